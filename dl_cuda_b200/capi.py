@@ -71,6 +71,14 @@ SIGNATURES = {
     "dlb_loss_bwd": (_i, [_i, _p, _p, _p, _i64, _i, _p]),
     "dlb_ce_from_ids_fwd": (_i, [_p, _p, _p, _i, _i, _f, _p]),
     "dlb_ce_from_ids_bwd": (_i, [_p, _p, _p, _i, _i, _f, _p]),
+    "dlb_attn_fwd_workspace_bytes": (_sz, [_p]),
+    "dlb_attn_fwd": (_i, [_p, _p, _sz, _p]),
+    "dlb_attn_bwd_workspace_bytes": (_sz, [_p, _p]),
+    "dlb_attn_bwd": (_i, [_p, _p, _p, _sz, _p]),
+    "dlb_rel_bucket_map_host": (_i, [_p, _i, _i, _i]),
+    "dlb_rel_bias_fwd": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _p]),
+    "dlb_rel_bias_bwd_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "dlb_rel_bias_bwd": (_i, [_p, _p, _p, _p, _sz, _i, _i, _i, _i, _i, _i, _i, _i, _p]),
 }
 
 
@@ -82,6 +90,27 @@ class PeerGroup(C.Structure):
     _fields_ = [("n_ranks", _i), ("my_rank", _i), ("cap_rows", _i), ("small_n", _i), ("timeout_ms", _i),
                 ("reserved", _i), ("flags", _p * MAX_PEERS), ("recv", _p * MAX_PEERS), ("grad", _p * MAX_PEERS),
                 ("small", _p * MAX_PEERS), ("stage", _p * MAX_PEERS), ("status", _p)]
+
+
+ATTN_MAX_HEAD_DIM, ATTN_MAX_BUCKETS, ATTN_MAX_DISTANCE = 128, 64, 1024
+
+
+class Heads(C.Structure):
+    """dlb_heads: an address and the strides (in elements) of batch, token and head."""
+    _fields_ = [("ptr", _p), ("batch_stride", _i64), ("token_stride", _i64), ("head_stride", _i64)]
+
+
+class Attn(C.Structure):
+    """dlb_attn of include/dlcuda_b200.h."""
+    _fields_ = [("batch", _i), ("heads", _i), ("kv_heads", _i), ("q_len", _i), ("kv_len", _i), ("head_dim", _i),
+                ("dtype", _i), ("causal", _i), ("scale", _f), ("cap", _f), ("buckets", _i), ("max_distance", _i),
+                ("kv_lens", _p), ("q_start", _p), ("prefix", _p), ("q_docs", _p), ("kv_docs", _p), ("slopes", _p),
+                ("table", _p), ("bucket_of", _p), ("q", Heads), ("k", Heads), ("v", Heads), ("o", Heads), ("lse", _p)]
+
+
+class AttnGrad(C.Structure):
+    """dlb_attn_grad of include/dlcuda_b200.h."""
+    _fields_ = [("dout", Heads), ("dq", Heads), ("dk", Heads), ("dv", Heads), ("dtable", _p)]
 
 
 class DlbError(RuntimeError):

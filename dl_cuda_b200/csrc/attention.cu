@@ -1,0 +1,276 @@
+// Entry points of the attention operators: argument checks, the choice between the kernels, and the
+// workspace layout.  The kernels: attn_generic.cuh (fp32 pipes, everything).
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_generic.cuh"
+
+namespace dlb {
+namespace {
+
+int check_heads(const char *call, const char *name, const dlb_heads &h, long long elements) {
+  DLB_REQUIRE(h.ptr != nullptr || elements == 0, DLB_ERR_INVALID_ARG, "%s: null pointer %s", call, name);
+  DLB_REQUIRE(h.batch_stride >= 0 && h.token_stride >= 0 && h.head_stride >= 0, DLB_ERR_INVALID_ARG,
+              "%s: negative stride of %s", call, name);
+  return DLB_OK;
+}
+
+// An output whose elements coincide would be written by several threads at once.
+int check_output(const char *call, const char *name, const dlb_heads &h, int batch, int tokens, int heads) {
+  DLB_REQUIRE((batch <= 1 || h.batch_stride > 0) && (tokens <= 1 || h.token_stride > 0) && (heads <= 1 || h.head_stride > 0),
+              DLB_ERR_INVALID_ARG, "%s: output %s has a stride of 0", call, name);
+  return DLB_OK;
+}
+
+int check(const char *call, const dlb_attn *a) {
+  DLB_REQUIRE(a != nullptr, DLB_ERR_INVALID_ARG, "%s: null argument block", call);
+  DLB_REQUIRE(a->batch >= 0 && a->q_len >= 0 && a->kv_len >= 0 && a->heads > 0 && a->kv_heads > 0 && a->head_dim > 0,
+              DLB_ERR_INVALID_ARG, "%s: batch=%d heads=%d kv_heads=%d q_len=%d kv_len=%d head_dim=%d", call, a->batch,
+              a->heads, a->kv_heads, a->q_len, a->kv_len, a->head_dim);
+  DLB_REQUIRE(a->heads % a->kv_heads == 0, DLB_ERR_INVALID_ARG, "%s: heads=%d is no multiple of kv_heads=%d", call,
+              a->heads, a->kv_heads);
+  DLB_REQUIRE(a->dtype == DLB_F32 || a->dtype == DLB_BF16, DLB_ERR_INVALID_ARG, "%s: dtype=%d", call, a->dtype);
+  DLB_REQUIRE(a->causal == 0 || a->causal == 1, DLB_ERR_INVALID_ARG, "%s: causal=%d", call, a->causal);
+  DLB_REQUIRE(std::isfinite(a->scale), DLB_ERR_INVALID_ARG, "%s: scale=%g", call, a->scale);
+  DLB_REQUIRE(std::isfinite(a->cap) && a->cap >= 0.f, DLB_ERR_INVALID_ARG, "%s: cap=%g", call, a->cap);
+  DLB_REQUIRE((a->q_docs == nullptr) == (a->kv_docs == nullptr), DLB_ERR_INVALID_ARG,
+              "%s: document numbers are needed for queries and keys, or for neither", call);
+  if (a->table) {
+    DLB_REQUIRE(a->bucket_of != nullptr, DLB_ERR_INVALID_ARG, "%s: table without bucket_of", call);
+    DLB_REQUIRE(a->buckets > 0 && a->max_distance >= 0, DLB_ERR_INVALID_ARG, "%s: buckets=%d max_distance=%d", call,
+                a->buckets, a->max_distance);
+    DLB_REQUIRE(a->buckets <= DLB_ATTN_MAX_BUCKETS && a->max_distance <= DLB_ATTN_MAX_DISTANCE, DLB_ERR_UNSUPPORTED,
+                "%s: buckets=%d (at most %d), max_distance=%d (at most %d)", call, a->buckets, DLB_ATTN_MAX_BUCKETS,
+                a->max_distance, DLB_ATTN_MAX_DISTANCE);
+  }
+  DLB_REQUIRE(a->head_dim <= DLB_ATTN_MAX_HEAD_DIM, DLB_ERR_UNSUPPORTED, "%s: head_dim=%d (at most %d)", call,
+              a->head_dim, DLB_ATTN_MAX_HEAD_DIM);
+  constexpr int kMaxLen = 1 << 29;
+  DLB_REQUIRE(a->q_len <= kMaxLen && a->kv_len <= kMaxLen, DLB_ERR_UNSUPPORTED, "%s: q_len=%d kv_len=%d", call,
+              a->q_len, a->kv_len);
+  // rows are numbered in 64 bits, tiles of rows by a 32-bit grid
+  const long long tiles = static_cast<long long>(a->batch) * a->heads * (ceil_div(std::max(a->q_len, a->kv_len), 64) + 1);
+  DLB_REQUIRE(tiles < (1ll << 31), DLB_ERR_UNSUPPORTED, "%s: batch=%d heads=%d lengths %d, %d make too many tiles", call,
+              a->batch, a->heads, a->q_len, a->kv_len);
+  const long long nq = static_cast<long long>(a->batch) * a->q_len, nk = static_cast<long long>(a->batch) * a->kv_len;
+  if (int st = check_heads(call, "q", a->q, nq)) return st;
+  if (int st = check_heads(call, "k", a->k, nk)) return st;
+  if (int st = check_heads(call, "v", a->v, nk)) return st;
+  return check_heads(call, "o", a->o, nq);
+}
+
+Heads heads_of(const dlb_heads &h) { return {h.ptr, h.batch_stride, h.token_stride, h.head_stride}; }
+
+AttnArgs args_of(const dlb_attn *a) {
+  AttnArgs p = {};
+  p.batch = a->batch;
+  p.heads = a->heads;
+  p.kv_heads = a->kv_heads;
+  p.group = a->heads / a->kv_heads;
+  p.q_len = a->q_len;
+  p.kv_len = a->kv_len;
+  p.dim = a->head_dim;
+  p.causal = a->causal;
+  p.scale = a->scale;
+  p.cap = a->cap;
+  p.kv_lens = a->kv_lens;
+  p.q_start = a->q_start;
+  p.prefix = a->prefix;
+  p.q_docs = a->q_docs;
+  p.kv_docs = a->kv_docs;
+  p.slopes = a->slopes;
+  p.table = a->table;
+  p.buckets = a->table ? a->buckets : 0;
+  p.reach = a->table ? a->max_distance : 0;
+  p.bucket_of = a->table ? a->bucket_of : nullptr;
+  p.q = heads_of(a->q);
+  p.k = heads_of(a->k);
+  p.v = heads_of(a->v);
+  p.o = heads_of(a->o);
+  p.lse = a->lse;
+  p.splits = 1;
+  return p;
+}
+
+// Can rows be read 16 bytes at a time?
+bool vector_rows(const Heads &h, int dim, int esize) {
+  const int v = 16 / esize;
+  return aligned16(h.ptr) && dim % v == 0 && h.batch % v == 0 && h.token % v == 0 && h.head % v == 0;
+}
+
+template <typename F>
+auto by_width(int dim, F &&f) {
+  if (dim <= 16) return f(std::integral_constant<int, 16>());
+  if (dim <= 32) return f(std::integral_constant<int, 32>());
+  if (dim <= 64) return f(std::integral_constant<int, 64>());
+  return f(std::integral_constant<int, 128>());
+}
+
+// Lets a kernel use `smem` bytes of dynamic shared memory.
+template <typename K>
+int allow_smem(K kern, size_t smem, const char *name) {
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  DLB_REQUIRE(e == cudaSuccess, DLB_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
+  return DLB_OK;
+}
+
+struct FwdPlan {
+  int pack, splits;
+  size_t bytes;
+};
+
+// Few queries: the heads that share a key/value head go into one tile, and the keys are split until
+// the grid fills the GPU twice (a share keeps at least two tiles).
+FwdPlan plan_fwd(const dlb_attn *a) {
+  FwdPlan p = {1, 1, 0};
+  const int group = a->heads / a->kv_heads;
+  if (static_cast<long long>(a->q_len) * group <= kGenTile) p.pack = group;
+  const long long ctas = static_cast<long long>(a->batch) * (a->heads / p.pack) *
+                         ceil_div(static_cast<long long>(a->q_len) * p.pack, static_cast<long long>(kGenTile));
+  const int key_tiles = ceil_div(a->kv_len, kGenTile);
+  if (ctas > 0 && ctas < sm_count())
+    p.splits = static_cast<int>(std::max(1ll, std::min({2ll * sm_count() / ctas, key_tiles / 2ll, 256ll})));
+  if (p.splits > 1) {
+    const size_t rows = static_cast<size_t>(a->batch) * a->heads * a->q_len * p.splits;
+    p.bytes = rows * (sizeof(float2) + sizeof(float) * a->head_dim);
+  }
+  return p;
+}
+
+template <typename T>
+int launch_fwd(AttnArgs p, const FwdPlan &plan, cudaStream_t st) {
+  const bool vec = vector_rows(p.q, p.dim, sizeof(T)) && vector_rows(p.k, p.dim, sizeof(T)) && vector_rows(p.v, p.dim, sizeof(T));
+  const int tiles = ceil_div(p.q_len * plan.pack, kGenTile);
+  const int rc = by_width(p.dim, [&](auto width) -> int {
+    constexpr int DP = decltype(width)::value;
+    const size_t smem = sizeof(float) * (3 * kGenTile * (DP + 4) + kGenTile * kGenScoreStride);
+    auto kern = attn_fwd_generic_kernel<T, DP>;
+    if (int s = allow_smem(kern, smem, "attn_fwd")) return s;
+    launch_pdl(kern, dim3(tiles * (p.heads / plan.pack) * p.batch, plan.splits), dim3(kGenThreads), smem, st, p, plan.pack, vec);
+    DLB_LAUNCH_CHECK("attn_fwd_generic");
+    return DLB_OK;
+  });
+  if (rc != DLB_OK || plan.splits == 1) return rc;
+  const size_t rows = static_cast<size_t>(p.batch) * p.heads * p.q_len;
+  launch_pdl(attn_join_kernel<T>, dim3(static_cast<unsigned>(ceil_div(rows, size_t{8}))), dim3(256), 0, st, p);
+  DLB_LAUNCH_CHECK("attn_join");
+  return DLB_OK;
+}
+
+struct BwdPlan {
+  int parts;  // partial tables per head
+  size_t stats_bytes, bytes;
+};
+
+BwdPlan plan_bwd(const dlb_attn *a, const dlb_attn_grad *g) {
+  BwdPlan p;
+  const size_t rows = static_cast<size_t>(a->batch) * a->heads * a->q_len;
+  p.stats_bytes = (rows * sizeof(float2) + 255) / 256 * 256;
+  p.parts = a->batch * ceil_div(a->q_len, kGenTile);
+  p.bytes = p.stats_bytes;
+  if (g->dtable && a->table) p.bytes += sizeof(float) * static_cast<size_t>(a->heads) * p.parts * a->buckets;
+  return p;
+}
+
+template <typename T>
+int launch_bwd(const AttnArgs &p, cudaStream_t st) {
+  const bool vec = vector_rows(p.q, p.dim, sizeof(T)) && vector_rows(p.k, p.dim, sizeof(T)) &&
+                   vector_rows(p.v, p.dim, sizeof(T)) && vector_rows(p.dout, p.dim, sizeof(T));
+  const size_t rows = static_cast<size_t>(p.batch) * p.heads * p.q_len;
+  if (rows > 0) {
+    launch_pdl(attn_row_stats_kernel<T>, dim3(static_cast<unsigned>(ceil_div(rows, size_t{8}))), dim3(256), 0, st, p);
+    DLB_LAUNCH_CHECK("attn_row_stats");
+  }
+  return by_width(p.dim, [&](auto width) -> int {
+    constexpr int DP = decltype(width)::value;
+    const size_t smem = sizeof(float) * (4 * kGenTile * (DP + 4) + 2 * kGenTile * kGenScoreStride);
+    if (p.kv_len > 0) {
+      auto kern = attn_bwd_generic_kernel<T, DP, true>;
+      if (int s = allow_smem(kern, smem, "attn_bwd")) return s;
+      launch_pdl(kern, dim3(ceil_div(p.kv_len, kGenTile) * p.kv_heads * p.batch), dim3(kGenThreads), smem, st, p, vec);
+      DLB_LAUNCH_CHECK("attn_bwd_generic");
+    }
+    if (p.q_len > 0) {
+      auto kern = attn_bwd_generic_kernel<T, DP, false>;
+      const size_t more = p.dtable ? sizeof(float) * 2 * p.buckets * kGenTile : 0;
+      if (int s = allow_smem(kern, smem + more, "attn_bwd")) return s;
+      launch_pdl(kern, dim3(ceil_div(p.q_len, kGenTile) * p.heads * p.batch), dim3(kGenThreads), smem + more, st, p, vec);
+      DLB_LAUNCH_CHECK("attn_bwd_generic");
+    }
+    return DLB_OK;
+  });
+}
+
+int check_workspace(const char *call, const void *workspace, size_t have, size_t need) {
+  DLB_REQUIRE(need == 0 || (workspace != nullptr && have >= need && aligned16(workspace)), DLB_ERR_WORKSPACE,
+              "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", call, need, have);
+  return DLB_OK;
+}
+
+}  // namespace
+}  // namespace dlb
+
+using namespace dlb;
+
+extern "C" size_t dlb_attn_fwd_workspace_bytes(const dlb_attn *a) {
+  if (check("attn_fwd", a) != DLB_OK) return 0;
+  return plan_fwd(a).bytes;
+}
+
+extern "C" int dlb_attn_fwd(const dlb_attn *a, void *workspace, size_t workspace_bytes, void *stream) {
+  if (int st = check("attn_fwd", a)) return st;
+  if (int st = check_output("attn_fwd", "o", a->o, a->batch, a->q_len, a->heads)) return st;
+  if (a->batch == 0 || a->q_len == 0) return DLB_OK;
+  const FwdPlan plan = plan_fwd(a);
+  if (int st = check_workspace("attn_fwd", workspace, workspace_bytes, plan.bytes)) return st;
+  AttnArgs p = args_of(a);
+  p.splits = plan.splits;
+  if (plan.splits > 1) {
+    p.part_ml = static_cast<float2 *>(workspace);
+    p.part_o = reinterpret_cast<float *>(p.part_ml + static_cast<size_t>(a->batch) * a->heads * a->q_len * plan.splits);
+  }
+  return a->dtype == DLB_F32 ? launch_fwd<float>(p, plan, as_stream(stream))
+                             : launch_fwd<__nv_bfloat16>(p, plan, as_stream(stream));
+}
+
+extern "C" size_t dlb_attn_bwd_workspace_bytes(const dlb_attn *a, const dlb_attn_grad *g) {
+  if (check("attn_bwd", a) != DLB_OK || g == nullptr) return 0;
+  return plan_bwd(a, g).bytes;
+}
+
+extern "C" int dlb_attn_bwd(const dlb_attn *a, const dlb_attn_grad *g, void *workspace, size_t workspace_bytes,
+                            void *stream) {
+  if (int st = check("attn_bwd", a)) return st;
+  DLB_REQUIRE(g != nullptr, DLB_ERR_INVALID_ARG, "attn_bwd: null gradient block");
+  const long long nq = static_cast<long long>(a->batch) * a->q_len, nk = static_cast<long long>(a->batch) * a->kv_len;
+  if (int st = check_heads("attn_bwd", "dout", g->dout, nq)) return st;
+  if (int st = check_heads("attn_bwd", "dq", g->dq, nq)) return st;
+  if (int st = check_heads("attn_bwd", "dk", g->dk, nk)) return st;
+  if (int st = check_heads("attn_bwd", "dv", g->dv, nk)) return st;
+  if (int st = check_output("attn_bwd", "dq", g->dq, a->batch, a->q_len, a->heads)) return st;
+  if (int st = check_output("attn_bwd", "dk", g->dk, a->batch, a->kv_len, a->kv_heads)) return st;
+  if (int st = check_output("attn_bwd", "dv", g->dv, a->batch, a->kv_len, a->kv_heads)) return st;
+  DLB_REQUIRE(a->lse != nullptr || nq == 0, DLB_ERR_INVALID_ARG, "attn_bwd: lse is needed");
+  DLB_REQUIRE(g->dtable == nullptr || a->table != nullptr, DLB_ERR_INVALID_ARG, "attn_bwd: dtable without table");
+  const BwdPlan plan = plan_bwd(a, g);
+  if (int st = check_workspace("attn_bwd", workspace, workspace_bytes, plan.bytes)) return st;
+  AttnArgs p = args_of(a);
+  p.dout = heads_of(g->dout);
+  p.dq = heads_of(g->dq);
+  p.dk = heads_of(g->dk);
+  p.dv = heads_of(g->dv);
+  p.dtable = g->dtable;
+  p.row_stats = static_cast<float2 *>(workspace);
+  p.table_part = reinterpret_cast<float *>(static_cast<char *>(workspace) + plan.stats_bytes);
+  p.table_parts = plan.parts;
+  cudaStream_t st = as_stream(stream);
+  if (a->batch > 0) {
+    const int rc = a->dtype == DLB_F32 ? launch_bwd<float>(p, st) : launch_bwd<__nv_bfloat16>(p, st);
+    if (rc != DLB_OK) return rc;
+  }
+  if (p.dtable) {
+    launch_pdl(attn_table_sum_kernel, dim3(p.heads * p.buckets), dim3(128), 0, st, p);
+    DLB_LAUNCH_CHECK("attn_table_sum");
+  }
+  return DLB_OK;
+}

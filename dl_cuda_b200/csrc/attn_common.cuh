@@ -1,0 +1,96 @@
+// What the attention kernels share: the arguments as they travel to the GPU, who sees whom, and
+// the score of a visible pair.  Scores are kept times log2(e), so that a probability is one exp2.
+#pragma once
+
+#include <climits>
+#include <cmath>
+
+#include "common.cuh"
+
+namespace dlb {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kHidesBelow = -1e30f;  // table entries under this hide their keys
+
+struct Heads {
+  void *ptr;
+  long long batch, token, head;  // strides in elements
+};
+
+struct AttnArgs {
+  int batch, heads, kv_heads, group, q_len, kv_len, dim, causal;
+  float scale, cap;
+  int buckets, reach;  // reach: max_distance of the bucket map
+  const int *kv_lens, *q_start, *prefix, *q_docs, *kv_docs;
+  const float *slopes, *table;
+  const int *bucket_of;
+  Heads q, k, v, o;
+  float *lse;
+  Heads dout, dq, dk, dv;  // backward only
+  float *dtable;
+  float2 *row_stats;       // backward: {lse * log2(e), delta} per (b, h, i)
+  float *table_part;       // backward: [heads][parts][buckets]
+  int table_parts;
+  // forward split over the keys: partial outputs [split][b, h, i][dim] and {max, sum} [split][b, h, i]
+  float *part_o;
+  float2 *part_ml;
+  int splits;
+};
+
+// Per batch: query i stands at start + i; keys from `end` on are reached by no query.
+struct BatchView {
+  int start, len, prefix, end;
+};
+
+__device__ __forceinline__ BatchView batch_view(const AttnArgs &a, int b) {
+  BatchView v;
+  v.start = a.q_start ? max(-(1 << 30), min(1 << 30, a.q_start[b])) : 0;
+  v.len = a.kv_lens ? max(0, min(a.kv_len, a.kv_lens[b])) : a.kv_len;
+  v.prefix = (a.causal && a.prefix) ? max(0, min(a.kv_len, a.prefix[b])) : 0;
+  v.end = a.causal ? min(v.len, max(max(v.start + a.q_len, 0), v.prefix)) : v.len;
+  return v;
+}
+
+// Keys [0, row_end) are visible to query i, as far as documents allow.
+__device__ __forceinline__ int row_end(const AttnArgs &a, const BatchView &v, int i) {
+  return a.causal ? min(v.len, max(v.start + i + 1, v.prefix)) : v.len;
+}
+
+// First query that sees key j (queries behind it see it too: row_end never falls with i).
+__device__ __forceinline__ int first_query(const AttnArgs &a, const BatchView &v, int j) {
+  return (!a.causal || j < v.prefix) ? 0 : max(0, j - v.start);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// tanh(x) = sign(x) * (1 - 2 / (1 + exp(2|x|))): near zero the difference cancels (absolute error
+// about 1e-7), where cap * tanh(x / cap) would lose relative precision in small scores; there the
+// odd series x - x^3/3 + 2x^5/15 - 17x^7/315 + 62x^9/2835 is used, whose first dropped term is under
+// 1e-8 of x for |x| < 0.25.
+__device__ __forceinline__ float tanh_score(float x) {
+  const float ax = fabsf(x), x2 = x * x;
+  const float e = ex2(ax * (2.f * kLog2e));
+  const float far = copysignf(1.f - __fdividef(2.f, 1.f + e), x);
+  float p = fmaf(x2, 62.f / 2835.f, -17.f / 315.f);
+  p = fmaf(x2, p, 2.f / 15.f);
+  p = fmaf(x2, p, -1.f / 3.f);
+  const float near = fmaf(x * x2, p, x);
+  return ax < 0.25f ? near : far;
+}
+
+// Table value of a bucket times log2(e), with the entries that hide their keys as -infinity.
+__device__ __forceinline__ float table_entry(const AttnArgs &a, int h, int bucket) {
+  const float t = a.table[h * a.buckets + bucket];
+  return t < kHidesBelow ? -INFINITY : t * kLog2e;
+}
+
+__device__ __forceinline__ int bucket_at(const AttnArgs &a, int distance) {
+  const int d = max(-a.reach, min(a.reach, distance)) + a.reach;
+  return min(max(a.bucket_of[d], 0), a.buckets - 1);
+}
+
+}  // namespace dlb

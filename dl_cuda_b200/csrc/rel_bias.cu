@@ -1,0 +1,205 @@
+// Learned relative position bias by buckets for programs that hold scores as a matrix: the add in
+// front of the softmax, and the gradient of the table.  Both are bound by HBM.
+#include <algorithm>
+#include <cmath>
+
+#include "common.cuh"
+
+namespace dlb {
+namespace {
+
+constexpr int kBiasThreads = 256;
+
+struct BiasArgs {
+  const void *in;  // scores (may be NULL) or dscores
+  const float *table;
+  const int *bucket_of;
+  void *out;
+  float *part;
+  int batch, heads, q_len, kv_len, start, buckets, reach;
+};
+
+__device__ __forceinline__ int bias_bucket(const BiasArgs &a, int distance) {
+  const int d = max(-a.reach, min(a.reach, distance)) + a.reach;
+  return min(max(a.bucket_of[d], 0), a.buckets - 1);
+}
+
+// A CTA takes rows of one head and keeps that head's bias by distance in shared memory.
+template <typename T>
+__global__ void __launch_bounds__(kBiasThreads) rel_bias_fwd_kernel(const __grid_constant__ BiasArgs a, int rows_per_cta, bool vec) {
+  pdl_prologue();
+  extern __shared__ float by_distance[];
+  const int row_tiles = (a.q_len + rows_per_cta - 1) / rows_per_cta;
+  const int tile = blockIdx.x % row_tiles, h = (blockIdx.x / row_tiles) % a.heads, b = blockIdx.x / (row_tiles * a.heads);
+  for (int d = threadIdx.x; d <= 2 * a.reach; d += kBiasThreads)
+    by_distance[d] = a.table[h * a.buckets + bias_bucket(a, d - a.reach)];
+  __syncthreads();
+  const int i1 = min(a.q_len, (tile + 1) * rows_per_cta);
+  for (int i = tile * rows_per_cta; i < i1; i++) {
+    const size_t row = (static_cast<size_t>(b) * a.heads + h) * a.q_len + i;
+    const T *src = a.in ? static_cast<const T *>(a.in) + row * a.kv_len : nullptr;
+    T *dst = static_cast<T *>(a.out) + row * a.kv_len;
+    const int shift = a.reach - (a.start + i);
+    if (vec) {
+      constexpr int V = Store<T>::kPerVec;
+      for (int j = threadIdx.x * V; j < a.kv_len; j += kBiasThreads * V) {
+        float f[V];
+#pragma unroll
+        for (int k = 0; k < V; k++) f[k] = 0.f;
+        if (src) Store<T>::unpack(ld_stream(src + j), f);
+#pragma unroll
+        for (int k = 0; k < V; k++) f[k] += by_distance[max(0, min(2 * a.reach, j + k + shift))];
+        st_stream(dst + j, Store<T>::pack(f));
+      }
+    } else {
+      for (int j = threadIdx.x; j < a.kv_len; j += kBiasThreads)
+        dst[j] = Store<T>::from_float((src ? Store<T>::to_float(ld_co(src + j)) : 0.f) + by_distance[max(0, min(2 * a.reach, j + shift))]);
+    }
+  }
+}
+
+// part[h][cta][bucket]: a CTA takes rows of one head of all batches; every thread adds up runs of one
+// bucket in a register and keeps a column of its own per bucket in shared memory.
+template <typename T>
+__global__ void __launch_bounds__(kBiasThreads) rel_bias_bwd_kernel(const __grid_constant__ BiasArgs a, int parts) {
+  pdl_prologue();
+  extern __shared__ float sums[];  // [buckets][threads]
+  const int part = blockIdx.x % parts, h = blockIdx.x / parts, tid = threadIdx.x;
+  for (int n = 0; n < a.buckets; n++) sums[n * kBiasThreads + tid] = 0.f;
+  const long long rows = static_cast<long long>(a.batch) * a.q_len;
+  for (long long r = part; r < rows; r += parts) {
+    const int b = r / a.q_len, i = r % a.q_len;
+    const T *src = static_cast<const T *>(a.in) + ((static_cast<size_t>(b) * a.heads + h) * a.q_len + i) * a.kv_len;
+    int now = -1;
+    float sum = 0.f;
+    for (int j = tid; j < a.kv_len; j += kBiasThreads) {
+      const int n = bias_bucket(a, j - (a.start + i));
+      if (n != now) {
+        if (now >= 0) sums[now * kBiasThreads + tid] += sum;
+        now = n;
+        sum = 0.f;
+      }
+      sum += Store<T>::to_float(ld_co(src + j));
+    }
+    if (now >= 0) sums[now * kBiasThreads + tid] += sum;
+  }
+  __syncthreads();
+  const int warp = tid / 32, lane = tid & 31;
+  for (int n = warp; n < a.buckets; n += kBiasThreads / 32) {
+    float s = 0.f;
+    for (int t = lane; t < kBiasThreads; t += 32) s += sums[n * kBiasThreads + t];
+    s = warp_sum(s);
+    if (lane == 0) a.part[(static_cast<size_t>(h) * parts + part) * a.buckets + n] = s;
+  }
+}
+
+__global__ void __launch_bounds__(128) rel_bias_sum_kernel(const float *part, float *out, int parts, int buckets) {
+  pdl_prologue();
+  __shared__ double warp_part[4];
+  const int h = blockIdx.x / buckets, n = blockIdx.x % buckets;
+  double sum = 0.0;
+  for (int p = threadIdx.x; p < parts; p += 128) sum += ld_co(part + (static_cast<size_t>(h) * parts + p) * buckets + n);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x / 32] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) out[blockIdx.x] = static_cast<float>(warp_part[0] + warp_part[1] + warp_part[2] + warp_part[3]);
+}
+
+int check_shape(const char *call, int batch, int heads, int q_len, int kv_len, int q_start, int buckets, int reach, int dtype) {
+  DLB_REQUIRE(batch >= 0 && heads >= 0 && q_len >= 0 && kv_len >= 0 && buckets > 0 && reach >= 0, DLB_ERR_INVALID_ARG,
+              "%s: batch=%d heads=%d q_len=%d kv_len=%d buckets=%d max_distance=%d", call, batch, heads, q_len, kv_len,
+              buckets, reach);
+  DLB_REQUIRE(dtype == DLB_F32 || dtype == DLB_BF16, DLB_ERR_INVALID_ARG, "%s: dtype=%d", call, dtype);
+  DLB_REQUIRE(buckets <= DLB_ATTN_MAX_BUCKETS && reach <= DLB_ATTN_MAX_DISTANCE, DLB_ERR_UNSUPPORTED,
+              "%s: buckets=%d (at most %d), max_distance=%d (at most %d)", call, buckets, DLB_ATTN_MAX_BUCKETS, reach,
+              DLB_ATTN_MAX_DISTANCE);
+  constexpr int kMax = 1 << 29;
+  DLB_REQUIRE(q_len <= kMax && kv_len <= kMax && q_start >= -2 * kMax && q_start <= 2 * kMax, DLB_ERR_UNSUPPORTED,
+              "%s: q_len=%d kv_len=%d q_start=%d", call, q_len, kv_len, q_start);
+  DLB_REQUIRE(static_cast<long long>(batch) * heads * q_len < (1ll << 31), DLB_ERR_UNSUPPORTED,
+              "%s: batch=%d heads=%d q_len=%d make too many rows", call, batch, heads, q_len);
+  return DLB_OK;
+}
+
+// Row groups of a head: enough CTAs for six per SM, at most one per row.
+int bias_parts(int batch, int heads, int q_len) {
+  const long long rows = static_cast<long long>(batch) * q_len;
+  return static_cast<int>(std::max(1ll, std::min<long long>(rows, ceil_div(6 * sm_count(), std::max(heads, 1)))));
+}
+
+}  // namespace
+}  // namespace dlb
+
+using namespace dlb;
+
+extern "C" int dlb_rel_bucket_map_host(int32_t *h_bucket_of, int buckets, int max_distance, int both_directions) {
+  DLB_REQUIRE(h_bucket_of != nullptr, DLB_ERR_INVALID_ARG, "rel_bucket_map: null pointer");
+  const int each = both_directions ? buckets / 2 : buckets;
+  const int own = each / 2;  // distances with a bucket of their own
+  DLB_REQUIRE(buckets > 0 && own >= 1 && (!both_directions || buckets % 2 == 0) && max_distance > own, DLB_ERR_INVALID_ARG,
+              "rel_bucket_map: buckets=%d max_distance=%d both_directions=%d", buckets, max_distance, both_directions);
+  DLB_REQUIRE(buckets <= DLB_ATTN_MAX_BUCKETS && max_distance <= DLB_ATTN_MAX_DISTANCE, DLB_ERR_UNSUPPORTED,
+              "rel_bucket_map: buckets=%d (at most %d), max_distance=%d (at most %d)", buckets, DLB_ATTN_MAX_BUCKETS,
+              max_distance, DLB_ATTN_MAX_DISTANCE);
+  const int wide = each - own;
+  auto of = [&](int distance) {
+    if (distance < own) return distance;
+    // log spacing; 1e-9 puts a border that falls on a whole distance into the upper bucket whatever log rounds to
+    const double at = std::log(static_cast<double>(distance) / own) / std::log(static_cast<double>(max_distance) / own) * wide;
+    return own + std::min(wide - 1, static_cast<int>(std::floor(at + 1e-9)));
+  };
+  for (int r = -max_distance; r <= max_distance; r++)
+    h_bucket_of[r + max_distance] = both_directions ? (r <= 0 ? of(-r) : each + of(r)) : of(std::max(-r, 0));
+  return DLB_OK;
+}
+
+extern "C" int dlb_rel_bias_fwd(const void *scores, const float *table, const int32_t *bucket_of, void *out, int batch,
+                                int heads, int q_len, int kv_len, int q_start, int buckets, int max_distance, int dtype,
+                                void *stream) {
+  if (int st = check_shape("rel_bias_fwd", batch, heads, q_len, kv_len, q_start, buckets, max_distance, dtype)) return st;
+  if (batch == 0 || heads == 0 || q_len == 0 || kv_len == 0) return DLB_OK;
+  DLB_REQUIRE(table && bucket_of && out, DLB_ERR_INVALID_ARG, "rel_bias_fwd: null pointer");
+  BiasArgs a = {scores, table, bucket_of, out, nullptr, batch, heads, q_len, kv_len, q_start, buckets, max_distance};
+  const int v = dtype == DLB_F32 ? 4 : 8;
+  const bool vec = aligned16(scores) && aligned16(out) && kv_len % v == 0;
+  const int rows_per_cta = 16;
+  const dim3 grid(ceil_div(q_len, rows_per_cta) * heads * batch);
+  const size_t smem = sizeof(float) * (2 * max_distance + 1);
+  if (dtype == DLB_F32)
+    launch_pdl(rel_bias_fwd_kernel<float>, grid, dim3(kBiasThreads), smem, as_stream(stream), a, rows_per_cta, vec);
+  else
+    launch_pdl(rel_bias_fwd_kernel<__nv_bfloat16>, grid, dim3(kBiasThreads), smem, as_stream(stream), a, rows_per_cta, vec);
+  DLB_LAUNCH_CHECK("rel_bias_fwd");
+  return DLB_OK;
+}
+
+extern "C" size_t dlb_rel_bias_bwd_workspace_bytes(int batch, int heads, int q_len, int kv_len, int buckets) {
+  if (check_shape("rel_bias_bwd", batch, heads, q_len, kv_len, 0, buckets, 0, DLB_F32) != DLB_OK) return 0;
+  return sizeof(float) * static_cast<size_t>(heads) * bias_parts(batch, heads, q_len) * buckets;
+}
+
+extern "C" int dlb_rel_bias_bwd(const void *dscores, const int32_t *bucket_of, float *dtable, void *workspace,
+                                size_t workspace_bytes, int batch, int heads, int q_len, int kv_len, int q_start,
+                                int buckets, int max_distance, int dtype, void *stream) {
+  if (int st = check_shape("rel_bias_bwd", batch, heads, q_len, kv_len, q_start, buckets, max_distance, dtype)) return st;
+  if (heads == 0) return DLB_OK;
+  const bool empty = batch == 0 || q_len == 0 || kv_len == 0;
+  DLB_REQUIRE((dscores || empty) && bucket_of && dtable, DLB_ERR_INVALID_ARG, "rel_bias_bwd: null pointer");
+  const size_t need = dlb_rel_bias_bwd_workspace_bytes(batch, heads, q_len, kv_len, buckets);
+  DLB_REQUIRE(workspace != nullptr && workspace_bytes >= need && aligned16(workspace), DLB_ERR_WORKSPACE,
+              "rel_bias_bwd: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
+  const int parts = bias_parts(batch, heads, q_len);
+  BiasArgs a = {dscores, nullptr, bucket_of, nullptr, static_cast<float *>(workspace), batch, heads, q_len, kv_len,
+                q_start, buckets, max_distance};
+  const size_t smem = sizeof(float) * buckets * kBiasThreads;
+  auto kern = dtype == DLB_F32 ? rel_bias_bwd_kernel<float> : rel_bias_bwd_kernel<__nv_bfloat16>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  DLB_REQUIRE(e == cudaSuccess, DLB_ERR_CUDA, "rel_bias_bwd: %s", cudaGetErrorString(e));
+  launch_pdl(kern, dim3(heads * parts), dim3(kBiasThreads), smem, as_stream(stream), a, parts);
+  DLB_LAUNCH_CHECK("rel_bias_bwd");
+  launch_pdl(rel_bias_sum_kernel, dim3(heads * buckets), dim3(128), 0, as_stream(stream),
+             static_cast<const float *>(a.part), dtable, parts, buckets);
+  DLB_LAUNCH_CHECK("rel_bias_sum");
+  return DLB_OK;
+}

@@ -490,6 +490,113 @@ DLB_API int dlb_ce_from_ids_bwd(const int32_t *target_ids, const float *y_pred,
                                 float *grad, int n, int classes, float epsilon,
                                 void *stream);
 
+/* ---- attention without a score matrix in memory -------------------------------
+ * For every batch b, head h (key/value head h / (heads / kv_heads)), query i at position
+ * p = (q_start ? q_start[b] : 0) + i, and key j:
+ *   x = scale * <q_i, k_j>;   s = cap > 0 ? cap * tanh(x / cap) : x;
+ *   s -= slopes[h] * |p - j|                         (slopes given)
+ *   s += table[h*buckets + bucket_of[clamp(j - p, -max_distance, max_distance) + max_distance]]
+ *                                                    (table given)
+ * Key j is visible to query i when
+ *   j < (kv_lens ? kv_lens[b] : kv_len), and
+ *   !causal, or j <= p, or j < prefix[b]             (prefix given), and
+ *   q_docs[b*q_len + i] == kv_docs[b*kv_len + j]     (documents given; any numbers, any order).
+ * o_i = softmax over the visible keys of s, times v;  lse_i = log of the sum of exp(s).  A query
+ * that sees no key gets o = 0 and lse = -infinity, and no gradient flows through it.  A table
+ * entry below -1e30 hides its keys, as -infinity does.
+ *
+ * q, o [batch, q_len, heads, head_dim] and k, v [batch, kv_len, kv_heads, head_dim] are given by
+ * an address and three strides in elements (columns are contiguous), so that the views of one
+ * fused projection, a cache larger than kv_len and [batch, head, token] layouts go in as they
+ * are; a stride of 0 repeats an input.  Outputs must not overlap anything else the call touches.
+ * k and v at keys that no query of the batch may reach (j >= kv_lens[b], or behind the last
+ * query's position and the prefix under a causal mask) may hold anything, NaN included; the
+ * values in front of that bound have to be finite, masked or not.
+ * kv_lens, q_start, prefix and the document arrays are int32 DEVICE arrays read by the kernels, so
+ * a captured graph sees what they hold when it is replayed; lengths and prefixes are clamped to
+ * [0, kv_len], starts to +-2^30.
+ *
+ * One entry point serves whole sequences and single tokens (q_len = 1 against a cache: the keys
+ * are split over the GPU and joined, through `workspace`).  Storage DLB_F32 keeps every product
+ * in fp32; DLB_BF16 multiplies on the tensor cores with fp32 sums and softmax statistics and
+ * rounds probabilities to bf16 in front of the second product.  head_dim 1..128; bf16 with
+ * head_dim, strides and addresses in multiples of 16 bytes takes the tensor cores, anything else
+ * plain CUDA kernels.  The result does not depend on scheduling: same call, same bits.
+ *
+ * Replaces the chain attnScoresKernel, applyCausalMaskKernel, softmaxForwardKernel and
+ * attnApplyKernel (src/transformer.cuh:8-58, call sites :441-486) for programs that do not need
+ * the probabilities in memory; caps, distance and bucket biases, documents, prefixes, lengths and
+ * shared key/value heads have no counterpart in the reference. */
+#define DLB_ATTN_MAX_HEAD_DIM 128
+#define DLB_ATTN_MAX_BUCKETS 64
+#define DLB_ATTN_MAX_DISTANCE 1024
+
+/* Element (b, token, head, column) lives at ptr[b*batch + token*token_stride + head*head_stride + column]. */
+typedef struct dlb_heads {
+  void *ptr;
+  int64_t batch_stride, token_stride, head_stride;
+} dlb_heads;
+
+typedef struct dlb_attn {
+  int batch, heads, kv_heads, q_len, kv_len, head_dim;
+  int dtype;  /* storage of q, k, v, o and their gradients */
+  int causal; /* 0 | 1 */
+  float scale;
+  float cap; /* 0: scores are not capped */
+  int buckets, max_distance; /* of table / bucket_of; ignored without a table */
+  const int32_t *kv_lens, *q_start, *prefix; /* [batch] or NULL */
+  const int32_t *q_docs, *kv_docs;           /* [batch, q_len], [batch, kv_len]: both or neither */
+  const float *slopes;                       /* [heads] or NULL */
+  const float *table;                        /* [heads, buckets] or NULL */
+  const int32_t *bucket_of;                  /* [2*max_distance + 1], values 0..buckets-1 (clamped) */
+  dlb_heads q, k, v, o;
+  float *lse; /* [batch, heads, q_len]; dlb_attn_fwd writes it (NULL: not wanted), dlb_attn_bwd reads it */
+} dlb_attn;
+
+DLB_API size_t dlb_attn_fwd_workspace_bytes(const dlb_attn *a);
+DLB_API int dlb_attn_fwd(const dlb_attn *a, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Gradients of q, k, v (storage type, overwritten) and of the table (fp32 [heads, buckets],
+ * overwritten; NULL: not wanted) from dout, with o and lse as dlb_attn_fwd left them.  Shared
+ * key/value heads get the sum over their query heads, table entries the sum over the batch; the
+ * probabilities are rebuilt from lse.  Keys that no query reaches get zero.  Every sum has a fixed
+ * order.  dout has to be finite, and lse within about +-1e4: the rebuilt probabilities carry a
+ * relative error of |lse| * 2^-23.  slopes are constants: they get no gradient.
+ * Replaces the attention part of TransformerLayer::backward (src/transformer.cuh:604-664:
+ * attnScoresKernel, attnApplyKernel, softmaxBackwardKernel, scaleBufferKernel, matMulATKernel). */
+typedef struct dlb_attn_grad {
+  dlb_heads dout, dq, dk, dv;
+  float *dtable;
+} dlb_attn_grad;
+
+DLB_API size_t dlb_attn_bwd_workspace_bytes(const dlb_attn *a, const dlb_attn_grad *g);
+DLB_API int dlb_attn_bwd(const dlb_attn *a, const dlb_attn_grad *g, void *workspace,
+                         size_t workspace_bytes, void *stream);
+
+/* ---- learned relative position bias by buckets --------------------------------
+ * Host map bucket_of[0 .. 2*max_distance] of j - p = -max_distance .. max_distance: with n buckets
+ * per direction (both_directions: n = buckets/2, keys behind the query use n..2n-1; else
+ * n = buckets and keys behind the query use bucket 0), distances below n/2 have their own bucket,
+ * larger ones share logarithmically spaced buckets up to max_distance, everything beyond is in
+ * the last.  A border that falls on a whole distance belongs to the upper bucket.
+ * No counterpart in the reference; built on the host as dlb_pe_build_table_host's table is. */
+DLB_API int dlb_rel_bucket_map_host(int32_t *h_bucket_of, int buckets, int max_distance,
+                                    int both_directions);
+
+/* For programs that hold scores as a matrix (dlb_gemm_f32 -> here -> dlb_softmax_fwd):
+ *   out[b,h,i,j] = (scores ? scores[b,h,i,j] : 0) + table[h, bucket_of[j - (q_start + i)]]
+ * over contiguous [batch, heads, q_len, kv_len]; out may be scores.  The gradient of the table is
+ * the sum of dscores over the batch and the positions of each bucket, in a fixed order.  dtype is
+ * the storage of scores, out and dscores; table and dtable are fp32.  No counterpart in the reference. */
+DLB_API int dlb_rel_bias_fwd(const void *scores, const float *table, const int32_t *bucket_of, void *out,
+                             int batch, int heads, int q_len, int kv_len, int q_start, int buckets,
+                             int max_distance, int dtype, void *stream);
+DLB_API size_t dlb_rel_bias_bwd_workspace_bytes(int batch, int heads, int q_len, int kv_len, int buckets);
+DLB_API int dlb_rel_bias_bwd(const void *dscores, const int32_t *bucket_of, float *dtable,
+                             void *workspace, size_t workspace_bytes, int batch, int heads,
+                             int q_len, int kv_len, int q_start, int buckets, int max_distance,
+                             int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

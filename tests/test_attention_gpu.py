@@ -1,0 +1,390 @@
+"""The attention operators against their formulas in 64 bits (tests/attention_reference.py holds the
+formulas and the bounds, entry by entry)."""
+import math
+
+import pytest
+import torch
+
+from attention_reference import check, reference
+from dl_cuda_b200 import capi, ops
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16}
+
+
+def make(seed, dtype, B, Sq, Sk, H, Hk, D, layout="fused", std=1.5):
+    """q, k, v, dout on the GPU, as views of what programs hold."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    dt = DTYPES[dtype]
+
+    def normal(*shape, scale=1.0):
+        return (torch.randn(*shape, generator=gen, device="cuda") * scale).to(dt)
+
+    if layout == "fused" and Sq == Sk:  # one projection: heads side by side
+        x = normal(B, Sq, H + 2 * Hk, D, scale=std)
+        q, k, v = x[:, :, :H], x[:, :, H:H + Hk], x[:, :, H + Hk:]
+    elif layout == "heads_first":  # [batch, head, token, column]
+        q, k, v = (normal(B, h, s, D, scale=std).transpose(1, 2) for h, s in ((H, Sq), (Hk, Sk), (Hk, Sk)))
+    else:
+        q, k, v = (normal(B, s, h, D, scale=std) for h, s in ((H, Sq), (Hk, Sk), (Hk, Sk)))
+    return q, k, v, normal(B, Sq, H, D)
+
+
+def ints(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def options(kind, B, Sq, Sk, H, seed=0):
+    gen = torch.Generator().manual_seed(seed + 17)
+    how = {}
+    for part in kind.split("+"):
+        if part == "causal":
+            how["causal"] = True
+        elif part == "cap":
+            how["cap"] = 5.0  # far into the bend
+        elif part == "slopes":
+            how["slopes"] = torch.rand(H, generator=gen).cuda()
+        elif part in ("table", "table1"):
+            both = part == "table"
+            how["bucket_of"] = ops.rel_bucket_map(16, 40, both).cuda()
+            how["table"] = torch.randn(H, 16, generator=gen).cuda()
+        elif part == "docs":
+            n = max(Sq, Sk)
+            d = torch.randint(0, 3, (B, n), generator=gen).sort(1)[0].int().cuda()
+            how["q_docs"], how["kv_docs"] = d[:, n - Sq:].contiguous(), d[:, :Sk].contiguous()
+        elif part == "mixed_docs":  # in no order, with queries whose document has no key
+            how["q_docs"] = torch.randint(0, 5, (B, Sq), generator=gen).int().cuda()
+            how["kv_docs"] = torch.randint(1, 4, (B, Sk), generator=gen).int().cuda()
+        elif part == "lens":
+            how["kv_lens"] = torch.randint(0, Sk + 1, (B,), generator=gen).int().cuda()
+            how["kv_lens"][0] = 0  # a sequence without a key
+        elif part == "prefix":
+            how["prefix"] = torch.randint(0, Sk + 1, (B,), generator=gen).int().cuda()
+        elif part == "start":
+            how["q_start"] = torch.randint(-3, Sk, (B,), generator=gen).int().cuda()
+    return how
+
+
+def run_both(q, k, v, dout, how, grads=True):
+    values, bounds = reference(q, k, v, dout if grads else None, **how)
+    o, lse = ops.attn_fwd(q, k, v, **how)
+    got = dict(o=o, lse=lse)
+    if grads:
+        dq, dk, dv, dtable = ops.attn_bwd(dout, q, k, v, o, lse, **how)
+        got.update(dq=dq, dk=dk, dv=dv, dtable=dtable)
+    check(got, values, bounds)
+    assert capi.pipeline_timeouts() == 0
+    return got
+
+
+KINDS = ["plain", "causal", "cap+causal", "slopes+causal", "table", "table1+causal", "cap+table+docs", "docs+causal",
+         "mixed_docs", "lens", "lens+causal+start", "prefix+causal", "prefix+causal+lens+slopes",
+         "cap+slopes+table+causal+docs+lens+prefix"]
+SHAPES = [  # B, Sq, Sk, H, Hk, D
+    (2, 1, 1, 2, 2, 16), (1, 64, 64, 2, 1, 64), (3, 65, 65, 4, 2, 32), (2, 130, 130, 4, 4, 64), (1, 257, 257, 3, 1, 128),
+    (2, 33, 190, 4, 2, 80), (2, 200, 70, 2, 2, 128), (1, 300, 300, 2, 2, 8),
+]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_forward_and_backward(shape, kind, dtype):
+    B, Sq, Sk, H, Hk, D = shape
+    q, k, v, dout = make(sum(shape), dtype, *shape)
+    run_both(q, k, v, dout, options(kind, B, Sq, Sk, H))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("D", [1, 3, 4, 17, 24, 40, 63, 72, 96, 100, 120, 127])
+def test_head_widths(D, dtype):
+    q, k, v, dout = make(D, dtype, 1, 70, 70, 4, 2, D)
+    run_both(q, k, v, dout, dict(causal=True))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("layout", ["fused", "heads_first", "plain"])
+@pytest.mark.parametrize("D", [64, 20])
+def test_layouts(layout, D, dtype):
+    q, k, v, dout = make(5, dtype, 2, 96, 96, 4, 2, D, layout)
+    run_both(q, k, v, dout.transpose(1, 2).contiguous().transpose(1, 2) if layout == "heads_first" else dout, dict(causal=True))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_repeated_inputs_and_strided_outputs(dtype):
+    """Keys of one sequence broadcast over the batch (stride 0), a broadcast gradient, outputs inside larger buffers."""
+    q, k, v, dout = make(9, dtype, 3, 70, 70, 4, 2, 64, "plain")
+    k, v = k[:1].expand(3, -1, -1, -1), v[:1].expand(3, -1, -1, -1)
+    dout = dout[:, :1].expand(-1, 70, -1, -1)
+    how = dict(causal=True)
+    values, bounds = reference(q, k, v, dout, **how)
+    wide = torch.full((3, 70, 8, 64), 7.0, dtype=q.dtype, device="cuda")
+    o, lse = ops.attn_fwd(q, k, v, out=wide[:, :, 2:6], **how)
+    room = [torch.full((3, 72, h + 1, 64), 7.0, dtype=q.dtype, device="cuda") for h in (4, 2, 2)]
+    views = [r[:, 1:71, :h] for r, h in zip(room, (4, 2, 2))]
+    dq, dk, dv, _ = ops.attn_bwd(dout, q, k, v, o, lse, dq=views[0], dk=views[1], dv=views[2], **how)
+    check(dict(o=o, lse=lse, dq=dq, dk=dk, dv=dv), values, bounds)
+    assert (wide[:, :, :2] == 7).all() and (wide[:, :, 6:] == 7).all()
+    for r, h in zip(room, (4, 2, 2)):
+        assert (r[:, 0] == 7).all() and (r[:, 71:] == 7).all() and (r[:, :, h] == 7).all()
+
+
+@pytest.mark.parametrize("offset", [1, 2, 3, 4, 8])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_addresses_off_the_vector_grid(dtype, offset):
+    q, k, v, dout = make(11, dtype, 1, 66, 66, 2, 2, 64, "plain")
+
+    def moved(t):
+        flat = torch.zeros(t.numel() + 64, dtype=t.dtype, device="cuda")
+        view = flat[offset:offset + t.numel()].view(t.shape)
+        view.copy_(t)
+        return view
+
+    run_both(moved(q), moved(k), moved(v), moved(dout), dict(causal=True))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("G", [1, 2, 4, 7, 8, 16, 24])
+@pytest.mark.parametrize("q_len", [1, 2, 5])
+def test_few_queries_against_a_cache(q_len, G, dtype):
+    """Single and few new tokens against ragged caches whose unused part holds NaN."""
+    B, Sk, Hk, D = 5, 700, 2, 128
+    q, k, v, _ = make(q_len * 31 + G, dtype, B, q_len, Sk, G * Hk, Hk, D, "plain")
+    lens = ints([q_len, 64, 129, 700, 333])
+    for b, n in enumerate(lens.tolist()):
+        k[b, n:] = math.nan
+        v[b, n:] = math.nan
+    for extra in ({}, dict(cap=5.0), options("slopes", B, q_len, Sk, G * Hk), options("table1", B, q_len, Sk, G * Hk)):
+        how = dict(causal=True, kv_lens=lens, q_start=lens - q_len, **extra)
+        run_both(q, k, v, None, how, grads=False)
+    # without lengths the causal bound alone keeps the unused part out
+    run_both(q, k, v, None, dict(causal=True, q_start=lens - q_len), grads=False)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("D", [16, 20, 64, 80, 128])
+@pytest.mark.parametrize("Sk", [1, 63, 64, 65, 1000, 5000])
+def test_one_token_lengths_and_widths(Sk, D, dtype):
+    q, k, v, _ = make(Sk + D, dtype, 2, 1, Sk, 8, 2, D, "plain")
+    run_both(q, k, v, None, dict(kv_lens=ints([Sk, (Sk + 1) // 2])), grads=False)
+    run_both(q, k, v, None, options("mixed_docs", 2, 1, Sk, 8), grads=False)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_unused_keys_may_hold_anything_in_training(dtype):
+    B, S = 3, 200
+    q, k, v, dout = make(21, dtype, B, S, S, 4, 2, 64, "plain")
+    lens = ints([1, 131, 200])
+    for b, n in enumerate(lens.tolist()):
+        k[b, n:] = math.nan
+        v[b, n:] = math.inf
+    got = run_both(q, k, v, dout, dict(kv_lens=lens))
+    for b, n in enumerate(lens.tolist()):
+        assert (got["dk"][b, n:] == 0).all() and (got["dv"][b, n:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_table_entries_that_hide_their_keys(dtype):
+    q, k, v, dout = make(23, dtype, 2, 150, 150, 2, 2, 64)
+    how = options("table", 2, 150, 150, 2)
+    how["table"][0, 3:9] = -math.inf
+    how["table"][1, 9:] = torch.finfo(torch.float32).min
+    run_both(q, k, v, dout, how)
+    how["table"][1] = torch.finfo(torch.float32).min  # head 1 sees nothing at all
+    got = run_both(q, k, v, dout, how)
+    assert (got["o"][:, :, 1] == 0).all() and (got["dq"][:, :, 1] == 0).all() and (got["dv"][:, :, 1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_large_scores(dtype):
+    """Scores of some hundreds: the running maximum has to carry them."""
+    q, k, v, dout = make(25, dtype, 1, 190, 190, 2, 2, 64, std=8.0)
+    run_both(q, k, v, dout, dict(causal=True))
+    run_both(q, k, v, dout, dict(causal=True, cap=30.0))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_empty_sizes(dtype):
+    dt = DTYPES[dtype]
+    e = lambda *s: torch.zeros(*s, dtype=dt, device="cuda")  # noqa: E731
+    o, lse = ops.attn_fwd(e(0, 5, 2, 16), e(0, 7, 2, 16), e(0, 7, 2, 16))
+    assert o.shape == (0, 5, 2, 16) and lse.shape == (0, 2, 5)
+    o, lse = ops.attn_fwd(e(2, 0, 2, 16), e(2, 7, 2, 16), e(2, 7, 2, 16))
+    assert o.numel() == 0
+    q = e(2, 5, 2, 16) + 1
+    o, lse = ops.attn_fwd(q, e(2, 0, 2, 16), e(2, 0, 2, 16))
+    assert (o == 0).all() and (lse == -math.inf).all()
+    dq, dk, dv, _ = ops.attn_bwd(q, q, e(2, 0, 2, 16), e(2, 0, 2, 16), o, lse)
+    assert (dq == 0).all() and dk.numel() == 0
+    k = e(2, 7, 2, 16) + 1
+    how = options("table", 2, 0, 7, 2)
+    none = e(2, 0, 2, 16)
+    dq, dk, dv, dtable = ops.attn_bwd(none, none, k, k, none, torch.zeros(2, 2, 0, device="cuda"), **how)
+    assert dq.numel() == 0 and (dk == 0).all() and (dv == 0).all() and (dtable == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("D", [64, 20])
+def test_same_bits_every_time_and_in_a_graph(D, dtype):
+    """The second call gives the first one's bits; a captured step follows lengths that change between replays."""
+    B, S, H = 2, 300, 4
+    q, k, v, dout = make(27, dtype, B, S, S, H, 2, D)
+    how = options("cap+table1+causal+docs", B, S, S, H)
+    lens = ints([300, 211])
+    how["kv_lens"] = lens
+
+    def step():
+        o, lse = ops.attn_fwd(q, k, v, **how)
+        return (o, lse) + ops.attn_bwd(dout, q, k, v, o, lse, **how)
+
+    first = step()
+    for a, b in zip(first, step()):
+        assert torch.equal(a, b)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    graph.replay()
+    for a, b in zip(first, held):
+        assert torch.equal(a, b)
+    lens.copy_(ints([17, 300]))
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(step(), held):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_two_streams_at_once(dtype):
+    """Two calls in flight, each with its own workspace, do not disturb each other."""
+    sets = [make(40 + n, dtype, 2, 1, 3000, 8, 2, 64, "plain")[:3] for n in range(2)]
+    want = [ops.attn_fwd(*s)[0].clone() for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [None, None]
+    for _ in range(10):
+        for n, (s, stream) in enumerate(zip(sets, streams)):
+            with torch.cuda.stream(stream):
+                got[n] = ops.attn_fwd(*s)[0]
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind", ["causal", "cap+table1+causal"])
+def test_gradients_against_differences(kind):
+    """Central differences of the 64-bit forward along random directions, against the kernels' fp32 gradients."""
+    B, S, H, Hk, D = 1, 70, 2, 1, 16
+    q, k, v, dout = make(51, "fp32", B, S, S, H, Hk, D, "plain")
+    how = options(kind, B, S, S, H)
+    o, lse = ops.attn_fwd(q, k, v, **how)
+    grads = dict(zip(("q", "k", "v", "table"), ops.attn_bwd(dout, q, k, v, o, lse, **how)))
+    inputs = dict(q=q, k=k, v=v, table=how.get("table"))
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    h = 1e-4  # the difference quotient is off by about h^2 of the third derivative: 1e-8
+    for name, x in inputs.items():
+        if x is None:
+            continue
+        along = torch.randn(x.shape, generator=gen, device="cuda", dtype=torch.float64)
+
+        def loss(sign):
+            moved = {n: (y.double() + sign * h * along if n == name else y) for n, y in inputs.items()}
+            rest = {n: y for n, y in how.items() if n != "table"}
+            if moved["table"] is not None:
+                rest["table"] = moved["table"]
+            return (reference(moved["q"].double(), moved["k"].double(), moved["v"].double(), **rest)[0]["o"] * dout.double()).sum()
+
+        want = ((loss(1) - loss(-1)) / (2 * h)).item()
+        got = (grads[name].double() * along).sum().item()
+        size = (grads[name].double() * along).abs().sum().item()
+        assert abs(got - want) <= 2e-6 * size + 1e-6, (name, got, want)
+
+
+def test_wrong_device_and_wrong_arguments():
+    q, k, v, dout = make(61, "fp32", 1, 8, 8, 2, 2, 16, "plain")
+    o, lse = ops.attn_fwd(q, k, v)
+    with pytest.raises(ValueError):
+        ops.attn_fwd(q.cpu(), k, v)
+    with pytest.raises(ValueError):
+        ops.attn_fwd(q, k.cpu(), v)
+    with pytest.raises(TypeError):
+        ops.attn_fwd(q, k.bfloat16(), v)
+    with pytest.raises(TypeError):
+        ops.attn_fwd(q.half(), k.half(), v.half())
+    with pytest.raises(ValueError):
+        ops.attn_fwd(q.transpose(2, 3), k, v)
+    with pytest.raises(ValueError):
+        ops.attn_fwd(q, k, v, kv_lens=torch.zeros(1, dtype=torch.int64, device="cuda"))
+    with pytest.raises(ValueError):
+        ops.attn_fwd(q, k, v, table=torch.zeros(2, 4, device="cuda"))
+    with pytest.raises(capi.DlbError):
+        ops.attn_fwd(q, k, v, q_docs=torch.zeros(1, 8, dtype=torch.int32, device="cuda"))
+    with pytest.raises(capi.DlbError):
+        ops.attn_fwd(q, k[:, :, :1].expand(-1, -1, 3, -1), v[:, :, :1].expand(-1, -1, 3, -1))
+    with pytest.raises(capi.DlbError):
+        ops.attn_fwd(q, k, v, out=o[:, :1].expand(-1, 8, -1, -1))
+    with pytest.raises(ValueError):
+        ops.attn_bwd(dout[:, :4], q, k, v, o, lse)
+
+
+# --- bucketed position bias on a score matrix ------------------------------------------------------
+BIAS_SHAPES = [(1, 1, 1, 1), (2, 3, 64, 64), (1, 4, 33, 130), (3, 2, 127, 65), (2, 2, 5, 1000), (1, 12, 200, 200)]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("q_start", [0, 7, -200])
+@pytest.mark.parametrize("shape", BIAS_SHAPES)
+def test_bias_matrix(shape, q_start, dtype):
+    B, H, Sq, Sk = shape
+    gen = torch.Generator(device="cuda").manual_seed(sum(shape))
+    dt, u = DTYPES[dtype], 2.0 ** -8 if dtype == "bf16" else 2.0 ** -24
+    scores = torch.randn(shape, generator=gen, device="cuda").to(dt)
+    table = torch.randn(H, 32, generator=gen, device="cuda")
+    for both in (True, False):
+        bucket_of = ops.rel_bucket_map(32, 50, both).cuda()
+        rel = torch.arange(Sk, device="cuda")[None] - (q_start + torch.arange(Sq, device="cuda"))[:, None]
+        bucket = bucket_of.long()[rel.clamp(-50, 50) + 50]
+        bias = table.double()[:, bucket]
+        for s in (scores, None):
+            out = ops.rel_bias_fwd(table, bucket_of, scores=s, shape=shape, q_start=q_start, dtype=dt)
+            want = bias[None].expand(shape) if s is None else s.double() + bias
+            # one fp32 addition, one rounding to the storage type
+            assert ((out.double() - want).abs() <= (u + 2.0 ** -24) * want.abs() + 1e-30).all()
+        inside = scores.clone()
+        ops.rel_bias_fwd(table, bucket_of, scores=inside, q_start=q_start, out=inside)
+        assert torch.equal(inside, ops.rel_bias_fwd(table, bucket_of, scores=scores, q_start=q_start))
+        d = ops.rel_bias_bwd(scores, bucket_of, 32, q_start=q_start)
+        assert torch.equal(d, ops.rel_bias_bwd(scores, bucket_of, 32, q_start=q_start))
+        one = torch.nn.functional.one_hot(bucket, 32).double()
+        want = torch.einsum("bhij,ijn->hn", scores.double(), one)
+        size = torch.einsum("bhij,ijn->hn", scores.double().abs(), one)
+        # at most B * Sq * (Sk / 256 + 2) fp32 additions stand one behind another, shared out over the row groups
+        chain = B * Sq * (Sk / 256 + 2) / max(1, min(B * Sq, 888 // H)) + Sk / 256 + 300
+        assert ((d.double() - want).abs() <= chain * 2.0 ** -24 * size + 1e-30).all()
+
+
+def test_bias_matrix_in_the_unfused_chain():
+    """Scores by dlb_gemm_f32, the bias, dlb_softmax_fwd and the product with the values: the fused call's result,
+    and the same gradient of the table by both ways."""
+    B, S, H, D = 2, 70, 3, 16
+    q, k, v, dout = make(71, "fp32", B, S, S, H, H, D, "plain")
+    how = options("table", B, S, S, H)
+    values, bounds = reference(q, k, v, dout, **how)
+    hf = lambda x: x.permute(0, 2, 1, 3).reshape(B * H, S, D).contiguous()  # noqa: E731
+    scores = ops.gemm(hf(q), hf(k).transpose(1, 2), alpha=D ** -0.5).view(B, H, S, S)
+    biased = ops.rel_bias_fwd(how["table"], how["bucket_of"], scores=scores)
+    p = ops.softmax_fwd(biased)
+    o = ops.gemm(p.view(B * H, S, S), hf(v)).view(B, H, S, D).permute(0, 2, 1, 3)
+    check(dict(o=o), values, bounds)
+    fused, lse = ops.attn_fwd(q, k, v, **how)
+    check(dict(o=fused, lse=lse), values, bounds)
+    dp = ops.gemm(hf(dout), hf(v).transpose(1, 2)).view(B, H, S, S)
+    ds = ops.softmax_bwd(dp, p)
+    by_matrix = ops.rel_bias_bwd(ds, how["bucket_of"], 16)
+    by_fusion = ops.attn_bwd(dout, q, k, v, fused, lse, **how)[3]
+    check(dict(dtable=by_matrix), values, bounds)
+    check(dict(dtable=by_fusion), values, bounds)
