@@ -4,6 +4,7 @@
 #include <type_traits>
 
 #include "attn_generic.cuh"
+#include "attn_mma.cuh"
 
 namespace dlb {
 namespace {
@@ -113,6 +114,9 @@ int allow_smem(K kern, size_t smem, const char *name) {
   DLB_REQUIRE(e == cudaSuccess, DLB_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
   return DLB_OK;
 }
+
+// From this many queries on, bf16 goes to the tensor cores.
+constexpr int kMmaQueries = 17;
 
 struct FwdPlan {
   int pack, splits;
@@ -228,6 +232,10 @@ extern "C" int dlb_attn_fwd(const dlb_attn *a, void *workspace, size_t workspace
   if (plan.splits > 1) {
     p.part_ml = static_cast<float2 *>(workspace);
     p.part_o = reinterpret_cast<float *>(p.part_ml + static_cast<size_t>(a->batch) * a->heads * a->q_len * plan.splits);
+  }
+  if (a->dtype == DLB_BF16 && a->q_len >= kMmaQueries && attn_mma_fits(p, false)) {
+    p.splits = 1;
+    return attn_fwd_mma(p, as_stream(stream));
   }
   return a->dtype == DLB_F32 ? launch_fwd<float>(p, plan, as_stream(stream))
                              : launch_fwd<__nv_bfloat16>(p, plan, as_stream(stream));

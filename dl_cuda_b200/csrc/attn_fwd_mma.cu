@@ -1,0 +1,503 @@
+// Attention forward on the tensor cores (bf16).
+//
+// A CTA owns two tiles of 128 queries of one head and walks over the tiles of 128 keys that any of
+// them sees.  Eight softmax warps and two more: one thread copies K and V tiles into a ring (TMA), one issues the products,
+// and each query tile has four warps for its softmax, one thread per row:
+//     S = Q K^T (TMEM, fp32) -> scores, running maximum, P = 2^(s - m) (bf16, written over S) -> O += P V
+// The two query tiles take turns: while one's softmax runs, the other's products do.  O stays in TMEM;
+// it is rescaled only when a row's maximum has grown by more than 2^8 since the last time, which P, the
+// sum and O all bear in fp32/bf16 range (the quotient is the same).  The sum behind the quotient adds
+// the ROUNDED probabilities, so that a row's weights add up to one exactly as the product sees them;
+// lse comes from the unrounded ones.
+#include <algorithm>
+
+#include "attn_mma.cuh"
+
+namespace dlb {
+namespace {
+
+constexpr int kFwdThreads = 384, kMmaWarp = 9, kLoadWarp = 8;
+// Registers: launched with 168 each (384 * 168 = 64512); the eight softmax warps go up to 208, the four
+// others down to 88 (256 * 208 + 128 * 88 = 64512).
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
+
+template <int NB>
+struct FwdShape {
+  static constexpr int kStages = NB == 2 ? 2 : 3;
+  static constexpr int kTileBytes = NB * kBlockBytes;
+  static constexpr int kRing = 2 * kTileBytes;                       // behind the two Q tiles
+  static constexpr int kLut = kRing + 2 * kStages * kTileBytes;      // K ring, V ring
+};
+
+struct FwdMaps {
+  CUtensorMap q, k, v;
+};
+
+template <int NB, bool CAP, int BIAS>
+__global__ void __launch_bounds__(kFwdThreads, 1)
+attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ FwdMaps maps, unsigned int *timeouts) {
+  using Shape = FwdShape<NB>;
+  constexpr int ST = Shape::kStages;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  unsigned char *ks = smem + Shape::kRing, *vs = ks + ST * Shape::kTileBytes;
+  float *lut = reinterpret_cast<float *>(smem + Shape::kLut);
+  unsigned char *flags = smem + Shape::kLut + (BIAS == kTable ? sizeof(float) * lut_floats(a.reach) : 0);
+  __shared__ uint64_t q_full, k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], s_full[2], p_full[2], o_full[2], drain;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int dead_flag;
+  __shared__ int doc_range[4];
+  volatile int *dead = &dead_flag;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    mbar_init(&q_full, 1);
+    for (int s = 0; s < ST; s++) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    for (int t = 0; t < 2; t++) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&o_full[t], 1);
+    }
+    mbar_init(&drain, 1);
+    dead_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == kMmaWarp) tmem_alloc(&tmem_slot, 512);
+  if (tid == kLoadWarp * 32) {
+    prefetch_map(&maps.q);
+    prefetch_map(&maps.k);
+    prefetch_map(&maps.v);
+  }
+  pdl_prologue();
+
+  // Pairs of query tiles are the slowest index, last pair first: long causal rows start early, and the
+  // heads that share keys run at the same time.
+  const int pairs = (a.q_len + 2 * kTileRows - 1) / (2 * kTileRows), per_pair = a.heads * a.batch;
+  const int pair = pairs - 1 - static_cast<int>(blockIdx.x) / per_pair;
+  const int h = blockIdx.x % a.heads, b = (blockIdx.x / a.heads) % a.batch, hk = h / a.group;
+  const int row0 = pair * 2 * kTileRows;
+  const BatchView view = batch_view(a, b);
+
+  // flags[n]: bit 2t: tile t sees some of key tile n; bit 2t + 1: every row of it sees all of it.
+  int first_end[2], last_end[2];
+#pragma unroll
+  for (int t = 0; t < 2; t++) {
+    const int r0 = row0 + t * kTileRows, r1 = min(a.q_len, r0 + kTileRows) - 1;
+    first_end[t] = r0 < a.q_len ? row_end(a, view, r0) : 0;
+    last_end[t] = r0 < a.q_len ? row_end(a, view, r1) : 0;
+  }
+  const int n_tiles = (max(last_end[0], last_end[1]) + kTileRows - 1) / kTileRows;
+  if (a.q_docs) {
+    if (warp < 2) {
+      int lo = INT_MAX, hi = INT_MIN;
+      for (int r = row0 + warp * kTileRows + lane; r < min(a.q_len, row0 + (warp + 1) * kTileRows); r += 32) {
+        const int d = ld_co(a.q_docs + static_cast<long long>(b) * a.q_len + r);
+        lo = min(lo, d);
+        hi = max(hi, d);
+      }
+      lo = warp_min(lo);
+      hi = warp_max(hi);
+      if (lane == 0) {
+        doc_range[2 * warp] = lo;
+        doc_range[2 * warp + 1] = hi;
+      }
+    }
+    __syncthreads();
+  }
+  for (int n = warp; n < n_tiles; n += kFwdThreads / 32) {
+    const int j0 = n * kTileRows;
+    int lo = 0, hi = 0;
+    if (a.kv_docs) {
+      lo = INT_MAX;
+      hi = INT_MIN;
+      for (int j = j0 + lane; j < min(view.end, j0 + kTileRows); j += 32) {
+        const int d = ld_co(a.kv_docs + static_cast<long long>(b) * a.kv_len + j);
+        lo = min(lo, d);
+        hi = max(hi, d);
+      }
+      lo = warp_min(lo);
+      hi = warp_max(hi);
+    }
+    int f = 0;
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      bool active = j0 < last_end[t], full = j0 + kTileRows <= first_end[t];
+      if (a.kv_docs) {
+        const int qlo = doc_range[2 * t], qhi = doc_range[2 * t + 1];
+        active = active && lo <= qhi && qlo <= hi;
+        full = full && lo == hi && qlo == qhi && lo == qlo;
+      }
+      if (active) f |= (full ? 3 : 1) << (2 * t);
+    }
+    if (lane == 0) flags[n] = static_cast<unsigned char>(f);
+  }
+  if (BIAS == kTable) fill_lut(lut, a, h, tid, kFwdThreads);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp < kLoadWarp) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    const int t = warp >> 2, i = row0 + t * kTileRows + (tid & 127);
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + lane_base + t * 128, o_at = tmem + lane_base + 256 + t * 128;
+    const bool valid = i < a.q_len;
+    const int end = valid ? row_end(a, view, i) : 0, pos = view.start + i;
+    const int doc = (a.q_docs && valid) ? ld_co(a.q_docs + static_cast<long long>(b) * a.q_len + i) : 0;
+    const float slope = (BIAS != kNoBias && a.slopes) ? ld_co(a.slopes + h) * kLog2e : 0.f;
+    const float to_log2 = CAP ? a.cap * kLog2e : a.scale * kLog2e, inside = CAP ? a.scale / a.cap : 0.f;
+    constexpr bool kRaw = !CAP && BIAS == kNoBias;  // maximum and exponent from the products themselves
+    const int tail = view.end % kTileRows && view.end < a.kv_len ? view.end / kTileRows : -1;
+    float m = -INFINITY, sum = 0.f, sum_rounded = 0.f;
+    int it = -1, done = 0;
+    for (int n = 0; n < n_tiles; n++) {
+      const int f = flags[n];
+      if (!f) continue;
+      it++;
+      if (!(f >> (2 * t) & 1)) continue;
+      const int j0 = n * kTileRows;
+      mbar_wait(&s_full[t], done & 1, dead, timeouts);
+      tc_fence_after();
+      uint32_t raw[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; c++) tmem_load32(s_at + c * 32, raw[c]);
+#pragma unroll
+      for (int c = 0; c < 4; c++) tmem_loaded(raw[c]);
+      float top = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        float x[32];
+#pragma unroll
+        for (int e = 0; e < 32; e++) x[e] = __uint_as_float(raw[c][e]);
+        if (CAP) tanh_scores(x, inside);
+        if (!kRaw) {
+          const float2 k2 = make_float2(to_log2, to_log2);
+          const int d0 = j0 + c * 32 - pos;
+          if (BIAS == kNoBias) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 y = mul2(make_float2(x[e], x[e + 1]), k2);
+              x[e] = y.x;
+              x[e + 1] = y.y;
+            }
+          } else {
+            float bias[32];
+#pragma unroll
+            for (int e = 0; e < 32; e++) bias[e] = 0.f;
+            if (BIAS == kTable) {
+              const bool left = d0 + 31 <= -a.reach, right = d0 >= a.reach;
+              if (__all_sync(0xffffffffu, left || right)) {
+                const float far = left ? lut[0] : lut[2 * (a.reach + kLutPad)];
+#pragma unroll
+                for (int e = 0; e < 32; e++) bias[e] = far;
+              } else {
+                // within 31 + 31 of the reach on either side: the padded table covers every index
+                const float *at = lut + d0 + a.reach + kLutPad;
+#pragma unroll
+                for (int e = 0; e < 32; e++) bias[e] = at[e];
+              }
+            }
+            if (BIAS == kSlope || a.slopes) {
+              const float d = static_cast<float>(d0);
+#pragma unroll
+              for (int e = 0; e < 32; e++) bias[e] = fmaf(-slope, fabsf(d + static_cast<float>(e)), bias[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 y = fma2(make_float2(x[e], x[e + 1]), k2, make_float2(bias[e], bias[e + 1]));
+              x[e] = y.x;
+              x[e + 1] = y.y;
+            }
+          }
+        }
+        if (!(f >> (2 * t + 1) & 1)) {
+          if (a.kv_docs) {
+            const int *docs = a.kv_docs + static_cast<long long>(b) * a.kv_len + j0 + c * 32;
+#pragma unroll
+            for (int e = 0; e < 32; e++) {
+              const int j = j0 + c * 32 + e;
+              if (j >= end || ld_co(docs + e) != doc) x[e] = -INFINITY;
+            }
+          } else {
+            const int room = end - (j0 + c * 32);
+#pragma unroll
+            for (int e = 0; e < 32; e++)
+              if (e >= room) x[e] = -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e++) {
+          top = fmaxf(top, x[e]);
+          raw[c][e] = __float_as_uint(x[e]);
+        }
+      }
+      if (kRaw) top *= to_log2;
+      const bool grow = top > m + 8.f;  // with m = -inf: whenever the row sees anything
+      if (__any_sync(0xffffffffu, grow)) {
+        const float keep = grow ? ex2(m - top) : 1.f;
+        if (grow) m = top;
+        sum *= keep;
+        sum_rounded *= keep;
+        if (done > 0) {
+          const float2 k2 = make_float2(keep, keep);
+          for (int c = 0; c < a.dim; c += 32) {
+            uint32_t o[32];
+            tmem_load32(o_at + c, o);
+            tmem_loaded(o);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 y = mul2(make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1])), k2);
+              o[e] = __float_as_uint(y.x);
+              o[e + 1] = __float_as_uint(y.y);
+            }
+            tmem_store32(o_at + c, o);
+          }
+        }
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+      const float2 mult = make_float2(kRaw ? to_log2 : 1.f, kRaw ? to_log2 : 1.f), minus = make_float2(-base, -base);
+      float2 part = make_float2(0.f, 0.f), part_rounded = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        uint32_t packed[32];
+#pragma unroll
+        for (int e = 0; e < 32; e++) {
+          const float2 y = fma2(make_float2(__uint_as_float(raw[2 * c + e / 16][2 * (e % 16)]),
+                                            __uint_as_float(raw[2 * c + e / 16][2 * (e % 16) + 1])), mult, minus);
+          const float2 p = make_float2(ex2(y.x), ex2(y.y));
+          packed[e] = pack_bf16(p.x, p.y);
+          part = add2(part, p);
+          part_rounded = add2(part_rounded, make_float2(__uint_as_float(packed[e] << 16), __uint_as_float(packed[e] & 0xffff0000u)));
+        }
+        tmem_store32(s_at + c * 32, packed);
+      }
+      sum += part.x + part.y;
+      sum_rounded += part_rounded.x + part_rounded.y;
+      if (n == tail) {
+        // Rows of V behind the last key any query reaches may hold anything, and 0 * NaN is NaN.
+        const int s = it % ST;
+        mbar_wait(&v_full[s], (it / ST) & 1, dead, timeouts);
+        const int from = view.end - j0;
+        for (int e = tid & 127; e < (kTileRows - from) * NB * 8; e += 128) {
+          const int r = from + e / (NB * 8), x = e % (NB * 8);
+          *reinterpret_cast<uint4 *>(vs + s * Shape::kTileBytes + (x / 8) * kBlockBytes + r * 128 + (x % 8) * 16) =
+              make_uint4(0, 0, 0, 0);
+        }
+        fence_async_smem();
+      }
+      tmem_stored();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[t]);
+      done++;
+    }
+    if (done > 0) mbar_wait(&o_full[t], 0, dead, timeouts);
+    tc_fence_after();
+    const float inv = sum_rounded > 0.f || sum_rounded != sum_rounded ? 1.f / sum_rounded : 0.f;
+    __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(a.o.ptr) + b * a.o.batch + static_cast<long long>(i) * a.o.token + h * a.o.head;
+    for (int c = 0; c < a.dim; c += 32) {
+      uint32_t o[32];
+      if (done > 0) {
+        tmem_load32(o_at + c, o);
+        tmem_loaded(o);
+      }
+#pragma unroll
+      for (int e = 0; e < 32; e += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          w[k] = inv == 0.f ? 0u : pack_bf16(__uint_as_float(o[e + 2 * k]) * inv, __uint_as_float(o[e + 2 * k + 1]) * inv);
+        if (valid && c + e < a.dim) *reinterpret_cast<uint4 *>(out + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    if (a.lse && valid)
+      a.lse[(static_cast<size_t>(b) * a.heads + h) * a.q_len + i] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
+    tc_fence_before();
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == kLoadWarp) {
+      if (lane == 0) {
+        const int q_tiles = row0 + kTileRows < a.q_len ? 2 : 1;
+        mbar_expect_tx(&q_full, q_tiles * Shape::kTileBytes);
+        for (int t = 0; t < q_tiles; t++)
+          for (int c = 0; c < NB; c++)
+            tma_load_rows(smem + (t * NB + c) * kBlockBytes, &maps.q, &q_full, c * kBlockCols, row0 + t * kTileRows, h, b);
+        int it = 0;
+        for (int n = 0; n < n_tiles; n++) {
+          if (!flags[n]) continue;
+          const int s = it % ST;
+          const unsigned use = it / ST;
+          if (use) mbar_wait(&k_empty[s], (use - 1) & 1, dead, timeouts);
+          if (*dead) break;
+          mbar_expect_tx(&k_full[s], Shape::kTileBytes);
+          for (int c = 0; c < NB; c++)
+            tma_load_rows(ks + (s * NB + c) * kBlockBytes, &maps.k, &k_full[s], c * kBlockCols, n * kTileRows, hk, b);
+          if (use) mbar_wait(&v_empty[s], (use - 1) & 1, dead, timeouts);
+          if (*dead) {
+            drain_wait(&k_full[s], use & 1);
+            break;
+          }
+          mbar_expect_tx(&v_full[s], Shape::kTileBytes);
+          for (int c = 0; c < NB; c++)
+            tma_load_rows(vs + (s * NB + c) * kBlockBytes, &maps.v, &v_full[s], c * kBlockCols, n * kTileRows, hk, b);
+          it++;
+        }
+        // The CTA must not end with copies in flight: after a wait that gave up they are waited for here.
+        if (*dead) {
+          drain_wait(&q_full, 0);
+          for (int i = max(0, it - ST); i < it; i++) {
+            drain_wait(&k_full[i % ST], (i / ST) & 1);
+            drain_wait(&v_full[i % ST], (i / ST) & 1);
+          }
+        }
+      }
+    } else if (warp == kMmaWarp) {
+      if (lane == 0) {
+        const int k_steps = (a.dim + 15) / 16, n_cols = k_steps * 16;
+        const uint32_t idesc_s = mma_desc(kTileRows, false), idesc_o = mma_desc(n_cols, true);
+        const uint32_t qa = smem_u32(smem), ka = smem_u32(ks), va = smem_u32(vs);
+        bool pending[2] = {false, false}, started[2] = {false, false};
+        unsigned p_phase[2] = {0, 0};
+        auto issue_pv = [&](int t, int s) {  // O_t += P_t V(stage s)
+          mbar_wait(&p_full[t], p_phase[t], dead, timeouts);
+          p_phase[t] ^= 1;
+          tc_fence_after();
+          const uint64_t vd = desc_mn_major(va + s * Shape::kTileBytes, kBlockBytes);
+          for (int k = 0; k < kTileRows / 16; k++)
+            mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, vd + k * (2048 >> 4), idesc_o, started[t] || k > 0);
+          started[t] = true;
+          pending[t] = false;
+        };
+        mbar_wait(&q_full, 0, dead, timeouts);
+        int it = 0;
+        for (int n = 0; n < n_tiles; n++) {
+          const int f = flags[n];
+          if (!f) continue;
+          const int s = it % ST, before = (it + ST - 1) % ST;
+          mbar_wait(&k_full[s], (it / ST) & 1, dead, timeouts);
+          if (it > 0) mbar_wait(&v_full[before], ((it - 1) / ST) & 1, dead, timeouts);
+          for (int t = 0; t < 2; t++) {
+            if (pending[t]) issue_pv(t, before);
+            if (f >> (2 * t) & 1) {
+              const uint64_t qd = desc_k_major(qa + t * Shape::kTileBytes), kd = desc_k_major(ka + s * Shape::kTileBytes);
+              for (int k = 0; k < k_steps; k++) {
+                const int at = (k / 4) * (kBlockBytes >> 4) + (k % 4) * 2;
+                mma_ss(tmem + t * 128, qd + at, kd + at, idesc_s, k > 0);
+              }
+              tc_commit(&s_full[t]);
+              pending[t] = true;
+            }
+          }
+          tc_commit(&k_empty[s]);
+          if (it > 0) tc_commit(&v_empty[before]);
+          it++;
+        }
+        if (it > 0) {
+          const int s = (it - 1) % ST;
+          mbar_wait(&v_full[s], ((it - 1) / ST) & 1, dead, timeouts);
+          for (int t = 0; t < 2; t++) {
+            if (pending[t]) issue_pv(t, s);
+            if (started[t]) tc_commit(&o_full[t]);
+          }
+        }
+        if (*dead) {
+          tc_commit(&drain);
+          drain_wait(&drain, 0);
+        }
+      }
+      }
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_free(tmem, 512);
+  }
+}
+
+}  // namespace
+
+int make_heads_map(CUtensorMap *map, const void *ptr, int dim, int tokens, int heads, int batch, long long token_stride,
+                   long long head_stride, long long batch_stride, int rows) {
+  using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                              const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static std::atomic<Encode> cached{nullptr};
+  Encode encode = cached.load(std::memory_order_acquire);
+  if (encode == nullptr) {
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found) != cudaSuccess || fn == nullptr)
+      return -1;
+    encode = reinterpret_cast<Encode>(fn);
+    cached.store(encode, std::memory_order_release);
+  }
+  // A stride of a dimension with one entry is never used: any valid value will do.
+  const cuuint64_t row = 16ull * ((dim * 2 + 15) / 16);
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(tokens), static_cast<cuuint64_t>(heads),
+                              static_cast<cuuint64_t>(batch)};
+  const cuuint64_t strides[3] = {tokens > 1 ? 2ull * token_stride : row, heads > 1 ? 2ull * head_stride : row,
+                                 batch > 1 ? 2ull * batch_stride : row};
+  const cuuint32_t box[4] = {kBlockCols, static_cast<cuuint32_t>(rows), 1, 1}, ones[4] = {1, 1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(ptr), dims, strides, box, ones,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
+namespace {
+
+// A tensor map wants positive strides in multiples of 16 bytes under 2^40; stores want the same grid.
+bool grid16(const Heads &h, int tokens, int heads, int batch) {
+  auto ok = [](int n, long long s) { return n <= 1 || (s > 0 && s % 8 == 0 && s < (1ll << 38)); };
+  return aligned16(h.ptr) && ok(tokens, h.token) && ok(heads, h.head) && ok(batch, h.batch);
+}
+
+}  // namespace
+
+bool attn_mma_fits(const AttnArgs &a, bool backward) {
+  if (a.dim % 8 != 0 || !(a.scale > 0.f) || a.q_len <= 0 || a.kv_len <= 0) return false;
+  if (a.kv_len > kMaxTiles * kTileRows || a.q_len > kMaxTiles * kTileRows) return false;
+  if (!grid16(a.q, a.q_len, a.heads, a.batch) || !grid16(a.o, a.q_len, a.heads, a.batch)) return false;
+  if (!grid16(a.k, a.kv_len, a.kv_heads, a.batch) || !grid16(a.v, a.kv_len, a.kv_heads, a.batch)) return false;
+  if (!backward) return true;
+  return grid16(a.dout, a.q_len, a.heads, a.batch) && grid16(a.dq, a.q_len, a.heads, a.batch) &&
+         grid16(a.dk, a.kv_len, a.kv_heads, a.batch) && grid16(a.dv, a.kv_len, a.kv_heads, a.batch);
+}
+
+int attn_fwd_mma(const AttnArgs &a, cudaStream_t st) {
+  FwdMaps maps;
+  int rc = make_heads_map(&maps.q, a.q.ptr, a.dim, a.q_len, a.heads, a.batch, a.q.token, a.q.head, a.q.batch, kTileRows);
+  if (!rc) rc = make_heads_map(&maps.k, a.k.ptr, a.dim, a.kv_len, a.kv_heads, a.batch, a.k.token, a.k.head, a.k.batch, kTileRows);
+  if (!rc) rc = make_heads_map(&maps.v, a.v.ptr, a.dim, a.kv_len, a.kv_heads, a.batch, a.v.token, a.v.head, a.v.batch, kTileRows);
+  DLB_REQUIRE(rc == 0, DLB_ERR_CUDA, "attn_fwd: tensor map refused (%d)", rc);
+  unsigned int *timeouts = wait_timeouts_counter();
+  DLB_REQUIRE(timeouts != nullptr, DLB_ERR_NO_DEVICE, "attn_fwd: no CUDA device");
+  const int tiles = ceil_div(a.kv_len, kTileRows);
+  auto launch = [&](auto kern, int blocks) -> int {
+    const size_t smem = 1024 + (blocks == 2 ? FwdShape<2>::kLut : FwdShape<1>::kLut) +
+                        (a.table ? sizeof(float) * lut_floats(a.reach) : 0) + ceil_div(tiles, 16) * 16;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    DLB_REQUIRE(e == cudaSuccess, DLB_ERR_CUDA, "attn_fwd: %s", cudaGetErrorString(e));
+    const int grid = ceil_div(a.q_len, 2 * kTileRows) * a.heads * a.batch;
+    launch_pdl(kern, dim3(grid), dim3(kFwdThreads), smem, st, a, maps, timeouts);
+    DLB_LAUNCH_CHECK("attn_fwd_mma");
+    return DLB_OK;
+  };
+  const int bias = a.table ? kTable : a.slopes ? kSlope : kNoBias;
+#define DLB_PICK(NB)                                                                                   \
+  (a.cap > 0.f ? (bias == kTable   ? launch(attn_fwd_mma_kernel<NB, true, kTable>, NB)                 \
+                  : bias == kSlope ? launch(attn_fwd_mma_kernel<NB, true, kSlope>, NB)                 \
+                                   : launch(attn_fwd_mma_kernel<NB, true, kNoBias>, NB))               \
+               : (bias == kTable   ? launch(attn_fwd_mma_kernel<NB, false, kTable>, NB)                \
+                  : bias == kSlope ? launch(attn_fwd_mma_kernel<NB, false, kSlope>, NB)                \
+                                   : launch(attn_fwd_mma_kernel<NB, false, kNoBias>, NB)))
+  return a.dim <= kBlockCols ? DLB_PICK(1) : DLB_PICK(2);
+#undef DLB_PICK
+}
+
+}  // namespace dlb
