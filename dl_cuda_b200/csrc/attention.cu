@@ -168,8 +168,7 @@ struct BwdPlan {
 
 BwdPlan plan_bwd(const dlb_attn *a, const dlb_attn_grad *g) {
   BwdPlan p;
-  const size_t rows = static_cast<size_t>(a->batch) * a->heads * a->q_len;
-  p.stats_bytes = (rows * sizeof(float2) + 255) / 256 * 256;
+  p.stats_bytes = static_cast<size_t>(a->batch) * a->heads * stat_tiles(a->q_len) * 2 * kStatRows * sizeof(float);
   p.parts = a->batch * ceil_div(a->q_len, kGenTile);
   p.bytes = p.stats_bytes;
   if (g->dtable && a->table) p.bytes += sizeof(float) * static_cast<size_t>(a->heads) * p.parts * a->buckets;
@@ -177,13 +176,17 @@ BwdPlan plan_bwd(const dlb_attn *a, const dlb_attn_grad *g) {
 }
 
 template <typename T>
-int launch_bwd(const AttnArgs &p, cudaStream_t st) {
+int launch_bwd(const AttnArgs &p, bool mma, cudaStream_t st) {
   const bool vec = vector_rows(p.q, p.dim, sizeof(T)) && vector_rows(p.k, p.dim, sizeof(T)) &&
                    vector_rows(p.v, p.dim, sizeof(T)) && vector_rows(p.dout, p.dim, sizeof(T));
-  const size_t rows = static_cast<size_t>(p.batch) * p.heads * p.q_len;
+  const size_t rows = static_cast<size_t>(p.batch) * p.heads * stat_tiles(p.q_len) * kStatRows;
   if (rows > 0) {
     launch_pdl(attn_row_stats_kernel<T>, dim3(static_cast<unsigned>(ceil_div(rows, size_t{8}))), dim3(256), 0, st, p);
     DLB_LAUNCH_CHECK("attn_row_stats");
+  }
+  if (mma) {
+    if (int s = attn_bwd_mma_keys(p, st)) return s;
+    return attn_bwd_mma_queries(p, st);
   }
   return by_width(p.dim, [&](auto width) -> int {
     constexpr int DP = decltype(width)::value;
@@ -268,12 +271,14 @@ extern "C" int dlb_attn_bwd(const dlb_attn *a, const dlb_attn_grad *g, void *wor
   p.dk = heads_of(g->dk);
   p.dv = heads_of(g->dv);
   p.dtable = g->dtable;
-  p.row_stats = static_cast<float2 *>(workspace);
+  p.row_stats = static_cast<float *>(workspace);
   p.table_part = reinterpret_cast<float *>(static_cast<char *>(workspace) + plan.stats_bytes);
   p.table_parts = plan.parts;
   cudaStream_t st = as_stream(stream);
   if (a->batch > 0) {
-    const int rc = a->dtype == DLB_F32 ? launch_bwd<float>(p, st) : launch_bwd<__nv_bfloat16>(p, st);
+    const bool mma = a->dtype == DLB_BF16 && attn_mma_fits(p, true) && attn_bwd_mma_room(p);
+    if (mma) p.table_parts = a->batch * ceil_div(a->q_len, kTileRows);
+    const int rc = a->dtype == DLB_F32 ? launch_bwd<float>(p, false, st) : launch_bwd<__nv_bfloat16>(p, mma, st);
     if (rc != DLB_OK) return rc;
   }
   if (p.dtable) {

@@ -1,0 +1,537 @@
+// Attention backward on the tensor cores (bf16): one kernel in two roles.
+//
+// A CTA keeps 128 rows X, Y (FOR_KEYS: a tile of K and V; else of Q and dO) and streams the other side
+// U, W (Q and dO of every head of the group; else K and V) past them in tiles of 64 rows:
+//     S = X U^T, G = Y W^T (TMEM) -> P = 2^(s - lse), D = P (G - delta), times the cap's derivative
+//     FOR_KEYS: dV += P W, dK += D U;   else dQ += D U                 (TMEM, scaled at the end)
+// with P and D written over S and G as bf16.  Two groups of four warps take alternate tiles, one
+// thread per row, so that the products of one tile run beside the exponentials of the other.
+//
+// Two passes rebuild S and G twice: 7 products of 2 * dim flop per pair where a single pass would need
+// 5.  In return no sum crosses a CTA: no fp32 copy of dQ in memory, no atomics, the same bits every time.
+#pragma once
+
+#include <algorithm>
+
+#include "attn_mma.cuh"
+
+namespace dlb {
+
+constexpr int kStreamRows = 64, kStreamBlock = kStreamRows * 128;
+constexpr int kBwdThreads = 320, kBwdLoadWarp = 8, kBwdMmaWarp = 9;
+constexpr int kStatsBytes = 2 * kStreamRows * sizeof(float);
+
+template <int NB, int ST>
+struct BwdShape {
+  static constexpr int kX = 0, kY = NB * kBlockBytes, kRing = 2 * NB * kBlockBytes;
+  static constexpr int kStage = 2 * NB * kStreamBlock;
+  static constexpr int kStats = kRing + ST * kStage, kRest = kStats + ST * kStatsBytes;
+};
+
+struct BwdMaps {
+  CUtensorMap x, y, u, w;
+};
+
+// Bytes behind the ring: bias by distance, bucket by distance, sums per bucket and row, tile flags.
+struct BwdRest {
+  int lut, buckets, sums, flags, total;
+};
+__host__ __device__ inline BwdRest bwd_rest(const AttnArgs &a, bool for_keys) {
+  const int tiles = ((for_keys ? a.q_len : a.kv_len) + kStreamRows - 1) / kStreamRows;
+  const bool table_sums = !for_keys && a.dtable != nullptr;
+  BwdRest r;
+  r.lut = 0;
+  r.buckets = r.lut + (a.table ? 4 * lut_floats(a.reach) : 0);
+  r.sums = r.buckets + (table_sums ? (lut_floats(a.reach) + 15) / 16 * 16 : 0);
+  r.flags = r.sums + (table_sums ? a.buckets * 2 * kTileRows * 8 : 0);
+  r.total = r.flags + (tiles + 15) / 16 * 16;
+  return r;
+}
+
+template <int NB, int ST, bool FOR_KEYS, bool CAP, int BIAS>
+static __global__ void __launch_bounds__(kBwdThreads, 1)
+attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ BwdMaps maps, unsigned int *timeouts) {
+  using Shape = BwdShape<NB, ST>;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  unsigned char *ring = smem + Shape::kRing;
+  const BwdRest rest = bwd_rest(a, FOR_KEYS);
+  float *lut = reinterpret_cast<float *>(smem + Shape::kRest + rest.lut);
+  unsigned char *bucket_lut = smem + Shape::kRest + rest.buckets;
+  float2 *sums = reinterpret_cast<float2 *>(smem + Shape::kRest + rest.sums);  // [group][bucket][row]
+  unsigned char *flags = smem + Shape::kRest + rest.flags;
+  __shared__ uint64_t x_full, full[ST], empty[ST], s_full[2], p_full[2], acc_full, drain;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int dead_flag, doc_range[2];
+  volatile int *dead = &dead_flag;
+  const bool table_sums = BIAS == kTable && !FOR_KEYS && a.dtable != nullptr;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    mbar_init(&x_full, 1);
+    for (int s = 0; s < ST; s++) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int t = 0; t < 2; t++) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 4);
+    }
+    mbar_init(&acc_full, 1);
+    mbar_init(&drain, 1);
+    dead_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == kBwdMmaWarp) tmem_alloc(&tmem_slot, 512);
+  if (tid == kBwdLoadWarp * 32) {
+    prefetch_map(&maps.x);
+    prefetch_map(&maps.y);
+    prefetch_map(&maps.u);
+    prefetch_map(&maps.w);
+  }
+  pdl_prologue();
+
+  // Tiles are the slowest index, those with most work under a causal mask first.
+  const int len = FOR_KEYS ? a.kv_len : a.q_len, units = FOR_KEYS ? a.kv_heads : a.heads;
+  const int tiles = (len + kTileRows - 1) / kTileRows;
+  int tile = blockIdx.x / (units * a.batch);
+  if (!FOR_KEYS) tile = tiles - 1 - tile;
+  const int unit = blockIdx.x % units, b = (blockIdx.x / units) % a.batch;
+  const int hk = FOR_KEYS ? unit : unit / a.group, heads_here = FOR_KEYS ? a.group : 1;
+  const int row0 = tile * kTileRows, row_last = min(len, row0 + kTileRows) - 1;
+  const BatchView view = batch_view(a, b);
+
+  // flags[n]: 1 when some row of the tile meets stream tile n, 3 when every row meets all of it.
+  int stream_end, from = 0;  // stream rows [from, stream_end) matter
+  int full_from = 0, full_end;
+  if (FOR_KEYS) {
+    stream_end = row0 < view.end ? a.q_len : 0;
+    from = first_query(a, view, row0);
+    full_from = first_query(a, view, row_last);
+    full_end = row0 + kTileRows <= view.end ? a.q_len : 0;
+  } else {
+    stream_end = row_end(a, view, row_last);
+    full_end = row_end(a, view, row0);
+  }
+  const int n_tiles = (stream_end + kStreamRows - 1) / kStreamRows;
+  if (a.q_docs) {
+    const int *docs = (FOR_KEYS ? a.kv_docs : a.q_docs) + static_cast<long long>(b) * len;
+    if (warp == 0) {
+      int lo = INT_MAX, hi = INT_MIN;
+      for (int r = row0 + lane; r <= row_last; r += 32) {
+        const int d = ld_co(docs + r);
+        lo = min(lo, d);
+        hi = max(hi, d);
+      }
+      lo = warp_min(lo);
+      hi = warp_max(hi);
+      if (lane == 0) {
+        doc_range[0] = lo;
+        doc_range[1] = hi;
+      }
+    }
+    __syncthreads();
+  }
+  const int *stream_docs = a.q_docs ? (FOR_KEYS ? a.q_docs : a.kv_docs) + static_cast<long long>(b) * (FOR_KEYS ? a.q_len : a.kv_len)
+                                    : nullptr;
+  for (int n = warp; n < n_tiles; n += kBwdThreads / 32) {
+    const int c0 = n * kStreamRows;
+    bool active = c0 + kStreamRows > from, whole = c0 >= full_from && c0 + kStreamRows <= full_end;
+    if (stream_docs) {
+      int lo = INT_MAX, hi = INT_MIN;
+      for (int c = c0 + lane; c < min(stream_end, c0 + kStreamRows); c += 32) {
+        const int d = ld_co(stream_docs + c);
+        lo = min(lo, d);
+        hi = max(hi, d);
+      }
+      lo = warp_min(lo);
+      hi = warp_max(hi);
+      active = active && lo <= doc_range[1] && doc_range[0] <= hi;
+      whole = whole && lo == hi && doc_range[0] == doc_range[1] && lo == doc_range[0];
+    }
+    if (lane == 0) flags[n] = active ? (whole ? 3 : 1) : 0;
+  }
+  if (BIAS == kTable && !FOR_KEYS) fill_lut(lut, a, unit, tid, kBwdThreads);
+  if (table_sums) {
+    for (int e = tid; e < 2 * (a.reach + kLutPad) + 1; e += kBwdThreads)
+      bucket_lut[e] = static_cast<unsigned char>(bucket_at(a, e - a.reach - kLutPad));
+    for (int e = tid; e < 2 * a.buckets * kTileRows; e += kBwdThreads) sums[e] = make_float2(0.f, 0.f);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == kBwdLoadWarp) {
+    if (lane == 0) {
+      const int x_head = FOR_KEYS ? hk : unit;
+      mbar_expect_tx(&x_full, 2 * NB * kBlockBytes);
+      for (int c = 0; c < NB; c++) {
+        tma_load_rows(smem + Shape::kX + c * kBlockBytes, &maps.x, &x_full, c * kBlockCols, row0, x_head, b);
+        tma_load_rows(smem + Shape::kY + c * kBlockBytes, &maps.y, &x_full, c * kBlockCols, row0, x_head, b);
+      }
+      int it = 0;
+      for (int g = 0; g < heads_here && !*dead; g++) {
+        const int head = FOR_KEYS ? hk * a.group + g : hk;  // of the streamed tensors
+        for (int n = 0; n < n_tiles; n++) {
+          if (!flags[n]) continue;
+          const int s = it % ST;
+          const unsigned use = it / ST;
+          if (use) mbar_wait(&empty[s], (use - 1) & 1, dead, timeouts);
+          if (*dead) break;
+          unsigned char *stage = ring + s * Shape::kStage;
+          mbar_expect_tx(&full[s], Shape::kStage + (FOR_KEYS ? kStatsBytes : 0));
+          for (int c = 0; c < NB; c++) {
+            tma_load_rows(stage + c * kStreamBlock, &maps.u, &full[s], c * kBlockCols, n * kStreamRows, head, b);
+            tma_load_rows(stage + (NB + c) * kStreamBlock, &maps.w, &full[s], c * kBlockCols, n * kStreamRows, head, b);
+          }
+          if (FOR_KEYS)
+            bulk_load(smem + Shape::kStats + s * kStatsBytes, stats_tile(a, b, head, n), kStatsBytes, &full[s]);
+          it++;
+        }
+      }
+      if (*dead) {  // no copy may be in flight when the CTA ends
+        drain_wait(&x_full, 0);
+        for (int i = max(0, it - ST); i < it; i++) drain_wait(&full[i % ST], (i / ST) & 1);
+      }
+    }
+  } else if (warp == kBwdMmaWarp) {
+    if (lane == 0) {
+      const int k_steps = (a.dim + 15) / 16, n_cols = k_steps * 16;
+      const uint32_t idesc_s = mma_desc(kStreamRows, false), idesc_acc = mma_desc(n_cols, true);
+      const uint64_t xd = desc_k_major(smem_u32(smem + Shape::kX)), yd = desc_k_major(smem_u32(smem + Shape::kY));
+      const uint32_t ring_at = smem_u32(ring);
+      auto accumulate = [&](int it) {  // with what the row threads made of tile `it`
+        const int s = it % ST, w = it & 1;
+        mbar_wait(&p_full[w], (it >> 1) & 1, dead, timeouts);
+        tc_fence_after();
+        const uint64_t ud = desc_mn_major(ring_at + s * Shape::kStage, kStreamBlock);
+        const uint64_t wd = desc_mn_major(ring_at + s * Shape::kStage + NB * kStreamBlock, kStreamBlock);
+        for (int k = 0; k < kStreamRows / 16; k++)
+          mma_ts(tmem + 256, tmem + w * 128 + 64 + k * 8, ud + k * (2048 >> 4), idesc_acc, it > 0 || k > 0);
+        if (FOR_KEYS)
+          for (int k = 0; k < kStreamRows / 16; k++)
+            mma_ts(tmem + 384, tmem + w * 128 + k * 8, wd + k * (2048 >> 4), idesc_acc, it > 0 || k > 0);
+        tc_commit(&empty[s]);
+      };
+      mbar_wait(&x_full, 0, dead, timeouts);
+      int it = 0;
+      for (int g = 0; g < heads_here && !*dead; g++)
+        for (int n = 0; n < n_tiles; n++) {
+          if (!flags[n]) continue;
+          const int s = it % ST, w = it & 1;
+          if (it >= 2) accumulate(it - 2);
+          mbar_wait(&full[s], (it / ST) & 1, dead, timeouts);
+          const uint64_t ud = desc_k_major(ring_at + s * Shape::kStage);
+          const uint64_t wd = desc_k_major(ring_at + s * Shape::kStage + NB * kStreamBlock);
+          for (int k = 0; k < k_steps; k++) {
+            const int xk = (k / 4) * (kBlockBytes >> 4) + (k % 4) * 2, uk = (k / 4) * (kStreamBlock >> 4) + (k % 4) * 2;
+            mma_ss(tmem + w * 128, xd + xk, ud + uk, idesc_s, k > 0);
+          }
+          for (int k = 0; k < k_steps; k++) {
+            const int xk = (k / 4) * (kBlockBytes >> 4) + (k % 4) * 2, uk = (k / 4) * (kStreamBlock >> 4) + (k % 4) * 2;
+            mma_ss(tmem + w * 128 + 64, yd + xk, wd + uk, idesc_s, k > 0);
+          }
+          tc_commit(&s_full[w]);
+          it++;
+        }
+      if (it >= 2) accumulate(it - 2);
+      if (it >= 1) accumulate(it - 1);
+      tc_commit(&acc_full);
+      if (*dead) {
+        tc_commit(&drain);
+        drain_wait(&drain, 0);
+      }
+    }
+  } else if (warp < kBwdLoadWarp) {
+    const int w = warp >> 2, row = tid & 127, x = row0 + row;
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + lane_base + w * 128, g_at = s_at + 64;
+    const bool valid = x < len && (!FOR_KEYS || x < view.end);
+    const int row_doc = (a.q_docs && valid) ? ld_co((FOR_KEYS ? a.kv_docs : a.q_docs) + static_cast<long long>(b) * len + x) : 0;
+    // Stream rows [see_from, see_end) are visible to this row, as far as documents allow.
+    const int see_from = !valid ? INT_MAX : FOR_KEYS ? first_query(a, view, x) : 0;
+    const int see_end = !valid ? 0 : FOR_KEYS ? a.q_len : row_end(a, view, x);
+    const float2 row_stat = (!FOR_KEYS && valid) ? stat_at(a, b, unit, x) : make_float2(-INFINITY, 0.f);
+    const float to_log2 = CAP ? a.cap * kLog2e : a.scale * kLog2e, inside = CAP ? a.scale / a.cap : 0.f;
+    const int tail = !FOR_KEYS && view.end % kStreamRows && view.end < a.kv_len ? view.end / kStreamRows : -1;
+    int bucket_now = 0;
+    float2 bucket_sum = make_float2(0.f, 0.f);
+    auto flush_bucket = [&](int next) {
+      float2 *at = sums + (w * a.buckets + bucket_now) * kTileRows + row;
+      float2 v = *at;
+      v.x += bucket_sum.x;
+      v.y += bucket_sum.y;
+      *at = v;
+      bucket_sum = make_float2(0.f, 0.f);
+      bucket_now = next;
+    };
+    int it = -1;
+    for (int g = 0; g < heads_here; g++) {
+      const int h = FOR_KEYS ? hk * a.group + g : unit;
+      const float slope = (BIAS != kNoBias && a.slopes) ? ld_co(a.slopes + h) * kLog2e : 0.f;
+      if (BIAS == kTable && FOR_KEYS) {
+        // this head's bias by distance; both groups of warps are past the last head's tiles here
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        fill_lut(lut, a, h, tid, 256);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+      }
+      for (int n = 0; n < n_tiles; n++) {
+        const int f = flags[n];
+        if (!f) continue;
+        it++;
+        if ((it & 1) != w) continue;
+        const int c0 = n * kStreamRows, s = it % ST;
+        mbar_wait(&full[s], (it / ST) & 1, dead, timeouts);  // the stage's statistics
+        mbar_wait(&s_full[w], (it >> 1) & 1, dead, timeouts);
+        tc_fence_after();
+        const float *stats = reinterpret_cast<const float *>(smem + Shape::kStats + s * kStatsBytes);
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+          const int c1 = c0 + half * 32;
+          uint32_t sr[32], gr[32];
+          tmem_load32(s_at + half * 32, sr);
+          tmem_load32(g_at + half * 32, gr);
+          tmem_loaded(sr);
+          tmem_loaded(gr);
+          float x32[32];
+#pragma unroll
+          for (int e = 0; e < 32; e++) x32[e] = __uint_as_float(sr[e]);
+          if (CAP) tanh_scores(x32, inside);
+          float bias[32];
+          const int d0 = FOR_KEYS ? x - (view.start + c1) : c1 - (view.start + x);  // distance j - p at e = 0
+          bool far = false;
+          int far_at = 0;
+          if (BIAS == kTable) {
+            const int lo = FOR_KEYS ? d0 - 31 : d0, hi = FOR_KEYS ? d0 : d0 + 31;
+            const bool left = hi <= -a.reach, right = lo >= a.reach;
+            far = __all_sync(0xffffffffu, left || right);
+            far_at = left ? 0 : 2 * (a.reach + kLutPad);
+            if (far) {
+              const float v = lut[far_at];
+#pragma unroll
+              for (int e = 0; e < 32; e++) bias[e] = v;
+            } else {
+              const float *at = lut + d0 + a.reach + kLutPad;
+#pragma unroll
+              for (int e = 0; e < 32; e++) bias[e] = at[FOR_KEYS ? -e : e];
+            }
+          } else if (BIAS == kSlope) {
+#pragma unroll
+            for (int e = 0; e < 32; e++) bias[e] = 0.f;
+          }
+          if (BIAS == kSlope || (BIAS == kTable && a.slopes)) {
+            const float d = static_cast<float>(d0);
+#pragma unroll
+            for (int e = 0; e < 32; e++)
+              bias[e] = fmaf(-slope, fabsf(FOR_KEYS ? d - static_cast<float>(e) : d + static_cast<float>(e)), bias[e]);
+          }
+          const float2 k2 = make_float2(to_log2, to_log2);
+          float p[32], ds[32];
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            float4 l4, d4;
+            if (FOR_KEYS) {
+              l4 = *reinterpret_cast<const float4 *>(stats + half * 32 + e);
+              d4 = *reinterpret_cast<const float4 *>(stats + kStreamRows + half * 32 + e);
+            } else {
+              l4 = make_float4(row_stat.x, row_stat.x, row_stat.x, row_stat.x);
+              d4 = make_float4(row_stat.y, row_stat.y, row_stat.y, row_stat.y);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; q += 2) {
+              float2 shift = q ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
+              const float2 minus = q ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);
+              if (BIAS != kNoBias) shift = add2(shift, make_float2(bias[e + q], bias[e + q + 1]));
+              const float2 y = fma2(make_float2(x32[e + q], x32[e + q + 1]), k2, shift);
+              p[e + q] = ex2(y.x);
+              p[e + q + 1] = ex2(y.y);
+              const float2 dp = add2(make_float2(__uint_as_float(gr[e + q]), __uint_as_float(gr[e + q + 1])), minus);
+              const float2 d2 = mul2(make_float2(p[e + q], p[e + q + 1]), dp);
+              ds[e + q] = d2.x;
+              ds[e + q + 1] = d2.y;
+            }
+          }
+          if (f != 3) {
+            if (stream_docs) {
+#pragma unroll
+              for (int e = 0; e < 32; e++)
+                if (c1 + e < see_from || c1 + e >= see_end || ld_co(stream_docs + c1 + e) != row_doc) p[e] = ds[e] = 0.f;
+            } else if (FOR_KEYS) {
+              const int skip = see_from - c1;  // see_end is q_len: rows behind it have -lse = -infinity
+#pragma unroll
+              for (int e = 0; e < 32; e++)
+                if (e < skip) p[e] = ds[e] = 0.f;
+            } else {
+              const int room = see_end - c1;
+#pragma unroll
+              for (int e = 0; e < 32; e++)
+                if (e >= room) p[e] = ds[e] = 0.f;
+            }
+          }
+          if (table_sums) {
+            // One run of columns per bucket: its sums stay in registers until the bucket changes.
+            if (far) {
+              const int n_now = bucket_lut[far_at];
+              if (n_now != bucket_now) flush_bucket(n_now);
+              float2 t = make_float2(0.f, 0.f);
+#pragma unroll
+              for (int e = 0; e < 32; e++) t = add2(t, make_float2(ds[e], p[e]));
+              bucket_sum = add2(bucket_sum, t);
+            } else {
+              const unsigned char *at = bucket_lut + d0 + a.reach + kLutPad;
+#pragma unroll
+              for (int e = 0; e < 32; e++) {
+                const int n_now = at[e];
+                if (n_now != bucket_now) flush_bucket(n_now);
+                bucket_sum = add2(bucket_sum, make_float2(ds[e], p[e]));
+              }
+            }
+          }
+          uint32_t packed[16];
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            float2 y = make_float2(ds[2 * e], ds[2 * e + 1]);
+            if (CAP) {  // d tanh = 1 - tanh^2
+              const float2 t = make_float2(x32[2 * e], x32[2 * e + 1]);
+              y = mul2(y, fma2(make_float2(-t.x, -t.y), t, make_float2(1.f, 1.f)));
+            }
+            packed[e] = pack_bf16(y.x, y.y);
+          }
+          tmem_store16(g_at + half * 16, packed);
+          if (FOR_KEYS) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) packed[e] = pack_bf16(p[2 * e], p[2 * e + 1]);
+            tmem_store16(s_at + half * 16, packed);
+          }
+        }
+        if (n == tail) {
+          // Rows of K that no query reaches may hold anything, and 0 * NaN is NaN.
+          const int first = view.end - c0;
+          for (int e = row; e < (kStreamRows - first) * NB * 8; e += 128) {
+            const int r = first + e / (NB * 8), q = e % (NB * 8);
+            *reinterpret_cast<uint4 *>(ring + s * Shape::kStage + (q / 8) * kStreamBlock + r * 128 + (q % 8) * 16) =
+                make_uint4(0, 0, 0, 0);
+          }
+          fence_async_smem();
+        }
+        tmem_stored();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[w]);
+      }
+    }
+    if (table_sums) flush_bucket(0);
+    mbar_wait(&acc_full, 0, dead, timeouts);
+    tc_fence_after();
+    // FOR_KEYS: the first group stores dK, the second dV; else they share the columns of dQ.
+    const Heads &to = !FOR_KEYS ? a.dq : w == 0 ? a.dk : a.dv;
+    const float by = FOR_KEYS && w == 1 ? 1.f : a.scale;
+    const uint32_t acc_at = tmem + lane_base + (FOR_KEYS && w == 1 ? 384 : 256);
+    __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(to.ptr) + b * to.batch + static_cast<long long>(x) * to.token + unit * to.head;
+    for (int c = FOR_KEYS ? 0 : w * 32; c < a.dim; c += FOR_KEYS ? 32 : 64) {
+      uint32_t o[32];
+      if (it >= 0) {
+        tmem_load32(acc_at + c, o);
+        tmem_loaded(o);
+      }
+#pragma unroll
+      for (int e = 0; e < 32; e += 8) {
+        uint32_t v[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          v[k] = it < 0 ? 0u : pack_bf16(__uint_as_float(o[e + 2 * k]) * by, __uint_as_float(o[e + 2 * k + 1]) * by);
+        if (x < len && c + e < a.dim) *reinterpret_cast<uint4 *>(out + c + e) = make_uint4(v[0], v[1], v[2], v[3]);
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (table_sums) {
+    // A row's gradients of its scores add up to zero: what rounding left (in delta above all, which
+    // comes from the rounded o) is taken off again in proportion to P.
+    if (tid < kTileRows) {
+      float e = 0.f, p = 0.f;
+      for (int n = 0; n < a.buckets; n++) {
+        float2 v = sums[n * kTileRows + tid];
+        const float2 other = sums[(a.buckets + n) * kTileRows + tid];
+        v.x += other.x;
+        v.y += other.y;
+        sums[n * kTileRows + tid] = v;
+        e += v.x;
+        p += v.y;
+      }
+      e = p > 0.f ? e / p : 0.f;
+      for (int n = 0; n < a.buckets; n++) {
+        const float2 v = sums[n * kTileRows + tid];
+        sums[n * kTileRows + tid].x = fmaf(-e, v.y, v.x);
+      }
+    }
+    __syncthreads();
+    float *part = a.table_part + (static_cast<size_t>(unit) * a.table_parts + b * tiles + tile) * a.buckets;
+    for (int n = warp; n < a.buckets; n += kBwdThreads / 32) {
+      float v = 0.f;
+      for (int r = lane; r < kTileRows; r += 32) v += sums[n * kTileRows + r].x;
+      v = warp_sum(v);
+      if (lane == 0) part[n] = v;
+    }
+  }
+  if (warp == kBwdMmaWarp) {
+    tc_fence_after();
+    tmem_free(tmem, 512);
+  }
+}
+
+template <bool FOR_KEYS>
+int bwd_mma_launch(const AttnArgs &a, cudaStream_t st) {
+  const char *name = FOR_KEYS ? "attn_bwd_mma (keys)" : "attn_bwd_mma (queries)";
+  BwdMaps maps;
+  auto q_map = [&](CUtensorMap *m, const Heads &h, int rows) {
+    return make_heads_map(m, h.ptr, a.dim, a.q_len, a.heads, a.batch, h.token, h.head, h.batch, rows);
+  };
+  auto k_map = [&](CUtensorMap *m, const Heads &h, int rows) {
+    return make_heads_map(m, h.ptr, a.dim, a.kv_len, a.kv_heads, a.batch, h.token, h.head, h.batch, rows);
+  };
+  int rc;
+  if (FOR_KEYS) {
+    rc = k_map(&maps.x, a.k, kTileRows);
+    if (!rc) rc = k_map(&maps.y, a.v, kTileRows);
+    if (!rc) rc = q_map(&maps.u, a.q, kStreamRows);
+    if (!rc) rc = q_map(&maps.w, a.dout, kStreamRows);
+  } else {
+    rc = q_map(&maps.x, a.q, kTileRows);
+    if (!rc) rc = q_map(&maps.y, a.dout, kTileRows);
+    if (!rc) rc = k_map(&maps.u, a.k, kStreamRows);
+    if (!rc) rc = k_map(&maps.w, a.v, kStreamRows);
+  }
+  DLB_REQUIRE(rc == 0, DLB_ERR_CUDA, "%s: tensor map refused (%d)", name, rc);
+  unsigned int *timeouts = wait_timeouts_counter();
+  DLB_REQUIRE(timeouts != nullptr, DLB_ERR_NO_DEVICE, "%s: no CUDA device", name);
+  auto launch = [&](auto kern, int ring_end) -> int {
+    const size_t smem = 1024 + ring_end + bwd_rest(a, FOR_KEYS).total;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    DLB_REQUIRE(e == cudaSuccess, DLB_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
+    const int grid = ceil_div(FOR_KEYS ? a.kv_len : a.q_len, kTileRows) * (FOR_KEYS ? a.kv_heads : a.heads) * a.batch;
+    launch_pdl(kern, dim3(grid), dim3(kBwdThreads), smem, st, a, maps, timeouts);
+    DLB_LAUNCH_CHECK(name);
+    return DLB_OK;
+  };
+  const bool cap = a.cap > 0.f;
+#define DLB_PICK(NB, ST, BIAS)                                                                     \
+  (cap ? launch(attn_bwd_mma_kernel<NB, ST, FOR_KEYS, true, BIAS>, BwdShape<NB, ST>::kRest)        \
+       : launch(attn_bwd_mma_kernel<NB, ST, FOR_KEYS, false, BIAS>, BwdShape<NB, ST>::kRest))
+  if (a.dim <= kBlockCols) {
+    if (a.table) return DLB_PICK(1, 4, kTable);
+    return a.slopes ? DLB_PICK(1, 4, kSlope) : DLB_PICK(1, 4, kNoBias);
+  }
+  if (a.table) {
+    // the sums per bucket and row leave room for two stages only
+    if constexpr (!FOR_KEYS)
+      if (a.dtable) return DLB_PICK(2, 2, kTable);
+    return DLB_PICK(2, 4, kTable);
+  }
+  return a.slopes ? DLB_PICK(2, 4, kSlope) : DLB_PICK(2, 4, kNoBias);
+#undef DLB_PICK
+}
+
+}  // namespace dlb

@@ -1,0 +1,6 @@
+// Gradients of the keys and values on the tensor cores (attn_bwd_mma.cuh).
+#include "attn_bwd_mma.cuh"
+
+namespace dlb {
+int attn_bwd_mma_keys(const AttnArgs &a, cudaStream_t st) { return bwd_mma_launch<true>(a, st); }
+}  // namespace dlb

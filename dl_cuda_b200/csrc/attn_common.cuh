@@ -28,7 +28,7 @@ struct AttnArgs {
   float *lse;
   Heads dout, dq, dk, dv;  // backward only
   float *dtable;
-  float2 *row_stats;       // backward: {lse * log2(e), delta} per (b, h, i)
+  float *row_stats;        // backward: see stats_tile
   float *table_part;       // backward: [heads][parts][buckets]
   int table_parts;
   // forward split over the keys: partial outputs [split][b, h, i][dim] and {max, sum} [split][b, h, i]
@@ -36,6 +36,19 @@ struct AttnArgs {
   float2 *part_ml;
   int splits;
 };
+
+// Backward: what it needs of a query row, in tiles of 64 rows per (b, h): 64 times -lse * log2(e)
+// (-infinity for a row that saw no key, and behind the last row: its probabilities are then
+// exp2(s - infinity) = 0), then 64 times -delta.  512 bytes a tile, on a 16-byte boundary for any q_len.
+constexpr int kStatRows = 64;
+__host__ __device__ inline int stat_tiles(int q_len) { return (q_len + kStatRows - 1) / kStatRows; }
+__device__ __forceinline__ float *stats_tile(const AttnArgs &a, int b, int h, int tile) {
+  return a.row_stats + ((static_cast<size_t>(b) * a.heads + h) * stat_tiles(a.q_len) + tile) * (2 * kStatRows);
+}
+__device__ __forceinline__ float2 stat_at(const AttnArgs &a, int b, int h, int i) {
+  const float *t = stats_tile(a, b, h, i / kStatRows) + i % kStatRows;
+  return make_float2(t[0], t[kStatRows]);
+}
 
 // Per batch: query i stands at start + i; keys from `end` on are reached by no query.
 struct BatchView {

@@ -310,26 +310,29 @@ static __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_cons
   if (a.lse && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
-// row_stats[b, h, i] = {lse * log2(e), delta}, delta = <dout_i, o_i> (= sum_j P_ij dP_ij); a row that
-// saw no key gets +infinity, which makes every rebuilt probability exp2(s - inf) = 0.  One warp per row.
+// Fills row_stats: -lse * log2(e) and -delta, delta = <dout_i, o_i> (= sum_j P_ij dP_ij).  One warp per row.
 template <typename T>
 static __global__ void __launch_bounds__(256) attn_row_stats_kernel(const __grid_constant__ AttnArgs a) {
   pdl_prologue();
-  const size_t rows = static_cast<size_t>(a.batch) * a.heads * a.q_len;
+  const int padded = stat_tiles(a.q_len) * kStatRows;
+  const size_t rows = static_cast<size_t>(a.batch) * a.heads * padded;
   const size_t row = static_cast<size_t>(blockIdx.x) * 8 + threadIdx.x / 32;
   if (row >= rows) return;
   const int lane = threadIdx.x & 31;
   // heads innermost: neighbouring warps read neighbouring memory of [token, head] layouts
-  const int h = row % a.heads, i = (row / a.heads) % a.q_len, b = row / (static_cast<size_t>(a.q_len) * a.heads);
-  const T *o = static_cast<const T *>(a.o.ptr) + b * a.o.batch + i * a.o.token + h * a.o.head;
-  const T *g = static_cast<const T *>(a.dout.ptr) + b * a.dout.batch + i * a.dout.token + h * a.dout.head;
+  const int h = row % a.heads, i = (row / a.heads) % padded, b = row / (static_cast<size_t>(padded) * a.heads);
   float sum = 0.f;
-  for (int c = lane; c < a.dim; c += 32) sum = fmaf(Store<T>::to_float(ld_co(o + c)), Store<T>::to_float(ld_co(g + c)), sum);
-  sum = warp_sum(sum);
+  if (i < a.q_len) {
+    const T *o = static_cast<const T *>(a.o.ptr) + b * a.o.batch + i * a.o.token + h * a.o.head;
+    const T *g = static_cast<const T *>(a.dout.ptr) + b * a.dout.batch + i * a.dout.token + h * a.dout.head;
+    for (int c = lane; c < a.dim; c += 32) sum = fmaf(Store<T>::to_float(ld_co(o + c)), Store<T>::to_float(ld_co(g + c)), sum);
+    sum = warp_sum(sum);
+  }
   if (lane == 0) {
-    const size_t at = (static_cast<size_t>(b) * a.heads + h) * a.q_len + i;
-    const float z = a.lse[at];
-    a.row_stats[at] = make_float2(z == -INFINITY ? INFINITY : z * kLog2e, sum);
+    float *at = stats_tile(a, b, h, i / kStatRows) + i % kStatRows;
+    at[0] = i < a.q_len ? -a.lse[(static_cast<size_t>(b) * a.heads + h) * a.q_len + i] * kLog2e : -INFINITY;
+    if (i < a.q_len && at[0] == INFINITY) at[0] = -INFINITY;  // lse = -infinity
+    at[kStatRows] = -sum;
   }
 }
 
@@ -385,8 +388,7 @@ attn_bwd_generic_kernel(const __grid_constant__ AttnArgs a, bool vec) {
     const int *docs = FOR_KEYS ? a.kv_docs : a.q_docs;
     row_doc[r] = (docs && valid) ? docs[static_cast<long long>(b) * len + x] : 0;
     end[r] = (!FOR_KEYS && valid) ? row_end(a, view, x) : 0;
-    row_stat[r] = (!FOR_KEYS && valid) ? a.row_stats[(static_cast<size_t>(b) * a.heads + unit) * a.q_len + x]
-                                       : make_float2(INFINITY, 0.f);
+    row_stat[r] = (!FOR_KEYS && valid) ? stat_at(a, b, unit, x) : make_float2(-INFINITY, 0.f);
   }
   float acc_x[4][N], acc_y[4][N];
 #pragma unroll
@@ -408,8 +410,7 @@ attn_bwd_generic_kernel(const __grid_constant__ AttnArgs a, bool vec) {
         const int *docs = FOR_KEYS ? a.q_docs : a.kv_docs;
         col_doc[c] = (docs && c < cols) ? docs[static_cast<long long>(b) * (FOR_KEYS ? a.q_len : a.kv_len) + c0 + c] : 0;
         if (FOR_KEYS)
-          col_stats[c] = c < cols ? a.row_stats[(static_cast<size_t>(b) * a.heads + h) * a.q_len + c0 + c]
-                                  : make_float2(INFINITY, 0.f);
+          col_stats[c] = c < cols ? stat_at(a, b, h, c0 + c) : make_float2(-INFINITY, 0.f);
       }
       __syncthreads();
       if (a.kv_docs) {
@@ -441,8 +442,8 @@ attn_bwd_generic_kernel(const __grid_constant__ AttnArgs a, bool vec) {
           const float2 stat = FOR_KEYS ? col_stats[tx + 16 * c] : row_stat[r];
           float dcap, p = 0.f, grad = 0.f;
           if (seen) {
-            p = ex2(gen_score(a, s[r][c], h, slope, j - (view.start + i), &dcap) - stat.x);
-            grad = p * (dp[r][c] - stat.y);
+            p = ex2(gen_score(a, s[r][c], h, slope, j - (view.start + i), &dcap) + stat.x);
+            grad = p * (dp[r][c] + stat.y);
           } else {
             dcap = 0.f;
           }

@@ -60,6 +60,9 @@ __host__ __device__ inline int lut_floats(int reach) { return 2 * (reach + kLutP
 // The tensor cores need 16-byte aligned rows, and a scale that keeps the order of the scores.
 bool attn_mma_fits(const AttnArgs &a, bool backward);
 int attn_fwd_mma(const AttnArgs &a, cudaStream_t st);
+bool attn_bwd_mma_room(const AttnArgs &a);  // does its shared memory fit?
+int attn_bwd_mma_keys(const AttnArgs &a, cudaStream_t st);
+int attn_bwd_mma_queries(const AttnArgs &a, cudaStream_t st);
 
 // Waits for copies or MMAs still in flight after another wait of the CTA gave up (bounded as well).
 __device__ __forceinline__ void drain_wait(uint64_t *bar, unsigned parity) {
