@@ -5,6 +5,7 @@
 
 #include "attn_generic.cuh"
 #include "attn_mma.cuh"
+#include "attn_step.cuh"
 
 namespace dlb {
 namespace {
@@ -115,30 +116,48 @@ int allow_smem(K kern, size_t smem, const char *name) {
   return DLB_OK;
 }
 
-// From this many queries on, bf16 goes to the tensor cores.
+// From this many queries on, bf16 goes to the 128-row tiles of the tensor cores; below, the whole
+// matrix product is one row tile and the cache is what takes time.
 constexpr int kMmaQueries = 17;
 
+enum FwdKind { kGeneric, kMma, kStep };
+
 struct FwdPlan {
+  FwdKind kind;
   int pack, splits;
   size_t bytes;
 };
 
-// Few queries: the heads that share a key/value head go into one tile, and the keys are split until
-// the grid fills the GPU twice (a share keeps at least two tiles).
-FwdPlan plan_fwd(const dlb_attn *a) {
-  FwdPlan p = {1, 1, 0};
+FwdPlan plan_fwd(const dlb_attn *a, const AttnArgs &args) {
+  FwdPlan p = {kGeneric, 1, 1, 0};
   const int group = a->heads / a->kv_heads;
-  if (static_cast<long long>(a->q_len) * group <= kGenTile) p.pack = group;
-  const long long ctas = static_cast<long long>(a->batch) * (a->heads / p.pack) *
-                         ceil_div(static_cast<long long>(a->q_len) * p.pack, static_cast<long long>(kGenTile));
-  const int key_tiles = ceil_div(a->kv_len, kGenTile);
-  if (ctas > 0 && ctas < sm_count())
-    p.splits = static_cast<int>(std::max(1ll, std::min({2ll * sm_count() / ctas, key_tiles / 2ll, 256ll})));
+  if (a->dtype == DLB_BF16 && attn_mma_fits(args, false)) p.kind = a->q_len >= kMmaQueries ? kMma : kStep;
+  if (p.kind == kMma) return p;
+  if (p.kind == kStep) {
+    p.splits = attn_step_splits(a->batch, a->kv_heads, a->q_len * group, a->kv_len);
+  } else {
+    // Few queries: the heads that share a key/value head go into one tile, and the keys are split until
+    // the grid fills the GPU twice (a share keeps at least two tiles).
+    if (static_cast<long long>(a->q_len) * group <= kGenTile) p.pack = group;
+    const long long ctas = static_cast<long long>(a->batch) * (a->heads / p.pack) *
+                           ceil_div(static_cast<long long>(a->q_len) * p.pack, static_cast<long long>(kGenTile));
+    const int key_tiles = ceil_div(a->kv_len, kGenTile);
+    if (ctas > 0 && ctas < sm_count())
+      p.splits = static_cast<int>(std::max(1ll, std::min({2ll * sm_count() / ctas, key_tiles / 2ll, 256ll})));
+  }
   if (p.splits > 1) {
     const size_t rows = static_cast<size_t>(a->batch) * a->heads * a->q_len * p.splits;
-    p.bytes = rows * (sizeof(float2) + sizeof(float) * a->head_dim);
+    p.bytes = (rows * sizeof(float2) + 15) / 16 * 16 + rows * sizeof(float) * a->head_dim;
   }
   return p;
+}
+
+template <typename T>
+int launch_join(const AttnArgs &p, cudaStream_t st) {
+  const size_t rows = static_cast<size_t>(p.batch) * p.heads * p.q_len;
+  launch_pdl(attn_join_kernel<T>, dim3(static_cast<unsigned>(ceil_div(rows, size_t{8}))), dim3(256), 0, st, p);
+  DLB_LAUNCH_CHECK("attn_join");
+  return DLB_OK;
 }
 
 template <typename T>
@@ -154,11 +173,7 @@ int launch_fwd(AttnArgs p, const FwdPlan &plan, cudaStream_t st) {
     DLB_LAUNCH_CHECK("attn_fwd_generic");
     return DLB_OK;
   });
-  if (rc != DLB_OK || plan.splits == 1) return rc;
-  const size_t rows = static_cast<size_t>(p.batch) * p.heads * p.q_len;
-  launch_pdl(attn_join_kernel<T>, dim3(static_cast<unsigned>(ceil_div(rows, size_t{8}))), dim3(256), 0, st, p);
-  DLB_LAUNCH_CHECK("attn_join");
-  return DLB_OK;
+  return rc != DLB_OK || plan.splits == 1 ? rc : launch_join<T>(p, st);
 }
 
 struct BwdPlan {
@@ -220,28 +235,30 @@ int check_workspace(const char *call, const void *workspace, size_t have, size_t
 using namespace dlb;
 
 extern "C" size_t dlb_attn_fwd_workspace_bytes(const dlb_attn *a) {
-  if (check("attn_fwd", a) != DLB_OK) return 0;
-  return plan_fwd(a).bytes;
+  if (check("attn_fwd", a) != DLB_OK || a->batch == 0 || a->q_len == 0) return 0;
+  return plan_fwd(a, args_of(a)).bytes;
 }
 
 extern "C" int dlb_attn_fwd(const dlb_attn *a, void *workspace, size_t workspace_bytes, void *stream) {
   if (int st = check("attn_fwd", a)) return st;
   if (int st = check_output("attn_fwd", "o", a->o, a->batch, a->q_len, a->heads)) return st;
   if (a->batch == 0 || a->q_len == 0) return DLB_OK;
-  const FwdPlan plan = plan_fwd(a);
-  if (int st = check_workspace("attn_fwd", workspace, workspace_bytes, plan.bytes)) return st;
   AttnArgs p = args_of(a);
+  const FwdPlan plan = plan_fwd(a, p);
+  if (int rc = check_workspace("attn_fwd", workspace, workspace_bytes, plan.bytes)) return rc;
+  cudaStream_t st = as_stream(stream);
   p.splits = plan.splits;
   if (plan.splits > 1) {
+    const size_t rows = static_cast<size_t>(a->batch) * a->heads * a->q_len * plan.splits;
     p.part_ml = static_cast<float2 *>(workspace);
-    p.part_o = reinterpret_cast<float *>(p.part_ml + static_cast<size_t>(a->batch) * a->heads * a->q_len * plan.splits);
+    p.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + (rows * sizeof(float2) + 15) / 16 * 16);
   }
-  if (a->dtype == DLB_BF16 && a->q_len >= kMmaQueries && attn_mma_fits(p, false)) {
-    p.splits = 1;
-    return attn_fwd_mma(p, as_stream(stream));
+  if (plan.kind == kMma) return attn_fwd_mma(p, st);
+  if (plan.kind == kStep) {
+    const int rc = attn_step(p, st);
+    return rc != DLB_OK || plan.splits == 1 ? rc : launch_join<__nv_bfloat16>(p, st);
   }
-  return a->dtype == DLB_F32 ? launch_fwd<float>(p, plan, as_stream(stream))
-                             : launch_fwd<__nv_bfloat16>(p, plan, as_stream(stream));
+  return a->dtype == DLB_F32 ? launch_fwd<float>(p, plan, st) : launch_fwd<__nv_bfloat16>(p, plan, st);
 }
 
 extern "C" size_t dlb_attn_bwd_workspace_bytes(const dlb_attn *a, const dlb_attn_grad *g) {

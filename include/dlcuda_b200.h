@@ -553,6 +553,8 @@ typedef struct dlb_attn {
   float *lse; /* [batch, heads, q_len]; dlb_attn_fwd writes it (NULL: not wanted), dlb_attn_bwd reads it */
 } dlb_attn;
 
+/* The size holds for the block as it will be passed: addresses and strides take part in the choice
+ * of the kernel. */
 DLB_API size_t dlb_attn_fwd_workspace_bytes(const dlb_attn *a);
 DLB_API int dlb_attn_fwd(const dlb_attn *a, void *workspace, size_t workspace_bytes, void *stream);
 
