@@ -143,7 +143,8 @@ FwdPlan plan_fwd(const dlb_attn *a, const AttnArgs &args) {
                            ceil_div(static_cast<long long>(a->q_len) * p.pack, static_cast<long long>(kGenTile));
     const int key_tiles = ceil_div(a->kv_len, kGenTile);
     if (ctas > 0 && ctas < sm_count())
-      p.splits = static_cast<int>(std::max(1ll, std::min({2ll * sm_count() / ctas, key_tiles / 2ll, 256ll})));
+      p.splits = static_cast<int>(std::max(1ll, std::min({2ll * sm_count() / ctas, key_tiles / 2ll,
+                                                          static_cast<long long>(kMaxSplits)})));
   }
   if (p.splits > 1) {
     const size_t rows = static_cast<size_t>(a->batch) * a->heads * a->q_len * p.splits;
@@ -155,7 +156,7 @@ FwdPlan plan_fwd(const dlb_attn *a, const AttnArgs &args) {
 template <typename T>
 int launch_join(const AttnArgs &p, cudaStream_t st) {
   const size_t rows = static_cast<size_t>(p.batch) * p.heads * p.q_len;
-  launch_pdl(attn_join_kernel<T>, dim3(static_cast<unsigned>(ceil_div(rows, size_t{8}))), dim3(256), 0, st, p);
+  launch_pdl(attn_join_kernel<T>, dim3(static_cast<unsigned>(rows)), dim3(kJoinThreads), 0, st, p);
   DLB_LAUNCH_CHECK("attn_join");
   return DLB_OK;
 }

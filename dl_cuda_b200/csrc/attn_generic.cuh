@@ -270,44 +270,58 @@ attn_fwd_generic_kernel(const __grid_constant__ AttnArgs a, int pack, bool vec) 
   }
 }
 
-// Joins the shares of the keys: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  One warp per row.
+// Joins the shares of the keys: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  One CTA per row: with
+// one user there are few rows and many shares, which four warps then read side by side.
+constexpr int kJoinThreads = 128, kMaxSplits = 256;
+
 template <typename T>
-static __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnArgs a) {
+static __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_constant__ AttnArgs a) {
   pdl_prologue();
-  const size_t rows = static_cast<size_t>(a.batch) * a.heads * a.q_len;
-  const size_t row = static_cast<size_t>(blockIdx.x) * 8 + threadIdx.x / 32;
-  if (row >= rows) return;
-  const int lane = threadIdx.x & 31;
+  __shared__ float weight[kMaxSplits], part[4][DLB_ATTN_MAX_HEAD_DIM], warp_value[4];
+  const size_t rows = static_cast<size_t>(a.batch) * a.heads * a.q_len, row = blockIdx.x;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  float2 ml[kMaxSplits / kJoinThreads];
   float m = -INFINITY;
-  for (int s = lane; s < a.splits; s += 32) m = fmaxf(m, a.part_ml[s * rows + row].x);
+#pragma unroll
+  for (int k = 0; k < kMaxSplits / kJoinThreads; k++) {
+    const int s = tid + k * kJoinThreads;
+    ml[k] = s < a.splits ? a.part_ml[s * rows + row] : make_float2(-INFINITY, 0.f);
+    m = fmaxf(m, ml[k].x);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) warp_value[warp] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(warp_value[0], warp_value[1]), fmaxf(warp_value[2], warp_value[3]));
   const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = 0; s0 < a.splits; s0 += 32) {
-    float w = 0.f;
-    if (s0 + lane < a.splits) {
-      const float2 ml = a.part_ml[(s0 + lane) * rows + row];
-      w = ex2(ml.x - base);
-      l += w * ml.y;
-    }
-    for (int s = 0; s < min(32, a.splits - s0); s++) {
-      const float ws = __shfl_sync(0xffffffffu, w, s);
-      if (ws == 0.f) continue;  // an empty share may hold no output at all
-      const float *src = a.part_o + ((s0 + s) * rows + row) * a.dim;
+  float l = 0.f;
 #pragma unroll
-      for (int n = 0; n < 4; n++)
-        if (lane + 32 * n < a.dim) acc[n] = fmaf(ws, src[lane + 32 * n], acc[n]);
-    }
+  for (int k = 0; k < kMaxSplits / kJoinThreads; k++) {
+    const float w = ex2(ml[k].x - base);
+    weight[tid + k * kJoinThreads] = w;
+    l = fmaf(w, ml[k].y, l);
   }
   l = warp_sum(l);
+  __syncthreads();
+  if (lane == 0) warp_value[warp] = l;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = warp; s < a.splits; s += 4) {
+    const float *src = a.part_o + (s * rows + row) * a.dim;
+    const float w = weight[s];
+#pragma unroll
+    for (int n = 0; n < 4; n++)
+      if (lane + 32 * n < a.dim) acc[n] = fmaf(w, src[lane + 32 * n], acc[n]);
+  }
+#pragma unroll
+  for (int n = 0; n < 4; n++) part[warp][lane + 32 * n] = acc[n];
+  __syncthreads();
+  l = warp_value[0] + warp_value[1] + warp_value[2] + warp_value[3];
   const int i = row % a.q_len, h = (row / a.q_len) % a.heads, b = row / (static_cast<size_t>(a.q_len) * a.heads);
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
   T *out = static_cast<T *>(a.o.ptr) + b * a.o.batch + i * a.o.token + h * a.o.head;
-#pragma unroll
-  for (int n = 0; n < 4; n++)
-    if (lane + 32 * n < a.dim) out[lane + 32 * n] = Store<T>::from_float(acc[n] * inv);
-  if (a.lse && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  if (tid < a.dim) out[tid] = Store<T>::from_float((part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid]) * inv);
+  if (a.lse && tid == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 // Fills row_stats: -lse * log2(e) and -delta, delta = <dout_i, o_i> (= sum_j P_ij dP_ij).  One warp per row.

@@ -1,11 +1,12 @@
 // Attention of a few queries against a long cache (bf16): bound by reading K and V once.
 //
-// The queries of all heads that share a key/value head are the 16 rows of warp-level matrix products
-// (mma.sync m16n8k16: with this few rows the products are free and the tensor memory of tcgen05, with
-// its 128 lanes, would stand empty).  Nothing is staged in shared memory: a product's inner index may
-// run in any order, so each lane loads 16 adjacent bytes of a K row and of the Q row and uses them as
-// the fragments of two steps, and 16 adjacent bytes of V rows become the fragments of eight column
-// tiles by byte permutations.  Every lane has its 16 loads of 16 keys in flight at once.
+// The queries of all heads that share a key/value head are the columns, 8 or 16, of warp-level matrix
+// products (mma.sync m16n8k16: with this few the products are free, and the tensor memory of tcgen05,
+// with its 128 lanes, would stand empty): S^T = K Q^T over 16 keys, O^T += V^T P^T over those keys.
+// Nothing is staged in shared memory: a product's inner index may run in any order, so a lane loads 16
+// adjacent bytes of a K row, and of the Q row, and uses them as the fragments of two steps; 16 adjacent
+// bytes of four V rows become the fragments of four 16-column tiles by byte permutations.  Every lane
+// has its 16 loads for 16 keys in flight at once.
 //
 // The keys are split over CTAs (blockIdx.y) until the GPU is full several times, so that sequences of
 // different lengths even out; the four warps of a CTA take every fourth 16 keys and are joined in
@@ -18,7 +19,7 @@
 namespace dlb {
 namespace {
 
-constexpr int kStepWarps = 4, kStepThreads = 32 * kStepWarps, kStepRows = 16, kStepKeys = 16;
+constexpr int kStepWarps = 4, kStepThreads = 32 * kStepWarps, kStepKeys = 16;
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -27,69 +28,95 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ float quad_max(float v) {
-  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+// The 8x8 matrix of 16-bit values that the warp holds one row per four lanes, transposed.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __shfl_xor_sync(0xffffffffu, v, 1);
-  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+
+// Over the eight lanes that hold a column (lane ids equal mod 4).
+__device__ __forceinline__ float col_max(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o *= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float col_sum(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o *= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 
 // Word x of a 16-byte vector (x is a compile-time constant where this is used).
 __device__ __forceinline__ uint32_t word(const uint4 &v, int x) { return x == 0 ? v.x : x == 1 ? v.y : x == 2 ? v.z : v.w; }
 
-template <int NT>  // head_dim up to 32 * NT
-__global__ void __launch_bounds__(kStepThreads, 3) attn_step_kernel(const __grid_constant__ AttnArgs a) {
+// NT: head_dim up to 32 * NT; NR: up to 8 * NR queries (rows of q x heads of the group) per CTA.
+template <int NT, int NR>
+__global__ void __launch_bounds__(kStepThreads, NR == 1 ? 4 : 3) attn_step_kernel(const __grid_constant__ AttnArgs a) {
   pdl_prologue();
   constexpr int NB = (NT + 1) / 2;  // blocks of 64 columns of V and O
-  constexpr int W = NB * 64;
-  __shared__ float out_s[kStepWarps][kStepRows][W + 4];
-  __shared__ float m_s[kStepWarps][kStepRows], l_s[kStepWarps][kStepRows], r_s[kStepWarps][kStepRows];
+  constexpr int W = NB * 64, kRows = 8 * NR;
+  __shared__ float out_s[kStepWarps][kRows][W + 4];
+  __shared__ float m_s[kStepWarps][kRows], l_s[kStepWarps][kRows], r_s[kStepWarps][kRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int rows = a.q_len * a.group, row_tiles = (rows + kStepRows - 1) / kStepRows;
+  const int rows = a.q_len * a.group, row_tiles = (rows + kRows - 1) / kRows;
   const int tile = blockIdx.x % row_tiles, hk = (blockIdx.x / row_tiles) % a.kv_heads, b = blockIdx.x / (row_tiles * a.kv_heads);
   const BatchView view = batch_view(a, b);
-  const int row_last = min(rows, (tile + 1) * kStepRows) - 1;
+  const int row_last = min(rows, (tile + 1) * kRows) - 1;
   const int last = row_end(a, view, row_last / a.group);  // row_end never falls with the query
   // this CTA's share of the keys, in multiples of what its warps take in one turn
   const int turn = kStepWarps * kStepKeys, turns = (last + turn - 1) / turn;
   const int share = (turns + a.splits - 1) / a.splits * turn;
   const int s0 = min(static_cast<long long>(last), static_cast<long long>(blockIdx.y) * share), s1 = min(last, s0 + share);
 
-  int pos[2], end[2], head[2], doc[2];
-  float slope[2], far_left[2];
-  uint4 q[2][NT];
+  // this lane's columns of S^T and O^T: rows 8y + 2c + x of the tile
+  int pos[NR][2], end[NR][2], head[NR][2], doc[NR][2];
+  float slope[NR][2], far_left[NR][2];
 #pragma unroll
-  for (int x = 0; x < 2; x++) {
-    const int r = tile * kStepRows + g + 8 * x, i = r / a.group;
-    const bool valid = r < rows;
-    head[x] = hk * a.group + r % a.group;
-    pos[x] = view.start + i;
-    end[x] = valid ? row_end(a, view, i) : 0;
-    doc[x] = (a.q_docs && valid) ? ld_co(a.q_docs + static_cast<long long>(b) * a.q_len + i) : 0;
-    slope[x] = (a.slopes && valid) ? ld_co(a.slopes + head[x]) * kLog2e : 0.f;
-    far_left[x] = (a.table && valid) ? table_entry(a, head[x], bucket_at(a, -a.reach)) : 0.f;
-    const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(a.q.ptr) + b * a.q.batch + static_cast<long long>(i) * a.q.token +
-                               head[x] * a.q.head;
+  for (int y = 0; y < NR; y++)
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      const int r = tile * kRows + 8 * y + 2 * c + x, i = r / a.group;
+      const bool valid = r < rows;
+      head[y][x] = hk * a.group + r % a.group;
+      pos[y][x] = view.start + i;
+      end[y][x] = valid ? min(s1, row_end(a, view, i)) : 0;
+      doc[y][x] = (a.q_docs && valid) ? ld_co(a.q_docs + static_cast<long long>(b) * a.q_len + i) : 0;
+      slope[y][x] = (a.slopes && valid) ? ld_co(a.slopes + head[y][x]) * kLog2e : 0.f;
+      far_left[y][x] = (a.table && valid) ? table_entry(a, head[y][x], bucket_at(a, -a.reach)) : 0.f;
+    }
+  uint4 q[NR][NT];  // row 8y + g
+#pragma unroll
+  for (int y = 0; y < NR; y++) {
+    const int r = tile * kRows + 8 * y + g;
+    const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(a.q.ptr) + b * a.q.batch +
+                               static_cast<long long>(r / a.group) * a.q.token + (hk * a.group + r % a.group) * a.q.head;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
       const int col = (4 * t + c) * 8;
-      q[x][t] = valid && col < a.dim ? ld_keep(src + col) : make_uint4(0, 0, 0, 0);
+      q[y][t] = r < rows && col < a.dim ? ld_keep(src + col) : make_uint4(0, 0, 0, 0);
     }
   }
   const __nv_bfloat16 *kb = static_cast<const __nv_bfloat16 *>(a.k.ptr) + b * a.k.batch + hk * a.k.head;
   const __nv_bfloat16 *vb = static_cast<const __nv_bfloat16 *>(a.v.ptr) + b * a.v.batch + hk * a.v.head;
   const float inside = a.cap > 0.f ? a.scale / a.cap : 0.f, to_log2 = (a.cap > 0.f ? a.cap : a.scale) * kLog2e;
-  const int far_to = min(view.start + (tile * kStepRows) / a.group, INT_MAX / 2) - a.reach;  // keys up to here are far left of all rows
+  const int far_to = view.start + (tile * kRows) / a.group - a.reach;  // keys up to here are beyond the reach of all rows
 
-  float acc[NB][8][4], m[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, sum_rounded[2] = {0.f, 0.f};
+  float acc[NR][NB][4][4], m[NR][2], sum[NR][2], sum_rounded[NR][2];
 #pragma unroll
-  for (int n = 0; n < NB; n++)
+  for (int y = 0; y < NR; y++) {
 #pragma unroll
-    for (int t = 0; t < 8; t++)
+    for (int x = 0; x < 2; x++) {
+      m[y][x] = -INFINITY;
+      sum[y][x] = sum_rounded[y][x] = 0.f;
+    }
 #pragma unroll
-      for (int e = 0; e < 4; e++) acc[n][t][e] = 0.f;
+    for (int n = 0; n < NB; n++)
+#pragma unroll
+      for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[y][n][t][e] = 0.f;
+  }
 
   for (int j0 = s0 + warp * kStepKeys; j0 < s1; j0 += turn) {
     uint4 k[2][NT], v[NB][4];
@@ -104,106 +131,109 @@ __global__ void __launch_bounds__(kStepThreads, 3) attn_step_kernel(const __grid
       }
     }
 #pragma unroll
-    for (int n = 0; n < NB; n++)
+    for (int x = 0; x < 4; x++) {
+      const int j = j0 + 2 * c + (x & 1) + 8 * (x >> 1);
+      const __nv_bfloat16 *src = vb + static_cast<long long>(j) * a.v.token;
 #pragma unroll
-      for (int x = 0; x < 4; x++) {
-        const int j = j0 + 2 * c + (x & 1) + 8 * (x >> 1), col = n * 64 + g * 8;
-        v[n][x] = j < s1 && col < a.dim ? ld_stream(vb + static_cast<long long>(j) * a.v.token + col) : make_uint4(0, 0, 0, 0);
-      }
-    float s[2][4];  // [key tile][row g: keys 2c, 2c + 1; row g + 8: the same]
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
-#pragma unroll
-      for (int e = 0; e < 4; e++) s[u][e] = 0.f;
-#pragma unroll
-      for (int t = 0; t < NT; t++) {
-        mma16816(s[u], q[0][t].x, q[1][t].x, q[0][t].y, q[1][t].y, k[u][t].x, k[u][t].y);
-        mma16816(s[u], q[0][t].z, q[1][t].z, q[0][t].w, q[1][t].w, k[u][t].z, k[u][t].w);
+      for (int n = 0; n < NB; n++) {
+        const int col = n * 64 + g * 8;
+        v[n][x] = j < s1 && col < a.dim ? ld_stream(src + col) : make_uint4(0, 0, 0, 0);
       }
     }
     const bool all_far = j0 + kStepKeys - 1 <= far_to;
-    float top[2] = {-INFINITY, -INFINITY};
+    float s[NR][4];  // {key g, key g + 8} x {row 2c, row 2c + 1}
+    bool grow = false;
 #pragma unroll
-    for (int u = 0; u < 2; u++)
+    for (int y = 0; y < NR; y++) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) s[y][e] = 0.f;
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        mma16816(s[y], k[0][t].x, k[1][t].x, k[0][t].y, k[1][t].y, q[y][t].x, q[y][t].y);
+        mma16816(s[y], k[0][t].z, k[1][t].z, k[0][t].w, k[1][t].w, q[y][t].z, q[y][t].w);
+      }
+      if (a.cap > 0.f) tanh_scores(s[y], inside);
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const int x = e >> 1, j = j0 + 8 * u + 2 * c + (e & 1), d = j - pos[x];
-        float y = s[u][e];
-        if (a.cap > 0.f) y = tanh_score(y * inside);
-        y *= to_log2;
-        if (a.slopes) y = fmaf(-slope[x], static_cast<float>(abs(d)), y);
-        if (a.table) y += all_far ? far_left[x] : table_entry(a, head[x], bucket_at(a, d));
-        bool seen = j < end[x] && j < s1;
-        if (a.kv_docs) seen = seen && ld_co(a.kv_docs + static_cast<long long>(b) * a.kv_len + j) == doc[x];
-        s[u][e] = seen ? y : -INFINITY;
-        top[x] = fmaxf(top[x], s[u][e]);
+        const int x = e & 1, j = j0 + 8 * (e >> 1) + g, d = j - pos[y][x];
+        float z = s[y][e] * to_log2;
+        if (a.slopes) z = fmaf(-slope[y][x], static_cast<float>(abs(d)), z);
+        if (a.table) z += all_far ? far_left[y][x] : table_entry(a, head[y][x], bucket_at(a, d));
+        bool seen = j < end[y][x];
+        if (a.kv_docs) seen = seen && ld_co(a.kv_docs + static_cast<long long>(b) * a.kv_len + j) == doc[y][x];
+        s[y][e] = seen ? z : -INFINITY;
+        grow = grow || s[y][e] > m[y][x] + 8.f;
       }
-    bool grow[2];
+    }
+    // The maximum a column's lanes share moves only when some score has outgrown it by 2^8.
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int y = 0; y < NR; y++)
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+          const float top = fmaxf(m[y][x], col_max(fmaxf(s[y][x], s[y][x + 2])));
+          const float keep = top > m[y][x] ? ex2(m[y][x] - top) : 1.f;
+          m[y][x] = top;
+          sum[y][x] *= keep;
+          sum_rounded[y][x] *= keep;
+#pragma unroll
+          for (int n = 0; n < NB; n++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+              acc[y][n][t][x] *= keep;
+              acc[y][n][t][x + 2] *= keep;
+            }
+        }
+    }
+    uint32_t p[NR][2];  // fragments of P^T: keys 2c, 2c + 1 (and 8 more) of row g
+#pragma unroll
+    for (int y = 0; y < NR; y++) {
+      const float base0 = m[y][0] == -INFINITY ? 0.f : m[y][0], base1 = m[y][1] == -INFINITY ? 0.f : m[y][1];
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const float p0 = ex2(s[y][2 * u] - base0), p1 = ex2(s[y][2 * u + 1] - base1);
+        const uint32_t packed = pack_bf16(p0, p1);
+        sum[y][0] += p0;
+        sum[y][1] += p1;
+        sum_rounded[y][0] += __uint_as_float(packed << 16);
+        sum_rounded[y][1] += __uint_as_float(packed & 0xffff0000u);
+        p[y][u] = transpose8x8(packed);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NB; n++)
+#pragma unroll
+      for (int t = 0; t < 4; t++) {
+        // columns 64 n + 8 g + 2 t (rows g of the fragment) and + 1 (rows g + 8)
+        const uint32_t w0 = word(v[n][0], t), w1 = word(v[n][1], t), w2 = word(v[n][2], t), w3 = word(v[n][3], t);
+        const uint32_t a0 = __byte_perm(w0, w1, 0x5410), a1 = __byte_perm(w0, w1, 0x7632);
+        const uint32_t a2 = __byte_perm(w2, w3, 0x5410), a3 = __byte_perm(w2, w3, 0x7632);
+#pragma unroll
+        for (int y = 0; y < NR; y++) mma16816(acc[y][n][t], a0, a1, a2, a3, p[y][0], p[y][1]);
+      }
+  }
+#pragma unroll
+  for (int y = 0; y < NR; y++)
 #pragma unroll
     for (int x = 0; x < 2; x++) {
-      top[x] = quad_max(top[x]);
-      grow[x] = top[x] > m[x] + 8.f;
-    }
-    if (__any_sync(0xffffffffu, grow[0] || grow[1])) {
-      float keep[2];
-#pragma unroll
-      for (int x = 0; x < 2; x++) {
-        keep[x] = grow[x] ? ex2(m[x] - top[x]) : 1.f;
-        if (grow[x]) m[x] = top[x];
-        sum[x] *= keep[x];
-        sum_rounded[x] *= keep[x];
+      const float l = col_sum(sum[y][x]), rounded = col_sum(sum_rounded[y][x]);
+      const int r = 8 * y + 2 * c + x;
+      if (g == 0) {
+        m_s[warp][r] = m[y][x];
+        l_s[warp][r] = l;
+        r_s[warp][r] = rounded;
       }
 #pragma unroll
       for (int n = 0; n < NB; n++)
 #pragma unroll
-        for (int t = 0; t < 8; t++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) acc[n][t][e] *= keep[e >> 1];
+        for (int t = 0; t < 4; t += 2)  // columns 64 n + 8 g + 2 t .. 2 t + 3
+          *reinterpret_cast<float4 *>(&out_s[warp][r][n * 64 + 8 * g + 2 * t]) =
+              make_float4(acc[y][n][t][x], acc[y][n][t][x + 2], acc[y][n][t + 1][x], acc[y][n][t + 1][x + 2]);
     }
-    uint32_t p[2][2];  // [key tile][row]
-#pragma unroll
-    for (int x = 0; x < 2; x++) {
-      const float base = m[x] == -INFINITY ? 0.f : m[x];
-#pragma unroll
-      for (int u = 0; u < 2; u++) {
-        const float p0 = ex2(s[u][2 * x] - base), p1 = ex2(s[u][2 * x + 1] - base);
-        p[u][x] = pack_bf16(p0, p1);
-        sum[x] += p0 + p1;
-        sum_rounded[x] += __uint_as_float(p[u][x] << 16) + __uint_as_float(p[u][x] & 0xffff0000u);
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < NB; n++)
-#pragma unroll
-      for (int t = 0; t < 8; t++) {
-        // column 64 n + 8 g + t of keys (2c, 2c + 1) and (2c + 8, 2c + 9)
-        const uint32_t pick = t & 1 ? 0x7632 : 0x5410;
-        const uint32_t b0 = __byte_perm(word(v[n][0], t / 2), word(v[n][1], t / 2), pick);
-        const uint32_t b1 = __byte_perm(word(v[n][2], t / 2), word(v[n][3], t / 2), pick);
-        mma16816(acc[n][t], p[0][0], p[0][1], p[1][0], p[1][1], b0, b1);
-      }
-  }
-#pragma unroll
-  for (int x = 0; x < 2; x++) {
-    sum[x] = quad_sum(sum[x]);
-    sum_rounded[x] = quad_sum(sum_rounded[x]);
-    if (c == 0) {
-      m_s[warp][g + 8 * x] = m[x];
-      l_s[warp][g + 8 * x] = sum[x];
-      r_s[warp][g + 8 * x] = sum_rounded[x];
-    }
-#pragma unroll
-    for (int n = 0; n < NB; n++)
-#pragma unroll
-      for (int half = 0; half < 2; half++)  // columns 64 n + 16 c + 8 half + 0..7
-#pragma unroll
-        for (int t = 0; t < 8; t += 4)
-          *reinterpret_cast<float4 *>(&out_s[warp][g + 8 * x][n * 64 + 16 * c + 8 * half + t]) =
-              make_float4(acc[n][t][2 * x + half], acc[n][t + 1][2 * x + half], acc[n][t + 2][2 * x + half], acc[n][t + 3][2 * x + half]);
-  }
   __syncthreads();
-  // Join of the four warps: eight threads a row.
-  const int r = threadIdx.x / 8, part = threadIdx.x % 8, rr = tile * kStepRows + r;
+  // Join of the four warps: 16 or 8 threads a row.
+  constexpr int kParts = kStepThreads / kRows;
+  const int r = threadIdx.x / kParts, part = threadIdx.x % kParts, rr = tile * kRows + r;
   if (rr >= rows) return;
   float top = -INFINITY;
 #pragma unroll
@@ -223,7 +253,7 @@ __global__ void __launch_bounds__(kStepThreads, 3) attn_step_kernel(const __grid
   const float to = rounded > 0.f || rounded != rounded ? (whole ? 1.f / rounded : l / rounded) : 0.f;
   const size_t at = static_cast<size_t>(blockIdx.y) * a.batch * a.heads * a.q_len + row;
   __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(a.o.ptr) + b * a.o.batch + static_cast<long long>(i) * a.o.token + h * a.o.head;
-  for (int col = part * 8; col < a.dim; col += 64) {
+  for (int col = part * 8; col < a.dim; col += kParts * 8) {
     float o[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
@@ -248,22 +278,37 @@ __global__ void __launch_bounds__(kStepThreads, 3) attn_step_kernel(const __grid
 
 }  // namespace
 
+namespace {
+// Rows of a CTA: one fragment of 8 where they all fit it, else two.
+int step_rows(int rows) { return rows <= 8 ? 8 : 16; }
+}  // namespace
+
 int attn_step_splits(int batch, int kv_heads, int rows, int kv_len) {
-  // Three CTAs fit an SM; six times that many even out sequences of different lengths (64 users with
-  // 4096 to 8192 keys: see the measurements beside the kernel), but a share keeps 256 keys.
-  const long long ctas = static_cast<long long>(batch) * kv_heads * ceil_div(rows, kStepRows);
-  const long long want = ceil_div(18ll * sm_count(), std::max(1ll, ctas));
-  return static_cast<int>(std::max(1ll, std::min({want, static_cast<long long>(kv_len / 256), 256ll})));
+  // Enough CTAs to fill the GPU once (four fit an SM) while a share keeps two turns of its warps, and to
+  // fill it four times, which evens out sequences of different lengths, while it keeps 16.
+  const long long ctas = static_cast<long long>(batch) * kv_heads * ceil_div(rows, step_rows(rows)), fill = 4ll * sm_count();
+  const long long once = std::min(ceil_div(fill, std::max(1ll, ctas)), kv_len / 128ll);
+  const long long often = std::min(ceil_div(4 * fill, std::max(1ll, ctas)), kv_len / 1024ll);
+  return static_cast<int>(std::max(1ll, std::min(std::max(once, often), 256ll)));
 }
 
 int attn_step(const AttnArgs &a, cudaStream_t st) {
-  const int rows = a.q_len * a.group;
-  const dim3 grid(ceil_div(rows, kStepRows) * a.kv_heads * a.batch, a.splits);
-  const int nt = ceil_div(a.dim, 32);
-  auto kern = nt == 1 ? attn_step_kernel<1> : nt == 2 ? attn_step_kernel<2> : nt == 3 ? attn_step_kernel<3> : attn_step_kernel<4>;
-  launch_pdl(kern, grid, dim3(kStepThreads), 0, st, a);
-  DLB_LAUNCH_CHECK("attn_step");
-  return DLB_OK;
+  const int rows = a.q_len * a.group, per_cta = step_rows(rows), nt = ceil_div(a.dim, 32);
+  const dim3 grid(ceil_div(rows, per_cta) * a.kv_heads * a.batch, a.splits);
+  auto launch = [&](auto kern) -> int {
+    launch_pdl(kern, grid, dim3(kStepThreads), 0, st, a);
+    DLB_LAUNCH_CHECK("attn_step");
+    return DLB_OK;
+  };
+  if (per_cta == 8)
+    return nt == 1   ? launch(attn_step_kernel<1, 1>)
+           : nt == 2 ? launch(attn_step_kernel<2, 1>)
+           : nt == 3 ? launch(attn_step_kernel<3, 1>)
+                     : launch(attn_step_kernel<4, 1>);
+  return nt == 1   ? launch(attn_step_kernel<1, 2>)
+         : nt == 2 ? launch(attn_step_kernel<2, 2>)
+         : nt == 3 ? launch(attn_step_kernel<3, 2>)
+                   : launch(attn_step_kernel<4, 2>);
 }
 
 }  // namespace dlb
