@@ -63,6 +63,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   __shared__ uint64_t x_full, full[ST], empty[ST], s_full[2], p_full[2], acc_full, drain;
   __shared__ uint32_t tmem_slot;
   __shared__ int dead_flag, doc_range[2];
+  __shared__ __align__(16) int doc_tile[2][kStreamRows];
   volatile int *dead = &dead_flag;
   const bool table_sums = BIAS == kTable && !FOR_KEYS && a.dtable != nullptr;
 
@@ -253,7 +254,9 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     const int see_from = !valid ? INT_MAX : FOR_KEYS ? first_query(a, view, x) : 0;
     const int see_end = !valid ? 0 : FOR_KEYS ? a.q_len : row_end(a, view, x);
     const float2 row_stat = (!FOR_KEYS && valid) ? stat_at(a, b, unit, x) : make_float2(-INFINITY, 0.f);
-    const float to_log2 = CAP ? a.cap * kLog2e : a.scale * kLog2e, inside = CAP ? a.scale / a.cap : 0.f;
+    const float to_log2 = CAP ? 1.f : a.scale * kLog2e;
+    const CapCoef cap = CAP ? cap_coef(a.scale, a.cap) : CapCoef();
+    const float2 uncap = both(CAP ? 1.f / cap.out : 0.f);
     const int tail = !FOR_KEYS && view.end % kStreamRows && view.end < a.kv_len ? view.end / kStreamRows : -1;
     int bucket_now = 0;
     float2 bucket_sum = make_float2(0.f, 0.f);
@@ -282,8 +285,16 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         it++;
         if ((it & 1) != w) continue;
         const int c0 = n * kStreamRows, s = it % ST;
+        const bool by_doc = f != 3 && stream_docs;
+        int col_doc = 0;
+        if (by_doc) col_doc = ld_co(stream_docs + min(c0 + (row & 63), (FOR_KEYS ? a.q_len : a.kv_len) - 1));
         mbar_wait(&full[s], (it / ST) & 1, dead, timeouts);  // the stage's statistics
         mbar_wait(&s_full[w], (it >> 1) & 1, dead, timeouts);
+        if (by_doc) {  // the group's document numbers of this tile
+          named_bar_sync(2 + w, 128);
+          if (row < kStreamRows) doc_tile[w][row] = col_doc;
+          named_bar_sync(2 + w, 128);
+        }
         tc_fence_after();
         const float *stats = reinterpret_cast<const float *>(smem + Shape::kStats + s * kStatsBytes);
 #pragma unroll
@@ -297,7 +308,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           float x32[32];
 #pragma unroll
           for (int e = 0; e < 32; e++) x32[e] = __uint_as_float(sr[e]);
-          if (CAP) tanh_scores(x32, inside);
+          if (CAP) cap_scores(x32, cap);
           float bias[32];
           const int d0 = FOR_KEYS ? x - (view.start + c1) : c1 - (view.start + x);  // distance j - p at e = 0
           bool far = false;
@@ -343,7 +354,8 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
               float2 shift = q ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
               const float2 minus = q ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);
               if (BIAS != kNoBias) shift = add2(shift, make_float2(bias[e + q], bias[e + q + 1]));
-              const float2 y = fma2(make_float2(x32[e + q], x32[e + q + 1]), k2, shift);
+              const float2 v = make_float2(x32[e + q], x32[e + q + 1]);
+              const float2 y = CAP ? add2(v, shift) : fma2(v, k2, shift);
               p[e + q] = ex2(y.x);
               p[e + q + 1] = ex2(y.y);
               const float2 dp = add2(make_float2(__uint_as_float(gr[e + q]), __uint_as_float(gr[e + q + 1])), minus);
@@ -355,9 +367,15 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           if (f != 3) {
             if (stream_docs) {
 #pragma unroll
-              for (int e = 0; e < 32; e++)
-                if (c1 + e < see_from || c1 + e >= see_end || ld_co(stream_docs + c1 + e) != row_doc) p[e] = ds[e] = 0.f;
-            } else if (FOR_KEYS) {
+              for (int e = 0; e < 32; e += 4) {
+                const int4 d = *reinterpret_cast<const int4 *>(&doc_tile[w][half * 32 + e]);
+                const int same[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                  if (same[q] != row_doc) p[e + q] = ds[e + q] = 0.f;
+              }
+            }
+            if (FOR_KEYS) {
               const int skip = see_from - c1;  // see_end is q_len: rows behind it have -lse = -infinity
 #pragma unroll
               for (int e = 0; e < 32; e++)
@@ -393,8 +411,8 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           for (int e = 0; e < 16; e++) {
             float2 y = make_float2(ds[2 * e], ds[2 * e + 1]);
             if (CAP) {  // d tanh = 1 - tanh^2
-              const float2 t = make_float2(x32[2 * e], x32[2 * e + 1]);
-              y = mul2(y, fma2(make_float2(-t.x, -t.y), t, make_float2(1.f, 1.f)));
+              const float2 t = mul2(make_float2(x32[2 * e], x32[2 * e + 1]), uncap);
+              y = mul2(y, fma2(make_float2(-t.x, -t.y), t, both(1.f)));
             }
             packed[e] = pack_bf16(y.x, y.y);
           }

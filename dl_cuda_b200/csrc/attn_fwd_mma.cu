@@ -47,6 +47,7 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   __shared__ uint32_t tmem_slot;
   __shared__ int dead_flag;
   __shared__ int doc_range[4];
+  __shared__ __align__(16) int doc_tile[2][kTileRows];
   volatile int *dead = &dead_flag;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -151,7 +152,8 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     const int end = valid ? row_end(a, view, i) : 0, pos = view.start + i;
     const int doc = (a.q_docs && valid) ? ld_co(a.q_docs + static_cast<long long>(b) * a.q_len + i) : 0;
     const float slope = (BIAS != kNoBias && a.slopes) ? ld_co(a.slopes + h) * kLog2e : 0.f;
-    const float to_log2 = CAP ? a.cap * kLog2e : a.scale * kLog2e, inside = CAP ? a.scale / a.cap : 0.f;
+    const float to_log2 = CAP ? 1.f : a.scale * kLog2e;
+    const CapCoef cap = CAP ? cap_coef(a.scale, a.cap) : CapCoef();
     constexpr bool kRaw = !CAP && BIAS == kNoBias;  // maximum and exponent from the products themselves
     const int tail = view.end % kTileRows && view.end < a.kv_len ? view.end / kTileRows : -1;
     float m = -INFINITY, sum = 0.f, sum_rounded = 0.f;
@@ -162,7 +164,15 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       it++;
       if (!(f >> (2 * t) & 1)) continue;
       const int j0 = n * kTileRows;
+      const bool whole = f >> (2 * t + 1) & 1;
+      int key_doc = 0;
+      if (!whole && a.kv_docs) key_doc = ld_co(a.kv_docs + static_cast<long long>(b) * a.kv_len + min(j0 + (tid & 127), a.kv_len - 1));
       mbar_wait(&s_full[t], done & 1, dead, timeouts);
+      if (!whole && a.kv_docs) {  // the group's document numbers of this tile
+        named_bar_sync(2 + t, 128);
+        doc_tile[t][tid & 127] = key_doc;
+        named_bar_sync(2 + t, 128);
+      }
       tc_fence_after();
       uint32_t raw[4][32];
 #pragma unroll
@@ -175,18 +185,11 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         float x[32];
 #pragma unroll
         for (int e = 0; e < 32; e++) x[e] = __uint_as_float(raw[c][e]);
-        if (CAP) tanh_scores(x, inside);
-        if (!kRaw) {
-          const float2 k2 = make_float2(to_log2, to_log2);
+        if (CAP) cap_scores(x, cap);
+        if (BIAS != kNoBias) {
+          const float2 k2 = both(to_log2);
           const int d0 = j0 + c * 32 - pos;
-          if (BIAS == kNoBias) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float2 y = mul2(make_float2(x[e], x[e + 1]), k2);
-              x[e] = y.x;
-              x[e + 1] = y.y;
-            }
-          } else {
+          {
             float bias[32];
 #pragma unroll
             for (int e = 0; e < 32; e++) bias[e] = 0.f;
@@ -216,26 +219,26 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             }
           }
         }
-        if (!(f >> (2 * t + 1) & 1)) {
+        if (!whole) {
+          const int room = end - (j0 + c * 32);
           if (a.kv_docs) {
-            const int *docs = a.kv_docs + static_cast<long long>(b) * a.kv_len + j0 + c * 32;
 #pragma unroll
-            for (int e = 0; e < 32; e++) {
-              const int j = j0 + c * 32 + e;
-              if (j >= end || ld_co(docs + e) != doc) x[e] = -INFINITY;
+            for (int e = 0; e < 32; e += 4) {
+              const int4 d = *reinterpret_cast<const int4 *>(&doc_tile[t][c * 32 + e]);
+              x[e] = d.x == doc ? x[e] : -INFINITY;
+              x[e + 1] = d.y == doc ? x[e + 1] : -INFINITY;
+              x[e + 2] = d.z == doc ? x[e + 2] : -INFINITY;
+              x[e + 3] = d.w == doc ? x[e + 3] : -INFINITY;
             }
-          } else {
-            const int room = end - (j0 + c * 32);
+          }
+          if (!a.kv_docs || room < 32) {
 #pragma unroll
-            for (int e = 0; e < 32; e++)
-              if (e >= room) x[e] = -INFINITY;
+            for (int e = 0; e < 32; e++) x[e] = e < room ? x[e] : -INFINITY;
           }
         }
+        top = fmaxf(top, max_of<32, false>(x));
 #pragma unroll
-        for (int e = 0; e < 32; e++) {
-          top = fmaxf(top, x[e]);
-          raw[c][e] = __float_as_uint(x[e]);
-        }
+        for (int e = 0; e < 32; e++) raw[c][e] = __float_as_uint(x[e]);
       }
       if (kRaw) top *= to_log2;
       const bool grow = top > m + 8.f;  // with m = -inf: whenever the row sees anything
@@ -261,24 +264,29 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         }
       }
       const float base = m == -INFINITY ? 0.f : m;
-      const float2 mult = make_float2(kRaw ? to_log2 : 1.f, kRaw ? to_log2 : 1.f), minus = make_float2(-base, -base);
-      float2 part = make_float2(0.f, 0.f), part_rounded = make_float2(0.f, 0.f);
+      const float2 mult = both(to_log2), minus = both(-base);
+      float2 part[4], part_rounded[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) part[k] = part_rounded[k] = both(0.f);
 #pragma unroll
       for (int c = 0; c < 2; c++) {
         uint32_t packed[32];
 #pragma unroll
         for (int e = 0; e < 32; e++) {
-          const float2 y = fma2(make_float2(__uint_as_float(raw[2 * c + e / 16][2 * (e % 16)]),
-                                            __uint_as_float(raw[2 * c + e / 16][2 * (e % 16) + 1])), mult, minus);
+          const float2 v = make_float2(__uint_as_float(raw[2 * c + e / 16][2 * (e % 16)]),
+                                       __uint_as_float(raw[2 * c + e / 16][2 * (e % 16) + 1]));
+          const float2 y = kRaw ? fma2(v, mult, minus) : add2(v, minus);
           const float2 p = make_float2(ex2(y.x), ex2(y.y));
           packed[e] = pack_bf16(p.x, p.y);
-          part = add2(part, p);
-          part_rounded = add2(part_rounded, make_float2(__uint_as_float(packed[e] << 16), __uint_as_float(packed[e] & 0xffff0000u)));
+          part[e % 4] = add2(part[e % 4], p);
+          part_rounded[e % 4] = add2(part_rounded[e % 4], make_float2(__uint_as_float(packed[e] << 16), __uint_as_float(packed[e] & 0xffff0000u)));
         }
         tmem_store32(s_at + c * 32, packed);
       }
-      sum += part.x + part.y;
-      sum_rounded += part_rounded.x + part_rounded.y;
+      part[0] = add2(add2(part[0], part[1]), add2(part[2], part[3]));
+      part_rounded[0] = add2(add2(part_rounded[0], part_rounded[1]), add2(part_rounded[2], part_rounded[3]));
+      sum += part[0].x + part[0].y;
+      sum_rounded += part_rounded[0].x + part_rounded[0].y;
       if (n == tail) {
         // Rows of V behind the last key any query reaches may hold anything, and 0 * NaN is NaN.
         const int s = it % ST;

@@ -13,40 +13,85 @@ constexpr int kLutPad = 160;                           // room on both sides of 
 constexpr int kMaxTiles = 4096;                        // key (or query) tiles a kernel can list
 enum { kNoBias = 0, kSlope = 1, kTable = 2 };          // kTable: with or without slopes
 
-// tanh(x) for |x| <= 1 as x * P(x^2), degree 6 in x^2: a least-squares fit of tanh(x) / x reweighted
-// until the relative error was level, 5e-8 before fp32 rounding and 1.2e-7 with it.
-__device__ __forceinline__ float2 tanh_small2(float2 x) {
+// Capped scores times log2(e), L tanh(k x) with L = cap * log2(e), k = scale / cap, as odd polynomials:
+// least-squares fits of tanh(x) / x in x^2, reweighted until the relative error was level.
+//   |k x| <= 0.4: degree 3, error 1.0e-7, with the powers of k and L folded into the coefficients
+//                 (5 operations a score; scores up to 0.4 cap are the usual case)
+//   |k x| <= 1:   degree 6, error 5e-8 (1.2e-7 in fp32), 10 operations
+// Anything larger takes two special-function operations per score.  A warp takes one road.
+struct CapCoef {
+  float c0, c1, c2, c3, k, out;
+  bool folded;  // k^7 must not fall under fp32's range
+};
+__device__ __forceinline__ CapCoef cap_coef(float scale, float cap) {
+  CapCoef c;
+  c.k = scale / cap;
+  c.out = cap * kLog2e;
+  const float kk = c.k * c.k;
+  c.c0 = 0.9999998807907104f * c.k * c.out;
+  c.c1 = -0.33331358432769775f * kk * c.k * c.out;
+  c.c2 = 0.132709339261055f * kk * kk * c.k * c.out;
+  c.c3 = -0.04755208641290665f * kk * kk * kk * c.k * c.out;
+  c.folded = c.k > 1e-4f && c.k < 1e4f;
+  return c;
+}
+
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+__device__ __forceinline__ float2 tanh_to_1(float2 x) {
   const float2 u = mul2(x, x);
-  auto c = [](float v) { return make_float2(v, v); };
-  float2 p = fma2(u, c(0.0010406870860606432f), c(-0.006202297285199165f));
-  p = fma2(p, u, c(0.020288638770580292f));
-  p = fma2(p, u, c(-0.053456228226423264f));
-  p = fma2(p, u, c(0.13325180113315582f));
-  p = fma2(p, u, c(-0.33332836627960205f));
-  p = fma2(p, u, c(0.9999999403953552f));
+  float2 p = fma2(u, both(0.0010406870860606432f), both(-0.006202297285199165f));
+  p = fma2(p, u, both(0.020288638770580292f));
+  p = fma2(p, u, both(-0.053456228226423264f));
+  p = fma2(p, u, both(0.13325180113315582f));
+  p = fma2(p, u, both(-0.33332836627960205f));
+  p = fma2(p, u, both(0.9999999403953552f));
   return mul2(p, x);
 }
 
-// tanh of N scores times `k`.  Scores well inside the cap (|x k| <= 1 in the whole warp, the usual
-// case) take the polynomial on the fp32 pipes, 9 instructions for two; a warp with a larger one pays
-// two special-function operations per score.
+// Largest value, in four chains of three-operand maxima.
+template <int N, bool ABS>
+__device__ __forceinline__ float max_of(const float (&x)[N]) {
+  constexpr int C = N < 8 ? 1 : 4;
+  float top[C];
+#pragma unroll
+  for (int c = 0; c < C; c++) top[c] = ABS ? 0.f : -INFINITY;
+#pragma unroll
+  for (int e = 0; e < N; e += 2 * C)
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+      const float p = x[e + 2 * c], q = x[e + 2 * c + 1];
+      top[c] = fmaxf(fmaxf(top[c], ABS ? fabsf(p) : p), ABS ? fabsf(q) : q);
+    }
+  if constexpr (C == 1) return top[0];
+  else return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+}
+
 template <int N>
-__device__ __forceinline__ void tanh_scores(float (&x)[N], float k) {
-  float top = 0.f;
+__device__ __forceinline__ void cap_scores(float (&x)[N], const CapCoef &c) {
+  // fmaxf drops NaN: a NaN score stays one on every road
+  const float top = max_of<N, true>(x) * c.k;
+  if (c.folded && __all_sync(0xffffffffu, top <= 0.4f)) {
 #pragma unroll
-  for (int c = 0; c < N; c++) top = fmaxf(top, fabsf(x[c]));
-  const bool small = top * fabsf(k) <= 1.f;  // false for NaN as well: fmaxf drops it, the slow side keeps it
-  if (__all_sync(0xffffffffu, small)) {
-    const float2 kk = make_float2(k, k);
+    for (int e = 0; e < N; e += 2) {
+      const float2 v = make_float2(x[e], x[e + 1]), u = mul2(v, v);
+      float2 p = fma2(u, both(c.c3), both(c.c2));
+      p = fma2(p, u, both(c.c1));
+      p = fma2(p, u, both(c.c0));
+      p = mul2(p, v);
+      x[e] = p.x;
+      x[e + 1] = p.y;
+    }
+  } else if (__all_sync(0xffffffffu, top <= 1.f)) {
 #pragma unroll
-    for (int c = 0; c < N; c += 2) {
-      const float2 t = tanh_small2(mul2(make_float2(x[c], x[c + 1]), kk));
-      x[c] = t.x;
-      x[c + 1] = t.y;
+    for (int e = 0; e < N; e += 2) {
+      const float2 t = mul2(tanh_to_1(mul2(make_float2(x[e], x[e + 1]), both(c.k))), both(c.out));
+      x[e] = t.x;
+      x[e + 1] = t.y;
     }
   } else {
 #pragma unroll
-    for (int c = 0; c < N; c++) x[c] = tanh_score(x[c] * k);
+    for (int e = 0; e < N; e++) x[e] = tanh_score(x[e] * c.k) * c.out;
   }
 }
 

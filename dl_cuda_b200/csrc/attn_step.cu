@@ -99,7 +99,8 @@ __global__ void __launch_bounds__(kStepThreads, NR == 1 ? 4 : 3) attn_step_kerne
   }
   const __nv_bfloat16 *kb = static_cast<const __nv_bfloat16 *>(a.k.ptr) + b * a.k.batch + hk * a.k.head;
   const __nv_bfloat16 *vb = static_cast<const __nv_bfloat16 *>(a.v.ptr) + b * a.v.batch + hk * a.v.head;
-  const float inside = a.cap > 0.f ? a.scale / a.cap : 0.f, to_log2 = (a.cap > 0.f ? a.cap : a.scale) * kLog2e;
+  const float to_log2 = a.cap > 0.f ? 1.f : a.scale * kLog2e;
+  const CapCoef cap = a.cap > 0.f ? cap_coef(a.scale, a.cap) : CapCoef();
   const int far_to = view.start + (tile * kRows) / a.group - a.reach;  // keys up to here are beyond the reach of all rows
 
   float acc[NR][NB][4][4], m[NR][2], sum[NR][2], sum_rounded[NR][2];
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(kStepThreads, NR == 1 ? 4 : 3) attn_step_kerne
         mma16816(s[y], k[0][t].x, k[1][t].x, k[0][t].y, k[1][t].y, q[y][t].x, q[y][t].y);
         mma16816(s[y], k[0][t].z, k[1][t].z, k[0][t].w, k[1][t].w, q[y][t].z, q[y][t].w);
       }
-      if (a.cap > 0.f) tanh_scores(s[y], inside);
+      if (a.cap > 0.f) cap_scores(s[y], cap);
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         const int x = e & 1, j = j0 + 8 * (e >> 1) + g, d = j - pos[y][x];
