@@ -197,52 +197,64 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       }
     }
   } else if (warp == kBwdMmaWarp) {
-    if (lane == 0) {
-      const int k_steps = (a.dim + 15) / 16, n_cols = k_steps * 16;
-      const uint32_t idesc_s = mma_desc(kStreamRows, false), idesc_acc = mma_desc(n_cols, true);
-      const uint64_t xd = desc_k_major(smem_u32(smem + Shape::kX)), yd = desc_k_major(smem_u32(smem + Shape::kY));
-      const uint32_t ring_at = smem_u32(ring);
-      auto accumulate = [&](int it) {  // with what the row threads made of tile `it`
-        const int s = it % ST, w = it & 1;
-        mbar_wait(&p_full[w], (it >> 1) & 1, dead, timeouts);
-        tc_fence_after();
-        const uint64_t ud = desc_mn_major(ring_at + s * Shape::kStage, kStreamBlock);
-        const uint64_t wd = desc_mn_major(ring_at + s * Shape::kStage + NB * kStreamBlock, kStreamBlock);
+    const int k_steps = (a.dim + 15) / 16, n_cols = k_steps * 16;
+    const uint32_t idesc_s = mma_desc(kStreamRows, false), idesc_acc = mma_desc(n_cols, true);
+    const uint64_t xd = desc_k_major(smem_u32(smem + Shape::kX)), yd = desc_k_major(smem_u32(smem + Shape::kY));
+    const uint64_t u_desc = desc_k_major(smem_u32(ring)), u_desc_mn = desc_mn_major(smem_u32(ring), kStreamBlock);
+    constexpr uint32_t kStageStep = Shape::kStage >> 4, kW = (NB * kStreamBlock) >> 4;  // in descriptor units
+    auto accumulate = [&](int it) {  // with what the row threads made of tile `it`
+      const int s = it % ST, w = it & 1;
+      mbar_wait(&p_full[w], (it >> 1) & 1, dead, timeouts);
+      tc_fence_after();
+      const uint64_t ud = u_desc_mn + s * kStageStep, wd = ud + kW;
+      const uint32_t p_at = tmem + w * 128;
+      if (elect_lane()) {
+#pragma unroll
         for (int k = 0; k < kStreamRows / 16; k++)
-          mma_ts(tmem + 256, tmem + w * 128 + 64 + k * 8, ud + k * (2048 >> 4), idesc_acc, it > 0 || k > 0);
-        if (FOR_KEYS)
+          mma_ts(tmem + 256, p_at + 64 + k * 8, ud + k * (2048 >> 4), idesc_acc, it > 0 || k > 0);
+        if (FOR_KEYS) {
+#pragma unroll
           for (int k = 0; k < kStreamRows / 16; k++)
-            mma_ts(tmem + 384, tmem + w * 128 + k * 8, wd + k * (2048 >> 4), idesc_acc, it > 0 || k > 0);
+            mma_ts(tmem + 384, p_at + k * 8, wd + k * (2048 >> 4), idesc_acc, it > 0 || k > 0);
+        }
         tc_commit(&empty[s]);
-      };
-      mbar_wait(&x_full, 0, dead, timeouts);
-      int it = 0;
-      for (int g = 0; g < heads_here && !*dead; g++)
-        for (int n = 0; n < n_tiles; n++) {
-          if (!flags[n]) continue;
-          const int s = it % ST, w = it & 1;
-          if (it >= 2) accumulate(it - 2);
-          mbar_wait(&full[s], (it / ST) & 1, dead, timeouts);
-          const uint64_t ud = desc_k_major(ring_at + s * Shape::kStage);
-          const uint64_t wd = desc_k_major(ring_at + s * Shape::kStage + NB * kStreamBlock);
-          for (int k = 0; k < k_steps; k++) {
+      }
+      __syncwarp();
+    };
+    mbar_wait(&x_full, 0, dead, timeouts);
+    int it = 0;
+    for (int g = 0; g < heads_here && !*dead; g++)
+      for (int n = 0; n < n_tiles; n++) {
+        if (!flags[n]) continue;
+        const int s = it % ST, w = it & 1;
+        if (it >= 2) accumulate(it - 2);
+        mbar_wait(&full[s], (it / ST) & 1, dead, timeouts);
+        const uint64_t ud = u_desc + s * kStageStep, wd = ud + kW;
+        const uint32_t s_to = tmem + w * 128;
+        if (elect_lane()) {
+#pragma unroll
+          for (int k = 0; k < NB * 4; k++) {
             const int xk = (k / 4) * (kBlockBytes >> 4) + (k % 4) * 2, uk = (k / 4) * (kStreamBlock >> 4) + (k % 4) * 2;
-            mma_ss(tmem + w * 128, xd + xk, ud + uk, idesc_s, k > 0);
+            if (k < k_steps) mma_ss(s_to, xd + xk, ud + uk, idesc_s, k > 0);
           }
-          for (int k = 0; k < k_steps; k++) {
+#pragma unroll
+          for (int k = 0; k < NB * 4; k++) {
             const int xk = (k / 4) * (kBlockBytes >> 4) + (k % 4) * 2, uk = (k / 4) * (kStreamBlock >> 4) + (k % 4) * 2;
-            mma_ss(tmem + w * 128 + 64, yd + xk, wd + uk, idesc_s, k > 0);
+            if (k < k_steps) mma_ss(s_to + 64, yd + xk, wd + uk, idesc_s, k > 0);
           }
           tc_commit(&s_full[w]);
-          it++;
         }
-      if (it >= 2) accumulate(it - 2);
-      if (it >= 1) accumulate(it - 1);
-      tc_commit(&acc_full);
-      if (*dead) {
-        tc_commit(&drain);
-        drain_wait(&drain, 0);
+        __syncwarp();
+        it++;
       }
+    if (it >= 2) accumulate(it - 2);
+    if (it >= 1) accumulate(it - 1);
+    if (elect_lane()) tc_commit(&acc_full);
+    __syncwarp();
+    if (*dead) {
+      if (elect_lane()) tc_commit(&drain);
+      __syncwarp();
+      drain_wait(&drain, 0);
     }
   } else if (warp < kBwdLoadWarp) {
     const int w = warp >> 2, row = tid & 127, x = row0 + row;

@@ -4,11 +4,13 @@
 // them sees.  Eight softmax warps and two more: one thread copies K and V tiles into a ring (TMA), one issues the products,
 // and each query tile has four warps for its softmax, one thread per row:
 //     S = Q K^T (TMEM, fp32) -> scores, running maximum, P = 2^(s - m) (bf16, written over S) -> O += P V
-// The two query tiles take turns: while one's softmax runs, the other's products do.  O stays in TMEM;
-// it is rescaled only when a row's maximum has grown by more than 2^8 since the last time, which P, the
-// sum and O all bear in fp32/bf16 range (the quotient is the same).  The sum behind the quotient adds
-// the ROUNDED probabilities, so that a row's weights add up to one exactly as the product sees them;
-// lse comes from the unrounded ones.
+// The two query tiles take turns: while one's softmax runs, the other's products do.  O stays in TMEM.
+// Exponentials are taken against a reference that moves only when a score leaves its range of 2^32, so
+// no maximum stands between a score and its exponential, and O is hardly ever rescaled; keys are walked
+// from the last tile to the first, which under a causal mask and a distance bias meets the largest
+// scores at once.  The sum behind the quotient adds the ROUNDED probabilities, so that a row's weights
+// add up to one exactly as the product sees them (bf16 output 1.9e-3 instead of 2.3e-3 from the exact
+// one, of which the output's own rounding is 1.7e-3); lse comes from the unrounded ones.
 #include <algorithm>
 
 #include "attn_mma.cuh"
@@ -19,6 +21,10 @@ namespace {
 constexpr int kFwdThreads = 384, kMmaWarp = 9, kLoadWarp = 8;
 // Registers: launched with 168 each (384 * 168 = 64512); the eight softmax warps go up to 208, the four
 // others down to 88 (256 * 208 + 128 * 88 = 64512).
+// A row's exponentials are taken against a reference m that its scores (in powers of two) have to stay
+// within 2^32 of from above; fp32 sums and bf16 probabilities bear that with room to spare, and the
+// reference divides out.  It starts at 0, which serves most rows from end to end.
+constexpr float kReach = 32.f;
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 
 template <int NB>
@@ -156,9 +162,9 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     const CapCoef cap = CAP ? cap_coef(a.scale, a.cap) : CapCoef();
     constexpr bool kRaw = !CAP && BIAS == kNoBias;  // maximum and exponent from the products themselves
     const int tail = view.end % kTileRows && view.end < a.kv_len ? view.end / kTileRows : -1;
-    float m = -INFINITY, sum = 0.f, sum_rounded = 0.f;
+    float m = 0.f, sum = 0.f, sum_rounded = 0.f;
     int it = -1, done = 0;
-    for (int n = 0; n < n_tiles; n++) {
+    for (int n = n_tiles - 1; n >= 0; n--) {
       const int f = flags[n];
       if (!f) continue;
       it++;
@@ -174,88 +180,103 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         named_bar_sync(2 + t, 128);
       }
       tc_fence_after();
-      uint32_t raw[4][32];
+      // One pass over the scores against the reference m, which the keys so far fit; only if one does not
+      // is m moved (and what has been summed rescaled) and the pass repeated.  P stays in registers until
+      // then: it is written over the scores.
+      uint32_t packed[2][32];
+      float2 part[4], part_rounded[4];
+      for (int pass = 0; pass < 2; pass++) {
+        float top = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < 4; c++) tmem_load32(s_at + c * 32, raw[c]);
+        for (int k = 0; k < 4; k++) part[k] = part_rounded[k] = both(0.f);
+        uint32_t raw[2][32];
+        tmem_load32(s_at, raw[0]);
 #pragma unroll
-      for (int c = 0; c < 4; c++) tmem_loaded(raw[c]);
-      float top = -INFINITY;
+        for (int c = 0; c < 4; c++) {
+          tmem_loaded(raw[c & 1]);
+          if (c < 3) tmem_load32(s_at + (c + 1) * 32, raw[(c + 1) & 1]);
+          float x[32];
 #pragma unroll
-      for (int c = 0; c < 4; c++) {
-        float x[32];
+          for (int e = 0; e < 32; e++) x[e] = __uint_as_float(raw[c & 1][e]);
+          if (CAP) cap_scores(x, cap);
+          if (BIAS != kNoBias) {
+            const float2 k2 = both(to_log2);
+            const int d0 = j0 + c * 32 - pos;
+            {
+              float bias[32];
 #pragma unroll
-        for (int e = 0; e < 32; e++) x[e] = __uint_as_float(raw[c][e]);
-        if (CAP) cap_scores(x, cap);
-        if (BIAS != kNoBias) {
-          const float2 k2 = both(to_log2);
-          const int d0 = j0 + c * 32 - pos;
-          {
-            float bias[32];
+              for (int e = 0; e < 32; e++) bias[e] = 0.f;
+              if (BIAS == kTable) {
+                const bool left = d0 + 31 <= -a.reach, right = d0 >= a.reach;
+                if (__all_sync(0xffffffffu, left || right)) {
+                  const float far = left ? lut[0] : lut[2 * (a.reach + kLutPad)];
 #pragma unroll
-            for (int e = 0; e < 32; e++) bias[e] = 0.f;
-            if (BIAS == kTable) {
-              const bool left = d0 + 31 <= -a.reach, right = d0 >= a.reach;
-              if (__all_sync(0xffffffffu, left || right)) {
-                const float far = left ? lut[0] : lut[2 * (a.reach + kLutPad)];
+                  for (int e = 0; e < 32; e++) bias[e] = far;
+                } else {
+                  // within 31 + 31 of the reach on either side: the padded table covers every index
+                  const float *at = lut + d0 + a.reach + kLutPad;
 #pragma unroll
-                for (int e = 0; e < 32; e++) bias[e] = far;
-              } else {
-                // within 31 + 31 of the reach on either side: the padded table covers every index
-                const float *at = lut + d0 + a.reach + kLutPad;
+                  for (int e = 0; e < 32; e++) bias[e] = at[e];
+                }
+              }
+              if (BIAS == kSlope || a.slopes) {
+                const float d = static_cast<float>(d0);
 #pragma unroll
-                for (int e = 0; e < 32; e++) bias[e] = at[e];
+                for (int e = 0; e < 32; e++) bias[e] = fmaf(-slope, fabsf(d + static_cast<float>(e)), bias[e]);
+              }
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                const float2 y = fma2(make_float2(x[e], x[e + 1]), k2, make_float2(bias[e], bias[e + 1]));
+                x[e] = y.x;
+                x[e + 1] = y.y;
               }
             }
-            if (BIAS == kSlope || a.slopes) {
-              const float d = static_cast<float>(d0);
+          }
+          if (!whole) {
+            const int room = end - (j0 + c * 32);
+            if (a.kv_docs) {
 #pragma unroll
-              for (int e = 0; e < 32; e++) bias[e] = fmaf(-slope, fabsf(d + static_cast<float>(e)), bias[e]);
+              for (int e = 0; e < 32; e += 4) {
+                const int4 d = *reinterpret_cast<const int4 *>(&doc_tile[t][c * 32 + e]);
+                x[e] = d.x == doc ? x[e] : -INFINITY;
+                x[e + 1] = d.y == doc ? x[e + 1] : -INFINITY;
+                x[e + 2] = d.z == doc ? x[e + 2] : -INFINITY;
+                x[e + 3] = d.w == doc ? x[e + 3] : -INFINITY;
+              }
             }
+            if (!a.kv_docs || room < 32) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float2 y = fma2(make_float2(x[e], x[e + 1]), k2, make_float2(bias[e], bias[e + 1]));
-              x[e] = y.x;
-              x[e + 1] = y.y;
+              for (int e = 0; e < 32; e++) x[e] = e < room ? x[e] : -INFINITY;
             }
+          }
+top = fmaxf(top, max_of<32, false>(x));
+          const float2 minus = both(-m);
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            const float2 v = make_float2(x[2 * e], x[2 * e + 1]);
+            const float2 y = kRaw ? fma2(v, both(to_log2), minus) : add2(v, minus);
+            const float2 p = make_float2(ex2(y.x), ex2(y.y));
+            const uint32_t w = pack_bf16(p.x, p.y);
+            packed[c / 2][(c & 1) * 16 + e] = w;
+            part[e % 4] = add2(part[e % 4], p);
+            part_rounded[e % 4] = add2(part_rounded[e % 4], make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)));
           }
         }
-        if (!whole) {
-          const int room = end - (j0 + c * 32);
-          if (a.kv_docs) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              const int4 d = *reinterpret_cast<const int4 *>(&doc_tile[t][c * 32 + e]);
-              x[e] = d.x == doc ? x[e] : -INFINITY;
-              x[e + 1] = d.y == doc ? x[e + 1] : -INFINITY;
-              x[e + 2] = d.z == doc ? x[e + 2] : -INFINITY;
-              x[e + 3] = d.w == doc ? x[e + 3] : -INFINITY;
-            }
-          }
-          if (!a.kv_docs || room < 32) {
-#pragma unroll
-            for (int e = 0; e < 32; e++) x[e] = e < room ? x[e] : -INFINITY;
-          }
-        }
-        top = fmaxf(top, max_of<32, false>(x));
-#pragma unroll
-        for (int e = 0; e < 32; e++) raw[c][e] = __float_as_uint(x[e]);
-      }
-      if (kRaw) top *= to_log2;
-      const bool grow = top > m + 8.f;  // with m = -inf: whenever the row sees anything
-      if (__any_sync(0xffffffffu, grow)) {
-        const float keep = grow ? ex2(m - top) : 1.f;
-        if (grow) m = top;
+        if (kRaw) top *= to_log2;
+        const bool above = top > m + kReach, below = sum == 0.f && top < m - kReach && top > -INFINITY;
+        if (!__any_sync(0xffffffffu, above || below)) break;
+        const float keep = above ? ex2(m - top) : below ? 0.f : 1.f;
+        if (above || below) m = top;
         sum *= keep;
         sum_rounded *= keep;
         if (done > 0) {
-          const float2 k2 = make_float2(keep, keep);
           for (int c = 0; c < a.dim; c += 32) {
             uint32_t o[32];
             tmem_load32(o_at + c, o);
             tmem_loaded(o);
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
-              const float2 y = mul2(make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1])), k2);
+              const float2 y = mul2(make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1])), both(keep));
               o[e] = __float_as_uint(y.x);
               o[e + 1] = __float_as_uint(y.y);
             }
@@ -263,26 +284,8 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           }
         }
       }
-      const float base = m == -INFINITY ? 0.f : m;
-      const float2 mult = both(to_log2), minus = both(-base);
-      float2 part[4], part_rounded[4];
-#pragma unroll
-      for (int k = 0; k < 4; k++) part[k] = part_rounded[k] = both(0.f);
-#pragma unroll
-      for (int c = 0; c < 2; c++) {
-        uint32_t packed[32];
-#pragma unroll
-        for (int e = 0; e < 32; e++) {
-          const float2 v = make_float2(__uint_as_float(raw[2 * c + e / 16][2 * (e % 16)]),
-                                       __uint_as_float(raw[2 * c + e / 16][2 * (e % 16) + 1]));
-          const float2 y = kRaw ? fma2(v, mult, minus) : add2(v, minus);
-          const float2 p = make_float2(ex2(y.x), ex2(y.y));
-          packed[e] = pack_bf16(p.x, p.y);
-          part[e % 4] = add2(part[e % 4], p);
-          part_rounded[e % 4] = add2(part_rounded[e % 4], make_float2(__uint_as_float(packed[e] << 16), __uint_as_float(packed[e] & 0xffff0000u)));
-        }
-        tmem_store32(s_at + c * 32, packed);
-      }
+      tmem_store32(s_at, packed[0]);
+      tmem_store32(s_at + 32, packed[1]);
       part[0] = add2(add2(part[0], part[1]), add2(part[2], part[3]));
       part_rounded[0] = add2(add2(part_rounded[0], part_rounded[1]), add2(part_rounded[2], part_rounded[3]));
       sum += part[0].x + part[0].y;
@@ -337,7 +340,7 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           for (int c = 0; c < NB; c++)
             tma_load_rows(smem + (t * NB + c) * kBlockBytes, &maps.q, &q_full, c * kBlockCols, row0 + t * kTileRows, h, b);
         int it = 0;
-        for (int n = 0; n < n_tiles; n++) {
+        for (int n = n_tiles - 1; n >= 0; n--) {
           if (!flags[n]) continue;
           const int s = it % ST;
           const unsigned use = it / ST;
@@ -366,60 +369,74 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         }
       }
     } else if (warp == kMmaWarp) {
-      if (lane == 0) {
-        const int k_steps = (a.dim + 15) / 16, n_cols = k_steps * 16;
-        const uint32_t idesc_s = mma_desc(kTileRows, false), idesc_o = mma_desc(n_cols, true);
-        const uint32_t qa = smem_u32(smem), ka = smem_u32(ks), va = smem_u32(vs);
-        bool pending[2] = {false, false}, started[2] = {false, false};
-        unsigned p_phase[2] = {0, 0};
-        auto issue_pv = [&](int t, int s) {  // O_t += P_t V(stage s)
-          mbar_wait(&p_full[t], p_phase[t], dead, timeouts);
-          p_phase[t] ^= 1;
-          tc_fence_after();
-          const uint64_t vd = desc_mn_major(va + s * Shape::kTileBytes, kBlockBytes);
+      const int k_steps = (a.dim + 15) / 16, n_cols = k_steps * 16;
+      const uint32_t idesc_s = mma_desc(kTileRows, false), idesc_o = mma_desc(n_cols, true);
+      const uint64_t q_desc = desc_k_major(smem_u32(smem)), k_desc = desc_k_major(smem_u32(ks));
+      const uint64_t v_desc = desc_mn_major(smem_u32(vs), kBlockBytes);
+      constexpr uint32_t kTileStep = Shape::kTileBytes >> 4;  // in descriptor units
+      bool pending[2] = {false, false}, started[2] = {false, false};
+      unsigned p_phase[2] = {0, 0};
+      auto issue_pv = [&](int t, int s) {  // O_t += P_t V(stage s)
+        mbar_wait(&p_full[t], p_phase[t], dead, timeouts);
+        p_phase[t] ^= 1;
+        tc_fence_after();
+        const uint64_t vd = v_desc + s * kTileStep;
+        if (elect_lane()) {
+#pragma unroll
           for (int k = 0; k < kTileRows / 16; k++)
             mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, vd + k * (2048 >> 4), idesc_o, started[t] || k > 0);
-          started[t] = true;
-          pending[t] = false;
-        };
-        mbar_wait(&q_full, 0, dead, timeouts);
-        int it = 0;
-        for (int n = 0; n < n_tiles; n++) {
-          const int f = flags[n];
-          if (!f) continue;
-          const int s = it % ST, before = (it + ST - 1) % ST;
-          mbar_wait(&k_full[s], (it / ST) & 1, dead, timeouts);
-          if (it > 0) mbar_wait(&v_full[before], ((it - 1) / ST) & 1, dead, timeouts);
-          for (int t = 0; t < 2; t++) {
-            if (pending[t]) issue_pv(t, before);
-            if (f >> (2 * t) & 1) {
-              const uint64_t qd = desc_k_major(qa + t * Shape::kTileBytes), kd = desc_k_major(ka + s * Shape::kTileBytes);
-              for (int k = 0; k < k_steps; k++) {
+        }
+        __syncwarp();
+        started[t] = true;
+        pending[t] = false;
+      };
+      auto commit = [&](uint64_t *bar) {
+        if (elect_lane()) tc_commit(bar);
+        __syncwarp();
+      };
+      mbar_wait(&q_full, 0, dead, timeouts);
+      int it = 0;
+      for (int n = n_tiles - 1; n >= 0; n--) {
+        const int f = flags[n];
+        if (!f) continue;
+        const int s = it % ST, before = (it + ST - 1) % ST;
+        mbar_wait(&k_full[s], (it / ST) & 1, dead, timeouts);
+        if (it > 0) mbar_wait(&v_full[before], ((it - 1) / ST) & 1, dead, timeouts);
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+          if (pending[t]) issue_pv(t, before);
+          if (f >> (2 * t) & 1) {
+            const uint64_t qd = q_desc + t * kTileStep, kd = k_desc + s * kTileStep;
+            if (elect_lane()) {
+#pragma unroll
+              for (int k = 0; k < NB * 4; k++) {
                 const int at = (k / 4) * (kBlockBytes >> 4) + (k % 4) * 2;
-                mma_ss(tmem + t * 128, qd + at, kd + at, idesc_s, k > 0);
+                if (k < k_steps) mma_ss(tmem + t * 128, qd + at, kd + at, idesc_s, k > 0);
               }
               tc_commit(&s_full[t]);
-              pending[t] = true;
             }
-          }
-          tc_commit(&k_empty[s]);
-          if (it > 0) tc_commit(&v_empty[before]);
-          it++;
-        }
-        if (it > 0) {
-          const int s = (it - 1) % ST;
-          mbar_wait(&v_full[s], ((it - 1) / ST) & 1, dead, timeouts);
-          for (int t = 0; t < 2; t++) {
-            if (pending[t]) issue_pv(t, s);
-            if (started[t]) tc_commit(&o_full[t]);
+            __syncwarp();
+            pending[t] = true;
           }
         }
-        if (*dead) {
-          tc_commit(&drain);
-          drain_wait(&drain, 0);
+        commit(&k_empty[s]);
+        if (it > 0) commit(&v_empty[before]);
+        it++;
+      }
+      if (it > 0) {
+        const int s = (it - 1) % ST;
+        mbar_wait(&v_full[s], ((it - 1) / ST) & 1, dead, timeouts);
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+          if (pending[t]) issue_pv(t, s);
+          if (started[t]) commit(&o_full[t]);
         }
       }
+      if (*dead) {
+        commit(&drain);
+        drain_wait(&drain, 0);
       }
+    }
   }
   __syncthreads();
   if (warp == kMmaWarp) {

@@ -88,6 +88,15 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       : "memory");
 }
 
+// One lane of a converged warp.  Issuing warps stay converged and elect the lane only around the
+// products, so that addresses and descriptors live in uniform registers: with a lane that runs alone
+// they are moved there one by one, which costs several times the product's own issue.
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(yes)::"memory");
+  return yes != 0;
+}
+
 #define DLB_R4(m, r, i) m(r[i]), m(r[i + 1]), m(r[i + 2]), m(r[i + 3])
 #define DLB_R16(m, r, i) DLB_R4(m, r, i), DLB_R4(m, r, i + 4), DLB_R4(m, r, i + 8), DLB_R4(m, r, i + 12)
 #define DLB_OUT(x) "=r"(x)
