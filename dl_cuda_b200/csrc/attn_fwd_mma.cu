@@ -1,8 +1,8 @@
 // Attention forward on the tensor cores (bf16).
 //
 // A CTA owns two tiles of 128 queries of one head and walks over the tiles of 128 keys that any of
-// them sees.  Eight softmax warps and two more: one thread copies K and V tiles into a ring (TMA), one issues the products,
-// and each query tile has four warps for its softmax, one thread per row:
+// them sees.  One warp copies K and V tiles into a ring (TMA), one issues the products, and each
+// query tile has eight warps for its softmax:
 //     S = Q K^T (TMEM, fp32) -> scores, running maximum, P = 2^(s - m) (bf16, written over S) -> O += P V
 // The two query tiles take turns: while one's softmax runs, the other's products do.  O stays in TMEM.
 // Exponentials are taken against a reference that moves only when a score leaves its range of 2^32, so
@@ -18,14 +18,17 @@
 namespace dlb {
 namespace {
 
-constexpr int kFwdThreads = 384, kMmaWarp = 9, kLoadWarp = 8;
-// Registers: launched with 168 each (384 * 168 = 64512); the eight softmax warps go up to 208, the four
-// others down to 88 (256 * 208 + 128 * 88 = 64512).
+// Eight softmax warps per query tile: a row belongs to two threads, 64 of a tile's 128 keys each.  (With
+// one thread a row, two warps a scheduler, nothing covered the latencies: 288 instead of 272 us
+// for 4096 x 4096 tokens, 32 heads of 128.)
+constexpr int kLoadWarp = 16, kMmaWarp = 17, kFwdThreads = 640, kHalf = kTileRows / 2;
+// Registers: launched with 96 each (640 * 96 = 61440); the softmax warps go up to 104, the four others
+// down to 64 (512 * 104 + 128 * 64 = 61440).
+constexpr int kSoftmaxRegs = 104, kOtherRegs = 64;
 // A row's exponentials are taken against a reference m that its scores (in powers of two) have to stay
 // within 2^32 of from above; fp32 sums and bf16 probabilities bear that with room to spare, and the
 // reference divides out.  It starts at 0, which serves most rows from end to end.
 constexpr float kReach = 32.f;
-constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 
 template <int NB>
 struct FwdShape {
@@ -38,6 +41,17 @@ struct FwdShape {
 struct FwdMaps {
   CUtensorMap q, k, v;
 };
+
+// Barrier of a query tile's 256 softmax threads that also tells whether any of them says yes.
+__device__ __forceinline__ bool any_of_group(int id, bool yes) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbarrier.cta.red.or.pred q, %1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(id), "r"(static_cast<uint32_t>(yes))
+      : "memory");
+  return any != 0;
+}
 
 template <int NB, bool CAP, int BIAS>
 __global__ void __launch_bounds__(kFwdThreads, 1)
@@ -54,6 +68,7 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   __shared__ int dead_flag;
   __shared__ int doc_range[4];
   __shared__ __align__(16) int doc_tile[2][kTileRows];
+  __shared__ float redo_top[2][2][kTileRows], redo_sum[2][2][kTileRows];  // [query tile][half][row]
   volatile int *dead = &dead_flag;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -67,7 +82,7 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     }
     for (int t = 0; t < 2; t++) {
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 4);
+      mbar_init(&p_full[t], 8);
       mbar_init(&o_full[t], 1);
     }
     mbar_init(&drain, 1);
@@ -151,105 +166,111 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 
   if (warp < kLoadWarp) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    const int t = warp >> 2, i = row0 + t * kTileRows + (tid & 127);
+    const int t = warp >> 3, half = warp >> 2 & 1, row = (warp & 3) * 32 + lane, i = row0 + t * kTileRows + row;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lane_base + t * 128, o_at = tmem + lane_base + 256 + t * 128;
+    const uint32_t s_at = tmem + lane_base + t * 128 + half * kHalf;  // this thread's scores
+    const uint32_t p_at = tmem + lane_base + t * 128 + half * (kHalf / 2), o_at = tmem + lane_base + 256 + t * 128;
     const bool valid = i < a.q_len;
     const int end = valid ? row_end(a, view, i) : 0, pos = view.start + i;
     const int doc = (a.q_docs && valid) ? ld_co(a.q_docs + static_cast<long long>(b) * a.q_len + i) : 0;
     const float slope = (BIAS != kNoBias && a.slopes) ? ld_co(a.slopes + h) * kLog2e : 0.f;
     const float to_log2 = CAP ? 1.f : a.scale * kLog2e;
     const CapCoef cap = CAP ? cap_coef(a.scale, a.cap) : CapCoef();
-    constexpr bool kRaw = !CAP && BIAS == kNoBias;  // maximum and exponent from the products themselves
+    constexpr bool kRaw = !CAP && BIAS == kNoBias;  // the exponent straight from the products
     const int tail = view.end % kTileRows && view.end < a.kv_len ? view.end / kTileRows : -1;
+
+    // Scores of 32 keys from j1 on, masked; times to_log2 still to come when kRaw.
+    auto scores = [&](float (&x)[32], int c, int j1, bool whole) {
+      uint32_t raw[32];
+      tmem_load32(s_at + c * 32, raw);
+      tmem_loaded(raw);
+#pragma unroll
+      for (int e = 0; e < 32; e++) x[e] = __uint_as_float(raw[e]);
+      if (CAP) cap_scores(x, cap);
+      if (BIAS != kNoBias) {
+        const int d0 = j1 - pos;
+        const float d = static_cast<float>(d0);
+        const bool slopes = BIAS == kSlope || a.slopes;
+        bool far = true;
+        const float *at = lut + d0 + a.reach + kLutPad;
+        float base = 0.f;
+        if (BIAS == kTable) {
+          // Either the warp's pairs are all beyond the reach, or all within 31 + 31 of it on either side,
+          // where the padded table covers every index.
+          const bool left = d0 + 31 <= -a.reach, right = d0 >= a.reach;
+          far = __all_sync(0xffffffffu, left || right);
+          if (far) base = left ? lut[0] : lut[2 * (a.reach + kLutPad)];
+        }
+        if (far && !slopes) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float2 y = fma2(make_float2(x[e], x[e + 1]), both(to_log2), both(base));
+            x[e] = y.x;
+            x[e + 1] = y.y;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float2 bias = BIAS == kTable && !far ? make_float2(at[e], at[e + 1]) : both(base);
+            if (slopes) {
+              bias.x = fmaf(-slope, fabsf(d + static_cast<float>(e)), bias.x);
+              bias.y = fmaf(-slope, fabsf(d + static_cast<float>(e + 1)), bias.y);
+            }
+            const float2 y = fma2(make_float2(x[e], x[e + 1]), both(to_log2), bias);
+            x[e] = y.x;
+            x[e + 1] = y.y;
+          }
+        }
+      }
+      if (!whole) {
+        const int room = end - j1;
+        if (a.kv_docs) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const int4 k = *reinterpret_cast<const int4 *>(&doc_tile[t][half * kHalf + c * 32 + e]);
+            x[e] = k.x == doc ? x[e] : -INFINITY;
+            x[e + 1] = k.y == doc ? x[e + 1] : -INFINITY;
+            x[e + 2] = k.z == doc ? x[e + 2] : -INFINITY;
+            x[e + 3] = k.w == doc ? x[e + 3] : -INFINITY;
+          }
+        }
+        if (room < 32) {
+#pragma unroll
+          for (int e = 0; e < 32; e++) x[e] = e < room ? x[e] : -INFINITY;
+        }
+      }
+    };
+
     float m = 0.f, sum = 0.f, sum_rounded = 0.f;
+    bool settled = false;  // the row has weight, or a reference of its own
     int it = -1, done = 0;
     for (int n = n_tiles - 1; n >= 0; n--) {
       const int f = flags[n];
       if (!f) continue;
       it++;
       if (!(f >> (2 * t) & 1)) continue;
-      const int j0 = n * kTileRows;
+      const int j0 = n * kTileRows, j1 = j0 + half * kHalf;
       const bool whole = f >> (2 * t + 1) & 1;
       int key_doc = 0;
-      if (!whole && a.kv_docs) key_doc = ld_co(a.kv_docs + static_cast<long long>(b) * a.kv_len + min(j0 + (tid & 127), a.kv_len - 1));
+      if (!whole && a.kv_docs && half == 0)
+        key_doc = ld_co(a.kv_docs + static_cast<long long>(b) * a.kv_len + min(j0 + row, a.kv_len - 1));
       mbar_wait(&s_full[t], done & 1, dead, timeouts);
-      if (!whole && a.kv_docs) {  // the group's document numbers of this tile
-        named_bar_sync(2 + t, 128);
-        doc_tile[t][tid & 127] = key_doc;
-        named_bar_sync(2 + t, 128);
+      if (!whole && a.kv_docs) {  // the tile's document numbers; the last use of the old ones lies behind a barrier
+        if (half == 0) doc_tile[t][row] = key_doc;
+        named_bar_sync(2 + t, 256);
       }
       tc_fence_after();
-      // One pass over the scores against the reference m, which the keys so far fit; only if one does not
-      // is m moved (and what has been summed rescaled) and the pass repeated.  P stays in registers until
-      // then: it is written over the scores.
-      uint32_t packed[2][32];
-      float2 part[4], part_rounded[4];
-      for (int pass = 0; pass < 2; pass++) {
-        float top = -INFINITY;
+      // One pass over the scores against the reference, which the keys so far fit.  Only if some row's
+      // sum says that it does not (too large, or nothing left of visible keys) the maximum is taken, the
+      // reference moved, what has been summed rescaled, and the pass repeated.
+      uint32_t packed[32];
+      float2 part, part_rounded;
+      for (int pass = 0;; pass++) {
+        float2 l[2] = {both(0.f), both(0.f)}, r[2] = {both(0.f), both(0.f)};
 #pragma unroll
-        for (int k = 0; k < 4; k++) part[k] = part_rounded[k] = both(0.f);
-        uint32_t raw[2][32];
-        tmem_load32(s_at, raw[0]);
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-          tmem_loaded(raw[c & 1]);
-          if (c < 3) tmem_load32(s_at + (c + 1) * 32, raw[(c + 1) & 1]);
+        for (int c = 0; c < 2; c++) {
           float x[32];
-#pragma unroll
-          for (int e = 0; e < 32; e++) x[e] = __uint_as_float(raw[c & 1][e]);
-          if (CAP) cap_scores(x, cap);
-          if (BIAS != kNoBias) {
-            const float2 k2 = both(to_log2);
-            const int d0 = j0 + c * 32 - pos;
-            {
-              float bias[32];
-#pragma unroll
-              for (int e = 0; e < 32; e++) bias[e] = 0.f;
-              if (BIAS == kTable) {
-                const bool left = d0 + 31 <= -a.reach, right = d0 >= a.reach;
-                if (__all_sync(0xffffffffu, left || right)) {
-                  const float far = left ? lut[0] : lut[2 * (a.reach + kLutPad)];
-#pragma unroll
-                  for (int e = 0; e < 32; e++) bias[e] = far;
-                } else {
-                  // within 31 + 31 of the reach on either side: the padded table covers every index
-                  const float *at = lut + d0 + a.reach + kLutPad;
-#pragma unroll
-                  for (int e = 0; e < 32; e++) bias[e] = at[e];
-                }
-              }
-              if (BIAS == kSlope || a.slopes) {
-                const float d = static_cast<float>(d0);
-#pragma unroll
-                for (int e = 0; e < 32; e++) bias[e] = fmaf(-slope, fabsf(d + static_cast<float>(e)), bias[e]);
-              }
-#pragma unroll
-              for (int e = 0; e < 32; e += 2) {
-                const float2 y = fma2(make_float2(x[e], x[e + 1]), k2, make_float2(bias[e], bias[e + 1]));
-                x[e] = y.x;
-                x[e + 1] = y.y;
-              }
-            }
-          }
-          if (!whole) {
-            const int room = end - (j0 + c * 32);
-            if (a.kv_docs) {
-#pragma unroll
-              for (int e = 0; e < 32; e += 4) {
-                const int4 d = *reinterpret_cast<const int4 *>(&doc_tile[t][c * 32 + e]);
-                x[e] = d.x == doc ? x[e] : -INFINITY;
-                x[e + 1] = d.y == doc ? x[e + 1] : -INFINITY;
-                x[e + 2] = d.z == doc ? x[e + 2] : -INFINITY;
-                x[e + 3] = d.w == doc ? x[e + 3] : -INFINITY;
-              }
-            }
-            if (!a.kv_docs || room < 32) {
-#pragma unroll
-              for (int e = 0; e < 32; e++) x[e] = e < room ? x[e] : -INFINITY;
-            }
-          }
-top = fmaxf(top, max_of<32, false>(x));
+          scores(x, c, j1 + c * 32, whole);
           const float2 minus = both(-m);
 #pragma unroll
           for (int e = 0; e < 16; e++) {
@@ -257,20 +278,38 @@ top = fmaxf(top, max_of<32, false>(x));
             const float2 y = kRaw ? fma2(v, both(to_log2), minus) : add2(v, minus);
             const float2 p = make_float2(ex2(y.x), ex2(y.y));
             const uint32_t w = pack_bf16(p.x, p.y);
-            packed[c / 2][(c & 1) * 16 + e] = w;
-            part[e % 4] = add2(part[e % 4], p);
-            part_rounded[e % 4] = add2(part_rounded[e % 4], make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)));
+            packed[c * 16 + e] = w;
+            l[e & 1] = add2(l[e & 1], p);
+            r[e & 1] = add2(r[e & 1], make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)));
           }
         }
+        part = add2(l[0], l[1]);
+        part_rounded = add2(r[0], r[1]);
+        const float total = part.x + part.y;
+        if (total > 0.f) settled = true;
+        const bool misfit = !(total <= 4294967296.f) || (!settled && total == 0.f && end > j1);
+        if (!any_of_group(4 + t, misfit) || pass == 1) break;
+        float top = -INFINITY;
+        for (int c = 0; c < 2; c++) {
+          float x[32];
+          scores(x, c, j1 + c * 32, whole);
+          top = fmaxf(top, max_of<32, false>(x));
+        }
         if (kRaw) top *= to_log2;
-        const bool above = top > m + kReach, below = sum == 0.f && top < m - kReach && top > -INFINITY;
-        if (!__any_sync(0xffffffffu, above || below)) break;
+        redo_top[t][half][row] = top;
+        redo_sum[t][half][row] = sum;
+        named_bar_sync(2 + t, 256);
+        top = fmaxf(top, redo_top[t][half ^ 1][row]);
+        const float row_sum = sum + redo_sum[t][half ^ 1][row];
+        named_bar_sync(2 + t, 256);
+        const bool above = top > m + kReach, below = row_sum == 0.f && top < m - kReach && top > -INFINITY;
         const float keep = above ? ex2(m - top) : below ? 0.f : 1.f;
         if (above || below) m = top;
+        settled = settled || row_sum > 0.f || top > -INFINITY;
         sum *= keep;
         sum_rounded *= keep;
         if (done > 0) {
-          for (int c = 0; c < a.dim; c += 32) {
+          for (int c = half * 32; c < a.dim; c += 64) {
             uint32_t o[32];
             tmem_load32(o_at + c, o);
             tmem_loaded(o);
@@ -284,18 +323,16 @@ top = fmaxf(top, max_of<32, false>(x));
           }
         }
       }
-      tmem_store32(s_at, packed[0]);
-      tmem_store32(s_at + 32, packed[1]);
-      part[0] = add2(add2(part[0], part[1]), add2(part[2], part[3]));
-      part_rounded[0] = add2(add2(part_rounded[0], part_rounded[1]), add2(part_rounded[2], part_rounded[3]));
-      sum += part[0].x + part[0].y;
-      sum_rounded += part_rounded[0].x + part_rounded[0].y;
+      // All of the tile's scores have been read (any_of_group is a barrier): P may go over them.
+      tmem_store32(p_at, packed);
+      sum += part.x + part.y;
+      sum_rounded += part_rounded.x + part_rounded.y;
       if (n == tail) {
         // Rows of V behind the last key any query reaches may hold anything, and 0 * NaN is NaN.
         const int s = it % ST;
         mbar_wait(&v_full[s], (it / ST) & 1, dead, timeouts);
         const int from = view.end - j0;
-        for (int e = tid & 127; e < (kTileRows - from) * NB * 8; e += 128) {
+        for (int e = half * 128 + row; e < (kTileRows - from) * NB * 8; e += 256) {
           const int r = from + e / (NB * 8), x = e % (NB * 8);
           *reinterpret_cast<uint4 *>(vs + s * Shape::kTileBytes + (x / 8) * kBlockBytes + r * 128 + (x % 8) * 16) =
               make_uint4(0, 0, 0, 0);
@@ -308,11 +345,16 @@ top = fmaxf(top, max_of<32, false>(x));
       if (lane == 0) mbar_arrive(&p_full[t]);
       done++;
     }
+    redo_top[t][half][row] = sum_rounded;
+    redo_sum[t][half][row] = sum;
+    named_bar_sync(2 + t, 256);
+    sum += redo_sum[t][half ^ 1][row];
+    sum_rounded += redo_top[t][half ^ 1][row];
     if (done > 0) mbar_wait(&o_full[t], 0, dead, timeouts);
     tc_fence_after();
     const float inv = sum_rounded > 0.f || sum_rounded != sum_rounded ? 1.f / sum_rounded : 0.f;
     __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(a.o.ptr) + b * a.o.batch + static_cast<long long>(i) * a.o.token + h * a.o.head;
-    for (int c = 0; c < a.dim; c += 32) {
+    for (int c = half * 32; c < a.dim; c += 64) {
       uint32_t o[32];
       if (done > 0) {
         tmem_load32(o_at + c, o);
@@ -327,7 +369,7 @@ top = fmaxf(top, max_of<32, false>(x));
         if (valid && c + e < a.dim) *reinterpret_cast<uint4 *>(out + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
-    if (a.lse && valid)
+    if (a.lse && valid && half == 0)
       a.lse[(static_cast<size_t>(b) * a.heads + h) * a.q_len + i] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
     tc_fence_before();
   } else {
