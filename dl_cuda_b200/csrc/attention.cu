@@ -1,5 +1,6 @@
 // Entry points of the attention operators: argument checks, the choice between the kernels, and the
-// workspace layout.  The kernels: attn_generic.cuh (fp32 pipes, everything).
+// workspace layout.  The kernels: attn_generic.cuh (fp32 arithmetic, any layout),
+// attn_fwd_mma.cu and attn_bwd_mma.cuh (bf16, whole sequences), attn_step.cu (bf16, few queries).
 #include <algorithm>
 #include <type_traits>
 
@@ -100,17 +101,26 @@ bool vector_rows(const Heads &h, int dim, int esize) {
   return aligned16(h.ptr) && dim % v == 0 && h.batch % v == 0 && h.token % v == 0 && h.head % v == 0;
 }
 
+// Head width, in the blocks of 32 columns that the fp32-arithmetic kernels are built for.
 template <typename F>
 auto by_width(int dim, F &&f) {
-  if (dim <= 16) return f(std::integral_constant<int, 16>());
   if (dim <= 32) return f(std::integral_constant<int, 32>());
   if (dim <= 64) return f(std::integral_constant<int, 64>());
+  if (dim <= 96) return f(std::integral_constant<int, 96>());
   return f(std::integral_constant<int, 128>());
 }
+// Groups of 16 rows per CTA.
+template <typename F>
+auto by_row_groups(int groups, F &&f) {
+  if (groups == 1) return f(std::integral_constant<int, 1>());
+  if (groups == 2) return f(std::integral_constant<int, 2>());
+  return f(std::integral_constant<int, 4>());
+}
 
-// Lets a kernel use `smem` bytes of dynamic shared memory.
+// Lets a kernel use `smem` bytes of dynamic shared memory (48 KB with the static are free to all).
 template <typename K>
 int allow_smem(K kern, size_t smem, const char *name) {
+  if (smem <= 40 * 1024) return DLB_OK;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   DLB_REQUIRE(e == cudaSuccess, DLB_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
   return DLB_OK;
@@ -124,12 +134,12 @@ enum FwdKind { kGeneric, kMma, kStep };
 
 struct FwdPlan {
   FwdKind kind;
-  int pack, splits;
+  int pack, splits, row_groups;
   size_t bytes;
 };
 
 FwdPlan plan_fwd(const dlb_attn *a, const AttnArgs &args) {
-  FwdPlan p = {kGeneric, 1, 1, 0};
+  FwdPlan p = {kGeneric, 1, 1, 4, 0};
   const int group = a->heads / a->kv_heads;
   if (a->dtype == DLB_BF16 && attn_mma_fits(args, false)) p.kind = a->q_len >= kMmaQueries ? kMma : kStep;
   if (p.kind == kMma) return p;
@@ -138,10 +148,11 @@ FwdPlan plan_fwd(const dlb_attn *a, const AttnArgs &args) {
   } else {
     // Few queries: the heads that share a key/value head go into one tile, and the keys are split until
     // the grid fills the GPU twice (a share keeps at least two tiles).
-    if (static_cast<long long>(a->q_len) * group <= kGenTile) p.pack = group;
-    const long long ctas = static_cast<long long>(a->batch) * (a->heads / p.pack) *
-                           ceil_div(static_cast<long long>(a->q_len) * p.pack, static_cast<long long>(kGenTile));
-    const int key_tiles = ceil_div(a->kv_len, kGenTile);
+    if (static_cast<long long>(a->q_len) * group <= 64) p.pack = group;
+    const long long rows = static_cast<long long>(a->q_len) * p.pack, units = static_cast<long long>(a->batch) * (a->heads / p.pack);
+    p.row_groups = rows <= 16 ? 1 : rows <= 32 || units * ceil_div(rows, 64ll) < 4 * sm_count() ? 2 : 4;
+    const long long ctas = units * ceil_div(rows, 16ll * p.row_groups);
+    const int key_tiles = ceil_div(a->kv_len, kGenCols);
     if (ctas > 0 && ctas < sm_count())
       p.splits = static_cast<int>(std::max(1ll, std::min({2ll * sm_count() / ctas, key_tiles / 2ll,
                                                           static_cast<long long>(kMaxSplits)})));
@@ -164,15 +175,17 @@ int launch_join(const AttnArgs &p, cudaStream_t st) {
 template <typename T>
 int launch_fwd(AttnArgs p, const FwdPlan &plan, cudaStream_t st) {
   const bool vec = vector_rows(p.q, p.dim, sizeof(T)) && vector_rows(p.k, p.dim, sizeof(T)) && vector_rows(p.v, p.dim, sizeof(T));
-  const int tiles = ceil_div(p.q_len * plan.pack, kGenTile);
   const int rc = by_width(p.dim, [&](auto width) -> int {
-    constexpr int DP = decltype(width)::value;
-    const size_t smem = sizeof(float) * (3 * kGenTile * (DP + 4) + kGenTile * kGenScoreStride);
-    auto kern = attn_fwd_generic_kernel<T, DP>;
-    if (int s = allow_smem(kern, smem, "attn_fwd")) return s;
-    launch_pdl(kern, dim3(tiles * (p.heads / plan.pack) * p.batch, plan.splits), dim3(kGenThreads), smem, st, p, plan.pack, vec);
-    DLB_LAUNCH_CHECK("attn_fwd_generic");
-    return DLB_OK;
+    return by_row_groups(plan.row_groups, [&](auto groups) -> int {
+      constexpr int DP = decltype(width)::value, RG = decltype(groups)::value;
+      const size_t smem = gen_fwd_smem<DP, RG>();
+      auto kern = attn_fwd_generic_kernel<T, DP, RG>;
+      if (int s = allow_smem(kern, smem, "attn_fwd")) return s;
+      const int tiles = ceil_div(p.q_len * plan.pack, 16 * RG);
+      launch_pdl(kern, dim3(tiles * (p.heads / plan.pack) * p.batch, plan.splits), dim3(kGenThreads), smem, st, p, plan.pack, vec);
+      DLB_LAUNCH_CHECK("attn_fwd_generic");
+      return DLB_OK;
+    });
   });
   return rc != DLB_OK || plan.splits == 1 ? rc : launch_join<T>(p, st);
 }
@@ -185,10 +198,17 @@ struct BwdPlan {
 BwdPlan plan_bwd(const dlb_attn *a, const dlb_attn_grad *g) {
   BwdPlan p;
   p.stats_bytes = static_cast<size_t>(a->batch) * a->heads * stat_tiles(a->q_len) * 2 * kStatRows * sizeof(float);
-  p.parts = a->batch * ceil_div(a->q_len, kGenTile);
+  p.parts = a->batch * ceil_div(a->q_len, 32);  // of the smallest tiles that any kernel uses
   p.bytes = p.stats_bytes;
   if (g->dtable && a->table) p.bytes += sizeof(float) * static_cast<size_t>(a->heads) * p.parts * a->buckets;
   return p;
+}
+
+int launch_table_sum(const AttnArgs &p, cudaStream_t st) {
+  if (!p.dtable) return DLB_OK;
+  launch_pdl(attn_table_sum_kernel, dim3(p.heads * p.buckets), dim3(128), 0, st, p);
+  DLB_LAUNCH_CHECK("attn_table_sum");
+  return DLB_OK;
 }
 
 template <typename T>
@@ -202,25 +222,32 @@ int launch_bwd(const AttnArgs &p, bool mma, cudaStream_t st) {
   }
   if (mma) {
     if (int s = attn_bwd_mma_keys(p, st)) return s;
-    return attn_bwd_mma_queries(p, st);
+    if (int s = attn_bwd_mma_queries(p, st)) return s;
+    return launch_table_sum(p, st);
   }
   return by_width(p.dim, [&](auto width) -> int {
-    constexpr int DP = decltype(width)::value;
-    const size_t smem = sizeof(float) * (4 * kGenTile * (DP + 4) + 2 * kGenTile * kGenScoreStride);
-    if (p.kv_len > 0) {
-      auto kern = attn_bwd_generic_kernel<T, DP, true>;
+    // 64-row tiles where they fill the GPU twice, else 32-row ones
+    auto blocks = [&](int rows, bool keys) {
+      return (keys ? ceil_div(p.kv_len, rows) * p.kv_heads : ceil_div(p.q_len, rows) * p.heads) * p.batch;
+    };
+    const bool fill = blocks(64, true) + blocks(64, false) >= 2 * sm_count() && blocks(64, true) >= sm_count();
+    // (the sums of more than 32 buckets do not fit beside the widest 64-row tiles)
+    const int groups = fill && !(p.dtable && p.buckets > 32 && p.dim > 64) ? 4 : 2;
+    auto launch = [&](auto row_groups) -> int {
+      constexpr int DP = decltype(width)::value, RG = decltype(row_groups)::value;
+      AttnArgs args = p;
+      args.table_parts = p.batch * ceil_div(p.q_len, 16 * RG);
+      const size_t smem = gen_bwd_smem<DP, RG>() + gen_table_bytes<RG>(p);
+      auto kern = attn_bwd_generic_kernel<T, DP, RG>;
       if (int s = allow_smem(kern, smem, "attn_bwd")) return s;
-      launch_pdl(kern, dim3(ceil_div(p.kv_len, kGenTile) * p.kv_heads * p.batch), dim3(kGenThreads), smem, st, p, vec);
-      DLB_LAUNCH_CHECK("attn_bwd_generic");
-    }
-    if (p.q_len > 0) {
-      auto kern = attn_bwd_generic_kernel<T, DP, false>;
-      const size_t more = p.dtable ? sizeof(float) * 2 * p.buckets * kGenTile : 0;
-      if (int s = allow_smem(kern, smem + more, "attn_bwd")) return s;
-      launch_pdl(kern, dim3(ceil_div(p.q_len, kGenTile) * p.heads * p.batch), dim3(kGenThreads), smem + more, st, p, vec);
-      DLB_LAUNCH_CHECK("attn_bwd_generic");
-    }
-    return DLB_OK;
+      const int key_blocks = blocks(16 * RG, true), all = key_blocks + blocks(16 * RG, false);
+      if (all > 0) {
+        launch_pdl(kern, dim3(all), dim3(kGenThreads), smem, st, args, vec, key_blocks);
+        DLB_LAUNCH_CHECK("attn_bwd_generic");
+      }
+      return launch_table_sum(args, st);
+    };
+    return groups == 4 ? launch(std::integral_constant<int, 4>()) : launch(std::integral_constant<int, 2>());
   });
 }
 
@@ -293,15 +320,8 @@ extern "C" int dlb_attn_bwd(const dlb_attn *a, const dlb_attn_grad *g, void *wor
   p.table_part = reinterpret_cast<float *>(static_cast<char *>(workspace) + plan.stats_bytes);
   p.table_parts = plan.parts;
   cudaStream_t st = as_stream(stream);
-  if (a->batch > 0) {
-    const bool mma = a->dtype == DLB_BF16 && attn_mma_fits(p, true) && attn_bwd_mma_room(p);
-    if (mma) p.table_parts = a->batch * ceil_div(a->q_len, kTileRows);
-    const int rc = a->dtype == DLB_F32 ? launch_bwd<float>(p, false, st) : launch_bwd<__nv_bfloat16>(p, mma, st);
-    if (rc != DLB_OK) return rc;
-  }
-  if (p.dtable) {
-    launch_pdl(attn_table_sum_kernel, dim3(p.heads * p.buckets), dim3(128), 0, st, p);
-    DLB_LAUNCH_CHECK("attn_table_sum");
-  }
-  return DLB_OK;
+  const bool mma = a->dtype == DLB_BF16 && a->batch > 0 && attn_mma_fits(p, true) && attn_bwd_mma_room(p);
+  if (mma) p.table_parts = a->batch * ceil_div(a->q_len, kTileRows);
+  return a->dtype == DLB_F32 ? launch_bwd<float>(p, false, st) : launch_bwd<__nv_bfloat16>(p, mma, st);
 }
+
