@@ -24,68 +24,127 @@ __device__ __forceinline__ int bias_bucket(const BiasArgs &a, int distance) {
   return min(max(a.bucket_of[d], 0), a.buckets - 1);
 }
 
-// A CTA takes rows of one head and keeps that head's bias by distance in shared memory.
+// A row is taken by one warp, 16 bytes a lane and four such loads in flight; a row that starts off the
+// 16-byte grid (odd kv_len) has up to V - 1 single elements in front and behind.
 template <typename T>
-__global__ void __launch_bounds__(kBiasThreads) rel_bias_fwd_kernel(const __grid_constant__ BiasArgs a, int rows_per_cta, bool vec) {
+struct RowCut {
+  static constexpr int V = Store<T>::kPerVec;
+  int head, vectors, tail;  // elements in front, 16-byte vectors, elements behind
+  __device__ __forceinline__ RowCut(const T *row, int n, bool vec) {
+    head = vec ? min(n, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / static_cast<int>(sizeof(T))) : n;
+    vectors = (n - head) / V;
+    tail = n - head - vectors * V;
+  }
+};
+
+constexpr int kBiasRows = 32;  // rows of a CTA: four per warp
+
+template <typename T>
+__global__ void __launch_bounds__(kBiasThreads) rel_bias_fwd_kernel(const __grid_constant__ BiasArgs a, bool vec) {
   pdl_prologue();
   extern __shared__ float by_distance[];
-  const int row_tiles = (a.q_len + rows_per_cta - 1) / rows_per_cta;
+  constexpr int V = Store<T>::kPerVec, kInFlight = 4;
+  const int row_tiles = (a.q_len + kBiasRows - 1) / kBiasRows;
   const int tile = blockIdx.x % row_tiles, h = (blockIdx.x / row_tiles) % a.heads, b = blockIdx.x / (row_tiles * a.heads);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   for (int d = threadIdx.x; d <= 2 * a.reach; d += kBiasThreads)
     by_distance[d] = a.table[h * a.buckets + bias_bucket(a, d - a.reach)];
   __syncthreads();
-  const int i1 = min(a.q_len, (tile + 1) * rows_per_cta);
-  for (int i = tile * rows_per_cta; i < i1; i++) {
+  const int i1 = min(a.q_len, (tile + 1) * kBiasRows);
+  for (int i = tile * kBiasRows + warp; i < i1; i += kBiasThreads / 32) {
     const size_t row = (static_cast<size_t>(b) * a.heads + h) * a.q_len + i;
     const T *src = a.in ? static_cast<const T *>(a.in) + row * a.kv_len : nullptr;
     T *dst = static_cast<T *>(a.out) + row * a.kv_len;
-    const int shift = a.reach - (a.start + i);
-    if (vec) {
-      constexpr int V = Store<T>::kPerVec;
-      for (int j = threadIdx.x * V; j < a.kv_len; j += kBiasThreads * V) {
+    const int shift = a.reach - (a.start + i);  // by_distance of column j is at j + shift, within 0..2 reach
+    auto bias_at = [&](int j) { return by_distance[max(0, min(2 * a.reach, j + shift))]; };
+    const RowCut<T> cut(dst, a.kv_len, vec);
+    for (int e = lane; e < cut.head + cut.tail; e += 32) {
+      const int j = e < cut.head ? e : cut.vectors * V + e;
+      dst[j] = Store<T>::from_float((src ? Store<T>::to_float(ld_co(src + j)) : 0.f) + bias_at(j));
+    }
+    for (int v0 = lane; v0 < cut.vectors; v0 += 32 * kInFlight) {
+      uint4 x[kInFlight];
+#pragma unroll
+      for (int k = 0; k < kInFlight; k++) {
+        const int v = v0 + 32 * k;
+        x[k] = src && v < cut.vectors ? ld_stream(src + cut.head + v * V) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int k = 0; k < kInFlight; k++) {
+        const int v = v0 + 32 * k, j = cut.head + v * V;
+        if (v >= cut.vectors) break;
         float f[V];
+        Store<T>::unpack(x[k], f);
+        if (j + V - 1 + shift <= 0 || j + shift >= 2 * a.reach) {  // beyond the reach: one value
+          const float far = bias_at(j);
 #pragma unroll
-        for (int k = 0; k < V; k++) f[k] = 0.f;
-        if (src) Store<T>::unpack(ld_stream(src + j), f);
+          for (int e = 0; e < V; e++) f[e] += far;
+        } else {
 #pragma unroll
-        for (int k = 0; k < V; k++) f[k] += by_distance[max(0, min(2 * a.reach, j + k + shift))];
+          for (int e = 0; e < V; e++) f[e] += bias_at(j + e);
+        }
         st_stream(dst + j, Store<T>::pack(f));
       }
-    } else {
-      for (int j = threadIdx.x; j < a.kv_len; j += kBiasThreads)
-        dst[j] = Store<T>::from_float((src ? Store<T>::to_float(ld_co(src + j)) : 0.f) + by_distance[max(0, min(2 * a.reach, j + shift))]);
     }
   }
 }
 
-// part[h][cta][bucket]: a CTA takes rows of one head of all batches; every thread adds up runs of one
-// bucket in a register and keeps a column of its own per bucket in shared memory.
+// part[h][cta][bucket]: a CTA takes rows of one head of all batches.  What lies beyond the reach has one
+// bucket on either side and is summed in two registers; nearer elements go to a column of their own
+// thread per bucket in shared memory.
 template <typename T>
-__global__ void __launch_bounds__(kBiasThreads) rel_bias_bwd_kernel(const __grid_constant__ BiasArgs a, int parts) {
+__global__ void __launch_bounds__(kBiasThreads) rel_bias_bwd_kernel(const __grid_constant__ BiasArgs a, int parts, bool vec) {
   pdl_prologue();
-  extern __shared__ float sums[];  // [buckets][threads]
-  const int part = blockIdx.x % parts, h = blockIdx.x / parts, tid = threadIdx.x;
+  extern __shared__ float sums[];  // [buckets][threads], then the bucket of every distance
+  constexpr int V = Store<T>::kPerVec, kInFlight = 4, kWarps = kBiasThreads / 32;
+  unsigned char *bucket_lut = reinterpret_cast<unsigned char *>(sums + a.buckets * kBiasThreads);
+  const int part = blockIdx.x % parts, h = blockIdx.x / parts, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   for (int n = 0; n < a.buckets; n++) sums[n * kBiasThreads + tid] = 0.f;
+  for (int d = tid; d <= 2 * a.reach; d += kBiasThreads) bucket_lut[d] = static_cast<unsigned char>(bias_bucket(a, d - a.reach));
+  __syncthreads();
+  float left = 0.f, right = 0.f;
   const long long rows = static_cast<long long>(a.batch) * a.q_len;
-  for (long long r = part; r < rows; r += parts) {
+  for (long long r = static_cast<long long>(part) * kWarps + warp; r < rows; r += static_cast<long long>(parts) * kWarps) {
     const int b = r / a.q_len, i = r % a.q_len;
     const T *src = static_cast<const T *>(a.in) + ((static_cast<size_t>(b) * a.heads + h) * a.q_len + i) * a.kv_len;
-    int now = -1;
-    float sum = 0.f;
-    for (int j = tid; j < a.kv_len; j += kBiasThreads) {
-      const int n = bias_bucket(a, j - (a.start + i));
-      if (n != now) {
-        if (now >= 0) sums[now * kBiasThreads + tid] += sum;
-        now = n;
-        sum = 0.f;
-      }
-      sum += Store<T>::to_float(ld_co(src + j));
+    const int shift = a.reach - (a.start + i);
+    auto add = [&](int j, float x) { sums[bucket_lut[max(0, min(2 * a.reach, j + shift))] * kBiasThreads + tid] += x; };
+    const RowCut<T> cut(src, a.kv_len, vec);
+    for (int e = lane; e < cut.head + cut.tail; e += 32) {
+      const int j = e < cut.head ? e : cut.vectors * V + e;
+      add(j, Store<T>::to_float(ld_co(src + j)));
     }
-    if (now >= 0) sums[now * kBiasThreads + tid] += sum;
+    for (int v0 = lane; v0 < cut.vectors; v0 += 32 * kInFlight) {
+      uint4 x[kInFlight];
+#pragma unroll
+      for (int k = 0; k < kInFlight; k++) {
+        const int v = v0 + 32 * k;
+        x[k] = v < cut.vectors ? ld_stream(src + cut.head + v * V) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int k = 0; k < kInFlight; k++) {
+        const int v = v0 + 32 * k, j = cut.head + v * V;
+        if (v >= cut.vectors) break;
+        float f[V];
+        Store<T>::unpack(x[k], f);
+        const bool far_left = j + V - 1 + shift <= 0, far_right = j + shift >= 2 * a.reach;
+        if (far_left || far_right) {
+          float s = 0.f;
+#pragma unroll
+          for (int e = 0; e < V; e++) s += f[e];
+          if (far_left) left += s;
+          else right += s;
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; e++) add(j + e, f[e]);
+        }
+      }
+    }
   }
+  sums[bucket_lut[0] * kBiasThreads + tid] += left;
+  sums[bucket_lut[2 * a.reach] * kBiasThreads + tid] += right;
   __syncthreads();
-  const int warp = tid / 32, lane = tid & 31;
-  for (int n = warp; n < a.buckets; n += kBiasThreads / 32) {
+  for (int n = warp; n < a.buckets; n += kWarps) {
     float s = 0.f;
     for (int t = lane; t < kBiasThreads; t += 32) s += sums[n * kBiasThreads + t];
     s = warp_sum(s);
@@ -122,10 +181,17 @@ int check_shape(const char *call, int batch, int heads, int q_len, int kv_len, i
   return DLB_OK;
 }
 
-// Row groups of a head: enough CTAs for six per SM, at most one per row.
+// Row groups of a head: enough CTAs for six per SM, with a row for each warp.
 int bias_parts(int batch, int heads, int q_len) {
   const long long rows = static_cast<long long>(batch) * q_len;
-  return static_cast<int>(std::max(1ll, std::min<long long>(rows, ceil_div(6 * sm_count(), std::max(heads, 1)))));
+  return static_cast<int>(std::max(1ll, std::min<long long>(ceil_div(rows, 8ll), ceil_div(6 * sm_count(), std::max(heads, 1)))));
+}
+
+// Can 16-byte accesses be used between the ragged ends of rows?  Addresses on element boundaries, and the
+// same place within 16 bytes for what is read and written.
+bool rows_can_be_cut(const void *p, const void *q, int esize) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(q);
+  return x % esize == 0 && (y == 0 || x % 16 == y % 16);
 }
 
 }  // namespace
@@ -161,15 +227,11 @@ extern "C" int dlb_rel_bias_fwd(const void *scores, const float *table, const in
   if (batch == 0 || heads == 0 || q_len == 0 || kv_len == 0) return DLB_OK;
   DLB_REQUIRE(table && bucket_of && out, DLB_ERR_INVALID_ARG, "rel_bias_fwd: null pointer");
   BiasArgs a = {scores, table, bucket_of, out, nullptr, batch, heads, q_len, kv_len, q_start, buckets, max_distance};
-  const int v = dtype == DLB_F32 ? 4 : 8;
-  const bool vec = aligned16(scores) && aligned16(out) && kv_len % v == 0;
-  const int rows_per_cta = 16;
-  const dim3 grid(ceil_div(q_len, rows_per_cta) * heads * batch);
+  const bool vec = rows_can_be_cut(out, scores, dtype == DLB_F32 ? 4 : 2);
+  const dim3 grid(ceil_div(q_len, kBiasRows) * heads * batch);
   const size_t smem = sizeof(float) * (2 * max_distance + 1);
-  if (dtype == DLB_F32)
-    launch_pdl(rel_bias_fwd_kernel<float>, grid, dim3(kBiasThreads), smem, as_stream(stream), a, rows_per_cta, vec);
-  else
-    launch_pdl(rel_bias_fwd_kernel<__nv_bfloat16>, grid, dim3(kBiasThreads), smem, as_stream(stream), a, rows_per_cta, vec);
+  auto kern = dtype == DLB_F32 ? rel_bias_fwd_kernel<float> : rel_bias_fwd_kernel<__nv_bfloat16>;
+  launch_pdl(kern, grid, dim3(kBiasThreads), smem, as_stream(stream), a, vec);
   DLB_LAUNCH_CHECK("rel_bias_fwd");
   return DLB_OK;
 }
@@ -192,11 +254,14 @@ extern "C" int dlb_rel_bias_bwd(const void *dscores, const int32_t *bucket_of, f
   const int parts = bias_parts(batch, heads, q_len);
   BiasArgs a = {dscores, nullptr, bucket_of, nullptr, static_cast<float *>(workspace), batch, heads, q_len, kv_len,
                 q_start, buckets, max_distance};
-  const size_t smem = sizeof(float) * buckets * kBiasThreads;
+  const size_t smem = sizeof(float) * buckets * kBiasThreads + 2 * max_distance + 1;
+  const bool vec = rows_can_be_cut(dscores, nullptr, dtype == DLB_F32 ? 4 : 2);
   auto kern = dtype == DLB_F32 ? rel_bias_bwd_kernel<float> : rel_bias_bwd_kernel<__nv_bfloat16>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  DLB_REQUIRE(e == cudaSuccess, DLB_ERR_CUDA, "rel_bias_bwd: %s", cudaGetErrorString(e));
-  launch_pdl(kern, dim3(heads * parts), dim3(kBiasThreads), smem, as_stream(stream), a, parts);
+  if (smem > 40 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    DLB_REQUIRE(e == cudaSuccess, DLB_ERR_CUDA, "rel_bias_bwd: %s", cudaGetErrorString(e));
+  }
+  launch_pdl(kern, dim3(heads * parts), dim3(kBiasThreads), smem, as_stream(stream), a, parts, vec);
   DLB_LAUNCH_CHECK("rel_bias_bwd");
   launch_pdl(rel_bias_sum_kernel, dim3(heads * buckets), dim3(128), 0, as_stream(stream),
              static_cast<const float *>(a.part), dtable, parts, buckets);

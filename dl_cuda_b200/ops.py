@@ -6,6 +6,8 @@ nothing is allocated inside a timed region) or are allocated here.
 """
 from __future__ import annotations
 
+from ctypes import byref
+
 import torch
 
 from . import capi
@@ -283,66 +285,96 @@ def softmax_bwd(dy, s, dx=None, scale=1.0):
 # --- attention ------------------------------------------------------------------------------
 def _heads(t):
     """capi.Heads of a [batch, token, head, column] tensor (any strides, columns contiguous)."""
-    return capi.Heads(ptr(t), t.stride(0), t.stride(1), t.stride(2))
+    stride = t.stride()
+    if stride[3] != 1 and t.shape[3] > 1:
+        raise ValueError("columns must be contiguous")
+    return capi.Heads(t.data_ptr(), stride[0], stride[1], stride[2])
 
 
-def _attn_args(q, k, v, scale, cap, causal, kv_lens, q_start, prefix, q_docs, kv_docs, slopes, table, bucket_of):
-    """The checked argument block without o and lse; shapes are checked here, values by the library."""
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 4:
-            raise ValueError(f"{name} must be [batch, token, head, column], got {tuple(t.shape)}")
-        if t.stride(3) != 1 and t.shape[3] > 1:
-            raise ValueError(f"the columns of {name} must be contiguous")
-        if t.dtype != q.dtype:
-            raise TypeError(f"{name} is {t.dtype}, q is {q.dtype}")
+def _int_array(name, t, shape, device):
+    if t is None:
+        return None
+    if t.dtype is not torch.int32 or t.shape != shape:
+        raise ValueError(f"{name} must be torch.int32 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    return _array(name, t, device)
+
+
+def _float_array(name, t, shape, device):
+    if t is None:
+        return None
+    if t.dtype is not torch.float32 or t.shape != shape:
+        raise ValueError(f"{name} must be torch.float32 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    return _array(name, t, device)
+
+
+def _array(name, t, device):
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t.data_ptr()
+
+
+def _like(name, t, q):
+    """t has q's shape, type and device."""
+    if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:
+        raise ValueError(f"{name} must be {q.dtype} {tuple(q.shape)} on {q.device}, "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _on_current_device(t):
+    if not t.is_cuda:
+        raise ValueError("device tensors required: the kernels have no CPU path")
+    if t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"tensors are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _attn_args(q, k, v, o, lse, scale, cap, causal, kv_lens, q_start, prefix, q_docs, kv_docs, slopes, table, bucket_of):
+    """The argument block; shapes, types and places are checked here, values by the library."""
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("q, k and v are [batch, token, head, column]")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"q is {q.dtype}, k {k.dtype}, v {v.dtype}")
     batch, q_len, heads, d = q.shape
+    _, kv_len, kv_heads, _ = k.shape
     if k.shape != v.shape or k.shape[0] != batch or k.shape[3] != d:
         raise ValueError(f"shapes do not fit: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-    kv_len, kv_heads = k.shape[1], k.shape[2]
+    _on_current_device(q)
+    device = q.device
+    if k.device != device or v.device != device:
+        raise ValueError(f"q, k and v are on {device}, {k.device} and {v.device}")
     if (table is None) != (bucket_of is None):
         raise ValueError("table and bucket_of go together")
-    wanted = (("kv_lens", kv_lens, (batch,), torch.int32), ("q_start", q_start, (batch,), torch.int32),
-              ("prefix", prefix, (batch,), torch.int32), ("q_docs", q_docs, (batch, q_len), torch.int32),
-              ("kv_docs", kv_docs, (batch, kv_len), torch.int32), ("slopes", slopes, (heads,), torch.float32),
-              ("table", table, (heads, table.shape[-1]) if table is not None else None, torch.float32),
-              ("bucket_of", bucket_of, (bucket_of.numel(),) if bucket_of is not None else None, torch.int32))
-    for name, t, shape, dtype in wanted:
-        if t is None:
-            continue
-        if tuple(t.shape) != shape or t.dtype != dtype:
-            raise ValueError(f"{name} must be {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
-    if bucket_of is not None and bucket_of.numel() % 2 == 0:
-        raise ValueError("bucket_of has 2 * max_distance + 1 entries")
-    _need_cuda(kv_lens, q_start, prefix, q_docs, kv_docs, slopes, table, bucket_of)
-    _same_device(q, k, v, kv_lens, q_start, prefix, q_docs, kv_docs, slopes, table, bucket_of)
-    a = capi.Attn(batch=batch, heads=heads, kv_heads=kv_heads, q_len=q_len, kv_len=kv_len, head_dim=d,
-                  dtype=dtype_of(q), causal=int(bool(causal)), scale=d ** -0.5 if scale is None else scale, cap=cap,
-                  buckets=table.shape[1] if table is not None else 0,
-                  max_distance=bucket_of.numel() // 2 if bucket_of is not None else 0,
-                  kv_lens=ptr(kv_lens), q_start=ptr(q_start), prefix=ptr(prefix), q_docs=ptr(q_docs),
-                  kv_docs=ptr(kv_docs), slopes=ptr(slopes), table=ptr(table), bucket_of=ptr(bucket_of))
-    a.q, a.k, a.v = _heads(q), _heads(k), _heads(v)
-    return a
+    buckets = reach = 0
+    if table is not None:
+        if table.dim() != 2 or bucket_of.dim() != 1 or bucket_of.numel() % 2 == 0:
+            raise ValueError("table is [heads, buckets], bucket_of has 2 * max_distance + 1 entries")
+        buckets, reach = table.shape[1], bucket_of.numel() // 2
+    per_batch = (batch,)
+    return capi.Attn(
+        batch, heads, kv_heads, q_len, kv_len, d, dtype_of(q), 1 if causal else 0, d ** -0.5 if scale is None else scale, cap,
+        buckets, reach, _int_array("kv_lens", kv_lens, per_batch, device), _int_array("q_start", q_start, per_batch, device),
+        _int_array("prefix", prefix, per_batch, device), _int_array("q_docs", q_docs, (batch, q_len), device),
+        _int_array("kv_docs", kv_docs, (batch, kv_len), device), _float_array("slopes", slopes, (heads,), device),
+        _float_array("table", table, (heads, buckets), device),
+        _int_array("bucket_of", bucket_of, (2 * reach + 1,), device), _heads(q), _heads(k), _heads(v), _heads(o), lse)
 
 
-def _same_device(first, *others):
-    if not first.is_cuda:
-        raise ValueError("device tensors required: the kernels have no CPU path")
-    if first.device.index != torch.cuda.current_device():
-        raise ValueError(f"tensors are on {first.device}, the current device is cuda:{torch.cuda.current_device()}")
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"tensors on {first.device} and {t.device}")
+def _lse(t, shape, device):
+    if t.shape != shape or t.dtype != torch.float32 or t.device != device or not t.is_contiguous():
+        raise ValueError(f"lse must be contiguous torch.float32 {shape} on {device}")
+    return t.data_ptr()
 
 
-def _check_like(name, t, shape, dtype, strided=False):
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-    if strided:
-        if t.stride(3) != 1 and t.shape[3] > 1:
-            raise ValueError(f"the columns of {name} must be contiguous")
-    elif not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
+def _space(workspace, need, device):
+    """(address, bytes) of the given workspace, or of a fresh one; keep the third alive over the call."""
+    if workspace is None:
+        if need == 0:
+            return None, 0, None
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    elif workspace.device != device or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be contiguous on {device}")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
 
 
 def attn_fwd(q, k, v, scale=None, cap=0.0, causal=False, kv_lens=None, q_start=None, prefix=None, q_docs=None,
@@ -350,31 +382,25 @@ def attn_fwd(q, k, v, scale=None, cap=0.0, causal=False, kv_lens=None, q_start=N
     """Returns (o, lse) of q [batch, q_len, heads, d] against k, v [batch, kv_len, kv_heads, d] (any strides with
     contiguous columns); lse is None when want_lse is False.  scale defaults to 1/sqrt(d).  Which keys a query
     sees, and how its scores are changed, is told at dlb_attn_fwd in the header.  A cache longer than kv_len goes
-    in as a slice; for one token against a cache pass q_start = kv_lens - 1."""
-    a = _attn_args(q, k, v, scale, cap, causal, kv_lens, q_start, prefix, q_docs, kv_docs, slopes, table, bucket_of)
-    batch, q_len, heads, d = q.shape
-    out = torch.empty(batch, q_len, heads, d, dtype=q.dtype, device=q.device) if out is None else out
-    _check_like("out", out, q.shape, q.dtype, strided=True)
+    in as a slice; for one token against a cache pass q_start = kv_lens - 1.  All tensors on the current device,
+    on whose current stream the call runs."""
+    if q.dim() != 4:
+        raise ValueError("q is [batch, token, head, column]")
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+    _like("out", out, q)
+    at = None
     if want_lse:
-        lse = torch.empty(batch, heads, q_len, dtype=torch.float32, device=q.device) if lse is None else lse
-        _check_like("lse", lse, (batch, heads, q_len), torch.float32)
+        shape = (q.shape[0], q.shape[2], q.shape[1])
+        lse = torch.empty(shape, dtype=torch.float32, device=q.device) if lse is None else lse
+        at = _lse(lse, shape, q.device)
     else:
         lse = None
-    _same_device(q, out, lse, workspace)
-    a.o, a.lse = _heads(out), ptr(lse)
-    workspace = attn_fwd_workspace(a, q.device) if workspace is None else workspace
-    check(capi.lib().dlb_attn_fwd(_ref(a), ptr(workspace), workspace.numel() * workspace.element_size(),
-                                  current_stream()))
+    a = _attn_args(q, k, v, out, at, scale, cap, causal, kv_lens, q_start, prefix, q_docs, kv_docs, slopes, table,
+                   bucket_of)
+    ref, library = byref(a), capi.lib()
+    space, size, _keep = _space(workspace, library.dlb_attn_fwd_workspace_bytes(ref) if workspace is None else 0, q.device)
+    check(library.dlb_attn_fwd(ref, space, size, current_stream()))
     return out, lse
-
-
-def _ref(struct):
-    import ctypes
-    return ctypes.byref(struct)
-
-
-def attn_fwd_workspace(args, device):
-    return _workspace(capi.lib().dlb_attn_fwd_workspace_bytes(_ref(args)), device)
 
 
 def attn_bwd(dout, q, k, v, o, lse, scale=None, cap=0.0, causal=False, kv_lens=None, q_start=None, prefix=None,
@@ -382,29 +408,25 @@ def attn_bwd(dout, q, k, v, o, lse, scale=None, cap=0.0, causal=False, kv_lens=N
              want_dtable=True, workspace=None):
     """Returns (dq, dk, dv, dtable) from dout, with o and lse as attn_fwd returned them for the same arguments;
     dtable (fp32 [heads, buckets]) is None without a table or when want_dtable is False."""
-    a = _attn_args(q, k, v, scale, cap, causal, kv_lens, q_start, prefix, q_docs, kv_docs, slopes, table, bucket_of)
-    batch, q_len, heads, d = q.shape
-
-    def fresh(like):
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
-
-    dq, dk, dv = (fresh(x) if g is None else g for g, x in ((dq, q), (dk, k), (dv, v)))
+    if q.dim() != 4:
+        raise ValueError("q is [batch, token, head, column]")
+    device = q.device
+    dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=device) if g is None else g
+                  for g, x in ((dq, q), (dk, k), (dv, v)))
     for name, t, like in (("dout", dout, q), ("o", o, q), ("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
-        _check_like(name, t, like.shape, q.dtype, strided=True)
-    _check_like("lse", lse, (batch, heads, q_len), torch.float32)
+        _like(name, t, like)
+    at = _lse(lse, (q.shape[0], q.shape[2], q.shape[1]), device)
+    a = _attn_args(q, k, v, o, at, scale, cap, causal, kv_lens, q_start, prefix, q_docs, kv_docs, slopes, table,
+                   bucket_of)
     if table is not None and want_dtable:
         dtable = torch.empty_like(table) if dtable is None else dtable
-        _check_like("dtable", dtable, table.shape, torch.float32)
+        to = _float_array("dtable", dtable, table.shape, device)
     else:
-        dtable = None
-    _same_device(q, dout, o, lse, dq, dk, dv, dtable, workspace)
-    a.o, a.lse = _heads(o), ptr(lse)
-    g = capi.AttnGrad(dtable=ptr(dtable))
-    g.dout, g.dq, g.dk, g.dv = _heads(dout), _heads(dq), _heads(dk), _heads(dv)
-    if workspace is None:
-        workspace = _workspace(capi.lib().dlb_attn_bwd_workspace_bytes(_ref(a), _ref(g)), q.device)
-    check(capi.lib().dlb_attn_bwd(_ref(a), _ref(g), ptr(workspace), workspace.numel() * workspace.element_size(),
-                                  current_stream()))
+        dtable = to = None
+    g = capi.AttnGrad(_heads(dout), _heads(dq), _heads(dk), _heads(dv), to)
+    ref, grad, library = byref(a), byref(g), capi.lib()
+    space, size, _keep = _space(workspace, library.dlb_attn_bwd_workspace_bytes(ref, grad) if workspace is None else 0, device)
+    check(library.dlb_attn_bwd(ref, grad, space, size, current_stream()))
     return dq, dk, dv, dtable
 
 
@@ -415,45 +437,45 @@ def rel_bucket_map(buckets, max_distance, both_directions=True):
     return t
 
 
-def _check_bucket_of(bucket_of):
-    if bucket_of.dim() != 1 or bucket_of.dtype != torch.int32 or bucket_of.numel() % 2 == 0:
-        raise ValueError("bucket_of must be an int32 vector of 2 * max_distance + 1 entries")
-
-
 def rel_bias_fwd(table, bucket_of, scores=None, shape=None, q_start=0, dtype=torch.float32, out=None):
     """scores [batch, heads, q_len, kv_len] (or zeros of `shape` and `dtype`) plus the bucketed position bias of
     table [heads, buckets]; out may be scores."""
-    _need_cuda(table, bucket_of, scores, out)
-    _check_bucket_of(bucket_of)
+    _on_current_device(table)
+    device = table.device
     if scores is not None:
-        shape, dtype = tuple(scores.shape), scores.dtype
-    if shape is None or len(shape) != 4:
-        raise ValueError("scores or a shape [batch, heads, q_len, kv_len] is needed")
+        shape, dtype = scores.shape, scores.dtype
+        _array("scores", scores, device)
+    if shape is None or len(shape) != 4 or table.dim() != 2 or bucket_of.dim() != 1 or bucket_of.numel() % 2 == 0:
+        raise ValueError("scores (or a shape) are [batch, heads, q_len, kv_len], table [heads, buckets], bucket_of has "
+                         "2 * max_distance + 1 entries")
     batch, heads, q_len, kv_len = shape
-    if table.dim() != 2 or table.shape[0] != heads or table.dtype != torch.float32:
-        raise ValueError(f"table must be float32 [{heads}, buckets], got {table.dtype} {tuple(table.shape)}")
-    out = torch.empty(shape, dtype=dtype, device=table.device) if out is None else out
-    _check_like("out", out, shape, dtype)
-    _same_device(table, bucket_of, scores, out)
-    check(capi.lib().dlb_rel_bias_fwd(ptr(scores), ptr(table), ptr(bucket_of), ptr(out), batch, heads, q_len, kv_len,
-                                      q_start, table.shape[1], bucket_of.numel() // 2, dtype_of(out), current_stream()))
+    buckets, reach = table.shape[1], bucket_of.numel() // 2
+    out = torch.empty(shape, dtype=dtype, device=device) if out is None else out
+    if out.shape != tuple(shape) or out.dtype != dtype:
+        raise ValueError(f"out must be {dtype} {tuple(shape)}, got {out.dtype} {tuple(out.shape)}")
+    check(capi.lib().dlb_rel_bias_fwd(ptr(scores), _float_array("table", table, (heads, buckets), device),
+                                      _int_array("bucket_of", bucket_of, (2 * reach + 1,), device),
+                                      _array("out", out, device), batch, heads, q_len, kv_len, q_start, buckets, reach,
+                                      dtype_of(out), current_stream()))
     return out
 
 
 def rel_bias_bwd(dscores, bucket_of, buckets, q_start=0, dtable=None, workspace=None):
     """dtable [heads, buckets]: the sum of dscores [batch, heads, q_len, kv_len] over each bucket's positions."""
-    _need_cuda(dscores, bucket_of, dtable, workspace)
-    _check_bucket_of(bucket_of)
+    _on_current_device(dscores)
+    device = dscores.device
+    if dscores.dim() != 4 or bucket_of.dim() != 1 or bucket_of.numel() % 2 == 0:
+        raise ValueError("dscores are [batch, heads, q_len, kv_len], bucket_of has 2 * max_distance + 1 entries")
     batch, heads, q_len, kv_len = dscores.shape
-    dtable = torch.empty(heads, buckets, dtype=torch.float32, device=dscores.device) if dtable is None else dtable
-    _check_like("dtable", dtable, (heads, buckets), torch.float32)
-    _same_device(dscores, bucket_of, dtable, workspace)
-    if workspace is None:
-        workspace = _workspace(capi.lib().dlb_rel_bias_bwd_workspace_bytes(batch, heads, q_len, kv_len, buckets),
-                               dscores.device)
-    check(capi.lib().dlb_rel_bias_bwd(ptr(dscores), ptr(bucket_of), ptr(dtable), ptr(workspace),
-                                      workspace.numel() * workspace.element_size(), batch, heads, q_len, kv_len, q_start,
-                                      buckets, bucket_of.numel() // 2, dtype_of(dscores), current_stream()))
+    reach = bucket_of.numel() // 2
+    dtable = torch.empty(heads, buckets, dtype=torch.float32, device=device) if dtable is None else dtable
+    library = capi.lib()
+    need = library.dlb_rel_bias_bwd_workspace_bytes(batch, heads, q_len, kv_len, buckets) if workspace is None else 0
+    space, size, _keep = _space(workspace, need, device)
+    check(library.dlb_rel_bias_bwd(_array("dscores", dscores, device),
+                                   _int_array("bucket_of", bucket_of, (2 * reach + 1,), device),
+                                   _float_array("dtable", dtable, (heads, buckets), device), space, size, batch, heads,
+                                   q_len, kv_len, q_start, buckets, reach, dtype_of(dscores), current_stream()))
     return dtable
 
 
