@@ -217,7 +217,9 @@ int launch_bwd(const AttnArgs &p, bool mma, cudaStream_t st) {
                    vector_rows(p.v, p.dim, sizeof(T)) && vector_rows(p.dout, p.dim, sizeof(T));
   const size_t rows = static_cast<size_t>(p.batch) * p.heads * stat_tiles(p.q_len) * kStatRows;
   if (rows > 0) {
-    launch_pdl(attn_row_stats_kernel<T>, dim3(static_cast<unsigned>(ceil_div(rows, size_t{8}))), dim3(256), 0, st, p);
+    const bool pairs = vector_rows(p.o, p.dim, sizeof(T)) && vector_rows(p.dout, p.dim, sizeof(T));
+    auto kern = pairs ? attn_row_stats_kernel<T, 8, true> : attn_row_stats_kernel<T, 32, false>;
+    launch_pdl(kern, dim3(static_cast<unsigned>(ceil_div(rows, size_t{pairs ? 32u : 8u}))), dim3(256), 0, st, p);
     DLB_LAUNCH_CHECK("attn_row_stats");
   }
   if (mma) {
@@ -232,7 +234,9 @@ int launch_bwd(const AttnArgs &p, bool mma, cudaStream_t st) {
     };
     const bool fill = blocks(64, true) + blocks(64, false) >= 2 * sm_count() && blocks(64, true) >= sm_count();
     // (the sums of more than 32 buckets do not fit beside the widest 64-row tiles)
-    const int groups = fill && !(p.dtable && p.buckets > 32 && p.dim > 64) ? 4 : 2;
+    // one 64-row tile may be the whole sequence: smaller ones would only load the other side twice
+    const bool short_rows = p.q_len <= 64 && p.kv_len <= 64;
+    const int groups = (fill || short_rows) && !(p.dtable && p.buckets > 32 && p.dim > 64) ? 4 : 2;
     auto launch = [&](auto row_groups) -> int {
       constexpr int DP = decltype(width)::value, RG = decltype(row_groups)::value;
       AttnArgs args = p;

@@ -4,8 +4,9 @@
 // U, W (Q and dO of every head of the group; else K and V) past them in tiles of 64 rows:
 //     S = X U^T, G = Y W^T (TMEM) -> P = 2^(s - lse), D = P (G - delta), times the cap's derivative
 //     FOR_KEYS: dV += P W, dK += D U;   else dQ += D U                 (TMEM, scaled at the end)
-// with P and D written over S and G as bf16.  Two groups of four warps take alternate tiles, one
-// thread per row, so that the products of one tile run beside the exponentials of the other.
+// with P and D written over S and G as bf16.  Two groups of warps take alternate tiles, so that the
+// products of one tile run beside the exponentials of the other.  A group has eight warps, two threads a
+// row (HALVES = 2), or four where the sums for the table leave no room for twice as many.
 //
 // Two passes rebuild S and G twice: 7 products of 2 * dim flop per pair where a single pass would need
 // 5.  In return no sum crosses a CTA: no fp32 copy of dQ in memory, no atomics, the same bits every time.
@@ -18,7 +19,14 @@
 namespace dlb {
 
 constexpr int kStreamRows = 64, kStreamBlock = kStreamRows * 128;
-constexpr int kBwdThreads = 320, kBwdLoadWarp = 8, kBwdMmaWarp = 9;
+// Registers with HALVES = 2: launched with 96 each (640 * 96 = 61440); the row warps go up to 104, the
+// four others down to 64 (512 * 104 + 128 * 64 = 61440).
+constexpr int kBwdRowRegs = 104, kBwdOtherRegs = 64;
+template <int HALVES>
+struct BwdWarps {
+  static constexpr int kRows = 8 * HALVES, kLoad = kRows, kMma = kRows + 1;
+  static constexpr int kThreads = HALVES == 2 ? 640 : 320;
+};
 constexpr int kStatsBytes = 2 * kStreamRows * sizeof(float);
 
 template <int NB, int ST>
@@ -36,29 +44,31 @@ struct BwdMaps {
 struct BwdRest {
   int lut, buckets, sums, flags, total;
 };
-__host__ __device__ inline BwdRest bwd_rest(const AttnArgs &a, bool for_keys) {
+__host__ __device__ inline BwdRest bwd_rest(const AttnArgs &a, bool for_keys, int halves) {
   const int tiles = ((for_keys ? a.q_len : a.kv_len) + kStreamRows - 1) / kStreamRows;
   const bool table_sums = !for_keys && a.dtable != nullptr;
   BwdRest r;
   r.lut = 0;
   r.buckets = r.lut + (a.table ? 4 * lut_floats(a.reach) : 0);
   r.sums = r.buckets + (table_sums ? (lut_floats(a.reach) + 15) / 16 * 16 : 0);
-  r.flags = r.sums + (table_sums ? a.buckets * 2 * kTileRows * 8 : 0);
+  r.flags = r.sums + (table_sums ? a.buckets * 2 * halves * kTileRows * 8 : 0);
   r.total = r.flags + (tiles + 15) / 16 * 16;
   return r;
 }
 
-template <int NB, int ST, bool FOR_KEYS, bool CAP, int BIAS>
-static __global__ void __launch_bounds__(kBwdThreads, 1)
+template <int NB, int ST, int HALVES, bool FOR_KEYS, bool CAP, int BIAS>
+static __global__ void __launch_bounds__(BwdWarps<HALVES>::kThreads, 1)
 attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ BwdMaps maps, unsigned int *timeouts) {
   using Shape = BwdShape<NB, ST>;
+  constexpr int kBwdLoadWarp = BwdWarps<HALVES>::kLoad, kBwdMmaWarp = BwdWarps<HALVES>::kMma;
+  constexpr int kBwdThreads = BwdWarps<HALVES>::kThreads, kGroup = 128 * HALVES;  // threads of a group
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   unsigned char *ring = smem + Shape::kRing;
-  const BwdRest rest = bwd_rest(a, FOR_KEYS);
+  const BwdRest rest = bwd_rest(a, FOR_KEYS, HALVES);
   float *lut = reinterpret_cast<float *>(smem + Shape::kRest + rest.lut);
   unsigned char *bucket_lut = smem + Shape::kRest + rest.buckets;
-  float2 *sums = reinterpret_cast<float2 *>(smem + Shape::kRest + rest.sums);  // [group][bucket][row]
+  float2 *sums = reinterpret_cast<float2 *>(smem + Shape::kRest + rest.sums);  // [group, half][bucket][row]
   unsigned char *flags = smem + Shape::kRest + rest.flags;
   __shared__ uint64_t x_full, full[ST], empty[ST], s_full[2], p_full[2], acc_full, drain;
   __shared__ uint32_t tmem_slot;
@@ -76,7 +86,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     }
     for (int t = 0; t < 2; t++) {
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 4);
+      mbar_init(&p_full[t], 4 * HALVES);
     }
     mbar_init(&acc_full, 1);
     mbar_init(&drain, 1);
@@ -156,108 +166,16 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   if (table_sums) {
     for (int e = tid; e < 2 * (a.reach + kLutPad) + 1; e += kBwdThreads)
       bucket_lut[e] = static_cast<unsigned char>(bucket_at(a, e - a.reach - kLutPad));
-    for (int e = tid; e < 2 * a.buckets * kTileRows; e += kBwdThreads) sums[e] = make_float2(0.f, 0.f);
+    for (int e = tid; e < 2 * HALVES * a.buckets * kTileRows; e += kBwdThreads) sums[e] = make_float2(0.f, 0.f);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  if (warp == kBwdLoadWarp) {
-    if (lane == 0) {
-      const int x_head = FOR_KEYS ? hk : unit;
-      mbar_expect_tx(&x_full, 2 * NB * kBlockBytes);
-      for (int c = 0; c < NB; c++) {
-        tma_load_rows(smem + Shape::kX + c * kBlockBytes, &maps.x, &x_full, c * kBlockCols, row0, x_head, b);
-        tma_load_rows(smem + Shape::kY + c * kBlockBytes, &maps.y, &x_full, c * kBlockCols, row0, x_head, b);
-      }
-      int it = 0;
-      for (int g = 0; g < heads_here && !*dead; g++) {
-        const int head = FOR_KEYS ? hk * a.group + g : hk;  // of the streamed tensors
-        for (int n = 0; n < n_tiles; n++) {
-          if (!flags[n]) continue;
-          const int s = it % ST;
-          const unsigned use = it / ST;
-          if (use) mbar_wait(&empty[s], (use - 1) & 1, dead, timeouts);
-          if (*dead) break;
-          unsigned char *stage = ring + s * Shape::kStage;
-          mbar_expect_tx(&full[s], Shape::kStage + (FOR_KEYS ? kStatsBytes : 0));
-          for (int c = 0; c < NB; c++) {
-            tma_load_rows(stage + c * kStreamBlock, &maps.u, &full[s], c * kBlockCols, n * kStreamRows, head, b);
-            tma_load_rows(stage + (NB + c) * kStreamBlock, &maps.w, &full[s], c * kBlockCols, n * kStreamRows, head, b);
-          }
-          if (FOR_KEYS)
-            bulk_load(smem + Shape::kStats + s * kStatsBytes, stats_tile(a, b, head, n), kStatsBytes, &full[s]);
-          it++;
-        }
-      }
-      if (*dead) {  // no copy may be in flight when the CTA ends
-        drain_wait(&x_full, 0);
-        for (int i = max(0, it - ST); i < it; i++) drain_wait(&full[i % ST], (i / ST) & 1);
-      }
-    }
-  } else if (warp == kBwdMmaWarp) {
-    const int k_steps = (a.dim + 15) / 16, n_cols = k_steps * 16;
-    const uint32_t idesc_s = mma_desc(kStreamRows, false), idesc_acc = mma_desc(n_cols, true);
-    const uint64_t xd = desc_k_major(smem_u32(smem + Shape::kX)), yd = desc_k_major(smem_u32(smem + Shape::kY));
-    const uint64_t u_desc = desc_k_major(smem_u32(ring)), u_desc_mn = desc_mn_major(smem_u32(ring), kStreamBlock);
-    constexpr uint32_t kStageStep = Shape::kStage >> 4, kW = (NB * kStreamBlock) >> 4;  // in descriptor units
-    auto accumulate = [&](int it) {  // with what the row threads made of tile `it`
-      const int s = it % ST, w = it & 1;
-      mbar_wait(&p_full[w], (it >> 1) & 1, dead, timeouts);
-      tc_fence_after();
-      const uint64_t ud = u_desc_mn + s * kStageStep, wd = ud + kW;
-      const uint32_t p_at = tmem + w * 128;
-      if (elect_lane()) {
-#pragma unroll
-        for (int k = 0; k < kStreamRows / 16; k++)
-          mma_ts(tmem + 256, p_at + 64 + k * 8, ud + k * (2048 >> 4), idesc_acc, it > 0 || k > 0);
-        if (FOR_KEYS) {
-#pragma unroll
-          for (int k = 0; k < kStreamRows / 16; k++)
-            mma_ts(tmem + 384, p_at + k * 8, wd + k * (2048 >> 4), idesc_acc, it > 0 || k > 0);
-        }
-        tc_commit(&empty[s]);
-      }
-      __syncwarp();
-    };
-    mbar_wait(&x_full, 0, dead, timeouts);
-    int it = 0;
-    for (int g = 0; g < heads_here && !*dead; g++)
-      for (int n = 0; n < n_tiles; n++) {
-        if (!flags[n]) continue;
-        const int s = it % ST, w = it & 1;
-        if (it >= 2) accumulate(it - 2);
-        mbar_wait(&full[s], (it / ST) & 1, dead, timeouts);
-        const uint64_t ud = u_desc + s * kStageStep, wd = ud + kW;
-        const uint32_t s_to = tmem + w * 128;
-        if (elect_lane()) {
-#pragma unroll
-          for (int k = 0; k < NB * 4; k++) {
-            const int xk = (k / 4) * (kBlockBytes >> 4) + (k % 4) * 2, uk = (k / 4) * (kStreamBlock >> 4) + (k % 4) * 2;
-            if (k < k_steps) mma_ss(s_to, xd + xk, ud + uk, idesc_s, k > 0);
-          }
-#pragma unroll
-          for (int k = 0; k < NB * 4; k++) {
-            const int xk = (k / 4) * (kBlockBytes >> 4) + (k % 4) * 2, uk = (k / 4) * (kStreamBlock >> 4) + (k % 4) * 2;
-            if (k < k_steps) mma_ss(s_to + 64, yd + xk, wd + uk, idesc_s, k > 0);
-          }
-          tc_commit(&s_full[w]);
-        }
-        __syncwarp();
-        it++;
-      }
-    if (it >= 2) accumulate(it - 2);
-    if (it >= 1) accumulate(it - 1);
-    if (elect_lane()) tc_commit(&acc_full);
-    __syncwarp();
-    if (*dead) {
-      if (elect_lane()) tc_commit(&drain);
-      __syncwarp();
-      drain_wait(&drain, 0);
-    }
-  } else if (warp < kBwdLoadWarp) {
-    const int w = warp >> 2, row = tid & 127, x = row0 + row;
+  if (warp < kBwdLoadWarp) {
+    if (HALVES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kBwdRowRegs));
+    const int w = warp / (4 * HALVES), half = HALVES == 2 ? warp >> 2 & 1 : 0, row = tid & 127, x = row0 + row;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lane_base + w * 128, g_at = s_at + 64;
     const bool valid = x < len && (!FOR_KEYS || x < view.end);
@@ -273,7 +191,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     int bucket_now = 0;
     float2 bucket_sum = make_float2(0.f, 0.f);
     auto flush_bucket = [&](int next) {
-      float2 *at = sums + (w * a.buckets + bucket_now) * kTileRows + row;
+      float2 *at = sums + ((w * HALVES + half) * a.buckets + bucket_now) * kTileRows + row;
       float2 v = *at;
       v.x += bucket_sum.x;
       v.y += bucket_sum.y;
@@ -287,9 +205,9 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       const float slope = (BIAS != kNoBias && a.slopes) ? ld_co(a.slopes + h) * kLog2e : 0.f;
       if (BIAS == kTable && FOR_KEYS) {
         // this head's bias by distance; both groups of warps are past the last head's tiles here
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        fill_lut(lut, a, h, tid, 256);
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        named_bar_sync(1, 2 * kGroup);
+        fill_lut(lut, a, h, tid, 2 * kGroup);
+        named_bar_sync(1, 2 * kGroup);
       }
       for (int n = 0; n < n_tiles; n++) {
         const int f = flags[n];
@@ -303,142 +221,131 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         mbar_wait(&full[s], (it / ST) & 1, dead, timeouts);  // the stage's statistics
         mbar_wait(&s_full[w], (it >> 1) & 1, dead, timeouts);
         if (by_doc) {  // the group's document numbers of this tile
-          named_bar_sync(2 + w, 128);
-          if (row < kStreamRows) doc_tile[w][row] = col_doc;
-          named_bar_sync(2 + w, 128);
+          named_bar_sync(2 + w, kGroup);
+          if (half == 0 && row < kStreamRows) doc_tile[w][row] = col_doc;
+          named_bar_sync(2 + w, kGroup);
         }
         tc_fence_after();
         const float *stats = reinterpret_cast<const float *>(smem + Shape::kStats + s * kStatsBytes);
+        // 16 columns at a time; a chunk's P and D go over the first 8 columns of its own S and G.
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
-          const int c1 = c0 + half * 32;
-          uint32_t sr[32], gr[32];
-          tmem_load32(s_at + half * 32, sr);
-          tmem_load32(g_at + half * 32, gr);
+        for (int q = 0; q < 4 / HALVES; q++) {
+          const int chunk = half * 2 + q, e0 = chunk * 16, c1 = c0 + e0;
+          uint32_t sr[16], gr[16];
+          tmem_load16(s_at + e0, sr);
+          tmem_load16(g_at + e0, gr);
           tmem_loaded(sr);
           tmem_loaded(gr);
-          float x32[32];
+          float x16[16];
 #pragma unroll
-          for (int e = 0; e < 32; e++) x32[e] = __uint_as_float(sr[e]);
-          if (CAP) cap_scores(x32, cap);
-          float bias[32];
+          for (int e = 0; e < 16; e++) x16[e] = __uint_as_float(sr[e]);
+          if (CAP) cap_scores(x16, cap);
           const int d0 = FOR_KEYS ? x - (view.start + c1) : c1 - (view.start + x);  // distance j - p at e = 0
-          bool far = false;
+          const float *lut_at = lut + d0 + a.reach + kLutPad;
+          bool far = true;
           int far_at = 0;
+          float far_bias = 0.f;
           if (BIAS == kTable) {
-            const int lo = FOR_KEYS ? d0 - 31 : d0, hi = FOR_KEYS ? d0 : d0 + 31;
+            const int lo = FOR_KEYS ? d0 - 15 : d0, hi = FOR_KEYS ? d0 : d0 + 15;
             const bool left = hi <= -a.reach, right = lo >= a.reach;
             far = __all_sync(0xffffffffu, left || right);
             far_at = left ? 0 : 2 * (a.reach + kLutPad);
-            if (far) {
-              const float v = lut[far_at];
-#pragma unroll
-              for (int e = 0; e < 32; e++) bias[e] = v;
-            } else {
-              const float *at = lut + d0 + a.reach + kLutPad;
-#pragma unroll
-              for (int e = 0; e < 32; e++) bias[e] = at[FOR_KEYS ? -e : e];
-            }
-          } else if (BIAS == kSlope) {
-#pragma unroll
-            for (int e = 0; e < 32; e++) bias[e] = 0.f;
+            if (far) far_bias = lut[far_at];
           }
-          if (BIAS == kSlope || (BIAS == kTable && a.slopes)) {
-            const float d = static_cast<float>(d0);
+          float p[16], ds[16];
 #pragma unroll
-            for (int e = 0; e < 32; e++)
-              bias[e] = fmaf(-slope, fabsf(FOR_KEYS ? d - static_cast<float>(e) : d + static_cast<float>(e)), bias[e]);
-          }
-          const float2 k2 = make_float2(to_log2, to_log2);
-          float p[32], ds[32];
-#pragma unroll
-          for (int e = 0; e < 32; e += 4) {
+          for (int e = 0; e < 16; e += 4) {
             float4 l4, d4;
             if (FOR_KEYS) {
-              l4 = *reinterpret_cast<const float4 *>(stats + half * 32 + e);
-              d4 = *reinterpret_cast<const float4 *>(stats + kStreamRows + half * 32 + e);
+              l4 = *reinterpret_cast<const float4 *>(stats + e0 + e);
+              d4 = *reinterpret_cast<const float4 *>(stats + kStreamRows + e0 + e);
             } else {
               l4 = make_float4(row_stat.x, row_stat.x, row_stat.x, row_stat.x);
               d4 = make_float4(row_stat.y, row_stat.y, row_stat.y, row_stat.y);
             }
 #pragma unroll
-            for (int q = 0; q < 4; q += 2) {
-              float2 shift = q ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
-              const float2 minus = q ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);
-              if (BIAS != kNoBias) shift = add2(shift, make_float2(bias[e + q], bias[e + q + 1]));
-              const float2 v = make_float2(x32[e + q], x32[e + q + 1]);
-              const float2 y = CAP ? add2(v, shift) : fma2(v, k2, shift);
-              p[e + q] = ex2(y.x);
-              p[e + q + 1] = ex2(y.y);
-              const float2 dp = add2(make_float2(__uint_as_float(gr[e + q]), __uint_as_float(gr[e + q + 1])), minus);
-              const float2 d2 = mul2(make_float2(p[e + q], p[e + q + 1]), dp);
-              ds[e + q] = d2.x;
-              ds[e + q + 1] = d2.y;
+            for (int k = 0; k < 4; k += 2) {
+              float2 shift = k ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
+              const float2 minus = k ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);
+              if (BIAS == kTable) {
+                const float2 bias = far ? both(far_bias)
+                                        : FOR_KEYS ? make_float2(lut_at[-(e + k)], lut_at[-(e + k + 1)])
+                                                   : make_float2(lut_at[e + k], lut_at[e + k + 1]);
+                shift = add2(shift, bias);
+              }
+              if (BIAS == kSlope || (BIAS == kTable && a.slopes)) {
+                const float d = static_cast<float>(d0), f0 = static_cast<float>(e + k), f1 = static_cast<float>(e + k + 1);
+                shift.x = fmaf(-slope, fabsf(FOR_KEYS ? d - f0 : d + f0), shift.x);
+                shift.y = fmaf(-slope, fabsf(FOR_KEYS ? d - f1 : d + f1), shift.y);
+              }
+              const float2 v = make_float2(x16[e + k], x16[e + k + 1]);
+              const float2 y = CAP ? add2(v, shift) : fma2(v, both(to_log2), shift);
+              p[e + k] = ex2(y.x);
+              p[e + k + 1] = ex2(y.y);
+              const float2 dp = add2(make_float2(__uint_as_float(gr[e + k]), __uint_as_float(gr[e + k + 1])), minus);
+              const float2 d2 = mul2(make_float2(p[e + k], p[e + k + 1]), dp);
+              ds[e + k] = d2.x;
+              ds[e + k + 1] = d2.y;
             }
           }
           if (f != 3) {
             if (stream_docs) {
 #pragma unroll
-              for (int e = 0; e < 32; e += 4) {
-                const int4 d = *reinterpret_cast<const int4 *>(&doc_tile[w][half * 32 + e]);
+              for (int e = 0; e < 16; e += 4) {
+                const int4 d = *reinterpret_cast<const int4 *>(&doc_tile[w][e0 + e]);
                 const int same[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
-                for (int q = 0; q < 4; q++)
-                  if (same[q] != row_doc) p[e + q] = ds[e + q] = 0.f;
+                for (int k = 0; k < 4; k++)
+                  if (same[k] != row_doc) p[e + k] = ds[e + k] = 0.f;
               }
             }
-            if (FOR_KEYS) {
-              const int skip = see_from - c1;  // see_end is q_len: rows behind it have -lse = -infinity
+            // Hidden: columns in front of the first query that sees the key (behind the last query
+            // -lse = -infinity has done it), or behind the last key that the query sees.
+            const int cut = FOR_KEYS ? see_from - c1 : see_end - c1;
 #pragma unroll
-              for (int e = 0; e < 32; e++)
-                if (e < skip) p[e] = ds[e] = 0.f;
-            } else {
-              const int room = see_end - c1;
-#pragma unroll
-              for (int e = 0; e < 32; e++)
-                if (e >= room) p[e] = ds[e] = 0.f;
-            }
+            for (int e = 0; e < 16; e++)
+              if (FOR_KEYS ? e < cut : e >= cut) p[e] = ds[e] = 0.f;
           }
           if (table_sums) {
             // One run of columns per bucket: its sums stay in registers until the bucket changes.
             if (far) {
               const int n_now = bucket_lut[far_at];
               if (n_now != bucket_now) flush_bucket(n_now);
-              float2 t = make_float2(0.f, 0.f);
+              float2 t = both(0.f);
 #pragma unroll
-              for (int e = 0; e < 32; e++) t = add2(t, make_float2(ds[e], p[e]));
+              for (int e = 0; e < 16; e++) t = add2(t, make_float2(ds[e], p[e]));
               bucket_sum = add2(bucket_sum, t);
             } else {
               const unsigned char *at = bucket_lut + d0 + a.reach + kLutPad;
 #pragma unroll
-              for (int e = 0; e < 32; e++) {
+              for (int e = 0; e < 16; e++) {
                 const int n_now = at[e];
                 if (n_now != bucket_now) flush_bucket(n_now);
                 bucket_sum = add2(bucket_sum, make_float2(ds[e], p[e]));
               }
             }
           }
-          uint32_t packed[16];
+          uint32_t packed[8];
 #pragma unroll
-          for (int e = 0; e < 16; e++) {
+          for (int e = 0; e < 8; e++) {
             float2 y = make_float2(ds[2 * e], ds[2 * e + 1]);
             if (CAP) {  // d tanh = 1 - tanh^2
-              const float2 t = mul2(make_float2(x32[2 * e], x32[2 * e + 1]), uncap);
+              const float2 t = mul2(make_float2(x16[2 * e], x16[2 * e + 1]), uncap);
               y = mul2(y, fma2(make_float2(-t.x, -t.y), t, both(1.f)));
             }
             packed[e] = pack_bf16(y.x, y.y);
           }
-          tmem_store16(g_at + half * 16, packed);
+          tmem_store8(g_at + e0, packed);
           if (FOR_KEYS) {
 #pragma unroll
-            for (int e = 0; e < 16; e++) packed[e] = pack_bf16(p[2 * e], p[2 * e + 1]);
-            tmem_store16(s_at + half * 16, packed);
+            for (int e = 0; e < 8; e++) packed[e] = pack_bf16(p[2 * e], p[2 * e + 1]);
+            tmem_store8(s_at + e0, packed);
           }
         }
         if (n == tail) {
           // Rows of K that no query reaches may hold anything, and 0 * NaN is NaN.
           const int first = view.end - c0;
-          for (int e = row; e < (kStreamRows - first) * NB * 8; e += 128) {
+          for (int e = half * 128 + row; e < (kStreamRows - first) * NB * 8; e += kGroup) {
             const int r = first + e / (NB * 8), q = e % (NB * 8);
             *reinterpret_cast<uint4 *>(ring + s * Shape::kStage + (q / 8) * kStreamBlock + r * 128 + (q % 8) * 16) =
                 make_uint4(0, 0, 0, 0);
@@ -454,12 +361,12 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     if (table_sums) flush_bucket(0);
     mbar_wait(&acc_full, 0, dead, timeouts);
     tc_fence_after();
-    // FOR_KEYS: the first group stores dK, the second dV; else they share the columns of dQ.
+    // FOR_KEYS: the first group stores dK, the second dV; else all share the columns of dQ.
     const Heads &to = !FOR_KEYS ? a.dq : w == 0 ? a.dk : a.dv;
     const float by = FOR_KEYS && w == 1 ? 1.f : a.scale;
     const uint32_t acc_at = tmem + lane_base + (FOR_KEYS && w == 1 ? 384 : 256);
     __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(to.ptr) + b * to.batch + static_cast<long long>(x) * to.token + unit * to.head;
-    for (int c = FOR_KEYS ? 0 : w * 32; c < a.dim; c += FOR_KEYS ? 32 : 64) {
+    for (int c = 32 * (FOR_KEYS ? half : w * HALVES + half); c < a.dim; c += 32 * HALVES * (FOR_KEYS ? 1 : 2)) {
       uint32_t o[32];
       if (it >= 0) {
         tmem_load32(acc_at + c, o);
@@ -475,6 +382,102 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       }
     }
     tc_fence_before();
+  } else {
+    if (HALVES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBwdOtherRegs));
+    if (warp == kBwdLoadWarp) {
+      if (lane == 0) {
+        const int x_head = FOR_KEYS ? hk : unit;
+        mbar_expect_tx(&x_full, 2 * NB * kBlockBytes);
+        for (int c = 0; c < NB; c++) {
+          tma_load_rows(smem + Shape::kX + c * kBlockBytes, &maps.x, &x_full, c * kBlockCols, row0, x_head, b);
+          tma_load_rows(smem + Shape::kY + c * kBlockBytes, &maps.y, &x_full, c * kBlockCols, row0, x_head, b);
+        }
+        int it = 0;
+        for (int g = 0; g < heads_here && !*dead; g++) {
+          const int head = FOR_KEYS ? hk * a.group + g : hk;  // of the streamed tensors
+          for (int n = 0; n < n_tiles; n++) {
+            if (!flags[n]) continue;
+            const int s = it % ST;
+            const unsigned use = it / ST;
+            if (use) mbar_wait(&empty[s], (use - 1) & 1, dead, timeouts);
+            if (*dead) break;
+            unsigned char *stage = ring + s * Shape::kStage;
+            mbar_expect_tx(&full[s], Shape::kStage + (FOR_KEYS ? kStatsBytes : 0));
+            for (int c = 0; c < NB; c++) {
+              tma_load_rows(stage + c * kStreamBlock, &maps.u, &full[s], c * kBlockCols, n * kStreamRows, head, b);
+              tma_load_rows(stage + (NB + c) * kStreamBlock, &maps.w, &full[s], c * kBlockCols, n * kStreamRows, head, b);
+            }
+            if (FOR_KEYS)
+              bulk_load(smem + Shape::kStats + s * kStatsBytes, stats_tile(a, b, head, n), kStatsBytes, &full[s]);
+            it++;
+          }
+        }
+        if (*dead) {  // no copy may be in flight when the CTA ends
+          drain_wait(&x_full, 0);
+          for (int i = max(0, it - ST); i < it; i++) drain_wait(&full[i % ST], (i / ST) & 1);
+        }
+      }
+    } else if (warp == kBwdMmaWarp) {
+      const int k_steps = (a.dim + 15) / 16, n_cols = k_steps * 16;
+      const uint32_t idesc_s = mma_desc(kStreamRows, false), idesc_acc = mma_desc(n_cols, true);
+      const uint64_t xd = desc_k_major(smem_u32(smem + Shape::kX)), yd = desc_k_major(smem_u32(smem + Shape::kY));
+      const uint64_t u_desc = desc_k_major(smem_u32(ring)), u_desc_mn = desc_mn_major(smem_u32(ring), kStreamBlock);
+      constexpr uint32_t kStageStep = Shape::kStage >> 4, kW = (NB * kStreamBlock) >> 4;  // in descriptor units
+      auto accumulate = [&](int it) {  // with what the row threads made of tile `it`
+        const int s = it % ST, w = it & 1;
+        mbar_wait(&p_full[w], (it >> 1) & 1, dead, timeouts);
+        tc_fence_after();
+        const uint64_t ud = u_desc_mn + s * kStageStep, wd = ud + kW;
+        const uint32_t p_at = tmem + w * 128;
+        if (elect_lane()) {
+#pragma unroll
+          for (int k = 0; k < kStreamRows / 16; k++)
+            mma_ts(tmem + 256, p_at + 64 + k * 16, ud + k * (2048 >> 4), idesc_acc, it > 0 || k > 0);
+          if (FOR_KEYS) {
+#pragma unroll
+            for (int k = 0; k < kStreamRows / 16; k++)
+              mma_ts(tmem + 384, p_at + k * 16, wd + k * (2048 >> 4), idesc_acc, it > 0 || k > 0);
+          }
+          tc_commit(&empty[s]);
+        }
+        __syncwarp();
+      };
+      mbar_wait(&x_full, 0, dead, timeouts);
+      int it = 0;
+      for (int g = 0; g < heads_here && !*dead; g++)
+        for (int n = 0; n < n_tiles; n++) {
+          if (!flags[n]) continue;
+          const int s = it % ST, w = it & 1;
+          if (it >= 2) accumulate(it - 2);
+          mbar_wait(&full[s], (it / ST) & 1, dead, timeouts);
+          const uint64_t ud = u_desc + s * kStageStep, wd = ud + kW;
+          const uint32_t s_to = tmem + w * 128;
+          if (elect_lane()) {
+#pragma unroll
+            for (int k = 0; k < NB * 4; k++) {
+              const int xk = (k / 4) * (kBlockBytes >> 4) + (k % 4) * 2, uk = (k / 4) * (kStreamBlock >> 4) + (k % 4) * 2;
+              if (k < k_steps) mma_ss(s_to, xd + xk, ud + uk, idesc_s, k > 0);
+            }
+#pragma unroll
+            for (int k = 0; k < NB * 4; k++) {
+              const int xk = (k / 4) * (kBlockBytes >> 4) + (k % 4) * 2, uk = (k / 4) * (kStreamBlock >> 4) + (k % 4) * 2;
+              if (k < k_steps) mma_ss(s_to + 64, yd + xk, wd + uk, idesc_s, k > 0);
+            }
+            tc_commit(&s_full[w]);
+          }
+          __syncwarp();
+          it++;
+        }
+      if (it >= 2) accumulate(it - 2);
+      if (it >= 1) accumulate(it - 1);
+      if (elect_lane()) tc_commit(&acc_full);
+      __syncwarp();
+      if (*dead) {
+        if (elect_lane()) tc_commit(&drain);
+        __syncwarp();
+        drain_wait(&drain, 0);
+      }
+    }
   }
   __syncthreads();
   if (table_sums) {
@@ -484,9 +487,8 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       float e = 0.f, p = 0.f;
       for (int n = 0; n < a.buckets; n++) {
         float2 v = sums[n * kTileRows + tid];
-        const float2 other = sums[(a.buckets + n) * kTileRows + tid];
-        v.x += other.x;
-        v.y += other.y;
+#pragma unroll
+        for (int k = 1; k < 2 * HALVES; k++) v = add2(v, sums[(k * a.buckets + n) * kTileRows + tid]);
         sums[n * kTileRows + tid] = v;
         e += v.x;
         p += v.y;
@@ -510,6 +512,20 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     tc_fence_after();
     tmem_free(tmem, 512);
   }
+}
+
+// The query pass with sums for the table: two stages, and two threads a row where their sums fit.
+struct BwdTableShape {
+  int halves;
+  size_t smem;
+};
+inline BwdTableShape bwd_table_shape(const AttnArgs &a) {
+  constexpr size_t kMaxSmem = 227 * 1024 - 2048;  // less the static part
+  BwdTableShape s = {2, 1024 + static_cast<size_t>(BwdShape<1, 2>::kRest) + bwd_rest(a, false, 2).total};
+  if (a.dim > kBlockCols || s.smem > kMaxSmem)
+    s = {1, 1024 + static_cast<size_t>(a.dim > kBlockCols ? BwdShape<2, 2>::kRest : BwdShape<1, 2>::kRest) + bwd_rest(a, false, 1).total};
+  if (s.smem > kMaxSmem) s.halves = 0;  // does not fit at all
+  return s;
 }
 
 template <bool FOR_KEYS>
@@ -537,30 +553,32 @@ int bwd_mma_launch(const AttnArgs &a, cudaStream_t st) {
   DLB_REQUIRE(rc == 0, DLB_ERR_CUDA, "%s: tensor map refused (%d)", name, rc);
   unsigned int *timeouts = wait_timeouts_counter();
   DLB_REQUIRE(timeouts != nullptr, DLB_ERR_NO_DEVICE, "%s: no CUDA device", name);
-  auto launch = [&](auto kern, int ring_end) -> int {
-    const size_t smem = 1024 + ring_end + bwd_rest(a, FOR_KEYS).total;
+  auto launch = [&](auto kern, int ring_end, int halves) -> int {
+    const size_t smem = 1024 + ring_end + bwd_rest(a, FOR_KEYS, halves).total;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     DLB_REQUIRE(e == cudaSuccess, DLB_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
     const int grid = ceil_div(FOR_KEYS ? a.kv_len : a.q_len, kTileRows) * (FOR_KEYS ? a.kv_heads : a.heads) * a.batch;
-    launch_pdl(kern, dim3(grid), dim3(kBwdThreads), smem, st, a, maps, timeouts);
+    launch_pdl(kern, dim3(grid), dim3(halves == 2 ? BwdWarps<2>::kThreads : BwdWarps<1>::kThreads), smem, st, a, maps, timeouts);
     DLB_LAUNCH_CHECK(name);
     return DLB_OK;
   };
   const bool cap = a.cap > 0.f;
-#define DLB_PICK(NB, ST, BIAS)                                                                     \
-  (cap ? launch(attn_bwd_mma_kernel<NB, ST, FOR_KEYS, true, BIAS>, BwdShape<NB, ST>::kRest)        \
-       : launch(attn_bwd_mma_kernel<NB, ST, FOR_KEYS, false, BIAS>, BwdShape<NB, ST>::kRest))
+#define DLB_PICK(NB, ST, HALVES, BIAS)                                                                             \
+  (cap ? launch(attn_bwd_mma_kernel<NB, ST, HALVES, FOR_KEYS, true, BIAS>, BwdShape<NB, ST>::kRest, HALVES)        \
+       : launch(attn_bwd_mma_kernel<NB, ST, HALVES, FOR_KEYS, false, BIAS>, BwdShape<NB, ST>::kRest, HALVES))
+  if constexpr (!FOR_KEYS) {
+    if (a.table && a.dtable) {  // as bwd_table_shape has it
+      const BwdTableShape shape = bwd_table_shape(a);
+      if (a.dim > kBlockCols) return DLB_PICK(2, 2, 1, kTable);
+      return shape.halves == 2 ? DLB_PICK(1, 2, 2, kTable) : DLB_PICK(1, 2, 1, kTable);
+    }
+  }
   if (a.dim <= kBlockCols) {
-    if (a.table) return DLB_PICK(1, 4, kTable);
-    return a.slopes ? DLB_PICK(1, 4, kSlope) : DLB_PICK(1, 4, kNoBias);
+    if (a.table) return DLB_PICK(1, 4, 2, kTable);
+    return a.slopes ? DLB_PICK(1, 4, 2, kSlope) : DLB_PICK(1, 4, 2, kNoBias);
   }
-  if (a.table) {
-    // the sums per bucket and row leave room for two stages only
-    if constexpr (!FOR_KEYS)
-      if (a.dtable) return DLB_PICK(2, 2, kTable);
-    return DLB_PICK(2, 4, kTable);
-  }
-  return a.slopes ? DLB_PICK(2, 4, kSlope) : DLB_PICK(2, 4, kNoBias);
+  if (a.table) return DLB_PICK(2, 4, 2, kTable);
+  return a.slopes ? DLB_PICK(2, 4, 2, kSlope) : DLB_PICK(2, 4, 2, kNoBias);
 #undef DLB_PICK
 }
 

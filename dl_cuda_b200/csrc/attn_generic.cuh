@@ -467,25 +467,38 @@ static __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __
   if (a.lse && tid == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
-// Fills row_stats: -lse * log2(e) and -delta, delta = <dout_i, o_i> (= sum_j P_ij dP_ij).  One warp per row.
-template <typename T>
+// Fills row_stats: -lse * log2(e) and -delta, delta = <dout_i, o_i> (= sum_j P_ij dP_ij).  A row is taken by
+// LANES lanes with one 16-byte vector of each at a time, or by a warp element by element.
+template <typename T, int LANES, bool VEC>
 static __global__ void __launch_bounds__(256) attn_row_stats_kernel(const __grid_constant__ AttnArgs a) {
   pdl_prologue();
   const int padded = stat_tiles(a.q_len) * kStatRows;
   const size_t rows = static_cast<size_t>(a.batch) * a.heads * padded;
-  const size_t row = static_cast<size_t>(blockIdx.x) * 8 + threadIdx.x / 32;
-  if (row >= rows) return;
-  const int lane = threadIdx.x & 31;
-  // heads innermost: neighbouring warps read neighbouring memory of [token, head] layouts
+  const size_t row = static_cast<size_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
+  const int lane = threadIdx.x % LANES;
+  const bool there = row < rows;
+  // heads innermost: neighbouring rows lie side by side in [token, head] layouts
   const int h = row % a.heads, i = (row / a.heads) % padded, b = row / (static_cast<size_t>(padded) * a.heads);
   float sum = 0.f;
-  if (i < a.q_len) {
+  if (there && i < a.q_len) {
     const T *o = static_cast<const T *>(a.o.ptr) + b * a.o.batch + i * a.o.token + h * a.o.head;
     const T *g = static_cast<const T *>(a.dout.ptr) + b * a.dout.batch + i * a.dout.token + h * a.dout.head;
-    for (int c = lane; c < a.dim; c += 32) sum = fmaf(Store<T>::to_float(ld_co(o + c)), Store<T>::to_float(ld_co(g + c)), sum);
-    sum = warp_sum(sum);
+    if constexpr (VEC) {
+      constexpr int V = Store<T>::kPerVec;
+      for (int c = lane * V; c < a.dim; c += LANES * V) {
+        float x[V], y[V];
+        Store<T>::unpack(ld_keep(o + c), x);
+        Store<T>::unpack(ld_keep(g + c), y);
+#pragma unroll
+        for (int e = 0; e < V; e++) sum = fmaf(x[e], y[e], sum);
+      }
+    } else {
+      for (int c = lane; c < a.dim; c += LANES) sum = fmaf(Store<T>::to_float(ld_co(o + c)), Store<T>::to_float(ld_co(g + c)), sum);
+    }
   }
-  if (lane == 0) {
+#pragma unroll
+  for (int k = LANES / 2; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+  if (there && lane == 0) {
     float *at = stats_tile(a, b, h, i / kStatRows) + i % kStatRows;
     at[0] = i < a.q_len ? -a.lse[(static_cast<size_t>(b) * a.heads + h) * a.q_len + i] * kLog2e : -INFINITY;
     if (i < a.q_len && at[0] == INFINITY) at[0] = -INFINITY;  // lse = -infinity

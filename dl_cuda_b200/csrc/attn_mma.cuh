@@ -105,7 +105,7 @@ __host__ __device__ inline int lut_floats(int reach) { return 2 * (reach + kLutP
 // The tensor cores need 16-byte aligned rows, and a scale that keeps the order of the scores.
 bool attn_mma_fits(const AttnArgs &a, bool backward);
 int attn_fwd_mma(const AttnArgs &a, cudaStream_t st);
-bool attn_bwd_mma_room(const AttnArgs &a);  // does its shared memory fit?
+bool attn_bwd_mma_room(const AttnArgs &a);  // do the sums for the table fit?
 int attn_bwd_mma_keys(const AttnArgs &a, cudaStream_t st);
 int attn_bwd_mma_queries(const AttnArgs &a, cudaStream_t st);
 

@@ -124,12 +124,19 @@ __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&r)[
       DLB_R16(DLB_IN, r, 0), DLB_R16(DLB_IN, r, 16)
       : "memory");
 }
-__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
-      DLB_R16(DLB_IN, r, 0)
-      : "memory");
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : DLB_R16(DLB_OUT, r, 0)
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_loaded(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : DLB_R16(DLB_INOUT, r, 0)::"memory");
+}
+__device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), DLB_R4(DLB_IN, r, 0),
+               DLB_R4(DLB_IN, r, 4)
+               : "memory");
 }
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
