@@ -1,12 +1,14 @@
 // Attention backward on the tensor cores (bf16): one kernel in two roles.
 //
 // A CTA keeps 128 rows X, Y (FOR_KEYS: a tile of K and V; else of Q and dO) and streams the other side
-// U, W (Q and dO of every head of the group; else K and V) past them in tiles of 64 rows:
+// U, W (Q and dO of every head of the group; else K and V) past them in tiles of 128 rows:
 //     S = X U^T, G = Y W^T (TMEM) -> P = 2^(s - lse), D = P (G - delta), times the cap's derivative
 //     FOR_KEYS: dV += P W, dK += D U;   else dQ += D U                 (TMEM, scaled at the end)
-// with P and D written over S and G as bf16.  Two groups of warps take alternate tiles, so that the
-// products of one tile run beside the exponentials of the other.  A group has eight warps, two threads a
-// row (HALVES = 2), or four where the sums for the table leave no room for twice as many.
+// with P and D written over S and G as bf16.  TMEM holds one S, one G and the sums, so the overlap is
+// within a tile: the row threads take the exponentials of S while the tensor cores make G and the last
+// tile's dK, and D while they make dV and the next S.  Tiles of 64 columns with two buffers each were
+// slower: a product of 128 x 64 takes the tensor cores as long as one of 128 x 128 (measured with the
+// clock: 65 cycles for 16 inner columns either way), so S and G cost twice as much.
 //
 // Two passes rebuild S and G twice: 7 products of 2 * dim flop per pair where a single pass would need
 // 5.  In return no sum crosses a CTA: no fp32 copy of dQ in memory, no atomics, the same bits every time.
@@ -18,21 +20,23 @@
 
 namespace dlb {
 
-constexpr int kStreamRows = 64, kStreamBlock = kStreamRows * 128;
-// Registers with HALVES = 2: launched with 96 each (640 * 96 = 61440); the row warps go up to 104, the
-// four others down to 64 (512 * 104 + 128 * 64 = 61440).
+constexpr int kStatsBytes = 2 * kStatRows * sizeof(float);
+static_assert(kStatRows == kTileRows, "a stage takes one tile of row statistics");
+
+// PARTS threads share a row's 128 columns: four, or two where the sums for the table leave no room for
+// more.  Registers with PARTS = 4: launched with 96 each (640 * 96 = 61440); the row warps go up to 104,
+// the four others down to 64 (512 * 104 + 128 * 64 = 61440).
 constexpr int kBwdRowRegs = 104, kBwdOtherRegs = 64;
-template <int HALVES>
+template <int PARTS>
 struct BwdWarps {
-  static constexpr int kRows = 8 * HALVES, kLoad = kRows, kMma = kRows + 1;
-  static constexpr int kThreads = HALVES == 2 ? 640 : 320;
+  static constexpr int kRows = 4 * PARTS, kLoad = kRows, kMma = kRows + 1;
+  static constexpr int kThreads = PARTS == 4 ? 640 : 320;
 };
-constexpr int kStatsBytes = 2 * kStreamRows * sizeof(float);
 
 template <int NB, int ST>
 struct BwdShape {
   static constexpr int kX = 0, kY = NB * kBlockBytes, kRing = 2 * NB * kBlockBytes;
-  static constexpr int kStage = 2 * NB * kStreamBlock;
+  static constexpr int kStage = 2 * NB * kBlockBytes;
   static constexpr int kStats = kRing + ST * kStage, kRest = kStats + ST * kStatsBytes;
 };
 
@@ -40,40 +44,53 @@ struct BwdMaps {
   CUtensorMap x, y, u, w;
 };
 
-// Bytes behind the ring: bias by distance, bucket by distance, sums per bucket and row, tile flags.
+// Where in the padded tables a warp's 16 pairs from distance d0 on (FOR_KEYS: back) lie when all its
+// rows' pairs are beyond the reach; -1 when some are not (then all are near enough for the padding).
+template <bool FOR_KEYS>
+__device__ __forceinline__ int far_side(const AttnArgs &a, int d0) {
+  const int lo = FOR_KEYS ? d0 - 15 : d0, hi = FOR_KEYS ? d0 : d0 + 15;
+  const bool left = hi <= -a.reach, right = lo >= a.reach;
+  if (!__all_sync(0xffffffffu, left || right)) return -1;
+  return left ? 0 : 2 * (a.reach + kLutPad);
+}
+
+// Bytes behind the ring: bias by distance, bucket by distance, sums per part, bucket and row (of the score
+// gradients in fp32, of the probabilities in bf16: they only weight a correction), tile flags.
 struct BwdRest {
-  int lut, buckets, sums, flags, total;
+  int lut, buckets, sums, p_sums, flags, total;
 };
-__host__ __device__ inline BwdRest bwd_rest(const AttnArgs &a, bool for_keys, int halves) {
-  const int tiles = ((for_keys ? a.q_len : a.kv_len) + kStreamRows - 1) / kStreamRows;
-  const bool table_sums = !for_keys && a.dtable != nullptr;
+__host__ __device__ inline BwdRest bwd_rest(const AttnArgs &a, bool for_keys, int parts) {
+  const int tiles = ((for_keys ? a.q_len : a.kv_len) + kTileRows - 1) / kTileRows;
+  const int slots = !for_keys && a.dtable != nullptr ? a.buckets * parts * kTileRows : 0;
   BwdRest r;
   r.lut = 0;
   r.buckets = r.lut + (a.table ? 4 * lut_floats(a.reach) : 0);
-  r.sums = r.buckets + (table_sums ? (lut_floats(a.reach) + 15) / 16 * 16 : 0);
-  r.flags = r.sums + (table_sums ? a.buckets * 2 * halves * kTileRows * 8 : 0);
+  r.sums = r.buckets + (slots ? (lut_floats(a.reach) + 15) / 16 * 16 : 0);
+  r.p_sums = r.sums + slots * 4;
+  r.flags = r.p_sums + slots * 2;
   r.total = r.flags + (tiles + 15) / 16 * 16;
   return r;
 }
 
-template <int NB, int ST, int HALVES, bool FOR_KEYS, bool CAP, int BIAS>
-static __global__ void __launch_bounds__(BwdWarps<HALVES>::kThreads, 1)
+template <int NB, int ST, int PARTS, bool FOR_KEYS, bool CAP, int BIAS>
+static __global__ void __launch_bounds__(BwdWarps<PARTS>::kThreads, 1)
 attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ BwdMaps maps, unsigned int *timeouts) {
   using Shape = BwdShape<NB, ST>;
-  constexpr int kBwdLoadWarp = BwdWarps<HALVES>::kLoad, kBwdMmaWarp = BwdWarps<HALVES>::kMma;
-  constexpr int kBwdThreads = BwdWarps<HALVES>::kThreads, kGroup = 128 * HALVES;  // threads of a group
+  constexpr int kBwdLoadWarp = BwdWarps<PARTS>::kLoad, kBwdMmaWarp = BwdWarps<PARTS>::kMma;
+  constexpr int kBwdThreads = BwdWarps<PARTS>::kThreads, kRowThreads = 128 * PARTS;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   unsigned char *ring = smem + Shape::kRing;
-  const BwdRest rest = bwd_rest(a, FOR_KEYS, HALVES);
+  const BwdRest rest = bwd_rest(a, FOR_KEYS, PARTS);
   float *lut = reinterpret_cast<float *>(smem + Shape::kRest + rest.lut);
   unsigned char *bucket_lut = smem + Shape::kRest + rest.buckets;
-  float2 *sums = reinterpret_cast<float2 *>(smem + Shape::kRest + rest.sums);  // [group, half][bucket][row]
+  float *sums = reinterpret_cast<float *>(smem + Shape::kRest + rest.sums);  // [part][bucket][row]
+  __nv_bfloat16 *p_sums = reinterpret_cast<__nv_bfloat16 *>(smem + Shape::kRest + rest.p_sums);
   unsigned char *flags = smem + Shape::kRest + rest.flags;
-  __shared__ uint64_t x_full, full[ST], empty[ST], s_full[2], p_full[2], acc_full, drain;
+  __shared__ uint64_t x_full, full[ST], empty[ST], s_full, g_full, p_full, d_full, acc_full, drain;
   __shared__ uint32_t tmem_slot;
   __shared__ int dead_flag, doc_range[2];
-  __shared__ __align__(16) int doc_tile[2][kStreamRows];
+  __shared__ __align__(16) int doc_tile[kTileRows];
   volatile int *dead = &dead_flag;
   const bool table_sums = BIAS == kTable && !FOR_KEYS && a.dtable != nullptr;
 
@@ -84,10 +101,10 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int t = 0; t < 2; t++) {
-      mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 4 * HALVES);
-    }
+    mbar_init(&s_full, 1);
+    mbar_init(&g_full, 1);
+    mbar_init(&p_full, 4 * PARTS);
+    mbar_init(&d_full, 4 * PARTS);
     mbar_init(&acc_full, 1);
     mbar_init(&drain, 1);
     dead_flag = 0;
@@ -124,7 +141,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     stream_end = row_end(a, view, row_last);
     full_end = row_end(a, view, row0);
   }
-  const int n_tiles = (stream_end + kStreamRows - 1) / kStreamRows;
+  const int n_tiles = (stream_end + kTileRows - 1) / kTileRows;
   if (a.q_docs) {
     const int *docs = (FOR_KEYS ? a.kv_docs : a.q_docs) + static_cast<long long>(b) * len;
     if (warp == 0) {
@@ -146,11 +163,11 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   const int *stream_docs = a.q_docs ? (FOR_KEYS ? a.q_docs : a.kv_docs) + static_cast<long long>(b) * (FOR_KEYS ? a.q_len : a.kv_len)
                                     : nullptr;
   for (int n = warp; n < n_tiles; n += kBwdThreads / 32) {
-    const int c0 = n * kStreamRows;
-    bool active = c0 + kStreamRows > from, whole = c0 >= full_from && c0 + kStreamRows <= full_end;
+    const int c0 = n * kTileRows;
+    bool active = c0 + kTileRows > from, whole = c0 >= full_from && c0 + kTileRows <= full_end;
     if (stream_docs) {
       int lo = INT_MAX, hi = INT_MIN;
-      for (int c = c0 + lane; c < min(stream_end, c0 + kStreamRows); c += 32) {
+      for (int c = c0 + lane; c < min(stream_end, c0 + kTileRows); c += 32) {
         const int d = ld_co(stream_docs + c);
         lo = min(lo, d);
         hi = max(hi, d);
@@ -166,7 +183,10 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   if (table_sums) {
     for (int e = tid; e < 2 * (a.reach + kLutPad) + 1; e += kBwdThreads)
       bucket_lut[e] = static_cast<unsigned char>(bucket_at(a, e - a.reach - kLutPad));
-    for (int e = tid; e < 2 * HALVES * a.buckets * kTileRows; e += kBwdThreads) sums[e] = make_float2(0.f, 0.f);
+    for (int e = tid; e < PARTS * a.buckets * kTileRows; e += kBwdThreads) {
+      sums[e] = 0.f;
+      p_sums[e] = __float2bfloat16_rn(0.f);
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -174,10 +194,11 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   const uint32_t tmem = tmem_slot;
 
   if (warp < kBwdLoadWarp) {
-    if (HALVES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kBwdRowRegs));
-    const int w = warp / (4 * HALVES), half = HALVES == 2 ? warp >> 2 & 1 : 0, row = tid & 127, x = row0 + row;
+    if (PARTS == 4) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kBwdRowRegs));
+    const int part = warp >> 2, row = tid & 127, x = row0 + row;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lane_base + w * 128, g_at = s_at + 64;
+    constexpr int kCols = kTileRows / PARTS, kChunks = kCols / 16;  // this thread's columns, 16 at a time
+    const uint32_t s_at = tmem + lane_base + part * kCols, g_at = s_at + 128;
     const bool valid = x < len && (!FOR_KEYS || x < view.end);
     const int row_doc = (a.q_docs && valid) ? ld_co((FOR_KEYS ? a.kv_docs : a.q_docs) + static_cast<long long>(b) * len + x) : 0;
     // Stream rows [see_from, see_end) are visible to this row, as far as documents allow.
@@ -187,16 +208,14 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     const float to_log2 = CAP ? 1.f : a.scale * kLog2e;
     const CapCoef cap = CAP ? cap_coef(a.scale, a.cap) : CapCoef();
     const float2 uncap = both(CAP ? 1.f / cap.out : 0.f);
-    const int tail = !FOR_KEYS && view.end % kStreamRows && view.end < a.kv_len ? view.end / kStreamRows : -1;
+    const int tail = !FOR_KEYS && view.end % kTileRows && view.end < a.kv_len ? view.end / kTileRows : -1;
     int bucket_now = 0;
-    float2 bucket_sum = make_float2(0.f, 0.f);
+    float2 bucket_sum = both(0.f);
     auto flush_bucket = [&](int next) {
-      float2 *at = sums + ((w * HALVES + half) * a.buckets + bucket_now) * kTileRows + row;
-      float2 v = *at;
-      v.x += bucket_sum.x;
-      v.y += bucket_sum.y;
-      *at = v;
-      bucket_sum = make_float2(0.f, 0.f);
+      const int at = (part * a.buckets + bucket_now) * kTileRows + row;
+      sums[at] += bucket_sum.x;
+      p_sums[at] = __float2bfloat16_rn(__bfloat162float(p_sums[at]) + bucket_sum.y);
+      bucket_sum = both(0.f);
       bucket_now = next;
     };
     int it = -1;
@@ -204,73 +223,59 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       const int h = FOR_KEYS ? hk * a.group + g : unit;
       const float slope = (BIAS != kNoBias && a.slopes) ? ld_co(a.slopes + h) * kLog2e : 0.f;
       if (BIAS == kTable && FOR_KEYS) {
-        // this head's bias by distance; both groups of warps are past the last head's tiles here
-        named_bar_sync(1, 2 * kGroup);
-        fill_lut(lut, a, h, tid, 2 * kGroup);
-        named_bar_sync(1, 2 * kGroup);
+        // this head's bias by distance, once all row threads are past the last head's tiles
+        named_bar_sync(1, kRowThreads);
+        fill_lut(lut, a, h, tid, kRowThreads);
+        named_bar_sync(1, kRowThreads);
       }
       for (int n = 0; n < n_tiles; n++) {
         const int f = flags[n];
         if (!f) continue;
         it++;
-        if ((it & 1) != w) continue;
-        const int c0 = n * kStreamRows, s = it % ST;
+        const int c0 = n * kTileRows, s = it % ST;
         const bool by_doc = f != 3 && stream_docs;
         int col_doc = 0;
-        if (by_doc) col_doc = ld_co(stream_docs + min(c0 + (row & 63), (FOR_KEYS ? a.q_len : a.kv_len) - 1));
-        mbar_wait(&full[s], (it / ST) & 1, dead, timeouts);  // the stage's statistics
-        mbar_wait(&s_full[w], (it >> 1) & 1, dead, timeouts);
-        if (by_doc) {  // the group's document numbers of this tile
-          named_bar_sync(2 + w, kGroup);
-          if (half == 0 && row < kStreamRows) doc_tile[w][row] = col_doc;
-          named_bar_sync(2 + w, kGroup);
+        if (by_doc && part == 0) col_doc = ld_co(stream_docs + min(c0 + row, (FOR_KEYS ? a.q_len : a.kv_len) - 1));
+        if (FOR_KEYS) mbar_wait(&full[s], (it / ST) & 1, dead, timeouts);  // the stage's statistics
+        mbar_wait(&s_full, it & 1, dead, timeouts);
+        if (by_doc) {  // the tile's document numbers
+          named_bar_sync(2, kRowThreads);
+          if (part == 0) doc_tile[row] = col_doc;
+          named_bar_sync(2, kRowThreads);
         }
         tc_fence_after();
-        const float *stats = reinterpret_cast<const float *>(smem + Shape::kStats + s * kStatsBytes);
-        // 16 columns at a time; a chunk's P and D go over the first 8 columns of its own S and G.
+        const float *stats = reinterpret_cast<const float *>(smem + Shape::kStats + s * kStatsBytes) + part * kCols;
+        // Probabilities, from S alone.  A chunk's P and D go over the first 8 columns of its own S and G.
+        float p[kCols], x_all[CAP ? kCols : 1];
 #pragma unroll
-        for (int q = 0; q < 4 / HALVES; q++) {
-          const int chunk = half * 2 + q, e0 = chunk * 16, c1 = c0 + e0;
-          uint32_t sr[16], gr[16];
+        for (int q = 0; q < kChunks; q++) {
+          const int e0 = q * 16, c1 = c0 + part * kCols + e0;
+          uint32_t sr[16];
           tmem_load16(s_at + e0, sr);
-          tmem_load16(g_at + e0, gr);
           tmem_loaded(sr);
-          tmem_loaded(gr);
           float x16[16];
 #pragma unroll
           for (int e = 0; e < 16; e++) x16[e] = __uint_as_float(sr[e]);
-          if (CAP) cap_scores(x16, cap);
+          if (CAP) {
+            cap_scores(x16, cap);
+#pragma unroll
+            for (int e = 0; e < 16; e++) x_all[CAP ? e0 + e : 0] = x16[e];
+          }
           const int d0 = FOR_KEYS ? x - (view.start + c1) : c1 - (view.start + x);  // distance j - p at e = 0
           const float *lut_at = lut + d0 + a.reach + kLutPad;
-          bool far = true;
-          int far_at = 0;
-          float far_bias = 0.f;
-          if (BIAS == kTable) {
-            const int lo = FOR_KEYS ? d0 - 15 : d0, hi = FOR_KEYS ? d0 : d0 + 15;
-            const bool left = hi <= -a.reach, right = lo >= a.reach;
-            far = __all_sync(0xffffffffu, left || right);
-            far_at = left ? 0 : 2 * (a.reach + kLutPad);
-            if (far) far_bias = lut[far_at];
-          }
-          float p[16], ds[16];
+          const int far_at = BIAS == kTable ? far_side<FOR_KEYS>(a, d0) : 0;
+          const float far_bias = BIAS == kTable && far_at >= 0 ? lut[far_at] : 0.f;
 #pragma unroll
           for (int e = 0; e < 16; e += 4) {
-            float4 l4, d4;
-            if (FOR_KEYS) {
-              l4 = *reinterpret_cast<const float4 *>(stats + e0 + e);
-              d4 = *reinterpret_cast<const float4 *>(stats + kStreamRows + e0 + e);
-            } else {
-              l4 = make_float4(row_stat.x, row_stat.x, row_stat.x, row_stat.x);
-              d4 = make_float4(row_stat.y, row_stat.y, row_stat.y, row_stat.y);
-            }
+            float4 l4 = make_float4(row_stat.x, row_stat.x, row_stat.x, row_stat.x);
+            if (FOR_KEYS) l4 = *reinterpret_cast<const float4 *>(stats + e0 + e);
 #pragma unroll
             for (int k = 0; k < 4; k += 2) {
               float2 shift = k ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
-              const float2 minus = k ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);
               if (BIAS == kTable) {
-                const float2 bias = far ? both(far_bias)
-                                        : FOR_KEYS ? make_float2(lut_at[-(e + k)], lut_at[-(e + k + 1)])
-                                                   : make_float2(lut_at[e + k], lut_at[e + k + 1]);
+                const float2 bias = far_at >= 0 ? both(far_bias)
+                                    : FOR_KEYS  ? make_float2(lut_at[-(e + k)], lut_at[-(e + k + 1)])
+                                                : make_float2(lut_at[e + k], lut_at[e + k + 1]);
                 shift = add2(shift, bias);
               }
               if (BIAS == kSlope || (BIAS == kTable && a.slopes)) {
@@ -280,23 +285,19 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
               }
               const float2 v = make_float2(x16[e + k], x16[e + k + 1]);
               const float2 y = CAP ? add2(v, shift) : fma2(v, both(to_log2), shift);
-              p[e + k] = ex2(y.x);
-              p[e + k + 1] = ex2(y.y);
-              const float2 dp = add2(make_float2(__uint_as_float(gr[e + k]), __uint_as_float(gr[e + k + 1])), minus);
-              const float2 d2 = mul2(make_float2(p[e + k], p[e + k + 1]), dp);
-              ds[e + k] = d2.x;
-              ds[e + k + 1] = d2.y;
+              p[e0 + e + k] = ex2(y.x);
+              p[e0 + e + k + 1] = ex2(y.y);
             }
           }
           if (f != 3) {
             if (stream_docs) {
 #pragma unroll
               for (int e = 0; e < 16; e += 4) {
-                const int4 d = *reinterpret_cast<const int4 *>(&doc_tile[w][e0 + e]);
+                const int4 d = *reinterpret_cast<const int4 *>(&doc_tile[part * kCols + e0 + e]);
                 const int same[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
                 for (int k = 0; k < 4; k++)
-                  if (same[k] != row_doc) p[e + k] = ds[e + k] = 0.f;
+                  if (same[k] != row_doc) p[e0 + e + k] = 0.f;
               }
             }
             // Hidden: columns in front of the first query that sees the key (behind the last query
@@ -304,16 +305,55 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             const int cut = FOR_KEYS ? see_from - c1 : see_end - c1;
 #pragma unroll
             for (int e = 0; e < 16; e++)
-              if (FOR_KEYS ? e < cut : e >= cut) p[e] = ds[e] = 0.f;
+              if (FOR_KEYS ? e < cut : e >= cut) p[e0 + e] = 0.f;
+          }
+          if (FOR_KEYS) {
+            uint32_t packed[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) packed[e] = pack_bf16(p[e0 + 2 * e], p[e0 + 2 * e + 1]);
+            tmem_store8(s_at + e0, packed);
+          }
+        }
+        if (FOR_KEYS) tmem_stored();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full);  // (S has been read, also where P is of no use)
+
+        mbar_wait(&g_full, it & 1, dead, timeouts);
+        tc_fence_after();
+#pragma unroll
+        for (int q = 0; q < kChunks; q++) {
+          const int e0 = q * 16, c1 = c0 + part * kCols + e0;
+          uint32_t gr[16];
+          tmem_load16(g_at + e0, gr);
+          tmem_loaded(gr);
+          float ds[16];
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            float4 d4 = make_float4(row_stat.y, row_stat.y, row_stat.y, row_stat.y);
+            if (FOR_KEYS) d4 = *reinterpret_cast<const float4 *>(stats + kTileRows + e0 + e);
+#pragma unroll
+            for (int k = 0; k < 4; k += 2) {
+              const float2 minus = k ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);
+              const float2 dp = add2(make_float2(__uint_as_float(gr[e + k]), __uint_as_float(gr[e + k + 1])), minus);
+              const float2 d2 = mul2(make_float2(p[e0 + e + k], p[e0 + e + k + 1]), dp);
+              ds[e + k] = d2.x;
+              ds[e + k + 1] = d2.y;
+            }
+          }
+          if (f != 3) {  // what is hidden may have met anything in V
+#pragma unroll
+            for (int e = 0; e < 16; e++) ds[e] = p[e0 + e] == 0.f ? 0.f : ds[e];
           }
           if (table_sums) {
             // One run of columns per bucket: its sums stay in registers until the bucket changes.
-            if (far) {
+            const int d0 = c1 - (view.start + x), far_at = far_side<FOR_KEYS>(a, d0);
+            if (far_at >= 0) {
               const int n_now = bucket_lut[far_at];
               if (n_now != bucket_now) flush_bucket(n_now);
               float2 t = both(0.f);
 #pragma unroll
-              for (int e = 0; e < 16; e++) t = add2(t, make_float2(ds[e], p[e]));
+              for (int e = 0; e < 16; e++) t = add2(t, make_float2(ds[e], p[e0 + e]));
               bucket_sum = add2(bucket_sum, t);
             } else {
               const unsigned char *at = bucket_lut + d0 + a.reach + kLutPad;
@@ -321,7 +361,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
               for (int e = 0; e < 16; e++) {
                 const int n_now = at[e];
                 if (n_now != bucket_now) flush_bucket(n_now);
-                bucket_sum = add2(bucket_sum, make_float2(ds[e], p[e]));
+                bucket_sum = add2(bucket_sum, make_float2(ds[e], p[e0 + e]));
               }
             }
           }
@@ -330,24 +370,19 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           for (int e = 0; e < 8; e++) {
             float2 y = make_float2(ds[2 * e], ds[2 * e + 1]);
             if (CAP) {  // d tanh = 1 - tanh^2
-              const float2 t = mul2(make_float2(x16[2 * e], x16[2 * e + 1]), uncap);
+              const float2 t = mul2(make_float2(x_all[CAP ? e0 + 2 * e : 0], x_all[CAP ? e0 + 2 * e + 1 : 0]), uncap);
               y = mul2(y, fma2(make_float2(-t.x, -t.y), t, both(1.f)));
             }
             packed[e] = pack_bf16(y.x, y.y);
           }
           tmem_store8(g_at + e0, packed);
-          if (FOR_KEYS) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) packed[e] = pack_bf16(p[2 * e], p[2 * e + 1]);
-            tmem_store8(s_at + e0, packed);
-          }
         }
         if (n == tail) {
           // Rows of K that no query reaches may hold anything, and 0 * NaN is NaN.
           const int first = view.end - c0;
-          for (int e = half * 128 + row; e < (kStreamRows - first) * NB * 8; e += kGroup) {
+          for (int e = part * 128 + row; e < (kTileRows - first) * NB * 8; e += kRowThreads) {
             const int r = first + e / (NB * 8), q = e % (NB * 8);
-            *reinterpret_cast<uint4 *>(ring + s * Shape::kStage + (q / 8) * kStreamBlock + r * 128 + (q % 8) * 16) =
+            *reinterpret_cast<uint4 *>(ring + s * Shape::kStage + (q / 8) * kBlockBytes + r * 128 + (q % 8) * 16) =
                 make_uint4(0, 0, 0, 0);
           }
           fence_async_smem();
@@ -355,18 +390,20 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         tmem_stored();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[w]);
+        if (lane == 0) mbar_arrive(&d_full);
       }
     }
     if (table_sums) flush_bucket(0);
     mbar_wait(&acc_full, 0, dead, timeouts);
     tc_fence_after();
-    // FOR_KEYS: the first group stores dK, the second dV; else all share the columns of dQ.
-    const Heads &to = !FOR_KEYS ? a.dq : w == 0 ? a.dk : a.dv;
-    const float by = FOR_KEYS && w == 1 ? 1.f : a.scale;
-    const uint32_t acc_at = tmem + lane_base + (FOR_KEYS && w == 1 ? 384 : 256);
+    // FOR_KEYS: the first half of the row warps stores dK, the other dV; else all share the columns of dQ.
+    constexpr int kSharers = FOR_KEYS ? PARTS / 2 : PARTS;
+    const bool second = FOR_KEYS && part >= PARTS / 2;
+    const Heads &to = !FOR_KEYS ? a.dq : second ? a.dv : a.dk;
+    const float by = second ? 1.f : a.scale;
+    const uint32_t acc_at = tmem + lane_base + (second ? 384 : 256);
     __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(to.ptr) + b * to.batch + static_cast<long long>(x) * to.token + unit * to.head;
-    for (int c = 32 * (FOR_KEYS ? half : w * HALVES + half); c < a.dim; c += 32 * HALVES * (FOR_KEYS ? 1 : 2)) {
+    for (int c = 32 * (part % kSharers); c < a.dim; c += 32 * kSharers) {
       uint32_t o[32];
       if (it >= 0) {
         tmem_load32(acc_at + c, o);
@@ -383,7 +420,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     }
     tc_fence_before();
   } else {
-    if (HALVES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBwdOtherRegs));
+    if (PARTS == 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBwdOtherRegs));
     if (warp == kBwdLoadWarp) {
       if (lane == 0) {
         const int x_head = FOR_KEYS ? hk : unit;
@@ -404,8 +441,8 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             unsigned char *stage = ring + s * Shape::kStage;
             mbar_expect_tx(&full[s], Shape::kStage + (FOR_KEYS ? kStatsBytes : 0));
             for (int c = 0; c < NB; c++) {
-              tma_load_rows(stage + c * kStreamBlock, &maps.u, &full[s], c * kBlockCols, n * kStreamRows, head, b);
-              tma_load_rows(stage + (NB + c) * kStreamBlock, &maps.w, &full[s], c * kBlockCols, n * kStreamRows, head, b);
+              tma_load_rows(stage + c * kBlockBytes, &maps.u, &full[s], c * kBlockCols, n * kTileRows, head, b);
+              tma_load_rows(stage + (NB + c) * kBlockBytes, &maps.w, &full[s], c * kBlockCols, n * kTileRows, head, b);
             }
             if (FOR_KEYS)
               bulk_load(smem + Shape::kStats + s * kStatsBytes, stats_tile(a, b, head, n), kStatsBytes, &full[s]);
@@ -419,26 +456,28 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       }
     } else if (warp == kBwdMmaWarp) {
       const int k_steps = (a.dim + 15) / 16, n_cols = k_steps * 16;
-      const uint32_t idesc_s = mma_desc(kStreamRows, false), idesc_acc = mma_desc(n_cols, true);
+      const uint32_t idesc_s = mma_desc(kTileRows, false), idesc_acc = mma_desc(n_cols, true);
       const uint64_t xd = desc_k_major(smem_u32(smem + Shape::kX)), yd = desc_k_major(smem_u32(smem + Shape::kY));
-      const uint64_t u_desc = desc_k_major(smem_u32(ring)), u_desc_mn = desc_mn_major(smem_u32(ring), kStreamBlock);
-      constexpr uint32_t kStageStep = Shape::kStage >> 4, kW = (NB * kStreamBlock) >> 4;  // in descriptor units
-      auto accumulate = [&](int it) {  // with what the row threads made of tile `it`
-        const int s = it % ST, w = it & 1;
-        mbar_wait(&p_full[w], (it >> 1) & 1, dead, timeouts);
-        tc_fence_after();
-        const uint64_t ud = u_desc_mn + s * kStageStep, wd = ud + kW;
-        const uint32_t p_at = tmem + w * 128;
+      const uint64_t u_desc = desc_k_major(smem_u32(ring)), u_desc_mn = desc_mn_major(smem_u32(ring), kBlockBytes);
+      constexpr uint32_t kStageStep = Shape::kStage >> 4, kW = (NB * kBlockBytes) >> 4;  // in descriptor units
+      // TMEM: S 0, G 128, dK or dQ 256, dV 384
+      auto scores = [&](uint32_t to, uint64_t ad, uint64_t bd, uint64_t *bar) {
         if (elect_lane()) {
 #pragma unroll
-          for (int k = 0; k < kStreamRows / 16; k++)
-            mma_ts(tmem + 256, p_at + 64 + k * 16, ud + k * (2048 >> 4), idesc_acc, it > 0 || k > 0);
-          if (FOR_KEYS) {
-#pragma unroll
-            for (int k = 0; k < kStreamRows / 16; k++)
-              mma_ts(tmem + 384, p_at + k * 16, wd + k * (2048 >> 4), idesc_acc, it > 0 || k > 0);
+          for (int k = 0; k < NB * 4; k++) {
+            const int at = (k / 4) * (kBlockBytes >> 4) + (k % 4) * 2;
+            if (k < k_steps) mma_ss(tmem + to, ad + at, bd + at, idesc_s, k > 0);
           }
-          tc_commit(&empty[s]);
+          tc_commit(bar);
+        }
+        __syncwarp();
+      };
+      auto accumulate = [&](uint32_t to, uint32_t from, uint64_t bd, bool add, uint64_t *bar) {
+        if (elect_lane()) {
+#pragma unroll
+          for (int k = 0; k < kTileRows / 16; k++)
+            mma_ts(tmem + to, tmem + from + k * 16, bd + k * (2048 >> 4), idesc_acc, add || k > 0);
+          if (bar) tc_commit(bar);
         }
         __syncwarp();
       };
@@ -447,29 +486,37 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       for (int g = 0; g < heads_here && !*dead; g++)
         for (int n = 0; n < n_tiles; n++) {
           if (!flags[n]) continue;
-          const int s = it % ST, w = it & 1;
-          if (it >= 2) accumulate(it - 2);
-          mbar_wait(&full[s], (it / ST) & 1, dead, timeouts);
-          const uint64_t ud = u_desc + s * kStageStep, wd = ud + kW;
-          const uint32_t s_to = tmem + w * 128;
-          if (elect_lane()) {
-#pragma unroll
-            for (int k = 0; k < NB * 4; k++) {
-              const int xk = (k / 4) * (kBlockBytes >> 4) + (k % 4) * 2, uk = (k / 4) * (kStreamBlock >> 4) + (k % 4) * 2;
-              if (k < k_steps) mma_ss(s_to, xd + xk, ud + uk, idesc_s, k > 0);
-            }
-#pragma unroll
-            for (int k = 0; k < NB * 4; k++) {
-              const int xk = (k / 4) * (kBlockBytes >> 4) + (k % 4) * 2, uk = (k / 4) * (kStreamBlock >> 4) + (k % 4) * 2;
-              if (k < k_steps) mma_ss(s_to + 64, yd + xk, wd + uk, idesc_s, k > 0);
-            }
-            tc_commit(&s_full[w]);
+          const int s = it % ST, before = (it + ST - 1) % ST;
+          if (it > 0) {
+            mbar_wait(&p_full, (it - 1) & 1, dead, timeouts);  // S is free, P there
+            tc_fence_after();
+            if (FOR_KEYS) accumulate(384, 0, u_desc_mn + before * kStageStep + kW, it > 1, nullptr);
           }
-          __syncwarp();
+          if (ST > 1 || it == 0) {
+            mbar_wait(&full[s], (it / ST) & 1, dead, timeouts);
+            scores(0, xd, u_desc + s * kStageStep, &s_full);
+          }
+          if (it > 0) {
+            mbar_wait(&d_full, (it - 1) & 1, dead, timeouts);  // D is there
+            tc_fence_after();
+            accumulate(256, 128, u_desc_mn + before * kStageStep, it > 1, &empty[before]);
+          }
+          if (ST == 1 && it > 0) {  // one stage: the next tile comes when the last is done with
+            mbar_wait(&full[s], (it / ST) & 1, dead, timeouts);
+            scores(0, xd, u_desc + s * kStageStep, &s_full);
+          }
+          scores(128, yd, u_desc + s * kStageStep + kW, &g_full);
           it++;
         }
-      if (it >= 2) accumulate(it - 2);
-      if (it >= 1) accumulate(it - 1);
+      if (it > 0) {
+        const int s = (it - 1) % ST;
+        mbar_wait(&p_full, (it - 1) & 1, dead, timeouts);
+        tc_fence_after();
+        if (FOR_KEYS) accumulate(384, 0, u_desc_mn + s * kStageStep + kW, it > 1, nullptr);
+        mbar_wait(&d_full, (it - 1) & 1, dead, timeouts);
+        tc_fence_after();
+        accumulate(256, 128, u_desc_mn + s * kStageStep, it > 1, nullptr);
+      }
       if (elect_lane()) tc_commit(&acc_full);
       __syncwarp();
       if (*dead) {
@@ -485,25 +532,29 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     // comes from the rounded o) is taken off again in proportion to P.
     if (tid < kTileRows) {
       float e = 0.f, p = 0.f;
-      for (int n = 0; n < a.buckets; n++) {
-        float2 v = sums[n * kTileRows + tid];
+      for (int n = 0; n < a.buckets; n++)
 #pragma unroll
-        for (int k = 1; k < 2 * HALVES; k++) v = add2(v, sums[(k * a.buckets + n) * kTileRows + tid]);
-        sums[n * kTileRows + tid] = v;
-        e += v.x;
-        p += v.y;
-      }
+        for (int k = 0; k < PARTS; k++) {
+          const int at = (k * a.buckets + n) * kTileRows + tid;
+          e += sums[at];
+          p += __bfloat162float(p_sums[at]);
+        }
       e = p > 0.f ? e / p : 0.f;
       for (int n = 0; n < a.buckets; n++) {
-        const float2 v = sums[n * kTileRows + tid];
-        sums[n * kTileRows + tid].x = fmaf(-e, v.y, v.x);
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < PARTS; k++) {
+          const int at = (k * a.buckets + n) * kTileRows + tid;
+          sum += fmaf(-e, __bfloat162float(p_sums[at]), sums[at]);
+        }
+        sums[n * kTileRows + tid] = sum;
       }
     }
     __syncthreads();
     float *part = a.table_part + (static_cast<size_t>(unit) * a.table_parts + b * tiles + tile) * a.buckets;
     for (int n = warp; n < a.buckets; n += kBwdThreads / 32) {
       float v = 0.f;
-      for (int r = lane; r < kTileRows; r += 32) v += sums[n * kTileRows + r].x;
+      for (int r = lane; r < kTileRows; r += 32) v += sums[n * kTileRows + r];
       v = warp_sum(v);
       if (lane == 0) part[n] = v;
     }
@@ -514,18 +565,19 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   }
 }
 
-// The query pass with sums for the table: two stages, and two threads a row where their sums fit.
+// The query pass with sums for the table: four threads a row where their sums fit, else two.
 struct BwdTableShape {
-  int halves;
+  int parts;
   size_t smem;
 };
 inline BwdTableShape bwd_table_shape(const AttnArgs &a) {
   constexpr size_t kMaxSmem = 227 * 1024 - 2048;  // less the static part
-  BwdTableShape s = {2, 1024 + static_cast<size_t>(BwdShape<1, 2>::kRest) + bwd_rest(a, false, 2).total};
-  if (a.dim > kBlockCols || s.smem > kMaxSmem)
-    s = {1, 1024 + static_cast<size_t>(a.dim > kBlockCols ? BwdShape<2, 2>::kRest : BwdShape<1, 2>::kRest) + bwd_rest(a, false, 1).total};
-  if (s.smem > kMaxSmem) s.halves = 0;  // does not fit at all
-  return s;
+  const size_t ring = 1024 + static_cast<size_t>(a.dim > kBlockCols ? BwdShape<2, 1>::kRest : BwdShape<1, 2>::kRest);
+  for (int parts = a.dim > kBlockCols ? 2 : 4; parts >= 2; parts -= 2) {
+    const size_t smem = ring + bwd_rest(a, false, parts).total;
+    if (smem <= kMaxSmem) return {parts, smem};
+  }
+  return {0, 0};  // does not fit at all
 }
 
 template <bool FOR_KEYS>
@@ -542,43 +594,42 @@ int bwd_mma_launch(const AttnArgs &a, cudaStream_t st) {
   if (FOR_KEYS) {
     rc = k_map(&maps.x, a.k, kTileRows);
     if (!rc) rc = k_map(&maps.y, a.v, kTileRows);
-    if (!rc) rc = q_map(&maps.u, a.q, kStreamRows);
-    if (!rc) rc = q_map(&maps.w, a.dout, kStreamRows);
+    if (!rc) rc = q_map(&maps.u, a.q, kTileRows);
+    if (!rc) rc = q_map(&maps.w, a.dout, kTileRows);
   } else {
     rc = q_map(&maps.x, a.q, kTileRows);
     if (!rc) rc = q_map(&maps.y, a.dout, kTileRows);
-    if (!rc) rc = k_map(&maps.u, a.k, kStreamRows);
-    if (!rc) rc = k_map(&maps.w, a.v, kStreamRows);
+    if (!rc) rc = k_map(&maps.u, a.k, kTileRows);
+    if (!rc) rc = k_map(&maps.w, a.v, kTileRows);
   }
   DLB_REQUIRE(rc == 0, DLB_ERR_CUDA, "%s: tensor map refused (%d)", name, rc);
   unsigned int *timeouts = wait_timeouts_counter();
   DLB_REQUIRE(timeouts != nullptr, DLB_ERR_NO_DEVICE, "%s: no CUDA device", name);
-  auto launch = [&](auto kern, int ring_end, int halves) -> int {
-    const size_t smem = 1024 + ring_end + bwd_rest(a, FOR_KEYS, halves).total;
+  auto launch = [&](auto kern, int ring_end, int parts) -> int {
+    const size_t smem = 1024 + ring_end + bwd_rest(a, FOR_KEYS, parts).total;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     DLB_REQUIRE(e == cudaSuccess, DLB_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
     const int grid = ceil_div(FOR_KEYS ? a.kv_len : a.q_len, kTileRows) * (FOR_KEYS ? a.kv_heads : a.heads) * a.batch;
-    launch_pdl(kern, dim3(grid), dim3(halves == 2 ? BwdWarps<2>::kThreads : BwdWarps<1>::kThreads), smem, st, a, maps, timeouts);
+    launch_pdl(kern, dim3(grid), dim3(parts == 4 ? BwdWarps<4>::kThreads : BwdWarps<2>::kThreads), smem, st, a, maps, timeouts);
     DLB_LAUNCH_CHECK(name);
     return DLB_OK;
   };
   const bool cap = a.cap > 0.f;
-#define DLB_PICK(NB, ST, HALVES, BIAS)                                                                             \
-  (cap ? launch(attn_bwd_mma_kernel<NB, ST, HALVES, FOR_KEYS, true, BIAS>, BwdShape<NB, ST>::kRest, HALVES)        \
-       : launch(attn_bwd_mma_kernel<NB, ST, HALVES, FOR_KEYS, false, BIAS>, BwdShape<NB, ST>::kRest, HALVES))
+#define DLB_PICK(NB, ST, PARTS, BIAS)                                                                            \
+  (cap ? launch(attn_bwd_mma_kernel<NB, ST, PARTS, FOR_KEYS, true, BIAS>, BwdShape<NB, ST>::kRest, PARTS)        \
+       : launch(attn_bwd_mma_kernel<NB, ST, PARTS, FOR_KEYS, false, BIAS>, BwdShape<NB, ST>::kRest, PARTS))
   if constexpr (!FOR_KEYS) {
     if (a.table && a.dtable) {  // as bwd_table_shape has it
-      const BwdTableShape shape = bwd_table_shape(a);
-      if (a.dim > kBlockCols) return DLB_PICK(2, 2, 1, kTable);
-      return shape.halves == 2 ? DLB_PICK(1, 2, 2, kTable) : DLB_PICK(1, 2, 1, kTable);
+      if (a.dim > kBlockCols) return DLB_PICK(2, 1, 2, kTable);
+      return bwd_table_shape(a).parts == 4 ? DLB_PICK(1, 2, 4, kTable) : DLB_PICK(1, 2, 2, kTable);
     }
   }
   if (a.dim <= kBlockCols) {
-    if (a.table) return DLB_PICK(1, 4, 2, kTable);
-    return a.slopes ? DLB_PICK(1, 4, 2, kSlope) : DLB_PICK(1, 4, 2, kNoBias);
+    if (a.table) return DLB_PICK(1, 4, 4, kTable);
+    return a.slopes ? DLB_PICK(1, 4, 4, kSlope) : DLB_PICK(1, 4, 4, kNoBias);
   }
-  if (a.table) return DLB_PICK(2, 4, 2, kTable);
-  return a.slopes ? DLB_PICK(2, 4, 2, kSlope) : DLB_PICK(2, 4, 2, kNoBias);
+  if (a.table) return DLB_PICK(2, 2, 4, kTable);
+  return a.slopes ? DLB_PICK(2, 2, 4, kSlope) : DLB_PICK(2, 2, 4, kNoBias);
 #undef DLB_PICK
 }
 

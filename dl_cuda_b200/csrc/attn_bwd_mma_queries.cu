@@ -2,7 +2,7 @@
 #include "attn_bwd_mma.cuh"
 
 namespace dlb {
-bool attn_bwd_mma_room(const AttnArgs &a) { return !(a.table && a.dtable) || bwd_table_shape(a).halves > 0; }
+bool attn_bwd_mma_room(const AttnArgs &a) { return !(a.table && a.dtable) || bwd_table_shape(a).parts > 0; }
 
 int attn_bwd_mma_queries(const AttnArgs &a, cudaStream_t st) { return bwd_mma_launch<false>(a, st); }
 }  // namespace dlb

@@ -37,10 +37,10 @@ struct AttnArgs {
   int splits;
 };
 
-// Backward: what it needs of a query row, in tiles of 64 rows per (b, h): 64 times -lse * log2(e)
+// Backward: what it needs of a query row, in tiles of 128 rows per (b, h): 128 times -lse * log2(e)
 // (-infinity for a row that saw no key, and behind the last row: its probabilities are then
-// exp2(s - infinity) = 0), then 64 times -delta.  512 bytes a tile, on a 16-byte boundary for any q_len.
-constexpr int kStatRows = 64;
+// exp2(s - infinity) = 0), then 128 times -delta.  1 KB a tile, on a 16-byte boundary for any q_len.
+constexpr int kStatRows = 128;
 __host__ __device__ inline int stat_tiles(int q_len) { return (q_len + kStatRows - 1) / kStatRows; }
 __device__ __forceinline__ float *stats_tile(const AttnArgs &a, int b, int h, int tile) {
   return a.row_stats + ((static_cast<size_t>(b) * a.heads + h) * stat_tiles(a.q_len) + tile) * (2 * kStatRows);
