@@ -4,9 +4,10 @@
 // U, W (Q and dO of every head of the group; else K and V) past them in tiles of 128 rows:
 //     S = X U^T, G = Y W^T (TMEM) -> P = 2^(s - lse), D = P (G - delta), times the cap's derivative
 //     FOR_KEYS: dV += P W, dK += D U;   else dQ += D U                 (TMEM, scaled at the end)
-// with P and D written over S and G as bf16.  TMEM holds one S, one G and the sums, so the overlap is
-// within a tile: the row threads take the exponentials of S while the tensor cores make G and the last
-// tile's dK, and D while they make dV and the next S.  Tiles of 64 columns with two buffers each were
+// with P and D written over S and G as bf16.  The row threads take the exponentials of S while the tensor
+// cores make G and the last tile's dK, and D while they make dV and the next S.  TMEM holds S, G and the
+// sums; where it has room for more, S does not wait for P: the query pass keeps two S where the ring has four stages to feed them, the key pass of
+// heads up to 64 wide keeps P beside S.  Tiles of 64 columns with two buffers each were
 // slower: a product of 128 x 64 takes the tensor cores as long as one of 128 x 128 (measured with the
 // clock: 65 cycles for 16 inner columns either way), so S and G cost twice as much.
 //
@@ -87,11 +88,17 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   float *sums = reinterpret_cast<float *>(smem + Shape::kRest + rest.sums);  // [part][bucket][row]
   __nv_bfloat16 *p_sums = reinterpret_cast<__nv_bfloat16 *>(smem + Shape::kRest + rest.p_sums);
   unsigned char *flags = smem + Shape::kRest + rest.flags;
-  __shared__ uint64_t x_full, full[ST], empty[ST], s_full, g_full, p_full, d_full, acc_full, drain;
+  __shared__ uint64_t x_full, full[ST], empty[ST], s_full[2], g_full, p_full[2], d_full, v_full, acc_full, drain;
   __shared__ uint32_t tmem_slot;
   __shared__ int dead_flag, doc_range[2];
   __shared__ __align__(16) int doc_tile[kTileRows];
   volatile int *dead = &dead_flag;
+  // s_full and p_full come in pairs, used in turn: with two S the tensor cores may finish the next tile's
+  // before a row thread has seen this one's.
+  // TMEM: S 0, G 128, dK or dQ 256; then dV 384 and P over S or at 448, or the second S at 384
+  constexpr bool kTwoS = !FOR_KEYS && ST >= 4, kOwnP = FOR_KEYS && NB == 1;
+  constexpr uint32_t kAccX = 256, kAccY = 384, kG = 128;
+  constexpr uint32_t kPStep = kOwnP ? 8 : 16;  // columns of P per 16 of S
   const bool table_sums = BIAS == kTable && !FOR_KEYS && a.dtable != nullptr;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -101,9 +108,12 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    mbar_init(&s_full, 1);
+    for (int t = 0; t < 2; t++) {
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 4 * PARTS);
+    }
     mbar_init(&g_full, 1);
-    mbar_init(&p_full, 4 * PARTS);
+    mbar_init(&v_full, 1);
     mbar_init(&d_full, 4 * PARTS);
     mbar_init(&acc_full, 1);
     mbar_init(&drain, 1);
@@ -198,7 +208,8 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     const int part = warp >> 2, row = tid & 127, x = row0 + row;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     constexpr int kCols = kTileRows / PARTS, kChunks = kCols / 16;  // this thread's columns, 16 at a time
-    const uint32_t s_at = tmem + lane_base + part * kCols, g_at = s_at + 128;
+    const uint32_t s_base = tmem + lane_base + part * kCols, g_at = s_base + kG;
+    const uint32_t p_at = kOwnP ? tmem + lane_base + 448 + part * (kCols / 2) : s_base;
     const bool valid = x < len && (!FOR_KEYS || x < view.end);
     const int row_doc = (a.q_docs && valid) ? ld_co((FOR_KEYS ? a.kv_docs : a.q_docs) + static_cast<long long>(b) * len + x) : 0;
     // Stream rows [see_from, see_end) are visible to this row, as far as documents allow.
@@ -237,7 +248,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         int col_doc = 0;
         if (by_doc && part == 0) col_doc = ld_co(stream_docs + min(c0 + row, (FOR_KEYS ? a.q_len : a.kv_len) - 1));
         if (FOR_KEYS) mbar_wait(&full[s], (it / ST) & 1, dead, timeouts);  // the stage's statistics
-        mbar_wait(&s_full, it & 1, dead, timeouts);
+        mbar_wait(&s_full[it & 1], (it >> 1) & 1, dead, timeouts);
         if (by_doc) {  // the tile's document numbers
           named_bar_sync(2, kRowThreads);
           if (part == 0) doc_tile[row] = col_doc;
@@ -246,6 +257,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         tc_fence_after();
         const float *stats = reinterpret_cast<const float *>(smem + Shape::kStats + s * kStatsBytes) + part * kCols;
         // Probabilities, from S alone.  A chunk's P and D go over the first 8 columns of its own S and G.
+        const uint32_t s_at = s_base + (kTwoS && (it & 1) ? 384 : 0);
         float p[kCols], x_all[CAP ? kCols : 1];
 #pragma unroll
         for (int q = 0; q < kChunks; q++) {
@@ -311,13 +323,14 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             uint32_t packed[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) packed[e] = pack_bf16(p[e0 + 2 * e], p[e0 + 2 * e + 1]);
-            tmem_store8(s_at + e0, packed);
+            if (kOwnP && q == 0 && it > 0) mbar_wait(&v_full, (it - 1) & 1, dead, timeouts);  // the last P has been used
+            tmem_store8(p_at + q * kPStep, packed);
           }
         }
         if (FOR_KEYS) tmem_stored();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full);  // (S has been read, also where P is of no use)
+        if (lane == 0) mbar_arrive(&p_full[it & 1]);  // (S has been read, also where P is of no use)
 
         mbar_wait(&g_full, it & 1, dead, timeouts);
         tc_fence_after();
@@ -401,7 +414,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     const bool second = FOR_KEYS && part >= PARTS / 2;
     const Heads &to = !FOR_KEYS ? a.dq : second ? a.dv : a.dk;
     const float by = second ? 1.f : a.scale;
-    const uint32_t acc_at = tmem + lane_base + (second ? 384 : 256);
+    const uint32_t acc_at = tmem + lane_base + (second ? kAccY : kAccX);
     __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(to.ptr) + b * to.batch + static_cast<long long>(x) * to.token + unit * to.head;
     for (int c = 32 * (part % kSharers); c < a.dim; c += 32 * kSharers) {
       uint32_t o[32];
@@ -460,7 +473,6 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       const uint64_t xd = desc_k_major(smem_u32(smem + Shape::kX)), yd = desc_k_major(smem_u32(smem + Shape::kY));
       const uint64_t u_desc = desc_k_major(smem_u32(ring)), u_desc_mn = desc_mn_major(smem_u32(ring), kBlockBytes);
       constexpr uint32_t kStageStep = Shape::kStage >> 4, kW = (NB * kBlockBytes) >> 4;  // in descriptor units
-      // TMEM: S 0, G 128, dK or dQ 256, dV 384
       auto scores = [&](uint32_t to, uint64_t ad, uint64_t bd, uint64_t *bar) {
         if (elect_lane()) {
 #pragma unroll
@@ -472,50 +484,71 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         }
         __syncwarp();
       };
-      auto accumulate = [&](uint32_t to, uint32_t from, uint64_t bd, bool add, uint64_t *bar) {
+      auto accumulate = [&](uint32_t to, uint32_t from, uint32_t step, uint64_t bd, bool add, uint64_t *bar) {
         if (elect_lane()) {
 #pragma unroll
           for (int k = 0; k < kTileRows / 16; k++)
-            mma_ts(tmem + to, tmem + from + k * 16, bd + k * (2048 >> 4), idesc_acc, add || k > 0);
+            mma_ts(tmem + to, tmem + from + k * step, bd + k * (2048 >> 4), idesc_acc, add || k > 0);
           if (bar) tc_commit(bar);
         }
         __syncwarp();
       };
+      auto make_s = [&](int it) {
+        mbar_wait(&full[it % ST], (it / ST) & 1, dead, timeouts);
+        scores(kTwoS && (it & 1) ? 384 : 0, xd, u_desc + (it % ST) * kStageStep, &s_full[it & 1]);
+      };
+      auto make_g = [&](int it) { scores(kG, yd, u_desc + (it % ST) * kStageStep + kW, &g_full); };
+      auto add_dv = [&](int it) {  // P of tile `it` is there
+        accumulate(kAccY, kOwnP ? 448 : 0, kPStep, u_desc_mn + (it % ST) * kStageStep + kW, it > 0, kOwnP ? &v_full : nullptr);
+      };
+      auto add_x = [&](int it) {  // dK or dQ, when D of tile `it` is there
+        mbar_wait(&d_full, it & 1, dead, timeouts);
+        tc_fence_after();
+        accumulate(kAccX, kG, 16, u_desc_mn + (it % ST) * kStageStep, it > 0, &empty[it % ST]);
+      };
+      auto wait_p = [&](int it) {  // S of tile `it` has been read, its P is there
+        mbar_wait(&p_full[it & 1], (it >> 1) & 1, dead, timeouts);
+        tc_fence_after();
+      };
       mbar_wait(&x_full, 0, dead, timeouts);
-      int it = 0;
-      for (int g = 0; g < heads_here && !*dead; g++)
-        for (int n = 0; n < n_tiles; n++) {
-          if (!flags[n]) continue;
-          const int s = it % ST, before = (it + ST - 1) % ST;
+      int total = 0;
+      for (int n = 0; n < n_tiles; n++) total += flags[n] != 0;
+      total *= heads_here;
+      if (kTwoS && total > 0) make_s(0);
+      for (int it = 0; it < total && !*dead; it++) {
+        if (kTwoS) {
+          if (it > 0) add_x(it - 1);
+          make_g(it);
+          if (it + 1 < total) {
+            if (it > 0) wait_p(it - 1);
+            make_s(it + 1);
+          }
+        } else if (ST > 1) {
           if (it > 0) {
-            mbar_wait(&p_full, (it - 1) & 1, dead, timeouts);  // S is free, P there
-            tc_fence_after();
-            if (FOR_KEYS) accumulate(384, 0, u_desc_mn + before * kStageStep + kW, it > 1, nullptr);
+            wait_p(it - 1);
+            if (FOR_KEYS && !kOwnP) add_dv(it - 1);
           }
-          if (ST > 1 || it == 0) {
-            mbar_wait(&full[s], (it / ST) & 1, dead, timeouts);
-            scores(0, xd, u_desc + s * kStageStep, &s_full);
-          }
+          make_s(it);
           if (it > 0) {
-            mbar_wait(&d_full, (it - 1) & 1, dead, timeouts);  // D is there
-            tc_fence_after();
-            accumulate(256, 128, u_desc_mn + before * kStageStep, it > 1, &empty[before]);
+            if (FOR_KEYS && kOwnP) add_dv(it - 1);
+            add_x(it - 1);
           }
-          if (ST == 1 && it > 0) {  // one stage: the next tile comes when the last is done with
-            mbar_wait(&full[s], (it / ST) & 1, dead, timeouts);
-            scores(0, xd, u_desc + s * kStageStep, &s_full);
+          make_g(it);
+        } else {  // one stage: the next tile comes when the last is done with
+          if (it > 0) {
+            wait_p(it - 1);
+            if (FOR_KEYS) add_dv(it - 1);
+            add_x(it - 1);
           }
-          scores(128, yd, u_desc + s * kStageStep + kW, &g_full);
-          it++;
+          make_s(it);
+          make_g(it);
         }
-      if (it > 0) {
-        const int s = (it - 1) % ST;
-        mbar_wait(&p_full, (it - 1) & 1, dead, timeouts);
-        tc_fence_after();
-        if (FOR_KEYS) accumulate(384, 0, u_desc_mn + s * kStageStep + kW, it > 1, nullptr);
-        mbar_wait(&d_full, (it - 1) & 1, dead, timeouts);
-        tc_fence_after();
-        accumulate(256, 128, u_desc_mn + s * kStageStep, it > 1, nullptr);
+      }
+      if (total > 0) {
+        if (kTwoS && total > 1) wait_p(total - 2);
+        wait_p(total - 1);
+        if (FOR_KEYS) add_dv(total - 1);
+        add_x(total - 1);
       }
       if (elect_lane()) tc_commit(&acc_full);
       __syncwarp();
