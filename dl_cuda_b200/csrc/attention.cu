@@ -223,8 +223,10 @@ int launch_bwd(const AttnArgs &p, bool mma, cudaStream_t st) {
     DLB_LAUNCH_CHECK("attn_row_stats");
   }
   if (mma) {
-    if (int s = attn_bwd_mma_keys(p, st)) return s;
-    if (int s = attn_bwd_mma_queries(p, st)) return s;
+    BwdMaps maps;
+    if (int s = make_bwd_maps(p, &maps)) return s;
+    if (int s = attn_bwd_mma_keys(p, maps, st)) return s;
+    if (int s = attn_bwd_mma_queries(p, maps, st)) return s;
     return launch_table_sum(p, st);
   }
   return by_width(p.dim, [&](auto width) -> int {

@@ -41,9 +41,6 @@ struct BwdShape {
   static constexpr int kStats = kRing + ST * kStage, kRest = kStats + ST * kStatsBytes;
 };
 
-struct BwdMaps {
-  CUtensorMap x, y, u, w;
-};
 
 // Where in the padded tables a warp's 16 pairs from distance d0 on (FOR_KEYS: back) lie when all its
 // rows' pairs are beyond the reach; -1 when some are not (then all are near enough for the padding).
@@ -122,10 +119,10 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   }
   if (warp == kBwdMmaWarp) tmem_alloc(&tmem_slot, 512);
   if (tid == kBwdLoadWarp * 32) {
-    prefetch_map(&maps.x);
-    prefetch_map(&maps.y);
-    prefetch_map(&maps.u);
-    prefetch_map(&maps.w);
+    prefetch_map(&(FOR_KEYS ? maps.k : maps.q));
+    prefetch_map(&(FOR_KEYS ? maps.v : maps.dout));
+    prefetch_map(&(FOR_KEYS ? maps.q : maps.k));
+    prefetch_map(&(FOR_KEYS ? maps.dout : maps.v));
   }
   pdl_prologue();
 
@@ -439,8 +436,8 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         const int x_head = FOR_KEYS ? hk : unit;
         mbar_expect_tx(&x_full, 2 * NB * kBlockBytes);
         for (int c = 0; c < NB; c++) {
-          tma_load_rows(smem + Shape::kX + c * kBlockBytes, &maps.x, &x_full, c * kBlockCols, row0, x_head, b);
-          tma_load_rows(smem + Shape::kY + c * kBlockBytes, &maps.y, &x_full, c * kBlockCols, row0, x_head, b);
+          tma_load_rows(smem + Shape::kX + c * kBlockBytes, &(FOR_KEYS ? maps.k : maps.q), &x_full, c * kBlockCols, row0, x_head, b);
+          tma_load_rows(smem + Shape::kY + c * kBlockBytes, &(FOR_KEYS ? maps.v : maps.dout), &x_full, c * kBlockCols, row0, x_head, b);
         }
         int it = 0;
         for (int g = 0; g < heads_here && !*dead; g++) {
@@ -454,8 +451,8 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             unsigned char *stage = ring + s * Shape::kStage;
             mbar_expect_tx(&full[s], Shape::kStage + (FOR_KEYS ? kStatsBytes : 0));
             for (int c = 0; c < NB; c++) {
-              tma_load_rows(stage + c * kBlockBytes, &maps.u, &full[s], c * kBlockCols, n * kTileRows, head, b);
-              tma_load_rows(stage + (NB + c) * kBlockBytes, &maps.w, &full[s], c * kBlockCols, n * kTileRows, head, b);
+              tma_load_rows(stage + c * kBlockBytes, &(FOR_KEYS ? maps.q : maps.k), &full[s], c * kBlockCols, n * kTileRows, head, b);
+              tma_load_rows(stage + (NB + c) * kBlockBytes, &(FOR_KEYS ? maps.dout : maps.v), &full[s], c * kBlockCols, n * kTileRows, head, b);
             }
             if (FOR_KEYS)
               bulk_load(smem + Shape::kStats + s * kStatsBytes, stats_tile(a, b, head, n), kStatsBytes, &full[s]);
@@ -614,28 +611,8 @@ inline BwdTableShape bwd_table_shape(const AttnArgs &a) {
 }
 
 template <bool FOR_KEYS>
-int bwd_mma_launch(const AttnArgs &a, cudaStream_t st) {
+int bwd_mma_launch(const AttnArgs &a, const BwdMaps &maps, cudaStream_t st) {
   const char *name = FOR_KEYS ? "attn_bwd_mma (keys)" : "attn_bwd_mma (queries)";
-  BwdMaps maps;
-  auto q_map = [&](CUtensorMap *m, const Heads &h, int rows) {
-    return make_heads_map(m, h.ptr, a.dim, a.q_len, a.heads, a.batch, h.token, h.head, h.batch, rows);
-  };
-  auto k_map = [&](CUtensorMap *m, const Heads &h, int rows) {
-    return make_heads_map(m, h.ptr, a.dim, a.kv_len, a.kv_heads, a.batch, h.token, h.head, h.batch, rows);
-  };
-  int rc;
-  if (FOR_KEYS) {
-    rc = k_map(&maps.x, a.k, kTileRows);
-    if (!rc) rc = k_map(&maps.y, a.v, kTileRows);
-    if (!rc) rc = q_map(&maps.u, a.q, kTileRows);
-    if (!rc) rc = q_map(&maps.w, a.dout, kTileRows);
-  } else {
-    rc = q_map(&maps.x, a.q, kTileRows);
-    if (!rc) rc = q_map(&maps.y, a.dout, kTileRows);
-    if (!rc) rc = k_map(&maps.u, a.k, kTileRows);
-    if (!rc) rc = k_map(&maps.w, a.v, kTileRows);
-  }
-  DLB_REQUIRE(rc == 0, DLB_ERR_CUDA, "%s: tensor map refused (%d)", name, rc);
   unsigned int *timeouts = wait_timeouts_counter();
   DLB_REQUIRE(timeouts != nullptr, DLB_ERR_NO_DEVICE, "%s: no CUDA device", name);
   auto launch = [&](auto kern, int ring_end, int parts) -> int {

@@ -2,5 +2,5 @@
 #include "attn_bwd_mma.cuh"
 
 namespace dlb {
-int attn_bwd_mma_keys(const AttnArgs &a, cudaStream_t st) { return bwd_mma_launch<true>(a, st); }
+int attn_bwd_mma_keys(const AttnArgs &a, const BwdMaps &maps, cudaStream_t st) { return bwd_mma_launch<true>(a, maps, st); }
 }  // namespace dlb

@@ -106,8 +106,12 @@ __host__ __device__ inline int lut_floats(int reach) { return 2 * (reach + kLutP
 bool attn_mma_fits(const AttnArgs &a, bool backward);
 int attn_fwd_mma(const AttnArgs &a, cudaStream_t st);
 bool attn_bwd_mma_room(const AttnArgs &a);  // do the sums for the table fit?
-int attn_bwd_mma_keys(const AttnArgs &a, cudaStream_t st);
-int attn_bwd_mma_queries(const AttnArgs &a, cudaStream_t st);
+struct BwdMaps {
+  CUtensorMap q, k, v, dout;
+};
+int make_bwd_maps(const AttnArgs &a, BwdMaps *maps);
+int attn_bwd_mma_keys(const AttnArgs &a, const BwdMaps &maps, cudaStream_t st);
+int attn_bwd_mma_queries(const AttnArgs &a, const BwdMaps &maps, cudaStream_t st);
 
 // Waits for copies or MMAs still in flight after another wait of the CTA gave up (bounded as well).
 __device__ __forceinline__ void drain_wait(uint64_t *bar, unsigned parity) {

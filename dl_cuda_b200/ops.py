@@ -6,7 +6,8 @@ nothing is allocated inside a timed region) or are allocated here.
 """
 from __future__ import annotations
 
-from ctypes import byref
+import ctypes
+import struct
 
 import torch
 
@@ -283,66 +284,60 @@ def softmax_bwd(dy, s, dx=None, scale=1.0):
 
 
 # --- attention ------------------------------------------------------------------------------
-def _heads(t):
-    """capi.Heads of a [batch, token, head, column] tensor (any strides, columns contiguous)."""
-    stride = t.stride()
-    if stride[3] != 1 and t.shape[3] > 1:
-        raise ValueError("columns must be contiguous")
-    return capi.Heads(t.data_ptr(), stride[0], stride[1], stride[2])
+# A call with small tensors is over before Python has made it, so this part builds the argument blocks with
+# struct.pack instead of ctypes structures and checks tensors by the cheapest means; the blocks are laid
+# out as capi.Attn and capi.AttnGrad are.
+_HEADS = "Pqqq"
+_ATTN = struct.Struct("@8i2f2i8P" + 4 * _HEADS + "P")
+_ATTN_GRAD = struct.Struct("@" + 4 * _HEADS + "P")
+assert _ATTN.size == ctypes.sizeof(capi.Attn) and _ATTN_GRAD.size == ctypes.sizeof(capi.AttnGrad)
 
 
-def _int_array(name, t, shape, device):
+def _current_device(t):
+    """The index of t's device, which has to be the current one."""
+    device = t.get_device()
+    if device < 0:
+        raise ValueError("device tensors required: the kernels have no CPU path")
+    if device != torch.cuda.current_device():
+        raise ValueError(f"tensors are on cuda:{device}, the current device is cuda:{torch.cuda.current_device()}")
+    return device
+
+
+def _stream(device):
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _address(name, t, dtype, shape, device):
+    """Address of a contiguous tensor of this type, shape and place; 0 for None."""
     if t is None:
-        return None
-    if t.dtype is not torch.int32 or t.shape != shape:
-        raise ValueError(f"{name} must be torch.int32 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-    return _array(name, t, device)
-
-
-def _float_array(name, t, shape, device):
-    if t is None:
-        return None
-    if t.dtype is not torch.float32 or t.shape != shape:
-        raise ValueError(f"{name} must be torch.float32 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-    return _array(name, t, device)
-
-
-def _array(name, t, device):
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
+        return 0
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {dtype} {tuple(shape)} on cuda:{device}, "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _like(name, t, q):
-    """t has q's shape, type and device."""
-    if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:
-        raise ValueError(f"{name} must be {q.dtype} {tuple(q.shape)} on {q.device}, "
+def _strided(name, t, dtype, shape, device):
+    """Address and strides of a [batch, token, head, column] tensor of this type, shape and place."""
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device:
+        raise ValueError(f"{name} must be {dtype} {tuple(shape)} on cuda:{device}, "
                          f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+    batch, token, head, column = t.stride()
+    if column != 1 and shape[3] > 1:
+        raise ValueError(f"the columns of {name} must be contiguous")
+    return t.data_ptr(), batch, token, head
 
 
-def _on_current_device(t):
-    if not t.is_cuda:
-        raise ValueError("device tensors required: the kernels have no CPU path")
-    if t.get_device() != torch.cuda.current_device():
-        raise ValueError(f"tensors are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-
-
-def _attn_args(q, k, v, o, lse, scale, cap, causal, kv_lens, q_start, prefix, q_docs, kv_docs, slopes, table, bucket_of):
-    """The argument block; shapes, types and places are checked here, values by the library."""
-    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
-        raise ValueError("q, k and v are [batch, token, head, column]")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError(f"q is {q.dtype}, k {k.dtype}, v {v.dtype}")
-    batch, q_len, heads, d = q.shape
-    _, kv_len, kv_heads, _ = k.shape
-    if k.shape != v.shape or k.shape[0] != batch or k.shape[3] != d:
-        raise ValueError(f"shapes do not fit: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-    _on_current_device(q)
-    device = q.device
-    if k.device != device or v.device != device:
-        raise ValueError(f"q, k and v are on {device}, {k.device} and {v.device}")
+def _attn_block(q, k, v, o, lse, device, scale, cap, causal, kv_lens, q_start, prefix, q_docs, kv_docs, slopes, table,
+                bucket_of):
+    """The packed argument block (o and lse: address and strides, address); values are checked by the library."""
+    q_shape, k_shape, dtype = q.shape, k.shape, q.dtype
+    if k.dtype is not dtype or v.dtype is not dtype:
+        raise TypeError(f"q is {dtype}, k {k.dtype}, v {v.dtype}")
+    if len(k_shape) != 4 or k_shape[0] != q_shape[0] or k_shape[3] != q_shape[3]:
+        raise ValueError(f"shapes do not fit: q {tuple(q_shape)}, k {tuple(k_shape)}, v {tuple(v.shape)}")
+    batch, q_len, heads, d = q_shape
+    _, kv_len, kv_heads, _ = k_shape
     if (table is None) != (bucket_of is None):
         raise ValueError("table and bucket_of go together")
     buckets = reach = 0
@@ -350,30 +345,27 @@ def _attn_args(q, k, v, o, lse, scale, cap, causal, kv_lens, q_start, prefix, q_
         if table.dim() != 2 or bucket_of.dim() != 1 or bucket_of.numel() % 2 == 0:
             raise ValueError("table is [heads, buckets], bucket_of has 2 * max_distance + 1 entries")
         buckets, reach = table.shape[1], bucket_of.numel() // 2
-    per_batch = (batch,)
-    return capi.Attn(
+    i32, f32 = torch.int32, torch.float32
+    return _ATTN.pack(
         batch, heads, kv_heads, q_len, kv_len, d, dtype_of(q), 1 if causal else 0, d ** -0.5 if scale is None else scale, cap,
-        buckets, reach, _int_array("kv_lens", kv_lens, per_batch, device), _int_array("q_start", q_start, per_batch, device),
-        _int_array("prefix", prefix, per_batch, device), _int_array("q_docs", q_docs, (batch, q_len), device),
-        _int_array("kv_docs", kv_docs, (batch, kv_len), device), _float_array("slopes", slopes, (heads,), device),
-        _float_array("table", table, (heads, buckets), device),
-        _int_array("bucket_of", bucket_of, (2 * reach + 1,), device), _heads(q), _heads(k), _heads(v), _heads(o), lse)
+        buckets, reach,
+        _address("kv_lens", kv_lens, i32, (batch,), device), _address("q_start", q_start, i32, (batch,), device),
+        _address("prefix", prefix, i32, (batch,), device), _address("q_docs", q_docs, i32, (batch, q_len), device),
+        _address("kv_docs", kv_docs, i32, (batch, kv_len), device), _address("slopes", slopes, f32, (heads,), device),
+        _address("table", table, f32, (heads, buckets), device),
+        _address("bucket_of", bucket_of, i32, (2 * reach + 1,), device),
+        *_strided("q", q, dtype, q_shape, device), *_strided("k", k, dtype, k_shape, device),
+        *_strided("v", v, dtype, k_shape, device), *o, lse)
 
 
-def _lse(t, shape, device):
-    if t.shape != shape or t.dtype != torch.float32 or t.device != device or not t.is_contiguous():
-        raise ValueError(f"lse must be contiguous torch.float32 {shape} on {device}")
-    return t.data_ptr()
-
-
-def _space(workspace, need, device):
+def _space(workspace, need, like):
     """(address, bytes) of the given workspace, or of a fresh one; keep the third alive over the call."""
     if workspace is None:
         if need == 0:
             return None, 0, None
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    elif workspace.device != device or not workspace.is_contiguous():
-        raise ValueError(f"workspace must be contiguous on {device}")
+        workspace = like.new_empty((need,), dtype=torch.uint8)
+    elif workspace.get_device() != like.get_device() or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be contiguous on {like.device}")
     return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
 
 
@@ -384,22 +376,26 @@ def attn_fwd(q, k, v, scale=None, cap=0.0, causal=False, kv_lens=None, q_start=N
     sees, and how its scores are changed, is told at dlb_attn_fwd in the header.  A cache longer than kv_len goes
     in as a slice; for one token against a cache pass q_start = kv_lens - 1.  All tensors on the current device,
     on whose current stream the call runs."""
-    if q.dim() != 4:
+    shape = q.shape
+    if len(shape) != 4:
         raise ValueError("q is [batch, token, head, column]")
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-    _like("out", out, q)
-    at = None
-    if want_lse:
-        shape = (q.shape[0], q.shape[2], q.shape[1])
-        lse = torch.empty(shape, dtype=torch.float32, device=q.device) if lse is None else lse
-        at = _lse(lse, shape, q.device)
-    else:
+    device = _current_device(q)
+    if out is None:
+        out = q.new_empty(shape)
+    to = _strided("out", out, q.dtype, shape, device)
+    lse_to = 0
+    if not want_lse:
         lse = None
-    a = _attn_args(q, k, v, out, at, scale, cap, causal, kv_lens, q_start, prefix, q_docs, kv_docs, slopes, table,
-                   bucket_of)
-    ref, library = byref(a), capi.lib()
-    space, size, _keep = _space(workspace, library.dlb_attn_fwd_workspace_bytes(ref) if workspace is None else 0, q.device)
-    check(library.dlb_attn_fwd(ref, space, size, current_stream()))
+    elif lse is None:
+        lse = q.new_empty((shape[0], shape[2], shape[1]), dtype=torch.float32)
+        lse_to = lse.data_ptr()
+    else:
+        lse_to = _address("lse", lse, torch.float32, (shape[0], shape[2], shape[1]), device)
+    block = _attn_block(q, k, v, to, lse_to, device, scale, cap, causal, kv_lens, q_start, prefix, q_docs, kv_docs,
+                        slopes, table, bucket_of)
+    library = capi.lib()
+    space, size, _keep = _space(workspace, library.dlb_attn_fwd_workspace_bytes(block) if workspace is None else 0, q)
+    check(library.dlb_attn_fwd(block, space, size, _stream(device)))
     return out, lse
 
 
@@ -408,25 +404,28 @@ def attn_bwd(dout, q, k, v, o, lse, scale=None, cap=0.0, causal=False, kv_lens=N
              want_dtable=True, workspace=None):
     """Returns (dq, dk, dv, dtable) from dout, with o and lse as attn_fwd returned them for the same arguments;
     dtable (fp32 [heads, buckets]) is None without a table or when want_dtable is False."""
-    if q.dim() != 4:
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 4:
         raise ValueError("q is [batch, token, head, column]")
-    device = q.device
-    dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=device) if g is None else g
-                  for g, x in ((dq, q), (dk, k), (dv, v)))
-    for name, t, like in (("dout", dout, q), ("o", o, q), ("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
-        _like(name, t, like)
-    at = _lse(lse, (q.shape[0], q.shape[2], q.shape[1]), device)
-    a = _attn_args(q, k, v, o, at, scale, cap, causal, kv_lens, q_start, prefix, q_docs, kv_docs, slopes, table,
-                   bucket_of)
-    if table is not None and want_dtable:
-        dtable = torch.empty_like(table) if dtable is None else dtable
-        to = _float_array("dtable", dtable, table.shape, device)
+    device = _current_device(q)
+    block = _attn_block(q, k, v, _strided("o", o, dtype, shape, device),
+                        _address("lse", lse, torch.float32, (shape[0], shape[2], shape[1]), device), device, scale, cap,
+                        causal, kv_lens, q_start, prefix, q_docs, kv_docs, slopes, table, bucket_of)
+    dq = q.new_empty(shape) if dq is None else dq
+    dk = q.new_empty(k.shape) if dk is None else dk
+    dv = q.new_empty(k.shape) if dv is None else dv
+    table_to = 0
+    if table is None or not want_dtable:
+        dtable = None
     else:
-        dtable = to = None
-    g = capi.AttnGrad(_heads(dout), _heads(dq), _heads(dk), _heads(dv), to)
-    ref, grad, library = byref(a), byref(g), capi.lib()
-    space, size, _keep = _space(workspace, library.dlb_attn_bwd_workspace_bytes(ref, grad) if workspace is None else 0, device)
-    check(library.dlb_attn_bwd(ref, grad, space, size, current_stream()))
+        dtable = table.new_empty(table.shape) if dtable is None else dtable
+        table_to = _address("dtable", dtable, torch.float32, table.shape, device)
+    grad = _ATTN_GRAD.pack(*_strided("dout", dout, dtype, shape, device), *_strided("dq", dq, dtype, shape, device),
+                           *_strided("dk", dk, dtype, k.shape, device), *_strided("dv", dv, dtype, k.shape, device),
+                           table_to)
+    library = capi.lib()
+    space, size, _keep = _space(workspace, library.dlb_attn_bwd_workspace_bytes(block, grad) if workspace is None else 0, q)
+    check(library.dlb_attn_bwd(block, grad, space, size, _stream(device)))
     return dq, dk, dv, dtable
 
 
@@ -440,42 +439,40 @@ def rel_bucket_map(buckets, max_distance, both_directions=True):
 def rel_bias_fwd(table, bucket_of, scores=None, shape=None, q_start=0, dtype=torch.float32, out=None):
     """scores [batch, heads, q_len, kv_len] (or zeros of `shape` and `dtype`) plus the bucketed position bias of
     table [heads, buckets]; out may be scores."""
-    _on_current_device(table)
-    device = table.device
+    device = _current_device(table)
     if scores is not None:
         shape, dtype = scores.shape, scores.dtype
-        _array("scores", scores, device)
     if shape is None or len(shape) != 4 or table.dim() != 2 or bucket_of.dim() != 1 or bucket_of.numel() % 2 == 0:
         raise ValueError("scores (or a shape) are [batch, heads, q_len, kv_len], table [heads, buckets], bucket_of has "
                          "2 * max_distance + 1 entries")
     batch, heads, q_len, kv_len = shape
     buckets, reach = table.shape[1], bucket_of.numel() // 2
-    out = torch.empty(shape, dtype=dtype, device=device) if out is None else out
-    if out.shape != tuple(shape) or out.dtype != dtype:
-        raise ValueError(f"out must be {dtype} {tuple(shape)}, got {out.dtype} {tuple(out.shape)}")
-    check(capi.lib().dlb_rel_bias_fwd(ptr(scores), _float_array("table", table, (heads, buckets), device),
-                                      _int_array("bucket_of", bucket_of, (2 * reach + 1,), device),
-                                      _array("out", out, device), batch, heads, q_len, kv_len, q_start, buckets, reach,
-                                      dtype_of(out), current_stream()))
+    out = table.new_empty(shape, dtype=dtype) if out is None else out
+    check(capi.lib().dlb_rel_bias_fwd(_address("scores", scores, dtype, shape, device) or None,
+                                      _address("table", table, torch.float32, (heads, buckets), device),
+                                      _address("bucket_of", bucket_of, torch.int32, (2 * reach + 1,), device),
+                                      _address("out", out, dtype, shape, device), batch, heads, q_len, kv_len, q_start,
+                                      buckets, reach, dtype_of(out), _stream(device)))
     return out
 
 
 def rel_bias_bwd(dscores, bucket_of, buckets, q_start=0, dtable=None, workspace=None):
     """dtable [heads, buckets]: the sum of dscores [batch, heads, q_len, kv_len] over each bucket's positions."""
-    _on_current_device(dscores)
-    device = dscores.device
-    if dscores.dim() != 4 or bucket_of.dim() != 1 or bucket_of.numel() % 2 == 0:
+    device = _current_device(dscores)
+    shape = dscores.shape
+    if len(shape) != 4 or bucket_of.dim() != 1 or bucket_of.numel() % 2 == 0:
         raise ValueError("dscores are [batch, heads, q_len, kv_len], bucket_of has 2 * max_distance + 1 entries")
-    batch, heads, q_len, kv_len = dscores.shape
+    batch, heads, q_len, kv_len = shape
     reach = bucket_of.numel() // 2
-    dtable = torch.empty(heads, buckets, dtype=torch.float32, device=device) if dtable is None else dtable
+    dtable = dscores.new_empty((heads, buckets), dtype=torch.float32) if dtable is None else dtable
     library = capi.lib()
     need = library.dlb_rel_bias_bwd_workspace_bytes(batch, heads, q_len, kv_len, buckets) if workspace is None else 0
-    space, size, _keep = _space(workspace, need, device)
-    check(library.dlb_rel_bias_bwd(_array("dscores", dscores, device),
-                                   _int_array("bucket_of", bucket_of, (2 * reach + 1,), device),
-                                   _float_array("dtable", dtable, (heads, buckets), device), space, size, batch, heads,
-                                   q_len, kv_len, q_start, buckets, reach, dtype_of(dscores), current_stream()))
+    space, size, _keep = _space(workspace, need, dscores)
+    check(library.dlb_rel_bias_bwd(_address("dscores", dscores, dscores.dtype, shape, device),
+                                   _address("bucket_of", bucket_of, torch.int32, (2 * reach + 1,), device),
+                                   _address("dtable", dtable, torch.float32, (heads, buckets), device), space, size,
+                                   batch, heads, q_len, kv_len, q_start, buckets, reach, dtype_of(dscores),
+                                   _stream(device)))
     return dtable
 
 
