@@ -144,7 +144,7 @@ FwdPlan plan_fwd(const dlb_attn *a, const AttnArgs &args) {
   if (a->dtype == DLB_BF16 && attn_mma_fits(args, false)) p.kind = a->q_len >= kMmaQueries ? kMma : kStep;
   if (p.kind == kMma) return p;
   if (p.kind == kStep) {
-    p.splits = attn_step_splits(a->batch, a->kv_heads, a->q_len * group, a->kv_len);
+    p.splits = attn_step_splits(a->batch, a->kv_heads, a->q_len * group, a->kv_len, a->head_dim);
   } else {
     // Few queries: the heads that share a key/value head go into one tile, and the keys are split until
     // the grid fills the GPU twice (a share keeps at least two tiles).

@@ -50,9 +50,14 @@ __device__ __forceinline__ float col_sum(float v) {
 // Word x of a 16-byte vector (x is a compile-time constant where this is used).
 __device__ __forceinline__ uint32_t word(const uint4 &v, int x) { return x == 0 ? v.x : x == 1 ? v.y : x == 2 ? v.z : v.w; }
 
+// CTAs that share an SM: as many as leave a lane the registers for its loads (wide heads keep the next 16
+// keys in flight beside the current 16: 5.1 -> 5.7 TB/s with three CTAs instead of four and no such
+// loads; at 64 columns four CTAs with them are best).
+constexpr int step_ctas_per_sm(int nt, int nr) { return nr == 2 ? 2 : nt > 2 ? 3 : 4; }
+
 // NT: head_dim up to 32 * NT; NR: up to 8 * NR queries (rows of q x heads of the group) per CTA.
 template <int NT, int NR>
-__global__ void __launch_bounds__(kStepThreads, NR == 1 ? 4 : 3) attn_step_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kStepThreads, step_ctas_per_sm(NT, NR)) attn_step_kernel(const __grid_constant__ AttnArgs a) {
   pdl_prologue();
   constexpr int NB = (NT + 1) / 2;  // blocks of 64 columns of V and O
   constexpr int W = NB * 64, kRows = 8 * NR;
@@ -119,8 +124,8 @@ __global__ void __launch_bounds__(kStepThreads, NR == 1 ? 4 : 3) attn_step_kerne
         for (int e = 0; e < 4; e++) acc[y][n][t][e] = 0.f;
   }
 
-  for (int j0 = s0 + warp * kStepKeys; j0 < s1; j0 += turn) {
-    uint4 k[2][NT], v[NB][4];
+  uint4 k[2][NT];
+  auto load_k = [&](int j0) {
 #pragma unroll
     for (int u = 0; u < 2; u++) {
       const int j = j0 + 8 * u + g;
@@ -131,6 +136,10 @@ __global__ void __launch_bounds__(kStepThreads, NR == 1 ? 4 : 3) attn_step_kerne
         k[u][t] = j < s1 && col < a.dim ? ld_stream(src + col) : make_uint4(0, 0, 0, 0);
       }
     }
+  };
+  load_k(s0 + warp * kStepKeys);
+  for (int j0 = s0 + warp * kStepKeys; j0 < s1; j0 += turn) {
+    uint4 v[NB][4];
 #pragma unroll
     for (int x = 0; x < 4; x++) {
       const int j = j0 + 2 * c + (x & 1) + 8 * (x >> 1);
@@ -153,6 +162,10 @@ __global__ void __launch_bounds__(kStepThreads, NR == 1 ? 4 : 3) attn_step_kerne
         mma16816(s[y], k[0][t].x, k[1][t].x, k[0][t].y, k[1][t].y, q[y][t].x, q[y][t].y);
         mma16816(s[y], k[0][t].z, k[1][t].z, k[0][t].w, k[1][t].w, q[y][t].z, q[y][t].w);
       }
+    }
+    load_k(j0 + turn);  // the next turn's keys are on their way while this one is finished
+#pragma unroll
+    for (int y = 0; y < NR; y++) {
       if (a.cap > 0.f) cap_scores(s[y], cap);
 #pragma unroll
       for (int e = 0; e < 4; e++) {
@@ -284,13 +297,15 @@ namespace {
 int step_rows(int rows) { return rows <= 8 ? 8 : 16; }
 }  // namespace
 
-int attn_step_splits(int batch, int kv_heads, int rows, int kv_len) {
-  // Enough CTAs to fill the GPU once (four fit an SM) while a share keeps two turns of its warps, and to
-  // fill it four times, which evens out sequences of different lengths, while it keeps 16.
-  const long long ctas = static_cast<long long>(batch) * kv_heads * ceil_div(rows, step_rows(rows)), fill = 4ll * sm_count();
-  const long long once = std::min(ceil_div(fill, std::max(1ll, ctas)), kv_len / 128ll);
-  const long long often = std::min(ceil_div(4 * fill, std::max(1ll, ctas)), kv_len / 1024ll);
-  return static_cast<int>(std::max(1ll, std::min(std::max(once, often), 256ll)));
+int attn_step_splits(int batch, int kv_heads, int rows, int kv_len, int dim) {
+  // Four rounds of CTAs even out sequences of different lengths; where that would leave a share less than
+  // 1024 keys, as many rounds as it does not, or, under two, just one (of shares down to 128 keys): a last
+  // round that is nearly empty costs as much as a full one (one user, 65536 keys: 76 us with 1.15 rounds).
+  const long long ctas = std::max(1ll, static_cast<long long>(batch) * kv_heads * ceil_div(rows, step_rows(rows)));
+  const long long fill = static_cast<long long>(step_ctas_per_sm(ceil_div(dim, 32), step_rows(rows) / 8)) * sm_count();
+  const long long even = std::min(ceil_div(4 * fill, ctas), kv_len / 1024ll);
+  const long long one_round = std::min(fill / ctas, kv_len / 128ll);
+  return static_cast<int>(std::max(1ll, std::min(even * ctas >= 2 * fill ? even : one_round, 256ll)));
 }
 
 int attn_step(const AttnArgs &a, cudaStream_t st) {
