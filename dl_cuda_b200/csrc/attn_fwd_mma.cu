@@ -7,8 +7,8 @@
 // The two query tiles take turns: while one's softmax runs, the other's products do.  O stays in TMEM.
 // Exponentials are taken against a reference that moves only when a score leaves its range of 2^32, so
 // no maximum stands between a score and its exponential, and O is hardly ever rescaled; keys are walked
-// from the last tile to the first, which under a causal mask and a distance bias meets the largest
-// scores at once.  The sum behind the quotient adds the ROUNDED probabilities, so that a row's weights
+// from where the queries stand outwards, so that a distance bias shows its largest scores at once (from
+// the far end of a prefix, every tile moved the reference: 64 instead of 53 us for 3 x 1531 tokens).  The sum behind the quotient adds the ROUNDED probabilities, so that a row's weights
 // add up to one exactly as the product sees them (bf16 output 1.9e-3 instead of 2.3e-3 from the exact
 // one, of which the output's own rounding is 1.7e-3); lse comes from the unrounded ones.
 #include <algorithm>
@@ -114,6 +114,9 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     last_end[t] = r0 < a.q_len ? row_end(a, view, r1) : 0;
   }
   const int n_tiles = (max(last_end[0], last_end[1]) + kTileRows - 1) / kTileRows;
+  // From the tile where the queries stand to the first, then on from there: the nearest keys first.
+  const int here = max(0, min(n_tiles - 1, (view.start + min(a.q_len, row0 + 2 * kTileRows) - 1) / kTileRows));
+  auto walk = [&](int k) { return k <= here ? here - k : k; };
   if (a.q_docs) {
     if (warp < 2) {
       int lo = INT_MAX, hi = INT_MIN;
@@ -244,7 +247,8 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     float m = 0.f, sum = 0.f, sum_rounded = 0.f;
     bool settled = false;  // the row has weight, or a reference of its own
     int it = -1, done = 0;
-    for (int n = n_tiles - 1; n >= 0; n--) {
+    for (int k = 0; k < n_tiles; k++) {
+      const int n = walk(k);
       const int f = flags[n];
       if (!f) continue;
       it++;
@@ -382,7 +386,8 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           for (int c = 0; c < NB; c++)
             tma_load_rows(smem + (t * NB + c) * kBlockBytes, &maps.q, &q_full, c * kBlockCols, row0 + t * kTileRows, h, b);
         int it = 0;
-        for (int n = n_tiles - 1; n >= 0; n--) {
+        for (int k = 0; k < n_tiles; k++) {
+          const int n = walk(k);
           if (!flags[n]) continue;
           const int s = it % ST;
           const unsigned use = it / ST;
@@ -438,7 +443,8 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       };
       mbar_wait(&q_full, 0, dead, timeouts);
       int it = 0;
-      for (int n = n_tiles - 1; n >= 0; n--) {
+      for (int k = 0; k < n_tiles; k++) {
+        const int n = walk(k);
         const int f = flags[n];
         if (!f) continue;
         const int s = it % ST, before = (it + ST - 1) % ST;
