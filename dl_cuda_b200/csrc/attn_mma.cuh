@@ -15,23 +15,22 @@ enum { kNoBias = 0, kSlope = 1, kTable = 2 };          // kTable: with or withou
 
 // Capped scores times log2(e), L tanh(k x) with L = cap * log2(e), k = scale / cap, as odd polynomials:
 // least-squares fits of tanh(x) / x in x^2, reweighted until the relative error was level.
-//   |k x| <= 0.4: degree 3, error 1.0e-7, with the powers of k and L folded into the coefficients
-//                 (5 operations a score; scores up to 0.4 cap are the usual case)
-//   |k x| <= 1:   degree 6, error 5e-8 (1.2e-7 in fp32), 10 operations
+//   |k x| <= 0.25: degree 2, error 4e-7 of a score, powers of k and L folded into the coefficients (4
+//                  operations a score; scores up to a quarter of the cap are the usual case)
+//   |k x| <= 1:    degree 6, error 5e-8 (1.2e-7 in fp32), 10 operations
 // Anything larger takes two special-function operations per score.  A warp takes one road.
 struct CapCoef {
-  float c0, c1, c2, c3, k, out;
-  bool folded;  // k^7 must not fall under fp32's range
+  float c0, c1, c2, k, out;
+  bool folded;  // k^5 must not fall under fp32's range
 };
 __device__ __forceinline__ CapCoef cap_coef(float scale, float cap) {
   CapCoef c;
   c.k = scale / cap;
   c.out = cap * kLog2e;
   const float kk = c.k * c.k;
-  c.c0 = 0.9999998807907104f * c.k * c.out;
-  c.c1 = -0.33331358432769775f * kk * c.k * c.out;
-  c.c2 = 0.132709339261055f * kk * kk * c.k * c.out;
-  c.c3 = -0.04755208641290665f * kk * kk * kk * c.k * c.out;
+  c.c0 = 0.9999995827674866f * c.k * c.out;
+  c.c1 = -0.3332189917564392f * kk * c.k * c.out;
+  c.c2 = 0.12841492891311646f * kk * kk * c.k * c.out;
   c.folded = c.k > 1e-4f && c.k < 1e4f;
   return c;
 }
@@ -71,12 +70,11 @@ template <int N>
 __device__ __forceinline__ void cap_scores(float (&x)[N], const CapCoef &c) {
   // fmaxf drops NaN: a NaN score stays one on every road
   const float top = max_of<N, true>(x) * c.k;
-  if (c.folded && __all_sync(0xffffffffu, top <= 0.4f)) {
+  if (c.folded && __all_sync(0xffffffffu, top <= 0.25f)) {
 #pragma unroll
     for (int e = 0; e < N; e += 2) {
       const float2 v = make_float2(x[e], x[e + 1]), u = mul2(v, v);
-      float2 p = fma2(u, both(c.c3), both(c.c2));
-      p = fma2(p, u, both(c.c1));
+      float2 p = fma2(u, both(c.c2), both(c.c1));
       p = fma2(p, u, both(c.c0));
       p = mul2(p, v);
       x[e] = p.x;
