@@ -51,10 +51,11 @@ int check(const char *call, const dlb_attn *a) {
   constexpr int kMaxLen = 1 << 29;
   DLB_REQUIRE(a->q_len <= kMaxLen && a->kv_len <= kMaxLen, DLB_ERR_UNSUPPORTED, "%s: q_len=%d kv_len=%d", call,
               a->q_len, a->kv_len);
-  // rows are numbered in 64 bits, tiles of rows by a 32-bit grid
+  // rows and tiles of rows are counted by 32-bit grids
   const long long tiles = static_cast<long long>(a->batch) * a->heads * (ceil_div(std::max(a->q_len, a->kv_len), 64) + 1);
-  DLB_REQUIRE(tiles < (1ll << 31), DLB_ERR_UNSUPPORTED, "%s: batch=%d heads=%d lengths %d, %d make too many tiles", call,
-              a->batch, a->heads, a->q_len, a->kv_len);
+  const long long rows = static_cast<long long>(a->batch) * a->heads * std::max(a->q_len, 1);
+  DLB_REQUIRE(tiles < (1ll << 31) && rows < (1ll << 31), DLB_ERR_UNSUPPORTED,
+              "%s: batch=%d heads=%d lengths %d, %d make too many rows", call, a->batch, a->heads, a->q_len, a->kv_len);
   const long long nq = static_cast<long long>(a->batch) * a->q_len, nk = static_cast<long long>(a->batch) * a->kv_len;
   if (int st = check_heads(call, "q", a->q, nq)) return st;
   if (int st = check_heads(call, "k", a->k, nk)) return st;
@@ -142,8 +143,9 @@ FwdPlan plan_fwd(const dlb_attn *a, const AttnArgs &args) {
   FwdPlan p = {kGeneric, 1, 1, 4, 0};
   const int group = a->heads / a->kv_heads;
   if (a->dtype == DLB_BF16 && attn_mma_fits(args, false)) p.kind = a->q_len >= kMmaQueries ? kMma : kStep;
-  if (p.kind == kMma) return p;
-  if (p.kind == kStep) {
+  if (p.kind == kMma) {
+    p.splits = attn_fwd_mma_splits(args);
+  } else if (p.kind == kStep) {
     p.splits = attn_step_splits(a->batch, a->kv_heads, a->q_len * group, a->kv_len, a->head_dim);
   } else {
     // Few queries: the heads that share a key/value head go into one tile, and the keys are split until
@@ -287,9 +289,8 @@ extern "C" int dlb_attn_fwd(const dlb_attn *a, void *workspace, size_t workspace
     p.part_ml = static_cast<float2 *>(workspace);
     p.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + (rows * sizeof(float2) + 15) / 16 * 16);
   }
-  if (plan.kind == kMma) return attn_fwd_mma(p, st);
-  if (plan.kind == kStep) {
-    const int rc = attn_step(p, st);
+  if (plan.kind != kGeneric) {
+    const int rc = plan.kind == kMma ? attn_fwd_mma(p, st) : attn_step(p, st);
     return rc != DLB_OK || plan.splits == 1 ? rc : launch_join<__nv_bfloat16>(p, st);
   }
   return a->dtype == DLB_F32 ? launch_fwd<float>(p, plan, st) : launch_fwd<__nv_bfloat16>(p, plan, st);

@@ -15,6 +15,8 @@
 // 5.  In return no sum crosses a CTA: no fp32 copy of dQ in memory, no atomics, the same bits every time.
 #pragma once
 
+#include <cuda_fp16.h>
+
 #include <algorithm>
 
 #include "attn_mma.cuh"
@@ -53,7 +55,8 @@ __device__ __forceinline__ int far_side(const AttnArgs &a, int d0) {
 }
 
 // Bytes behind the ring: bias by distance, bucket by distance, sums per part, bucket and row (of the score
-// gradients in fp32, of the probabilities in bf16: they only weight a correction), tile flags.
+// gradients in fp32, of the probabilities, at most 1 a row, in fp16: they only weight a correction of some
+// thousandths), tile flags.
 struct BwdRest {
   int lut, buckets, sums, p_sums, flags, total;
 };
@@ -83,7 +86,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   float *lut = reinterpret_cast<float *>(smem + Shape::kRest + rest.lut);
   unsigned char *bucket_lut = smem + Shape::kRest + rest.buckets;
   float *sums = reinterpret_cast<float *>(smem + Shape::kRest + rest.sums);  // [part][bucket][row]
-  __nv_bfloat16 *p_sums = reinterpret_cast<__nv_bfloat16 *>(smem + Shape::kRest + rest.p_sums);
+  __half *p_sums = reinterpret_cast<__half *>(smem + Shape::kRest + rest.p_sums);
   unsigned char *flags = smem + Shape::kRest + rest.flags;
   __shared__ uint64_t x_full, full[ST], empty[ST], s_full[2], g_full, p_full[2], d_full, v_full, acc_full, drain;
   __shared__ uint32_t tmem_slot;
@@ -192,7 +195,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       bucket_lut[e] = static_cast<unsigned char>(bucket_at(a, e - a.reach - kLutPad));
     for (int e = tid; e < PARTS * a.buckets * kTileRows; e += kBwdThreads) {
       sums[e] = 0.f;
-      p_sums[e] = __float2bfloat16_rn(0.f);
+      p_sums[e] = __float2half_rn(0.f);
     }
   }
   tc_fence_before();
@@ -222,7 +225,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     auto flush_bucket = [&](int next) {
       const int at = (part * a.buckets + bucket_now) * kTileRows + row;
       sums[at] += bucket_sum.x;
-      p_sums[at] = __float2bfloat16_rn(__bfloat162float(p_sums[at]) + bucket_sum.y);
+      p_sums[at] = __float2half_rn(__half2float(p_sums[at]) + bucket_sum.y);
       bucket_sum = both(0.f);
       bucket_now = next;
     };
@@ -567,7 +570,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         for (int k = 0; k < PARTS; k++) {
           const int at = (k * a.buckets + n) * kTileRows + tid;
           e += sums[at];
-          p += __bfloat162float(p_sums[at]);
+          p += __half2float(p_sums[at]);
         }
       e = p > 0.f ? e / p : 0.f;
       for (int n = 0; n < a.buckets; n++) {
@@ -575,7 +578,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 #pragma unroll
         for (int k = 0; k < PARTS; k++) {
           const int at = (k * a.buckets + n) * kTileRows + tid;
-          sum += fmaf(-e, __bfloat162float(p_sums[at]), sums[at]);
+          sum += fmaf(-e, __half2float(p_sums[at]), sums[at]);
         }
         sums[n * kTileRows + tid] = sum;
       }

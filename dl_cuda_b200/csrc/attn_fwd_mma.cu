@@ -29,6 +29,8 @@ constexpr int kSoftmaxRegs = 104, kOtherRegs = 64;
 // within 2^32 of from above; fp32 sums and bf16 probabilities bear that with room to spare, and the
 // reference divides out.  It starts at 0, which serves most rows from end to end.
 constexpr float kReach = 32.f;
+// A sum under this may have lost weights to underflow (or has none): 2^26 times the smallest it can hold.
+constexpr float kNothing = 1e-30f;
 
 template <int NB>
 struct FwdShape {
@@ -114,9 +116,13 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     last_end[t] = r0 < a.q_len ? row_end(a, view, r1) : 0;
   }
   const int n_tiles = (max(last_end[0], last_end[1]) + kTileRows - 1) / kTileRows;
-  // From the tile where the queries stand to the first, then on from there: the nearest keys first.
-  const int here = max(0, min(n_tiles - 1, (view.start + min(a.q_len, row0 + 2 * kTileRows) - 1) / kTileRows));
-  auto walk = [&](int k) { return k <= here ? here - k : k; };
+  // This CTA's share of them (blockIdx.y), from the tile where the queries stand to the first, then on
+  // from there: the nearest keys first.
+  const int share = (n_tiles + a.splits - 1) / a.splits;
+  const int n_first = min(n_tiles, static_cast<int>(blockIdx.y) * share), n_last = min(n_tiles, n_first + share);
+  const int n_count = n_last - n_first;
+  const int here = max(n_first, min(n_last - 1, (view.start + min(a.q_len, row0 + 2 * kTileRows) - 1) / kTileRows));
+  auto walk = [&](int k) { return k <= here - n_first ? here - k : n_first + k; };
   if (a.q_docs) {
     if (warp < 2) {
       int lo = INT_MAX, hi = INT_MIN;
@@ -134,7 +140,7 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     }
     __syncthreads();
   }
-  for (int n = warp; n < n_tiles; n += kFwdThreads / 32) {
+  for (int n = n_first + warp; n < n_last; n += kFwdThreads / 32) {
     const int j0 = n * kTileRows;
     int lo = 0, hi = 0;
     if (a.kv_docs) {
@@ -247,7 +253,7 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     float m = 0.f, sum = 0.f, sum_rounded = 0.f;
     bool settled = false;  // the row has weight, or a reference of its own
     int it = -1, done = 0;
-    for (int k = 0; k < n_tiles; k++) {
+    for (int k = 0; k < n_count; k++) {
       const int n = walk(k);
       const int f = flags[n];
       if (!f) continue;
@@ -290,8 +296,8 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         part = add2(l[0], l[1]);
         part_rounded = add2(r[0], r[1]);
         const float total = part.x + part.y;
-        if (total > 0.f) settled = true;
-        const bool misfit = !(total <= 4294967296.f) || (!settled && total == 0.f && end > j1);
+        if (total >= kNothing) settled = true;
+        const bool misfit = !(total <= 4294967296.f) || (!settled && end > j1);
         if (!any_of_group(4 + t, misfit) || pass == 1) break;
         float top = -INFINITY;
         for (int c = 0; c < 2; c++) {
@@ -306,10 +312,10 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         top = fmaxf(top, redo_top[t][half ^ 1][row]);
         const float row_sum = sum + redo_sum[t][half ^ 1][row];
         named_bar_sync(2 + t, 256);
-        const bool above = top > m + kReach, below = row_sum == 0.f && top < m - kReach && top > -INFINITY;
+        const bool above = top > m + kReach, below = row_sum < kNothing && top < m - kReach && top > -INFINITY;
         const float keep = above ? ex2(m - top) : below ? 0.f : 1.f;
         if (above || below) m = top;
-        settled = settled || row_sum > 0.f || top > -INFINITY;
+        settled = settled || row_sum >= kNothing || top > -INFINITY;
         sum *= keep;
         sum_rounded *= keep;
         if (done > 0) {
@@ -356,7 +362,11 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     sum_rounded += redo_top[t][half ^ 1][row];
     if (done > 0) mbar_wait(&o_full[t], 0, dead, timeouts);
     tc_fence_after();
-    const float inv = sum_rounded > 0.f || sum_rounded != sum_rounded ? 1.f / sum_rounded : 0.f;
+    const bool whole_row = a.splits == 1, any = sum_rounded > 0.f || sum_rounded != sum_rounded;
+    // A share's output is kept for a quotient by the unrounded sum, which the join uses.
+    const float by = !any ? 0.f : whole_row ? 1.f / sum_rounded : sum / sum_rounded;
+    const size_t at = (static_cast<size_t>(b) * a.heads + h) * a.q_len + i;
+    const size_t part_at = static_cast<size_t>(blockIdx.y) * a.batch * a.heads * a.q_len + at;
     __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(a.o.ptr) + b * a.o.batch + static_cast<long long>(i) * a.o.token + h * a.o.head;
     for (int c = half * 32; c < a.dim; c += 64) {
       uint32_t o[32];
@@ -366,15 +376,24 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       }
 #pragma unroll
       for (int e = 0; e < 32; e += 8) {
-        uint32_t w[4];
+        float f[8];
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-          w[k] = inv == 0.f ? 0u : pack_bf16(__uint_as_float(o[e + 2 * k]) * inv, __uint_as_float(o[e + 2 * k + 1]) * inv);
-        if (valid && c + e < a.dim) *reinterpret_cast<uint4 *>(out + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int k = 0; k < 8; k++) f[k] = by == 0.f ? 0.f : __uint_as_float(o[e + k]) * by;
+        if (!valid || c + e >= a.dim) continue;
+        if (whole_row) {
+          *reinterpret_cast<uint4 *>(out + c + e) = Store<__nv_bfloat16>::pack(f);
+        } else {
+          float4 *to = reinterpret_cast<float4 *>(a.part_o + part_at * a.dim + c + e);
+          to[0] = make_float4(f[0], f[1], f[2], f[3]);
+          to[1] = make_float4(f[4], f[5], f[6], f[7]);
+        }
       }
     }
-    if (a.lse && valid && half == 0)
-      a.lse[(static_cast<size_t>(b) * a.heads + h) * a.q_len + i] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
+    if (!whole_row) {
+      if (valid && half == 0) a.part_ml[part_at] = make_float2(sum == 0.f ? -INFINITY : m, sum);
+    } else if (a.lse && valid && half == 0) {
+      a.lse[at] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
+    }
     tc_fence_before();
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
@@ -386,7 +405,7 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           for (int c = 0; c < NB; c++)
             tma_load_rows(smem + (t * NB + c) * kBlockBytes, &maps.q, &q_full, c * kBlockCols, row0 + t * kTileRows, h, b);
         int it = 0;
-        for (int k = 0; k < n_tiles; k++) {
+        for (int k = 0; k < n_count; k++) {
           const int n = walk(k);
           if (!flags[n]) continue;
           const int s = it % ST;
@@ -443,7 +462,7 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       };
       mbar_wait(&q_full, 0, dead, timeouts);
       int it = 0;
-      for (int k = 0; k < n_tiles; k++) {
+      for (int k = 0; k < n_count; k++) {
         const int n = walk(k);
         const int f = flags[n];
         if (!f) continue;
@@ -542,6 +561,12 @@ bool attn_mma_fits(const AttnArgs &a, bool backward) {
          grid16(a.dk, a.kv_len, a.kv_heads, a.batch) && grid16(a.dv, a.kv_len, a.kv_heads, a.batch);
 }
 
+int attn_fwd_mma_splits(const AttnArgs &a) {
+  // Few queries against many keys: shares of the key tiles fill the GPU once, of four tiles at least.
+  const long long ctas = static_cast<long long>(ceil_div(a.q_len, 2 * kTileRows)) * a.heads * a.batch;
+  return static_cast<int>(std::max(1ll, std::min({sm_count() / ctas, ceil_div(a.kv_len, kTileRows) / 4ll, 256ll})));
+}
+
 int attn_fwd_mma(const AttnArgs &a, cudaStream_t st) {
   FwdMaps maps;
   int rc = make_heads_map(&maps.q, a.q.ptr, a.dim, a.q_len, a.heads, a.batch, a.q.token, a.q.head, a.q.batch, kTileRows);
@@ -557,7 +582,7 @@ int attn_fwd_mma(const AttnArgs &a, cudaStream_t st) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     DLB_REQUIRE(e == cudaSuccess, DLB_ERR_CUDA, "attn_fwd: %s", cudaGetErrorString(e));
     const int grid = ceil_div(a.q_len, 2 * kTileRows) * a.heads * a.batch;
-    launch_pdl(kern, dim3(grid), dim3(kFwdThreads), smem, st, a, maps, timeouts);
+    launch_pdl(kern, dim3(grid, a.splits), dim3(kFwdThreads), smem, st, a, maps, timeouts);
     DLB_LAUNCH_CHECK("attn_fwd_mma");
     return DLB_OK;
   };

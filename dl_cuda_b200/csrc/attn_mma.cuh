@@ -102,6 +102,7 @@ __host__ __device__ inline int lut_floats(int reach) { return 2 * (reach + kLutP
 
 // The tensor cores need 16-byte aligned rows, and a scale that keeps the order of the scores.
 bool attn_mma_fits(const AttnArgs &a, bool backward);
+int attn_fwd_mma_splits(const AttnArgs &a);  // shares of the keys that attn_fwd_mma wants
 int attn_fwd_mma(const AttnArgs &a, cudaStream_t st);
 bool attn_bwd_mma_room(const AttnArgs &a);  // do the sums for the table fit?
 struct BwdMaps {

@@ -12,7 +12,9 @@ the tensor cores in it (else w = 0), entry by entry:
     |dv' - dv| <= (d + w) P^T|dO| + u |dv|
     |dS' - dS| <= (d + w) |dS| + P (e_dp + e_delta) =: b, e_dp = (D + 8) 2^-24 |dO||V|,
          e_delta = |dO| . bound(o) + (D + 8) 2^-24 |dO| . |o|
-    |dq' - dq| <= scale b |K| + u |dq|, |dk' - dk| <= scale b^T |Q| + u |dk|
+    |dx' - dx| <= scale (c b + 4 d_s (|dS| + b)) =: bx for dx = scale c dS, c = 1 - tanh^2 off by at most
+         4 d_s (twice the tanh's error and a rounding): (c + e1)(dS + e2) - c dS = c e2 + e1 dS + e1 e2
+    |dq' - dq| <= bx |K| + u |dq|, |dk' - dk| <= bx^T |Q| + u |dk|
     dtable: sums of d |dS| + d P (|dP| + |delta|) + P e_dp, doubled: the rows' common error is taken off
 """
 import math
@@ -100,7 +102,7 @@ def reference(q, k, v, dout=None, scale=None, cap=0.0, causal=False, kv_lens=Non
         b_t = 2 * (d * dS.abs() + d * P * (dP.abs() + delta.abs()) + P * e_dp)
         bounds["dtable"] = torch.einsum("bhij,bijn->hn", b_t, one) + tiny
     dcap = (1 - t * t) if cap else torch.ones_like(x)
-    dx, b_x = dS * dcap * scale, (b_s * dcap.abs() + 4 * d_s * dS.abs()) * scale
+    dx, b_x = dS * dcap * scale, (b_s * dcap.abs() + 4 * d_s * (dS.abs() + b_s)) * scale
 
     def shared(y):  # sum over the query heads of a key/value head
         return y.unflatten(1, (Hk, G)).sum(2)

@@ -388,3 +388,104 @@ def test_bias_matrix_in_the_unfused_chain():
     by_fusion = ops.attn_bwd(dout, q, k, v, fused, lse, **how)[3]
     check(dict(dtable=by_matrix), values, bounds)
     check(dict(dtable=by_fusion), values, bounds)
+
+
+# --- what only long or unusual calls reach -----------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shift", [-95.0, -88.0, -86.0, -70.0, -30.0, 25.0, 60.0, 85.0])
+@pytest.mark.parametrize("q_len", [1, 150])
+def test_scores_far_from_zero(q_len, shift, dtype):
+    """A bias common to all keys changes lse alone, also where 2^score would leave fp32's range."""
+    B, S, H, D = 2, 300, 2, 64
+    q, k, v, dout = make(81, dtype, B, q_len, S, H, H, D, "plain")
+    how = options("table", B, q_len, S, H)
+    how["table"] = how["table"] + shift
+    run_both(q, k, v, dout, how, grads=q_len > 1)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("causal", [False, True])
+def test_steep_distance_bias(causal, dtype):
+    """Slopes that take neighbouring tiles 2^100 apart, keys on both sides, the near ones partly hidden."""
+    B, S, H, D = 2, 700, 2, 64
+    q, k, v, dout = make(83, dtype, B, S, S, H, H, D, "plain")
+    how = dict(causal=causal, slopes=torch.tensor([1.0, 0.7], device="cuda"), prefix=ints([650, 0]) if causal else None,
+               kv_lens=ints([700, 300]))
+    run_both(q, k, v, dout, how)
+
+
+@pytest.mark.parametrize("q_len,Sk,H,Hk,D", [(17, 5000, 8, 2, 128), (64, 3000, 2, 1, 64), (200, 2048, 1, 1, 80), (300, 900, 2, 2, 128),
+                                            (40, 1025, 4, 4, 32)])
+@pytest.mark.parametrize("kind", ["plain", "cap+causal", "table", "mixed_docs", "lens"])
+def test_a_chunk_against_a_long_cache(q_len, Sk, H, Hk, D, kind):
+    """More queries than a single-token call has, too few to fill the GPU: the key tiles are shared out."""
+    B = 2
+    q, k, v, _ = make(q_len + Sk, "bf16", B, q_len, Sk, H, Hk, D, "plain")
+    how = options(kind, B, q_len, Sk, H)
+    if how.get("causal"):
+        how["q_start"] = ints([Sk - q_len, Sk // 2])
+        how["kv_lens"] = ints([Sk, Sk // 2 + q_len])
+        k[1, Sk // 2 + q_len:] = math.nan
+        v[1, Sk // 2 + q_len:] = math.inf
+    run_both(q, k, v, None, how, grads=False)
+    assert torch.equal(ops.attn_fwd(q, k, v, **how)[0], ops.attn_fwd(q, k, v, **how)[0])
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_64_buckets_and_the_longest_map(D, dtype):
+    B, S, H = 1, 400, 2
+    q, k, v, dout = make(85, dtype, B, S, S, H, H, D, "plain")
+    gen = torch.Generator().manual_seed(1)
+    how = dict(table=torch.randn(H, 64, generator=gen).cuda(), bucket_of=ops.rel_bucket_map(64, 1024, True).cuda())
+    run_both(q, k, v, dout, how)
+    how["bucket_of"] = torch.randint(0, 64, (2 * 300 + 1,), generator=gen).int().cuda()  # a map of one's own
+    run_both(q, k, v, dout, how)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_bucket_map_edges(dtype):
+    """A map of one entry; values outside 0..buckets-1 count as the nearest bucket."""
+    q, k, v, dout = make(87, dtype, 1, 40, 40, 2, 2, 64, "plain")
+    table = torch.randn(2, 4, generator=torch.Generator().manual_seed(2)).cuda()
+    run_both(q, k, v, dout, dict(table=table, bucket_of=ints([2])))
+    run_both(q, k, v, dout, dict(table=table, bucket_of=ints([-7, 1, 9, 3, 2])))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_positions_far_out(dtype):
+    """Starts at the ends of the range that is served, and beyond it (clamped)."""
+    q, k, v, dout = make(89, dtype, 4, 30, 50, 2, 2, 64, "plain")
+    starts = torch.tensor([2 ** 30, -2 ** 30, 2 ** 31 - 1, -2 ** 31], dtype=torch.int64).int().cuda()
+    run_both(q, k, v, dout, dict(q_start=starts, causal=True))
+    how = options("table", 4, 30, 50, 2)
+    run_both(q, k, v, dout, dict(q_start=starts, **how))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_negative_and_zero_scales(dtype):
+    q, k, v, dout = make(91, dtype, 1, 90, 90, 2, 1, 64, "plain")
+    for scale in (0.0, -0.2, 1e-3, 3.0):
+        run_both(q, k, v, dout, dict(scale=scale, causal=True))
+
+
+@pytest.mark.parametrize("cap", [1e-3, 0.5, 200.0, 1e5])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_caps_from_tight_to_loose(cap, dtype):
+    q, k, v, dout = make(93, dtype, 1, 150, 150, 2, 1, 64, "plain")
+    run_both(q, k, v, dout, dict(cap=cap, causal=True))
+    run_both(q[:, :1], k, v, None, dict(cap=cap), grads=False)
+
+
+def test_rows_behind_the_outputs_stay_as_they_were():
+    """Outputs that are the front part of larger buffers: nothing is written behind them."""
+    for dtype in ("fp32", "bf16"):
+        for q_len, Sk in ((1, 900), (5, 100), (100, 100), (130, 260)):
+            q, k, v, dout = make(95, dtype, 2, q_len, Sk, 4, 2, 64, "plain")
+            room = {n: torch.full((2, t + 3, h, 64), 7.0, dtype=q.dtype, device="cuda")
+                    for n, t, h in (("o", q_len, 4), ("dq", q_len, 4), ("dk", Sk, 2), ("dv", Sk, 2))}
+            o, lse = ops.attn_fwd(q, k, v, out=room["o"][:, :q_len])
+            ops.attn_bwd(dout, q, k, v, o, lse, dq=room["dq"][:, :q_len], dk=room["dk"][:, :Sk], dv=room["dv"][:, :Sk])
+            for n, t in (("o", q_len), ("dq", q_len), ("dk", Sk), ("dv", Sk)):
+                assert (room[n][:, t:] == 7).all(), (dtype, q_len, n)
+                assert not (room[n][:, :t] == 7).all()
