@@ -6,10 +6,15 @@
 //     FOR_KEYS: dV += P W, dK += D U;   else dQ += D U                 (TMEM, scaled at the end)
 // with P and D written over S and G as bf16.  The row threads take the exponentials of S while the tensor
 // cores make G and the last tile's dK, and D while they make dV and the next S.  TMEM holds S, G and the
-// sums; where it has room for more, S does not wait for P: the query pass keeps two S where the ring has four stages to feed them, the key pass of
-// heads up to 64 wide keeps P beside S.  Tiles of 64 columns with two buffers each were
-// slower: a product of 128 x 64 takes the tensor cores as long as one of 128 x 128 (measured with the
-// clock: 65 cycles for 16 inner columns either way), so S and G cost twice as much.
+// sums; for heads up to 64 wide it has room for more, and S does not wait for P: the key pass keeps P
+// beside S, the query pass two S where its ring has four stages to feed them.
+//
+// Tiles of 64 columns with two buffers each were slower (889 instead of 811 us for both passes over 4096
+// x 4096 tokens, 32 heads of 128): a product of 128 x 64 takes the tensor cores as long as one of 128 x
+// 128, 65 cycles for 16 inner columns, so S and G cost twice as much.  What bounds the key pass now, by the
+// clock: 2800 cycles a tile, of which P takes 1430 (1024 of them are the special-function units' 16 a
+// clock) and dV with the next S, which cannot start before P is complete, 1260; the tensor cores are busy
+// for 2048.
 //
 // Two passes rebuild S and G twice: 7 products of 2 * dim flop per pair where a single pass would need
 // 5.  In return no sum crosses a CTA: no fp32 copy of dQ in memory, no atomics, the same bits every time.

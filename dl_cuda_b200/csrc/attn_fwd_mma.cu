@@ -11,6 +11,12 @@
 // the far end of a prefix, every tile moved the reference: 64 instead of 53 us for 3 x 1531 tokens).  The sum behind the quotient adds the ROUNDED probabilities, so that a row's weights
 // add up to one exactly as the product sees them (bf16 output 1.9e-3 instead of 2.3e-3 from the exact
 // one, of which the output's own rounding is 1.7e-3); lse comes from the unrounded ones.
+//
+// Measured (32 heads of 128, 4096 tokens): 270 us, 1.01 PFLOP/s, of the 1.66 that the library's plain
+// product reaches; causal 141 us, causal with a cap 177 us.  By the clock a pair of tiles takes 3500 cycles
+// where the tensor cores need 2470 of issue: a tile's own chain of scores, softmax (1700 cycles a tile,
+// half of which are exponentials) and product is what remains, since TMEM has no room for a second S.
+// Taking a quarter of the exponentials as polynomials on the fp32 pipes changed nothing (275 us).
 #include <algorithm>
 
 #include "attn_mma.cuh"

@@ -15,6 +15,11 @@
 // the second product wants inner indexes c and c + 4, so the streamed rows 2c, 2c + 1 are loaded for
 // them, 16 bytes serving four 8-column tiles of the result.  Rows of a tile are multiples of 128 bytes
 // with their 16-byte chunks permuted (chunk_of) so that both kinds of load hit every bank once.
+//
+// Measured, fp32: forward of 2 x 1000 tokens, 16 heads of 64, in packed documents 105 us (137 us with the
+// scalar tiles); forward of 2 x 2048 tokens, causal, 546 us = 31 TFLOP/s, backward 1.75 ms = 25 TFLOP/s.
+// The tensor pipe is busy for a third of the time: splitting operands and waiting for one product after
+// another in few warps take the rest.
 #pragma once
 
 #include "attn_common.cuh"

@@ -514,14 +514,15 @@ DLB_API int dlb_ce_from_ids_bwd(const int32_t *target_ids, const float *y_pred,
  * values in front of that bound have to be finite, masked or not.
  * kv_lens, q_start, prefix and the document arrays are int32 DEVICE arrays read by the kernels, so
  * a captured graph sees what they hold when it is replayed; lengths and prefixes are clamped to
- * [0, kv_len], starts to +-2^30.
+ * [0, kv_len], starts to +-2^30.  q, and dout in the backward, have to be finite in every row.
  *
  * One entry point serves whole sequences and single tokens (q_len = 1 against a cache: the keys
  * are split over the GPU and joined, through `workspace`).  Storage DLB_F32 keeps every product
  * in fp32; DLB_BF16 multiplies on the tensor cores with fp32 sums and softmax statistics and
  * rounds probabilities to bf16 in front of the second product.  head_dim 1..128; bf16 with
  * head_dim, strides and addresses in multiples of 16 bytes takes the tensor cores, anything else
- * plain CUDA kernels.  The result does not depend on scheduling: same call, same bits.
+ * kernels with fp32 arithmetic.  The result does not depend on scheduling: same call, same bits.
+ * As with the other pipelined kernels, make the first call of a kind on a device before capturing.
  *
  * Replaces the chain attnScoresKernel, applyCausalMaskKernel, softmaxForwardKernel and
  * attnApplyKernel (src/transformer.cuh:8-58, call sites :441-486) for programs that do not need
