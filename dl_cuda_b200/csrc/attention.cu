@@ -118,15 +118,6 @@ auto by_row_groups(int groups, F &&f) {
   return f(std::integral_constant<int, 4>());
 }
 
-// Lets a kernel use `smem` bytes of dynamic shared memory (48 KB with the static are free to all).
-template <typename K>
-int allow_smem(K kern, size_t smem, const char *name) {
-  if (smem <= 40 * 1024) return DLB_OK;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  DLB_REQUIRE(e == cudaSuccess, DLB_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
-  return DLB_OK;
-}
-
 // From this many queries on, bf16 goes to the 128-row tiles of the tensor cores; below, the cache is what
 // takes time, and the 16 rows of the few-queries kernel are enough.  Measured for 8 sequences, 8192 keys,
 // 32 query heads on 8 key heads of 128 (this kernel / the 128-row tiles): 1 query 59 / 225 us, 8 queries

@@ -609,11 +609,10 @@ struct BwdTableShape {
   size_t smem;
 };
 inline BwdTableShape bwd_table_shape(const AttnArgs &a) {
-  constexpr size_t kMaxSmem = 227 * 1024 - 2048;  // less the static part
   const size_t ring = 1024 + static_cast<size_t>(a.dim > kBlockCols ? BwdShape<2, 1>::kRest : BwdShape<1, 2>::kRest);
   for (int parts = a.dim > kBlockCols ? 2 : 4; parts >= 2; parts -= 2) {
     const size_t smem = ring + bwd_rest(a, false, parts).total;
-    if (smem <= kMaxSmem) return {parts, smem};
+    if (smem <= kMaxDynamicSmem) return {parts, smem};
   }
   return {0, 0};  // does not fit at all
 }
@@ -625,8 +624,7 @@ int bwd_mma_launch(const AttnArgs &a, const BwdMaps &maps, cudaStream_t st) {
   DLB_REQUIRE(timeouts != nullptr, DLB_ERR_NO_DEVICE, "%s: no CUDA device", name);
   auto launch = [&](auto kern, int ring_end, int parts) -> int {
     const size_t smem = 1024 + ring_end + bwd_rest(a, FOR_KEYS, parts).total;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    DLB_REQUIRE(e == cudaSuccess, DLB_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
+    if (int rc = allow_smem(kern, smem, name)) return rc;
     const int grid = ceil_div(FOR_KEYS ? a.kv_len : a.q_len, kTileRows) * (FOR_KEYS ? a.kv_heads : a.heads) * a.batch;
     launch_pdl(kern, dim3(grid), dim3(parts == 4 ? BwdWarps<4>::kThreads : BwdWarps<2>::kThreads), smem, st, a, maps, timeouts);
     DLB_LAUNCH_CHECK(name);

@@ -12,6 +12,19 @@ namespace dlb {
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kHidesBelow = -1e30f;  // table entries under this hide their keys
 
+// Lets a kernel use any amount of dynamic shared memory up to kMaxDynamicSmem (8 KB are left for static).
+// The limit is a property of the kernel, not of a launch: set to each call's own need, a smaller call on
+// one host thread would take it away from a larger one on another.
+constexpr size_t kMaxDynamicSmem = 227 * 1024 - 8192;
+template <typename K>
+int allow_smem(K kern, size_t smem, const char *name) {
+  DLB_REQUIRE(smem <= kMaxDynamicSmem, DLB_ERR_UNSUPPORTED, "%s: %zu bytes of shared memory", name, smem);
+  if (smem <= 40 * 1024) return DLB_OK;  // 48 KB with the static are free to all
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMaxDynamicSmem));
+  DLB_REQUIRE(e == cudaSuccess, DLB_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
+  return DLB_OK;
+}
+
 struct Heads {
   void *ptr;
   long long batch, token, head;  // strides in elements

@@ -585,8 +585,7 @@ int attn_fwd_mma(const AttnArgs &a, cudaStream_t st) {
   auto launch = [&](auto kern, int blocks) -> int {
     const size_t smem = 1024 + (blocks == 2 ? FwdShape<2>::kLut : FwdShape<1>::kLut) +
                         (a.table ? sizeof(float) * lut_floats(a.reach) : 0) + ceil_div(tiles, 16) * 16;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    DLB_REQUIRE(e == cudaSuccess, DLB_ERR_CUDA, "attn_fwd: %s", cudaGetErrorString(e));
+    if (int rc = allow_smem(kern, smem, "attn_fwd")) return rc;
     const int grid = ceil_div(a.q_len, 2 * kTileRows) * a.heads * a.batch;
     launch_pdl(kern, dim3(grid, a.splits), dim3(kFwdThreads), smem, st, a, maps, timeouts);
     DLB_LAUNCH_CHECK("attn_fwd_mma");

@@ -5,7 +5,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "common.cuh"
+#include "attn_common.cuh"
 
 namespace dlb {
 namespace {
@@ -259,10 +259,7 @@ extern "C" int dlb_rel_bias_bwd(const void *dscores, const int32_t *bucket_of, f
   const size_t smem = sizeof(float) * buckets * kBiasThreads + 2 * max_distance + 1;
   const bool vec = rows_can_be_cut(dscores, nullptr, dtype == DLB_F32 ? 4 : 2);
   auto kern = dtype == DLB_F32 ? rel_bias_bwd_kernel<float> : rel_bias_bwd_kernel<__nv_bfloat16>;
-  if (smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    DLB_REQUIRE(e == cudaSuccess, DLB_ERR_CUDA, "rel_bias_bwd: %s", cudaGetErrorString(e));
-  }
+  if (int rc = allow_smem(kern, smem, "rel_bias_bwd")) return rc;
   launch_pdl(kern, dim3(heads * parts), dim3(kBiasThreads), smem, as_stream(stream), a, parts, vec);
   DLB_LAUNCH_CHECK("rel_bias_bwd");
   launch_pdl(rel_bias_sum_kernel, dim3(heads * buckets), dim3(128), 0, as_stream(stream),

@@ -489,3 +489,35 @@ def test_rows_behind_the_outputs_stay_as_they_were():
             for n, t in (("o", q_len), ("dq", q_len), ("dk", Sk), ("dv", Sk)):
                 assert (room[n][:, t:] == 7).all(), (dtype, q_len, n)
                 assert not (room[n][:, :t] == 7).all()
+
+
+def test_two_host_threads():
+    """Calls of one kernel with different needs of shared memory from two host threads at once."""
+    import threading
+    sets = []
+    for n, (D, docs) in enumerate(((64, 40), (64, 3000))):
+        q, k, v, dout = make(97 + n, "bf16", 1, 130, docs, 2, 2, D, "plain")
+        how = dict(bucket_of=ops.rel_bucket_map(16, 40 + 900 * n, True).cuda(), table=torch.randn(2, 16, device="cuda"))
+        o, lse = ops.attn_fwd(q, k, v, **how)
+        sets.append(((q, k, v), how, dout, o, lse, ops.attn_bwd(dout, q, k, v, o, lse, **how)))
+    torch.cuda.synchronize()
+    failures = []
+
+    def work(n):
+        try:
+            (q, k, v), how, dout, o, lse, want = sets[n]
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(200):
+                    got = ops.attn_bwd(dout, q, k, v, *ops.attn_fwd(q, k, v, **how), **how)
+                torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(x, y) for x, y in zip(got, want)):
+                failures.append("results differ")
+        except Exception as e:  # noqa: BLE001
+            failures.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures
