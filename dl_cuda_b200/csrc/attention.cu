@@ -207,8 +207,16 @@ int launch_table_sum(const AttnArgs &p, cudaStream_t st) {
   return DLB_OK;
 }
 
+int launch_bwd_mma(const AttnArgs &p, cudaStream_t st) {
+  BwdMaps maps;
+  if (int s = make_bwd_maps(p, &maps)) return s;
+  if (int s = attn_bwd_mma_queries(p, maps, st)) return s;  // also fills the row statistics for the keys
+  if (int s = attn_bwd_mma_keys(p, maps, st)) return s;
+  return launch_table_sum(p, st);
+}
+
 template <typename T>
-int launch_bwd(const AttnArgs &p, bool mma, cudaStream_t st) {
+int launch_bwd(const AttnArgs &p, cudaStream_t st) {
   const bool vec = vector_rows(p.q, p.dim, sizeof(T)) && vector_rows(p.k, p.dim, sizeof(T)) &&
                    vector_rows(p.v, p.dim, sizeof(T)) && vector_rows(p.dout, p.dim, sizeof(T));
   const size_t rows = static_cast<size_t>(p.batch) * p.heads * stat_tiles(p.q_len) * kStatRows;
@@ -217,13 +225,6 @@ int launch_bwd(const AttnArgs &p, bool mma, cudaStream_t st) {
     auto kern = pairs ? attn_row_stats_kernel<T, 8, true> : attn_row_stats_kernel<T, 32, false>;
     launch_pdl(kern, dim3(static_cast<unsigned>(ceil_div(rows, size_t{pairs ? 32u : 8u}))), dim3(256), 0, st, p);
     DLB_LAUNCH_CHECK("attn_row_stats");
-  }
-  if (mma) {
-    BwdMaps maps;
-    if (int s = make_bwd_maps(p, &maps)) return s;
-    if (int s = attn_bwd_mma_keys(p, maps, st)) return s;
-    if (int s = attn_bwd_mma_queries(p, maps, st)) return s;
-    return launch_table_sum(p, st);
   }
   return by_width(p.dim, [&](auto width) -> int {
     // 64-row tiles where they fill the GPU twice, else 32-row ones
@@ -322,7 +323,10 @@ extern "C" int dlb_attn_bwd(const dlb_attn *a, const dlb_attn_grad *g, void *wor
   p.table_parts = plan.parts;
   cudaStream_t st = as_stream(stream);
   const bool mma = a->dtype == DLB_BF16 && a->batch > 0 && attn_mma_fits(p, true) && attn_bwd_mma_room(p);
-  if (mma) p.table_parts = a->batch * ceil_div(a->q_len, kTileRows);
-  return a->dtype == DLB_F32 ? launch_bwd<float>(p, false, st) : launch_bwd<__nv_bfloat16>(p, mma, st);
+  if (mma) {
+    p.table_parts = a->batch * ceil_div(a->q_len, kTileRows);
+    return launch_bwd_mma(p, st);
+  }
+  return a->dtype == DLB_F32 ? launch_bwd<float>(p, st) : launch_bwd<__nv_bfloat16>(p, st);
 }
 

@@ -59,6 +59,49 @@ __device__ __forceinline__ int far_side(const AttnArgs &a, int d0) {
   return left ? 0 : 2 * (a.reach + kLutPad);
 }
 
+// {-lse * log2(e), -delta} of query x (row `row` of tile `tile`), delta = <dout_x, o_x> by the PARTS threads
+// of the row, and its place in row_stats filled; rows behind the last query get {-infinity, 0}.
+template <int NB, int PARTS>
+__device__ __forceinline__ float2 make_row_stats(const AttnArgs &a, int b, int h, int tile, int x, int part, int row, bool valid,
+                                                 float (*delta_part)[kTileRows]) {
+  float sum = 0.f, lse = -INFINITY;
+  if (valid) {
+    using S = Store<__nv_bfloat16>;
+    const __nv_bfloat16 *o = static_cast<const __nv_bfloat16 *>(a.o.ptr) + b * a.o.batch + static_cast<long long>(x) * a.o.token + h * a.o.head;
+    const __nv_bfloat16 *g = static_cast<const __nv_bfloat16 *>(a.dout.ptr) + b * a.dout.batch +
+                             static_cast<long long>(x) * a.dout.token + h * a.dout.head;
+    constexpr int kLoads = NB * kBlockCols / (8 * PARTS);  // all in flight at once
+    uint4 ov[kLoads], gv[kLoads];
+#pragma unroll
+    for (int k = 0; k < kLoads; k++) {
+      const int c = (k * PARTS + part) * 8;
+      ov[k] = c < a.dim ? ld_keep(o + c) : make_uint4(0, 0, 0, 0);
+      gv[k] = c < a.dim ? ld_keep(g + c) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int k = 0; k < kLoads; k++) {
+      float u[8], v[8];
+      S::unpack(ov[k], u);
+      S::unpack(gv[k], v);
+#pragma unroll
+      for (int e = 0; e < 8; e++) sum = fmaf(u[e], v[e], sum);
+    }
+    lse = ld_co(a.lse + (static_cast<size_t>(b) * a.heads + h) * a.q_len + x);
+  }
+  delta_part[part][row] = sum;
+  named_bar_sync(1, 128 * PARTS);
+  sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < PARTS; k++) sum += delta_part[k][row];
+  const float2 stat = make_float2(lse == -INFINITY ? -INFINITY : -lse * kLog2e, -sum);
+  if (part == 0) {
+    float *to = stats_tile(a, b, h, tile) + row;
+    to[0] = stat.x;
+    to[kStatRows] = stat.y;
+  }
+  return stat;
+}
+
 // Bytes behind the ring: bias by distance, bucket by distance, sums per part, bucket and row (of the score
 // gradients in fp32, of the probabilities, at most 1 a row, in fp16: they only weight a correction of some
 // thousandths), tile flags.
@@ -96,6 +139,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   __shared__ uint64_t x_full, full[ST], empty[ST], s_full[2], g_full, p_full[2], d_full, v_full, acc_full, drain;
   __shared__ uint32_t tmem_slot;
   __shared__ int dead_flag, doc_range[2];
+  __shared__ float delta_part[FOR_KEYS ? 1 : PARTS][kTileRows];
   __shared__ __align__(16) int doc_tile[kTileRows];
   volatile int *dead = &dead_flag;
   // s_full and p_full come in pairs, used in turn: with two S the tensor cores may finish the next tile's
@@ -220,7 +264,8 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     // Stream rows [see_from, see_end) are visible to this row, as far as documents allow.
     const int see_from = !valid ? INT_MAX : FOR_KEYS ? first_query(a, view, x) : 0;
     const int see_end = !valid ? 0 : FOR_KEYS ? a.q_len : row_end(a, view, x);
-    const float2 row_stat = (!FOR_KEYS && valid) ? stat_at(a, b, unit, x) : make_float2(-INFINITY, 0.f);
+    // The query pass, which runs first, makes its rows' statistics itself and leaves them to the key pass.
+    const float2 row_stat = FOR_KEYS ? make_float2(-INFINITY, 0.f) : make_row_stats<NB, PARTS>(a, b, unit, tile, x, part, row, valid, delta_part);
     const float to_log2 = CAP ? 1.f : a.scale * kLog2e;
     const CapCoef cap = CAP ? cap_coef(a.scale, a.cap) : CapCoef();
     const float2 uncap = both(CAP ? 1.f / cap.out : 0.f);
