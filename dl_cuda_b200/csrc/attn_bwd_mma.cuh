@@ -368,6 +368,11 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 #pragma unroll
             for (int e = 0; e < 16; e++)
               if (FOR_KEYS ? e < cut : e >= cut) p[e0 + e] = 0.f;
+            if (CAP) {  // a hidden score may be NaN, and the cap's derivative of it
+#pragma unroll
+              for (int e = 0; e < 16; e++)
+                if (p[e0 + e] == 0.f) x_all[CAP ? e0 + e : 0] = 0.f;
+            }
           }
           if (FOR_KEYS) {
             uint32_t packed[8];
@@ -655,7 +660,7 @@ struct BwdTableShape {
 };
 inline BwdTableShape bwd_table_shape(const AttnArgs &a) {
   const size_t ring = 1024 + static_cast<size_t>(a.dim > kBlockCols ? BwdShape<2, 1>::kRest : BwdShape<1, 2>::kRest);
-  for (int parts = a.dim > kBlockCols ? 2 : 4; parts >= 2; parts -= 2) {
+  for (int parts = 4; parts >= 2; parts -= 2) {
     const size_t smem = ring + bwd_rest(a, false, parts).total;
     if (smem <= kMaxDynamicSmem) return {parts, smem};
   }
@@ -681,7 +686,7 @@ int bwd_mma_launch(const AttnArgs &a, const BwdMaps &maps, cudaStream_t st) {
        : launch(attn_bwd_mma_kernel<NB, ST, PARTS, FOR_KEYS, false, BIAS>, BwdShape<NB, ST>::kRest, PARTS))
   if constexpr (!FOR_KEYS) {
     if (a.table && a.dtable) {  // as bwd_table_shape has it
-      if (a.dim > kBlockCols) return DLB_PICK(2, 1, 2, kTable);
+      if (a.dim > kBlockCols) return bwd_table_shape(a).parts == 4 ? DLB_PICK(2, 1, 4, kTable) : DLB_PICK(2, 1, 2, kTable);
       return bwd_table_shape(a).parts == 4 ? DLB_PICK(1, 2, 4, kTable) : DLB_PICK(1, 2, 2, kTable);
     }
   }

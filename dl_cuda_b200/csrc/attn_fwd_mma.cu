@@ -3,14 +3,15 @@
 // A CTA owns two tiles of 128 queries of one head and walks over the tiles of 128 keys that any of
 // them sees.  One warp copies K and V tiles into a ring (TMA), one issues the products, and each
 // query tile has eight warps for its softmax:
-//     S = Q K^T (TMEM, fp32) -> scores, running maximum, P = 2^(s - m) (bf16, written over S) -> O += P V
+//     S = Q K^T (TMEM, fp32) -> scores s -> P = 2^(s - m) (bf16, written over S) -> O += P V
 // The two query tiles take turns: while one's softmax runs, the other's products do.  O stays in TMEM.
 // Exponentials are taken against a reference that moves only when a score leaves its range of 2^32, so
 // no maximum stands between a score and its exponential, and O is hardly ever rescaled; keys are walked
 // from where the queries stand outwards, so that a distance bias shows its largest scores at once (from
-// the far end of a prefix, every tile moved the reference: 64 instead of 53 us for 3 x 1531 tokens).  The sum behind the quotient adds the ROUNDED probabilities, so that a row's weights
-// add up to one exactly as the product sees them (bf16 output 1.9e-3 instead of 2.3e-3 from the exact
-// one, of which the output's own rounding is 1.7e-3); lse comes from the unrounded ones.
+// the far end of a prefix, every tile moved the reference: 64 instead of 53 us for 3 x 1531 tokens).
+// The sum behind the quotient adds the ROUNDED probabilities, so that a row's weights add up to one
+// exactly as the product sees them (bf16 output 1.9e-3 instead of 2.3e-3 from the exact one, of which the
+// output's own rounding is 1.7e-3); lse comes from the unrounded ones.
 //
 // Measured (32 heads of 128, 4096 tokens): 270 us, 1.01 PFLOP/s, of the 1.66 that the library's plain
 // product reaches; causal 141 us, causal with a cap 177 us.  By the clock a pair of tiles takes 3500 cycles

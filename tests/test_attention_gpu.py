@@ -179,9 +179,11 @@ def test_unused_keys_may_hold_anything_in_training(dtype):
     for b, n in enumerate(lens.tolist()):
         k[b, n:] = math.nan
         v[b, n:] = math.inf
-    got = run_both(q, k, v, dout, dict(kv_lens=lens))
-    for b, n in enumerate(lens.tolist()):
-        assert (got["dk"][b, n:] == 0).all() and (got["dv"][b, n:] == 0).all()
+    for extra in ({}, dict(cap=5.0), options("slopes", B, S, S, 4), options("table", B, S, S, 4),
+                  dict(cap=5.0, **options("table+docs", B, S, S, 4))):
+        got = run_both(q, k, v, dout, dict(kv_lens=lens, **extra))
+        for b, n in enumerate(lens.tolist()):
+            assert (got["dk"][b, n:] == 0).all() and (got["dv"][b, n:] == 0).all()
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
