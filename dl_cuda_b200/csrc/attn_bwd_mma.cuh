@@ -103,8 +103,9 @@ __device__ __forceinline__ float2 make_row_stats(const AttnArgs &a, int b, int h
 }
 
 // Bytes behind the ring: bias by distance, bucket by distance, sums per part, bucket and row (of the score
-// gradients in fp32, of the probabilities, at most 1 a row, in fp16: they only weight a correction of some
-// thousandths), tile flags.
+// gradients in fp32, of the probabilities, at most 1 a row, in fp16 times 2^15, which keeps 11 bits of them
+// down to 2^-29: they only weight a correction of some thousandths), tile flags.
+constexpr float kProbScale = 32768.f;
 struct BwdRest {
   int lut, buckets, sums, p_sums, flags, total;
 };
@@ -275,7 +276,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     auto flush_bucket = [&](int next) {
       const int at = (part * a.buckets + bucket_now) * kTileRows + row;
       sums[at] += bucket_sum.x;
-      p_sums[at] = __float2half_rn(__half2float(p_sums[at]) + bucket_sum.y);
+      p_sums[at] = __float2half_rn(fmaf(bucket_sum.y, kProbScale, __half2float(p_sums[at])));
       bucket_sum = both(0.f);
       bucket_now = next;
     };
@@ -625,7 +626,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         for (int k = 0; k < PARTS; k++) {
           const int at = (k * a.buckets + n) * kTileRows + tid;
           e += sums[at];
-          p += __half2float(p_sums[at]);
+          p += __half2float(p_sums[at]) * (1.f / kProbScale);
         }
       e = p > 0.f ? e / p : 0.f;
       for (int n = 0; n < a.buckets; n++) {
@@ -633,7 +634,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 #pragma unroll
         for (int k = 0; k < PARTS; k++) {
           const int at = (k * a.buckets + n) * kTileRows + tid;
-          sum += fmaf(-e, __half2float(p_sums[at]), sums[at]);
+          sum += fmaf(-e, __half2float(p_sums[at]) * (1.f / kProbScale), sums[at]);
         }
         sums[n * kTileRows + tid] = sum;
       }

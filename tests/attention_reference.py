@@ -8,14 +8,18 @@ The bounds count roundings.  A rounding to a type is off by at most u = finfo.ep
          where the backward rebuilds it from lse, plus (Sk / 32 + 32) 2^-24 for the sum
 the outputs obey, with w = u of the storage type where probabilities or score gradients pass through
 the tensor cores in it (else w = 0), entry by entry:
-    |o'  - o|  <= (d + w) P|V| + u |o|
+    |o'  - o|  <= (d + w) (P|V| + |o|) + u |o|: weights p(1 + e), |e| <= d + w, in the product and in the
+         sum behind the quotient give sum p e (v - o), and |v - o| <= |v| + |o|
     |dv' - dv| <= (d + w) P^T|dO| + u |dv|
     |dS' - dS| <= (d + w) |dS| + P (e_dp + e_delta) =: b, e_dp = (D + 8) 2^-24 |dO||V|,
          e_delta = |dO| . bound(o) + (D + 8) 2^-24 |dO| . |o|
     |dx' - dx| <= scale (c b + 4 d_s (|dS| + b)) =: bx for dx = scale c dS, c = 1 - tanh^2 off by at most
          4 d_s (twice the tanh's error and a rounding): (c + e1)(dS + e2) - c dS = c e2 + e1 dS + e1 e2
     |dq' - dq| <= bx |K| + u |dq|, |dk' - dk| <= bx^T |Q| + u |dk|
-    dtable: sums of d |dS| + d P (|dP| + |delta|) + P e_dp, doubled: the rows' common error is taken off
+    dtable: sums of d |dS| + d P (|dP| + |delta|) + P e_dp, doubled: the rows' common error is taken off;
+         on the tensor cores in proportion to sums of P that are kept in fp16 times 2^15: off by 2^-11 of the
+         sum, or by 2^-40 (half a step of the smallest fp16, 2^-24, over 2^15), an addition, at most
+         Sk / 128 + 2 of them by each of four threads; and the error taken off is at most e_delta + e_dp
 """
 import math
 
@@ -83,7 +87,7 @@ def reference(q, k, v, dout=None, scale=None, cap=0.0, causal=False, kv_lens=Non
     def tokens(y):
         return y.permute(0, 2, 1, 3)
 
-    b_o = (d + w) * (P @ vd.abs()) + u * o.abs()
+    b_o = (d + w) * (P @ vd.abs() + o.abs()) + u * o.abs()
     values, bounds = dict(o=tokens(o), lse=lse), dict(o=tokens(b_o) + tiny)
     bounds["lse"] = (2 * d_s)[..., 0] + 2.0 ** -23 * torch.where(lse.isinf(), 0.0, lse.abs()) + (Sk / 32 + 32) * 2.0 ** -24
     if dout is None:
@@ -101,6 +105,10 @@ def reference(q, k, v, dout=None, scale=None, cap=0.0, causal=False, kv_lens=Non
         values["dtable"] = torch.einsum("bhij,bijn->hn", dS, one)
         b_t = 2 * (d * dS.abs() + d * P * (dP.abs() + delta.abs()) + P * e_dp)
         bounds["dtable"] = torch.einsum("bhij,bijn->hn", b_t, one) + tiny
+        if w:
+            most = e_delta + (e_dp.amax(-1, keepdim=True) if Sk else 0.0)
+            bounds["dtable"] += (Sk / 128 + 2) * (2.0 ** -11 * torch.einsum("bhij,bijn->hn", P * most, one)
+                                                  + 4 * 2.0 ** -40 * most.sum((0, 2, 3))[:, None])
     dcap = (1 - t * t) if cap else torch.ones_like(x)
     dx, b_x = dS * dcap * scale, (b_s * dcap.abs() + 4 * d_s * (dS.abs() + b_s)) * scale
 
