@@ -517,16 +517,18 @@ DLB_API int dlb_ce_from_ids_bwd(const int32_t *target_ids, const float *y_pred,
  * [0, kv_len], starts to +-2^30.  q, and dout in the backward, have to be finite in every row.
  *
  * One entry point serves whole sequences and single tokens (q_len = 1 against a cache: the keys
- * are split over the GPU and joined, through `workspace`).  Storage DLB_F32 keeps every product
- * in fp32; DLB_BF16 multiplies on the tensor cores with fp32 sums and softmax statistics and
- * rounds probabilities to bf16 in front of the second product.  head_dim 1..128; bf16 with
+ * are split over the GPU and joined, through `workspace`).  With DLB_F32 every operand of a
+ * product is split into two parts of 11 bits and three of their products are summed in fp32, which
+ * leaves out 2^-21 of |x||y|; DLB_BF16 multiplies on the tensor cores with fp32 sums and softmax
+ * statistics and rounds probabilities (in the backward also the gradients of the scores) to bf16 in
+ * front of the next product.  head_dim 1..128; bf16 with
  * head_dim, strides and addresses in multiples of 16 bytes takes the tensor cores, anything else
  * kernels with fp32 arithmetic.  The result does not depend on scheduling: same call, same bits.
  * As with the other pipelined kernels, make the first call of a kind on a device before capturing.
  *
  * Replaces the chain attnScoresKernel, applyCausalMaskKernel, softmaxForwardKernel and
- * attnApplyKernel (src/transformer.cuh:8-58, call sites :441-486) for programs that do not need
- * the probabilities in memory; caps, distance and bucket biases, documents, prefixes, lengths and
+ * attnApplyKernel (src/transformer.cuh:8-58) for programs that do not need the probabilities in
+ * memory; caps, distance and bucket biases, documents, prefixes, lengths and
  * shared key/value heads have no counterpart in the reference. */
 #define DLB_ATTN_MAX_HEAD_DIM 128
 #define DLB_ATTN_MAX_BUCKETS 64
@@ -565,8 +567,8 @@ DLB_API int dlb_attn_fwd(const dlb_attn *a, void *workspace, size_t workspace_by
  * probabilities are rebuilt from lse.  Keys that no query reaches get zero.  Every sum has a fixed
  * order.  dout has to be finite, and lse within about +-1e4: the rebuilt probabilities carry a
  * relative error of |lse| * 2^-23.  slopes are constants: they get no gradient.
- * Replaces the attention part of TransformerLayer::backward (src/transformer.cuh:604-664:
- * attnScoresKernel, attnApplyKernel, softmaxBackwardKernel, scaleBufferKernel, matMulATKernel). */
+ * Replaces the attention products of TransformerLayer::backward with softmaxBackwardKernel and
+ * scaleBufferKernel between them (src/transformer.cuh:8-19, 47-108, 209-214). */
 typedef struct dlb_attn_grad {
   dlb_heads dout, dq, dk, dv;
   float *dtable;
