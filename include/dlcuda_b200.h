@@ -521,14 +521,13 @@ DLB_API int dlb_ce_from_ids_bwd(const int32_t *target_ids, const float *y_pred,
  * product is split into two parts of 11 bits and three of their products are summed in fp32, which
  * leaves out 2^-21 of |x||y|; DLB_BF16 multiplies on the tensor cores with fp32 sums and softmax
  * statistics and rounds probabilities (in the backward also the gradients of the scores) to bf16 in
- * front of the next product.  head_dim 1..128; bf16 with
- * head_dim, strides and addresses in multiples of 16 bytes takes the tensor cores, anything else
- * kernels with fp32 arithmetic.  The result does not depend on scheduling: same call, same bits.
+ * front of the next product.  head_dim 1..128; bf16 with head_dim, strides and addresses in
+ * multiples of 16 bytes takes the tensor cores, anything else kernels with fp32 arithmetic.  The result does not depend on scheduling: same call, same bits.
  * As with the other pipelined kernels, make the first call of a kind on a device before capturing.
  *
  * Replaces the chain attnScoresKernel, applyCausalMaskKernel, softmaxForwardKernel and
- * attnApplyKernel (src/transformer.cuh:8-58) for programs that do not need the probabilities in
- * memory; caps, distance and bucket biases, documents, prefixes, lengths and
+ * attnApplyKernel (launched at src/transformer.cuh:462-487) for programs that do not need the
+ * probabilities in memory; caps, distance and bucket biases, documents, prefixes, lengths and
  * shared key/value heads have no counterpart in the reference. */
 #define DLB_ATTN_MAX_HEAD_DIM 128
 #define DLB_ATTN_MAX_BUCKETS 64
@@ -567,8 +566,7 @@ DLB_API int dlb_attn_fwd(const dlb_attn *a, void *workspace, size_t workspace_by
  * probabilities are rebuilt from lse.  Keys that no query reaches get zero.  Every sum has a fixed
  * order.  dout has to be finite, and lse within about +-1e4: the rebuilt probabilities carry a
  * relative error of |lse| * 2^-23.  slopes are constants: they get no gradient.
- * Replaces the attention products of TransformerLayer::backward with softmaxBackwardKernel and
- * scaleBufferKernel between them (src/transformer.cuh:8-19, 47-108, 209-214). */
+ * Replaces the attention part of TransformerLayer::backward (src/transformer.cuh:604-658). */
 typedef struct dlb_attn_grad {
   dlb_heads dout, dq, dk, dv;
   float *dtable;
