@@ -522,8 +522,9 @@ DLB_API int dlb_ce_from_ids_bwd(const int32_t *target_ids, const float *y_pred,
  * leaves out 2^-21 of |x||y|; DLB_BF16 multiplies on the tensor cores with fp32 sums and softmax
  * statistics and rounds probabilities (in the backward also the gradients of the scores) to bf16 in
  * front of the next product.  head_dim 1..128; bf16 with head_dim, strides and addresses in
- * multiples of 16 bytes takes the tensor cores, anything else kernels with fp32 arithmetic.  The result does not depend on scheduling: same call, same bits.
- * As with the other pipelined kernels, make the first call of a kind on a device before capturing.
+ * multiples of 16 bytes takes the tensor cores, anything else kernels with fp32 arithmetic.
+ * The result does not depend on scheduling: same call, same bits.  As with the other pipelined
+ * kernels, make the first call of a kind on a device before capturing.
  *
  * Replaces the chain attnScoresKernel, applyCausalMaskKernel, softmaxForwardKernel and
  * attnApplyKernel (launched at src/transformer.cuh:462-487) for programs that do not need the
