@@ -36,8 +36,9 @@ int check(const char *call, const dlb_attn *a) {
   DLB_REQUIRE(a->causal == 0 || a->causal == 1, DLB_ERR_INVALID_ARG, "%s: causal=%d", call, a->causal);
   DLB_REQUIRE(std::isfinite(a->scale), DLB_ERR_INVALID_ARG, "%s: scale=%g", call, a->scale);
   DLB_REQUIRE(std::isfinite(a->cap) && a->cap >= 0.f, DLB_ERR_INVALID_ARG, "%s: cap=%g", call, a->cap);
-  DLB_REQUIRE((a->q_docs == nullptr) == (a->kv_docs == nullptr), DLB_ERR_INVALID_ARG,
-              "%s: document numbers are needed for queries and keys, or for neither", call);
+  // (an array without elements may have any address, NULL too: that of an empty tensor is)
+  DLB_REQUIRE(a->batch == 0 || a->q_len == 0 || a->kv_len == 0 || (a->q_docs == nullptr) == (a->kv_docs == nullptr),
+              DLB_ERR_INVALID_ARG, "%s: document numbers are needed for queries and keys, or for neither", call);
   if (a->table) {
     DLB_REQUIRE(a->bucket_of != nullptr, DLB_ERR_INVALID_ARG, "%s: table without bucket_of", call);
     DLB_REQUIRE(a->buckets > 0 && a->max_distance >= 0, DLB_ERR_INVALID_ARG, "%s: buckets=%d max_distance=%d", call,
@@ -80,8 +81,9 @@ AttnArgs args_of(const dlb_attn *a) {
   p.kv_lens = a->kv_lens;
   p.q_start = a->q_start;
   p.prefix = a->prefix;
-  p.q_docs = a->q_docs;
-  p.kv_docs = a->kv_docs;
+  const bool docs = a->q_docs && a->kv_docs;  // one alone: the other side is empty, and no pair is left to hide
+  p.q_docs = docs ? a->q_docs : nullptr;
+  p.kv_docs = docs ? a->kv_docs : nullptr;
   p.slopes = a->slopes;
   p.table = a->table;
   p.buckets = a->table ? a->buckets : 0;

@@ -548,7 +548,7 @@ typedef struct dlb_attn {
   float cap; /* 0: scores are not capped */
   int buckets, max_distance; /* of table / bucket_of; ignored without a table */
   const int32_t *kv_lens, *q_start, *prefix; /* [batch] or NULL */
-  const int32_t *q_docs, *kv_docs;           /* [batch, q_len], [batch, kv_len]: both or neither */
+  const int32_t *q_docs, *kv_docs;           /* [batch, q_len], [batch, kv_len]: both or neither (NULL will do for an empty one) */
   const float *slopes;                       /* [heads] or NULL */
   const float *table;                        /* [heads, buckets] or NULL */
   const int32_t *bucket_of;                  /* [2*max_distance + 1], values 0..buckets-1 (clamped) */

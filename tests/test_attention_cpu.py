@@ -66,6 +66,20 @@ def test_null_blocks_and_overlapping_outputs():
     assert lib.dlb_attn_bwd(ctypes.byref(block()), ctypes.byref(g), FAKE, 1 << 30, None) == capi.ERR_INVALID_ARG  # no lse
 
 
+def test_documents_of_an_empty_side():
+    """The address of an array without elements says nothing: an empty tensor's is NULL."""
+    lib = capi.lib()
+    h = capi.Heads(FAKE, 4096, 64, 16)
+    g = capi.AttnGrad(dout=h, dq=h, dk=h, dv=h)
+    for docs in (dict(q_docs=FAKE), dict(kv_docs=FAKE), dict(q_docs=FAKE, kv_docs=FAKE)):
+        assert lib.dlb_attn_fwd(ctypes.byref(block(q_len=0, **docs)), None, 0, None) == capi.OK
+        assert lib.dlb_attn_fwd(ctypes.byref(block(batch=0, **docs)), None, 0, None) == capi.OK
+        # refused for the workspace alone, not for the documents
+        a = block(kv_len=0, lse=FAKE, **docs)
+        assert lib.dlb_attn_bwd(ctypes.byref(a), ctypes.byref(g), None, 0, None) == capi.ERR_WORKSPACE
+        assert lib.dlb_attn_bwd_workspace_bytes(ctypes.byref(a), ctypes.byref(g)) > 0
+
+
 def test_workspace_is_asked_for():
     lib = capi.lib()
     a = block(lse=FAKE)

@@ -227,6 +227,21 @@ def test_empty_sizes(dtype):
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_empty_sizes_with_documents(dtype):
+    dt = DTYPES[dtype]
+    full = lambda *s: torch.ones(*s, dtype=dt, device="cuda")  # noqa: E731
+    docs = lambda b, n: torch.zeros(b, n, dtype=torch.int32, device="cuda")  # noqa: E731
+    for B, Sq, Sk in ((2, 5, 0), (2, 1, 0), (2, 0, 7), (0, 5, 7), (2, 0, 0)):
+        q, k = full(B, Sq, 2, 16), full(B, Sk, 2, 16)
+        how = dict(q_docs=docs(B, Sq), kv_docs=docs(B, Sk))
+        o, lse = ops.attn_fwd(q, k, k, **how)
+        assert (o == 0).all() and (lse == -math.inf).all()
+        dq, dk, dv, _ = ops.attn_bwd(q, q, k, k, o, lse, **how)
+        assert dq.shape == q.shape and dk.shape == k.shape
+        assert (dq == 0).all() and (dk == 0).all() and (dv == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("D", [64, 20])
 def test_same_bits_every_time_and_in_a_graph(D, dtype):
     """The second call gives the first one's bits; a captured step follows lengths that change between replays."""
