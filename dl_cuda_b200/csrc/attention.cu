@@ -245,10 +245,18 @@ int launch_bwd(const AttnArgs &p, cudaStream_t st) {
       const size_t smem = gen_bwd_smem<DP, RG>() + gen_table_bytes<RG>(p);
       auto kern = attn_bwd_generic_kernel<T, DP, RG>;
       if (int s = allow_smem(kern, smem, "attn_bwd")) return s;
-      const int key_blocks = blocks(16 * RG, true), all = key_blocks + blocks(16 * RG, false);
-      if (all > 0) {
-        launch_pdl(kern, dim3(all), dim3(kGenThreads), smem, st, args, vec, key_blocks);
+      const int key_blocks = blocks(16 * RG, true), query_blocks = blocks(16 * RG, false);
+      auto pass = [&](int all, int of_keys) -> int {
+        if (all == 0) return DLB_OK;
+        launch_pdl(kern, dim3(all), dim3(kGenThreads), smem, st, args, vec, of_keys);
         DLB_LAUNCH_CHECK("attn_bwd_generic");
+        return DLB_OK;
+      };
+      if (sizeof(T) == 2) {  // the query pass mends delta for the key pass
+        if (int s = pass(query_blocks, 0)) return s;
+        if (int s = pass(key_blocks, key_blocks)) return s;
+      } else {
+        if (int s = pass(key_blocks + query_blocks, key_blocks)) return s;
       }
       return launch_table_sum(args, st);
     };

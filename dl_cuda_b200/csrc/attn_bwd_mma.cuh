@@ -3,11 +3,11 @@
 // A CTA keeps 128 rows X, Y (FOR_KEYS: a tile of K and V; else of Q and dO) and streams the other side
 // U, W (Q and dO of every head of the group; else K and V) past them in tiles of 128 rows:
 //     S = X U^T, G = Y W^T (TMEM) -> P = 2^(s - lse), D = P (G - delta), times the cap's derivative
-//     FOR_KEYS: dV += P W, dK += D U;   else dQ += D U                 (TMEM, scaled at the end)
-// with P and D written over S and G as bf16.  The row threads take the exponentials of S while the tensor
-// cores make G and the last tile's dK, and D while they make dV and the next S.  TMEM holds S, G and the
-// sums; for heads up to 64 wide it has room for more, and S does not wait for P: the key pass keeps P
-// beside S, the query pass two S where its ring has four stages to feed them.
+//     FOR_KEYS: dV += P W, dK += D U;   else dQ += D U, R += P U        (TMEM, scaled at the end)
+// with P and D written over S and G as bf16 (P of the query pass beside D).  The row threads take the
+// exponentials of S while the tensor cores make G and the last tile's dK, and D while they make dV and the
+// next S.  TMEM holds S, G and the sums; for heads up to 64 wide it has room for more, and S does not wait
+// for P: the key pass keeps P beside S, the query pass two S where its ring has four stages to feed them.
 //
 // Tiles of 64 columns with two buffers each were slower (889 instead of 811 us for both passes over 4096
 // x 4096 tokens, 32 heads of 128): a product of 128 x 64 takes the tensor cores as long as one of 128 x
@@ -16,8 +16,17 @@
 // clock) and dV with the next S, which cannot start before P is complete, 1260; the tensor cores are busy
 // for 2048.
 //
-// Two passes rebuild S and G twice: 7 products of 2 * dim flop per pair where a single pass would need
+// Two passes rebuild S and G twice: 8 products of 2 * dim flop per pair where a single pass would need
 // 5.  In return no sum crosses a CTA: no fp32 copy of dQ in memory, no atomics, the same bits every time.
+//
+// delta.  <dout, o> from the bf16 output is off by its rounding, which moves every D of a row the same way:
+// where values have a common part (o large, D small) that is far more than D's own rounding.  The query
+// pass therefore takes it as a first guess only.  Its rows add up D in fp32; with the true delta a row's D
+// add up to zero, so the sum e is what the guess is off by, and
+//     dQ = scale (sum_j D_ij k_j - e_i R_i),  R_i = sum_j P_ij k_j (times the cap's derivative)
+// at the price of one product; delta + e goes to the key pass, which runs second.  dq and dk of 70 causal
+// tokens come from 2.7e-3 to 2.35e-3 of the exact ones (the output's and D's own rounding make 2.35e-3),
+// both passes over 4096 tokens, 32 heads of 128 on 8, causal with a cap, from 537 to 578 us.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -60,7 +69,8 @@ __device__ __forceinline__ int far_side(const AttnArgs &a, int d0) {
 }
 
 // {-lse * log2(e), -delta} of query x (row `row` of tile `tile`), delta = <dout_x, o_x> by the PARTS threads
-// of the row, and its place in row_stats filled; rows behind the last query get {-infinity, 0}.
+// of the row (a first guess, see above), and its place in row_stats filled; rows behind the last query get
+// {-infinity, 0}.
 template <int NB, int PARTS>
 __device__ __forceinline__ float2 make_row_stats(const AttnArgs &a, int b, int h, int tile, int x, int part, int row, bool valid,
                                                  float (*delta_part)[kTileRows]) {
@@ -140,14 +150,15 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   __shared__ uint64_t x_full, full[ST], empty[ST], s_full[2], g_full, p_full[2], d_full, v_full, acc_full, drain;
   __shared__ uint32_t tmem_slot;
   __shared__ int dead_flag, doc_range[2];
-  __shared__ float delta_part[FOR_KEYS ? 1 : PARTS][kTileRows];
+  __shared__ float delta_part[FOR_KEYS ? 1 : PARTS][kTileRows], sum_part[FOR_KEYS ? 1 : PARTS][kTileRows];
   __shared__ __align__(16) int doc_tile[kTileRows];
   volatile int *dead = &dead_flag;
   // s_full and p_full come in pairs, used in turn: with two S the tensor cores may finish the next tile's
   // before a row thread has seen this one's.
-  // TMEM: S 0, G 128, dK or dQ 256; then dV 384 and P over S or at 448, or the second S at 384
+  // TMEM: S 0, G 128, dK or dQ 256; then dV 384 and P over S or at 448, or the second S at 384 and R at
+  // 320 (heads up to 64 wide), or R at 384
   constexpr bool kTwoS = !FOR_KEYS && ST >= 4, kOwnP = FOR_KEYS && NB == 1;
-  constexpr uint32_t kAccX = 256, kAccY = 384, kG = 128;
+  constexpr uint32_t kAccX = 256, kAccY = !FOR_KEYS && NB == 1 ? 320 : 384, kG = 128;
   constexpr uint32_t kPStep = kOwnP ? 8 : 16;  // columns of P per 16 of S
   const bool table_sums = BIAS == kTable && !FOR_KEYS && a.dtable != nullptr;
 
@@ -280,6 +291,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       bucket_sum = both(0.f);
       bucket_now = next;
     };
+    float2 ds_sum[2] = {both(0.f), both(0.f)};  // of this thread's D, for e
     int it = -1;
     for (int g = 0; g < heads_here; g++) {
       const int h = FOR_KEYS ? hk * a.group + g : unit;
@@ -309,7 +321,8 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         const float *stats = reinterpret_cast<const float *>(smem + Shape::kStats + s * kStatsBytes) + part * kCols;
         // Probabilities, from S alone.  A chunk's P and D go over the first 8 columns of its own S and G.
         const uint32_t s_at = s_base + (kTwoS && (it & 1) ? 384 : 0);
-        float p[kCols], x_all[CAP ? kCols : 1];
+        float p[kCols], capped[CAP ? kCols : 1];  // P, P times the cap's derivative
+        auto through_cap = [&](int e) { return make_float2(CAP ? capped[CAP ? e : 0] : p[e], CAP ? capped[CAP ? e + 1 : 0] : p[e + 1]); };
 #pragma unroll
         for (int q = 0; q < kChunks; q++) {
           const int e0 = q * 16, c1 = c0 + part * kCols + e0;
@@ -319,11 +332,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           float x16[16];
 #pragma unroll
           for (int e = 0; e < 16; e++) x16[e] = __uint_as_float(sr[e]);
-          if (CAP) {
-            cap_scores(x16, cap);
-#pragma unroll
-            for (int e = 0; e < 16; e++) x_all[CAP ? e0 + e : 0] = x16[e];
-          }
+          if (CAP) cap_scores(x16, cap);
           const int d0 = FOR_KEYS ? x - (view.start + c1) : c1 - (view.start + x);  // distance j - p at e = 0
           const float *lut_at = lut + d0 + a.reach + kLutPad;
           const int far_at = BIAS == kTable ? far_side<FOR_KEYS>(a, d0) : 0;
@@ -372,7 +381,16 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             if (CAP) {  // a hidden score may be NaN, and the cap's derivative of it
 #pragma unroll
               for (int e = 0; e < 16; e++)
-                if (p[e0 + e] == 0.f) x_all[CAP ? e0 + e : 0] = 0.f;
+                if (p[e0 + e] == 0.f) x16[e] = 0.f;
+            }
+          }
+          if (CAP) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {  // d tanh = 1 - tanh^2
+              const float2 t = mul2(make_float2(x16[e], x16[e + 1]), uncap);
+              const float2 c = mul2(make_float2(p[e0 + e], p[e0 + e + 1]), fma2(make_float2(-t.x, -t.y), t, both(1.f)));
+              capped[CAP ? e0 + e : 0] = c.x;
+              capped[CAP ? e0 + e + 1 : 0] = c.y;
             }
           }
           if (FOR_KEYS) {
@@ -396,7 +414,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
           uint32_t gr[16];
           tmem_load16(g_at + e0, gr);
           tmem_loaded(gr);
-          float ds[16];
+          float dp[16];
 #pragma unroll
           for (int e = 0; e < 16; e += 4) {
             float4 d4 = make_float4(row_stat.y, row_stat.y, row_stat.y, row_stat.y);
@@ -404,15 +422,14 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 #pragma unroll
             for (int k = 0; k < 4; k += 2) {
               const float2 minus = k ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);
-              const float2 dp = add2(make_float2(__uint_as_float(gr[e + k]), __uint_as_float(gr[e + k + 1])), minus);
-              const float2 d2 = mul2(make_float2(p[e0 + e + k], p[e0 + e + k + 1]), dp);
-              ds[e + k] = d2.x;
-              ds[e + k + 1] = d2.y;
+              const float2 d2 = add2(make_float2(__uint_as_float(gr[e + k]), __uint_as_float(gr[e + k + 1])), minus);
+              dp[e + k] = d2.x;
+              dp[e + k + 1] = d2.y;
             }
           }
           if (f != 3) {  // what is hidden may have met anything in V
 #pragma unroll
-            for (int e = 0; e < 16; e++) ds[e] = p[e0 + e] == 0.f ? 0.f : ds[e];
+            for (int e = 0; e < 16; e++) dp[e] = p[e0 + e] == 0.f ? 0.f : dp[e];
           }
           if (table_sums) {
             // One run of columns per bucket: its sums stay in registers until the bucket changes.
@@ -422,7 +439,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
               if (n_now != bucket_now) flush_bucket(n_now);
               float2 t = both(0.f);
 #pragma unroll
-              for (int e = 0; e < 16; e++) t = add2(t, make_float2(ds[e], p[e0 + e]));
+              for (int e = 0; e < 16; e++) t = add2(t, make_float2(p[e0 + e] * dp[e], p[e0 + e]));
               bucket_sum = add2(bucket_sum, t);
             } else {
               const unsigned char *at = bucket_lut + d0 + a.reach + kLutPad;
@@ -430,21 +447,26 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
               for (int e = 0; e < 16; e++) {
                 const int n_now = at[e];
                 if (n_now != bucket_now) flush_bucket(n_now);
-                bucket_sum = add2(bucket_sum, make_float2(ds[e], p[e0 + e]));
+                bucket_sum = add2(bucket_sum, make_float2(p[e0 + e] * dp[e], p[e0 + e]));
               }
             }
           }
           uint32_t packed[8];
 #pragma unroll
           for (int e = 0; e < 8; e++) {
-            float2 y = make_float2(ds[2 * e], ds[2 * e + 1]);
-            if (CAP) {  // d tanh = 1 - tanh^2
-              const float2 t = mul2(make_float2(x_all[CAP ? e0 + 2 * e : 0], x_all[CAP ? e0 + 2 * e + 1 : 0]), uncap);
-              y = mul2(y, fma2(make_float2(-t.x, -t.y), t, both(1.f)));
-            }
+            const float2 d2 = make_float2(dp[2 * e], dp[2 * e + 1]), y = mul2(through_cap(e0 + 2 * e), d2);
+            if (!FOR_KEYS) ds_sum[e & 1] = fma2(make_float2(p[e0 + 2 * e], p[e0 + 2 * e + 1]), d2, ds_sum[e & 1]);
             packed[e] = pack_bf16(y.x, y.y);
           }
           tmem_store8(g_at + e0, packed);
+          if (!FOR_KEYS) {  // beside D
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+              const float2 y = through_cap(e0 + 2 * e);
+              packed[e] = pack_bf16(y.x, y.y);
+            }
+            tmem_store8(g_at + e0 + 8, packed);
+          }
         }
         if (n == tail) {
           // Rows of K that no query reaches may hold anything, and 0 * NaN is NaN.
@@ -463,6 +485,15 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       }
     }
     if (table_sums) flush_bucket(0);
+    float off = 0.f;  // what delta was off by
+    if constexpr (!FOR_KEYS) {
+      const float2 sum = add2(ds_sum[0], ds_sum[1]);
+      sum_part[part][row] = sum.x + sum.y;
+      named_bar_sync(1, kRowThreads);
+#pragma unroll
+      for (int k = 0; k < PARTS; k++) off += sum_part[k][row];
+      if (part == 0) stats_tile(a, b, unit, tile)[kStatRows + row] = row_stat.y - off;
+    }
     mbar_wait(&acc_full, 0, dead, timeouts);
     tc_fence_after();
     // FOR_KEYS: the first half of the row warps stores dK, the other dV; else all share the columns of dQ.
@@ -477,6 +508,13 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       if (it >= 0) {
         tmem_load32(acc_at + c, o);
         tmem_loaded(o);
+        if constexpr (!FOR_KEYS) {
+          uint32_t r[32];
+          tmem_load32(tmem + lane_base + kAccY + c, r);
+          tmem_loaded(r);
+#pragma unroll
+          for (int e = 0; e < 32; e++) o[e] = __float_as_uint(fmaf(-off, __uint_as_float(r[e]), __uint_as_float(o[e])));
+        }
       }
 #pragma unroll
       for (int e = 0; e < 32; e += 8) {
@@ -557,10 +595,12 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       auto add_dv = [&](int it) {  // P of tile `it` is there
         accumulate(kAccY, kOwnP ? 448 : 0, kPStep, u_desc_mn + (it % ST) * kStageStep + kW, it > 0, kOwnP ? &v_full : nullptr);
       };
-      auto add_x = [&](int it) {  // dK or dQ, when D of tile `it` is there
+      auto add_x = [&](int it) {  // dK, or dQ and R, when D of tile `it` is there
         mbar_wait(&d_full, it & 1, dead, timeouts);
         tc_fence_after();
-        accumulate(kAccX, kG, 16, u_desc_mn + (it % ST) * kStageStep, it > 0, &empty[it % ST]);
+        const uint64_t ud = u_desc_mn + (it % ST) * kStageStep;
+        if (!FOR_KEYS) accumulate(kAccY, kG + 8, 16, ud, it > 0, nullptr);
+        accumulate(kAccX, kG, 16, ud, it > 0, &empty[it % ST]);
       };
       auto wait_p = [&](int it) {  // S of tile `it` has been read, its P is there
         mbar_wait(&p_full[it & 1], (it >> 1) & 1, dead, timeouts);

@@ -472,8 +472,8 @@ static __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __
   if (a.lse && tid == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
-// Fills row_stats: -lse * log2(e) and -delta, delta = <dout_i, o_i> (= sum_j P_ij dP_ij).  A row is taken by
-// LANES lanes with one 16-byte vector of each at a time, or by a warp element by element.
+// Fills row_stats: -lse * log2(e) and -delta, delta = <dout_i, o_i> (= sum_j P_ij dP_ij; from a bf16 output
+// a first guess, see attn_bwd_generic).  A row is taken by LANES lanes with one 16-byte vector of each at a time, or by a warp element by element.
 template <typename T, int LANES, bool VEC>
 static __global__ void __launch_bounds__(256) attn_row_stats_kernel(const __grid_constant__ AttnArgs a) {
   pdl_prologue();
@@ -530,6 +530,9 @@ constexpr size_t gen_bwd_smem() {
 // other side streams by in tiles of 64 rows:
 //   P = exp2(s - lse), dS = P (dP - delta);  FOR_KEYS: dV += P^T dO, dK += dS^T Q over the heads of
 // the group, else dQ += dS K.  Each pass rebuilds the scores, so no sum crosses a CTA.
+// With bf16 storage delta comes from a rounded output; a row's dS add up to what that is off by, e, and the
+// query pass takes e sum_j P_j k_j off dQ again and leaves delta + e to the key pass, a launch of its own
+// then (attn_bwd_mma.cuh tells more).
 template <typename T, int DP, int RG, bool FOR_KEYS>
 __device__ __forceinline__ void attn_bwd_generic(const AttnArgs &a, bool vec, int block) {
   extern __shared__ __align__(16) float gen_smem[];
@@ -541,6 +544,8 @@ __device__ __forceinline__ void attn_bwd_generic(const AttnArgs &a, bool vec, in
   unsigned char *bucket_lut = reinterpret_cast<unsigned char *>(sums + 2 * a.buckets * kRows);  // by distance
   __shared__ float2 col_stat_tiles[2][kGenCols];
   __shared__ int col_doc_tiles[2][kGenCols];
+  constexpr bool kFixDelta = !FOR_KEYS && sizeof(T) == 2;
+  __shared__ float ds_sums[CG][kRows];
   const bool want_table = !FOR_KEYS && a.dtable != nullptr;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int r0 = (warp % RG) * 16, cg = warp / RG, w0 = cg * 8 * NT;  // this warp's rows and columns
@@ -583,7 +588,7 @@ __device__ __forceinline__ void attn_bwd_generic(const AttnArgs &a, bool vec, in
     end[x] = (!FOR_KEYS && valid) ? row_end(a, view, row0 + r) : 0;
     row_stat[x] = (!FOR_KEYS && valid) ? stat_at(a, b, unit, row0 + r) : make_float2(-INFINITY, 0.f);
   }
-  float acc_x[DP / 32][4][4], acc_y[DP / 32][4][4];
+  float acc_x[DP / 32][4][4], acc_y[DP / 32][4][4], ds_sum[2] = {0.f, 0.f};
 #pragma unroll
   for (int q = 0; q < DP / 32; q++)
 #pragma unroll
@@ -678,7 +683,8 @@ __device__ __forceinline__ void attn_bwd_generic(const AttnArgs &a, bool vec, in
             ds_tile[r * kPitch + cc] = grad;
             p_tile[r * kPitch + cc] = prob;
           }
-          p[k][e] = prob;
+          if (kFixDelta) ds_sum[x] += grad;
+          p[k][e] = kFixDelta ? prob * dcap * a.scale : prob;
           d[k][e] = grad * dcap * a.scale;  // through the cap and the scale: the gradient of <q, k>
         }
       if (want_table) {
@@ -707,7 +713,7 @@ __device__ __forceinline__ void attn_bwd_generic(const AttnArgs &a, bool vec, in
           }
         }
       }
-      if (FOR_KEYS) gen_accumulate<DP, NT>(acc_y, p, ws, w0, lane);
+      if (FOR_KEYS || kFixDelta) gen_accumulate<DP, NT>(acc_y, p, FOR_KEYS ? ws : us, w0, lane);
       gen_accumulate<DP, NT>(acc_x, d, us, w0, lane);
       __syncthreads();
       if (NBUF == 2) buf ^= 1;
@@ -715,6 +721,30 @@ __device__ __forceinline__ void attn_bwd_generic(const AttnArgs &a, bool vec, in
       step = next;
     }
     async_wait<0>();
+  }
+  if constexpr (kFixDelta) {
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      const float sum = quad_sum(ds_sum[x]);
+      if (c == 0) ds_sums[cg][r0 + g + 8 * x] = sum;
+    }
+    __syncthreads();
+    float off[2] = {0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < CG; k++)
+#pragma unroll
+      for (int x = 0; x < 2; x++) off[x] += ds_sums[k][r0 + g + 8 * x];
+#pragma unroll
+    for (int q = 0; q < DP / 32; q++)
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc_x[q][k][e] = fmaf(-off[e >> 1], acc_y[q][k][e], acc_x[q][k][e]);
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      const int r = r0 + g + 8 * x, i = row0 + r;
+      if (c == 0 && cg == 0 && r < rows) stats_tile(a, b, unit, i / kStatRows)[kStatRows + i % kStatRows] = row_stat[x].y - off[x];
+    }
   }
   float *us = ring;
   // Join of the column groups, through the place of the streamed tiles: [column group][row][column].
@@ -764,7 +794,8 @@ __device__ __forceinline__ void attn_bwd_generic(const AttnArgs &a, bool vec, in
   }
 }
 
-// Both passes in one launch: the first key_blocks CTAs make dK and dV, the others dQ and the table's parts.
+// Both passes in one launch, or one of them: the first key_blocks CTAs make dK and dV, the others dQ and the
+// table's parts.
 template <typename T, int DP, int RG>
 static __global__ void __launch_bounds__(kGenThreads, DP <= 64 ? 2 : 1)
 attn_bwd_generic_kernel(const __grid_constant__ AttnArgs a, bool vec, int key_blocks) {

@@ -13,6 +13,9 @@ the tensor cores in it (else w = 0), entry by entry:
     |dv' - dv| <= (d + w) P^T|dO| + u |dv|
     |dS' - dS| <= (d + w) |dS| + P (e_dp + e_delta) =: b, e_dp = (D + 8) 2^-24 |dO||V|,
          e_delta = |dO| . bound(o) + (D + 8) 2^-24 |dO| . |o|
+         or, where delta is told by the row's own sum of score gradients (exact_delta), which is off by their
+         errors: e_delta = d (P.|dP| + |delta| + f) + P.e_dp + w f, f being the e_delta above, which a row's
+         share of keys times that sum takes off again, rounded to w
     |dx' - dx| <= scale (c b + 4 d_s (|dS| + b)) =: bx for dx = scale c dS, c = 1 - tanh^2 off by at most
          4 d_s (twice the tanh's error and a rounding): (c + e1)(dS + e2) - c dS = c e2 + e1 dS + e1 e2
     |dq' - dq| <= bx |K| + u |dq|, |dk' - dk| <= bx^T |Q| + u |dk|
@@ -29,7 +32,7 @@ F64 = torch.float64
 
 
 def reference(q, k, v, dout=None, scale=None, cap=0.0, causal=False, kv_lens=None, q_start=None, prefix=None,
-              q_docs=None, kv_docs=None, slopes=None, table=None, bucket_of=None, tensor_cores=None):
+              q_docs=None, kv_docs=None, slopes=None, table=None, bucket_of=None, tensor_cores=None, exact_delta=False):
     """(values, bounds): dicts of o, lse and, with dout, dq, dk, dv, dtable in float64 on the inputs' device."""
     B, Sq, H, D = q.shape
     Sk, Hk = k.shape[1], k.shape[2]
@@ -98,6 +101,10 @@ def reference(q, k, v, dout=None, scale=None, cap=0.0, causal=False, kv_lens=Non
     dS = P * (dP - delta)
     e_dp = (D + 8) * 2.0 ** -24 * (g.abs() @ vd.abs().transpose(-1, -2))
     e_delta = (g.abs() * b_o).sum(-1, keepdim=True) + (D + 8) * 2.0 ** -24 * (g.abs() * o.abs()).sum(-1, keepdim=True)
+    from_output = e_delta
+    if exact_delta:
+        e_delta = d * ((P * dP.abs()).sum(-1, keepdim=True) + delta.abs() + from_output) + (P * e_dp).sum(-1, keepdim=True) \
+            + w * from_output
     b_s = (d + w) * dS.abs() + P * (e_dp + e_delta)
     if table is not None:
         n = table.shape[1]
@@ -106,7 +113,7 @@ def reference(q, k, v, dout=None, scale=None, cap=0.0, causal=False, kv_lens=Non
         b_t = 2 * (d * dS.abs() + d * P * (dP.abs() + delta.abs()) + P * e_dp)
         bounds["dtable"] = torch.einsum("bhij,bijn->hn", b_t, one) + tiny
         if w:
-            most = e_delta + (e_dp.amax(-1, keepdim=True) if Sk else 0.0)
+            most = from_output + (e_dp.amax(-1, keepdim=True) if Sk else 0.0)
             bounds["dtable"] += (Sk / 128 + 2) * (2.0 ** -11 * torch.einsum("bhij,bijn->hn", P * most, one)
                                                   + 4 * 2.0 ** -40 * most.sum((0, 2, 3))[:, None])
     dcap = (1 - t * t) if cap else torch.ones_like(x)

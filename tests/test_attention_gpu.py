@@ -226,6 +226,25 @@ def test_empty_sizes(dtype):
     assert dq.numel() == 0 and (dk == 0).all() and (dv == 0).all() and (dtable == 0).all()
 
 
+@pytest.mark.parametrize("kind", ["plain", "causal", "cap+causal", "slopes+causal", "table", "table64", "mixed_docs", "lens"])
+@pytest.mark.parametrize("shape", [(2, 19, 19, 4, 2, 64), (1, 200, 200, 2, 1, 128), (2, 130, 400, 2, 2, 20), (1, 700, 700, 2, 1, 16),
+                                   (1, 150, 150, 2, 2, 72)])
+def test_values_with_a_common_part(shape, kind):
+    """Values that share a large part: the output's rounding, times the output's gradient, is far more than the score
+    gradients, and must not reach dq and dk through delta."""
+    B, Sq, Sk, H, Hk, D = shape
+    q, k, v, dout = make(sum(shape) + 1, "bf16", *shape, layout="plain", std=1.0)
+    v = (v.float() * 0.25 + 6.0).bfloat16()
+    if kind == "table64":  # more buckets than leave room for four threads a row
+        how = dict(table=torch.randn(H, 64, generator=torch.Generator().manual_seed(4)).cuda(), bucket_of=ops.rel_bucket_map(64, 90).cuda())
+    else:
+        how = options(kind, B, Sq, Sk, H)
+    values, bounds = reference(q, k, v, dout, exact_delta=True, **how)
+    o, lse = ops.attn_fwd(q, k, v, **how)
+    dq, dk, dv, dtable = ops.attn_bwd(dout, q, k, v, o, lse, **how)
+    check(dict(o=o, lse=lse, dq=dq, dk=dk, dv=dv, dtable=dtable), values, bounds)
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_empty_sizes_with_documents(dtype):
     dt = DTYPES[dtype]
