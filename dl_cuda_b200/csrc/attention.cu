@@ -196,7 +196,8 @@ struct BwdPlan {
 BwdPlan plan_bwd(const dlb_attn *a, const dlb_attn_grad *g) {
   BwdPlan p;
   p.stats_bytes = static_cast<size_t>(a->batch) * a->heads * stat_tiles(a->q_len) * 2 * kStatRows * sizeof(float);
-  p.parts = a->batch * ceil_div(a->q_len, 32);  // of the smallest tiles that any kernel uses
+  // of the smallest tiles that any kernel uses: 32 queries, or 128 keys
+  p.parts = a->batch * std::max(ceil_div(a->q_len, 32), ceil_div(a->kv_len, kTileRows));
   p.bytes = p.stats_bytes;
   if (g->dtable && a->table) p.bytes += sizeof(float) * static_cast<size_t>(a->heads) * p.parts * a->buckets;
   return p;
@@ -332,9 +333,9 @@ extern "C" int dlb_attn_bwd(const dlb_attn *a, const dlb_attn_grad *g, void *wor
   p.table_part = reinterpret_cast<float *>(static_cast<char *>(workspace) + plan.stats_bytes);
   p.table_parts = plan.parts;
   cudaStream_t st = as_stream(stream);
-  const bool mma = a->dtype == DLB_BF16 && a->batch > 0 && attn_mma_fits(p, true) && attn_bwd_mma_room(p);
+  const bool mma = a->dtype == DLB_BF16 && a->batch > 0 && attn_mma_fits(p, true);
   if (mma) {
-    p.table_parts = a->batch * ceil_div(a->q_len, kTileRows);
+    p.table_parts = a->batch * ceil_div(a->kv_len, kTileRows);
     return launch_bwd_mma(p, st);
   }
   return a->dtype == DLB_F32 ? launch_bwd<float>(p, st) : launch_bwd<__nv_bfloat16>(p, st);

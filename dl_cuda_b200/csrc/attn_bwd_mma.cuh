@@ -29,8 +29,6 @@
 // both passes over 4096 tokens, 32 heads of 128 on 8, causal with a cap, from 537 to 578 us.
 #pragma once
 
-#include <cuda_fp16.h>
-
 #include <algorithm>
 
 #include "attn_mma.cuh"
@@ -112,22 +110,20 @@ __device__ __forceinline__ float2 make_row_stats(const AttnArgs &a, int b, int h
   return stat;
 }
 
-// Bytes behind the ring: bias by distance, bucket by distance, sums per part, bucket and row (of the score
-// gradients in fp32, of the probabilities, at most 1 a row, in fp16 times 2^15, which keeps 11 bits of them
-// down to 2^-29: they only weight a correction of some thousandths), tile flags.
-constexpr float kProbScale = 32768.f;
+// Bytes behind the ring: bias by distance, bucket by distance, sums of the score gradients per part, bucket
+// and row (a thread's own, so that no order is left to chance), tile flags.  The gradient of the table is
+// made by the key pass: its delta is exact, so that nothing has to be taken off a row's sums afterwards.
 struct BwdRest {
-  int lut, buckets, sums, p_sums, flags, total;
+  int lut, buckets, sums, flags, total;
 };
 __host__ __device__ inline BwdRest bwd_rest(const AttnArgs &a, bool for_keys, int parts) {
   const int tiles = ((for_keys ? a.q_len : a.kv_len) + kTileRows - 1) / kTileRows;
-  const int slots = !for_keys && a.dtable != nullptr ? a.buckets * parts * kTileRows : 0;
+  const int slots = for_keys && a.dtable != nullptr ? a.buckets * parts * kTileRows : 0;
   BwdRest r;
   r.lut = 0;
   r.buckets = r.lut + (a.table ? 4 * lut_floats(a.reach) : 0);
   r.sums = r.buckets + (slots ? (lut_floats(a.reach) + 15) / 16 * 16 : 0);
-  r.p_sums = r.sums + slots * 4;
-  r.flags = r.p_sums + slots * 2;
+  r.flags = r.sums + slots * 4;
   r.total = r.flags + (tiles + 15) / 16 * 16;
   return r;
 }
@@ -145,7 +141,6 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   float *lut = reinterpret_cast<float *>(smem + Shape::kRest + rest.lut);
   unsigned char *bucket_lut = smem + Shape::kRest + rest.buckets;
   float *sums = reinterpret_cast<float *>(smem + Shape::kRest + rest.sums);  // [part][bucket][row]
-  __half *p_sums = reinterpret_cast<__half *>(smem + Shape::kRest + rest.p_sums);
   unsigned char *flags = smem + Shape::kRest + rest.flags;
   __shared__ uint64_t x_full, full[ST], empty[ST], s_full[2], g_full, p_full[2], d_full, v_full, acc_full, drain;
   __shared__ uint32_t tmem_slot;
@@ -160,7 +155,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   constexpr bool kTwoS = !FOR_KEYS && ST >= 4, kOwnP = FOR_KEYS && NB == 1;
   constexpr uint32_t kAccX = 256, kAccY = !FOR_KEYS && NB == 1 ? 320 : 384, kG = 128;
   constexpr uint32_t kPStep = kOwnP ? 8 : 16;  // columns of P per 16 of S
-  const bool table_sums = BIAS == kTable && !FOR_KEYS && a.dtable != nullptr;
+  const bool table_sums = BIAS == kTable && FOR_KEYS && a.dtable != nullptr;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -254,10 +249,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   if (table_sums) {
     for (int e = tid; e < 2 * (a.reach + kLutPad) + 1; e += kBwdThreads)
       bucket_lut[e] = static_cast<unsigned char>(bucket_at(a, e - a.reach - kLutPad));
-    for (int e = tid; e < PARTS * a.buckets * kTileRows; e += kBwdThreads) {
-      sums[e] = 0.f;
-      p_sums[e] = __float2half_rn(0.f);
-    }
+    for (int e = tid; e < PARTS * a.buckets * kTileRows; e += kBwdThreads) sums[e] = 0.f;
   }
   tc_fence_before();
   __syncthreads();
@@ -283,12 +275,10 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     const float2 uncap = both(CAP ? 1.f / cap.out : 0.f);
     const int tail = !FOR_KEYS && view.end % kTileRows && view.end < a.kv_len ? view.end / kTileRows : -1;
     int bucket_now = 0;
-    float2 bucket_sum = both(0.f);
+    float bucket_sum = 0.f;
     auto flush_bucket = [&](int next) {
-      const int at = (part * a.buckets + bucket_now) * kTileRows + row;
-      sums[at] += bucket_sum.x;
-      p_sums[at] = __float2half_rn(fmaf(bucket_sum.y, kProbScale, __half2float(p_sums[at])));
-      bucket_sum = both(0.f);
+      sums[(part * a.buckets + bucket_now) * kTileRows + row] += bucket_sum;
+      bucket_sum = 0.f;
       bucket_now = next;
     };
     float2 ds_sum[2] = {both(0.f), both(0.f)};  // of this thread's D, for e
@@ -432,22 +422,24 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
             for (int e = 0; e < 16; e++) dp[e] = p[e0 + e] == 0.f ? 0.f : dp[e];
           }
           if (table_sums) {
-            // One run of columns per bucket: its sums stay in registers until the bucket changes.
-            const int d0 = c1 - (view.start + x), far_at = far_side<FOR_KEYS>(a, d0);
+            // One run of columns per bucket: its sum stays in a register until the bucket changes.
+            const int d0 = x - (view.start + c1), far_at = far_side<FOR_KEYS>(a, d0);
             if (far_at >= 0) {
               const int n_now = bucket_lut[far_at];
               if (n_now != bucket_now) flush_bucket(n_now);
-              float2 t = both(0.f);
+              float2 t[2] = {both(0.f), both(0.f)};
 #pragma unroll
-              for (int e = 0; e < 16; e++) t = add2(t, make_float2(p[e0 + e] * dp[e], p[e0 + e]));
-              bucket_sum = add2(bucket_sum, t);
+              for (int e = 0; e < 16; e += 2)
+                t[e >> 1 & 1] = fma2(make_float2(p[e0 + e], p[e0 + e + 1]), make_float2(dp[e], dp[e + 1]), t[e >> 1 & 1]);
+              const float2 u = add2(t[0], t[1]);
+              bucket_sum += u.x + u.y;
             } else {
               const unsigned char *at = bucket_lut + d0 + a.reach + kLutPad;
 #pragma unroll
               for (int e = 0; e < 16; e++) {
-                const int n_now = at[e];
+                const int n_now = at[-e];
                 if (n_now != bucket_now) flush_bucket(n_now);
-                bucket_sum = add2(bucket_sum, make_float2(p[e0 + e] * dp[e], p[e0 + e]));
+                bucket_sum = fmaf(p[e0 + e], dp[e], bucket_sum);
               }
             }
           }
@@ -483,8 +475,25 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         __syncwarp();
         if (lane == 0) mbar_arrive(&d_full);
       }
+      if (table_sums) {  // this head's part of its table's gradient; the sums start anew
+        flush_bucket(0);
+        named_bar_sync(1, kRowThreads);
+        float *to = a.table_part + (static_cast<size_t>(h) * a.table_parts + b * tiles + tile) * a.buckets;
+        for (int n = warp; n < a.buckets; n += BwdWarps<PARTS>::kRows) {
+          float v = 0.f;
+#pragma unroll
+          for (int k = 0; k < PARTS; k++)
+            for (int r = lane; r < kTileRows; r += 32) {
+              float &slot = sums[(k * a.buckets + n) * kTileRows + r];
+              v += slot;
+              slot = 0.f;
+            }
+          v = warp_sum(v);
+          if (lane == 0) to[n] = v;
+        }
+        // (the next head's sums wait for the barriers around its bias by distance)
+      }
     }
-    if (table_sums) flush_bucket(0);
     float off = 0.f;  // what delta was off by
     if constexpr (!FOR_KEYS) {
       const float2 sum = add2(ds_sum[0], ds_sum[1]);
@@ -656,57 +665,16 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     }
   }
   __syncthreads();
-  if (table_sums) {
-    // A row's gradients of its scores add up to zero: what rounding left (in delta above all, which
-    // comes from the rounded o) is taken off again in proportion to P.
-    if (tid < kTileRows) {
-      float e = 0.f, p = 0.f;
-      for (int n = 0; n < a.buckets; n++)
-#pragma unroll
-        for (int k = 0; k < PARTS; k++) {
-          const int at = (k * a.buckets + n) * kTileRows + tid;
-          e += sums[at];
-          p += __half2float(p_sums[at]) * (1.f / kProbScale);
-        }
-      e = p > 0.f ? e / p : 0.f;
-      for (int n = 0; n < a.buckets; n++) {
-        float sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < PARTS; k++) {
-          const int at = (k * a.buckets + n) * kTileRows + tid;
-          sum += fmaf(-e, __half2float(p_sums[at]) * (1.f / kProbScale), sums[at]);
-        }
-        sums[n * kTileRows + tid] = sum;
-      }
-    }
-    __syncthreads();
-    float *part = a.table_part + (static_cast<size_t>(unit) * a.table_parts + b * tiles + tile) * a.buckets;
-    for (int n = warp; n < a.buckets; n += kBwdThreads / 32) {
-      float v = 0.f;
-      for (int r = lane; r < kTileRows; r += 32) v += sums[n * kTileRows + r];
-      v = warp_sum(v);
-      if (lane == 0) part[n] = v;
-    }
-  }
   if (warp == kBwdMmaWarp) {
     tc_fence_after();
     tmem_free(tmem, 512);
   }
 }
 
-// The query pass with sums for the table: four threads a row where their sums fit, else two.
-struct BwdTableShape {
-  int parts;
-  size_t smem;
-};
-inline BwdTableShape bwd_table_shape(const AttnArgs &a) {
-  const size_t ring = 1024 + static_cast<size_t>(a.dim > kBlockCols ? BwdShape<2, 1>::kRest : BwdShape<1, 2>::kRest);
-  for (int parts = 4; parts >= 2; parts -= 2) {
-    const size_t smem = ring + bwd_rest(a, false, parts).total;
-    if (smem <= kMaxDynamicSmem) return {parts, smem};
-  }
-  return {0, 0};  // does not fit at all
-}
+// What the sums of the most buckets and the longest map leave room for.
+constexpr int kMostSums = 4 * DLB_ATTN_MAX_BUCKETS * kTileRows * 2, kMostLuts = 5 * (2 * (DLB_ATTN_MAX_DISTANCE + kLutPad) + 4) + 16;
+static_assert(1024 + BwdShape<1, 2>::kRest + kMostSums + kMostLuts + kMaxTiles <= kMaxDynamicSmem &&
+              1024 + BwdShape<2, 1>::kRest + kMostSums + kMostLuts + kMaxTiles <= kMaxDynamicSmem, "a table must fit in some shape");
 
 template <bool FOR_KEYS>
 int bwd_mma_launch(const AttnArgs &a, const BwdMaps &maps, cudaStream_t st) {
@@ -725,10 +693,18 @@ int bwd_mma_launch(const AttnArgs &a, const BwdMaps &maps, cudaStream_t st) {
 #define DLB_PICK(NB, ST, PARTS, BIAS)                                                                            \
   (cap ? launch(attn_bwd_mma_kernel<NB, ST, PARTS, FOR_KEYS, true, BIAS>, BwdShape<NB, ST>::kRest, PARTS)        \
        : launch(attn_bwd_mma_kernel<NB, ST, PARTS, FOR_KEYS, false, BIAS>, BwdShape<NB, ST>::kRest, PARTS))
-  if constexpr (!FOR_KEYS) {
-    if (a.table && a.dtable) {  // as bwd_table_shape has it
-      if (a.dim > kBlockCols) return bwd_table_shape(a).parts == 4 ? DLB_PICK(2, 1, 4, kTable) : DLB_PICK(2, 1, 2, kTable);
-      return bwd_table_shape(a).parts == 4 ? DLB_PICK(1, 2, 4, kTable) : DLB_PICK(1, 2, 2, kTable);
+  if constexpr (FOR_KEYS) {
+    if (a.dtable) {
+      // The sums for the table cost stages of the ring; the last shape holds the most buckets there can be.
+      auto fits = [&](int ring_end, int parts) { return 1024 + ring_end + bwd_rest(a, true, parts).total <= kMaxDynamicSmem; };
+      if (a.dim <= kBlockCols) {
+        if (fits(BwdShape<1, 4>::kRest, 4)) return DLB_PICK(1, 4, 4, kTable);
+        if (fits(BwdShape<1, 2>::kRest, 4)) return DLB_PICK(1, 2, 4, kTable);
+        return DLB_PICK(1, 2, 2, kTable);
+      }
+      if (fits(BwdShape<2, 2>::kRest, 4)) return DLB_PICK(2, 2, 4, kTable);
+      if (fits(BwdShape<2, 1>::kRest, 4)) return DLB_PICK(2, 1, 4, kTable);
+      return DLB_PICK(2, 1, 2, kTable);
     }
   }
   if (a.dim <= kBlockCols) {

@@ -1,4 +1,4 @@
-// Gradients of the keys and values on the tensor cores (attn_bwd_mma.cuh).
+// Gradients of the keys, the values and the bias table on the tensor cores (attn_bwd_mma.cuh).
 #include "attn_bwd_mma.cuh"
 
 namespace dlb {

@@ -104,7 +104,6 @@ __host__ __device__ inline int lut_floats(int reach) { return 2 * (reach + kLutP
 bool attn_mma_fits(const AttnArgs &a, bool backward);
 int attn_fwd_mma_splits(const AttnArgs &a);  // shares of the keys that attn_fwd_mma wants
 int attn_fwd_mma(const AttnArgs &a, cudaStream_t st);
-bool attn_bwd_mma_room(const AttnArgs &a);  // do the sums for the table fit?
 struct BwdMaps {
   CUtensorMap q, k, v, dout;
 };

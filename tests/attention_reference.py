@@ -22,7 +22,10 @@ the tensor cores in it (else w = 0), entry by entry:
     dtable: sums of d |dS| + d P (|dP| + |delta|) + P e_dp, doubled: the rows' common error is taken off;
          on the tensor cores in proportion to sums of P that are kept in fp16 times 2^15: off by 2^-11 of the
          sum, or by 2^-40 (half a step of the smallest fp16, 2^-24, over 2^15), an addition, at most
-         Sk / 128 + 2 of them by each of four threads; and the error taken off is at most e_delta + e_dp
+         Sk / 128 + 2 of them by each of four threads; and the error taken off is at most e_delta + e_dp.
+         With exact_delta nothing is taken off: sums of 2 (d |dS| + P e_dp) + P e_delta without the term in w,
+         and of (Sq / 4 + 32) 2^-24 |dS| for a thread's own additions (a quarter of a key's queries), its
+         warp's and its row's
 """
 import math
 
@@ -112,7 +115,10 @@ def reference(q, k, v, dout=None, scale=None, cap=0.0, causal=False, kv_lens=Non
         values["dtable"] = torch.einsum("bhij,bijn->hn", dS, one)
         b_t = 2 * (d * dS.abs() + d * P * (dP.abs() + delta.abs()) + P * e_dp)
         bounds["dtable"] = torch.einsum("bhij,bijn->hn", b_t, one) + tiny
-        if w:
+        if exact_delta:
+            b_t = 2 * (d * dS.abs() + P * e_dp) + P * (e_delta - w * from_output) + (Sq / 4 + 32) * 2.0 ** -24 * dS.abs()
+            bounds["dtable"] = torch.einsum("bhij,bijn->hn", b_t, one) + tiny
+        elif w:
             most = from_output + (e_dp.amax(-1, keepdim=True) if Sk else 0.0)
             bounds["dtable"] += (Sk / 128 + 2) * (2.0 ** -11 * torch.einsum("bhij,bijn->hn", P * most, one)
                                                   + 4 * 2.0 ** -40 * most.sum((0, 2, 3))[:, None])

@@ -245,6 +245,32 @@ def test_values_with_a_common_part(shape, kind):
     check(dict(o=o, lse=lse, dq=dq, dk=dk, dv=dv, dtable=dtable), values, bounds)
 
 
+@pytest.mark.parametrize("D,buckets", [(64, 2), (64, 64), (128, 2), (128, 32), (128, 64), (20, 2)])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_bucket_map_that_alternates(D, buckets, dtype):
+    """A map whose buckets change at every distance, over some 2000 keys: every addition to a bucket's sum counts.
+    An output that puts delta off by D shows what the sums' roundings are worth: the gradient of the table must not
+    move with it, since a row's score gradients add up to zero whatever delta is taken.  (dq and dk hold for the
+    forward's own output, and so does every bound.)"""
+    B, Sq, S, H = 1, 128, 1900, 2
+    gen = torch.Generator(device="cuda").manual_seed(D + buckets)
+    q = torch.zeros(B, Sq, H, D, device="cuda", dtype=DTYPES[dtype])
+    k, v = (torch.randn(B, S, H, D, generator=gen, device="cuda").to(DTYPES[dtype]) for _ in range(2))
+    dout = torch.ones_like(q)
+    how = dict(q_start=ints([S // 2 - Sq // 2]), table=torch.zeros(H, buckets, device="cuda"),
+               bucket_of=ints([0, 1, 1, 1] * 512 + [0]))
+    values, bounds = reference(q, k, v, dout, exact_delta=dtype == "bf16", **how)
+    o, lse = ops.attn_fwd(q, k, v, **how)
+    dq, dk, dv, dtable = ops.attn_bwd(dout, q, k, v, o, lse, **how)
+    check(dict(o=o, lse=lse, dq=dq, dk=dk, dv=dv, dtable=dtable), values, bounds)
+    moved = ops.attn_bwd(dout, q, k, v, torch.ones_like(o), lse, **how)[3]
+    # Each of Sq rows: D times the error of a bucket's share w of the probabilities.  In fp32 a sum of n additions is off
+    # by n / 2 steps of 2^-24 of it (its addends are alike), n <= S / 16 + 32 with four threads a row, twice that with
+    # two; the two buckets' errors move the share w by at most w (1 - w) each, and w is 1/4.
+    error = D * Sq * 2 * 0.1875 * (S / 8 + 64) * 2.0 ** -24 + D * Sq * 2.0 ** -21
+    assert ((moved.double() - values["dtable"]).abs() <= error + bounds["dtable"]).all()
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_empty_sizes_with_documents(dtype):
     dt = DTYPES[dtype]
