@@ -11,8 +11,9 @@
 namespace dlb {
 namespace {
 
-int check_heads(const char *call, const char *name, const dlb_heads &h, long long elements) {
+int check_heads(const char *call, const char *name, const dlb_heads &h, long long elements, int dtype) {
   DLB_REQUIRE(h.ptr != nullptr || elements == 0, DLB_ERR_INVALID_ARG, "%s: null pointer %s", call, name);
+  DLB_REQUIRE(on_elements(h.ptr, dtype == DLB_F32 ? 4 : 2), DLB_ERR_INVALID_ARG, "%s: address of %s is not on an element", call, name);
   DLB_REQUIRE(h.batch_stride >= 0 && h.token_stride >= 0 && h.head_stride >= 0, DLB_ERR_INVALID_ARG,
               "%s: negative stride of %s", call, name);
   return DLB_OK;
@@ -57,11 +58,15 @@ int check(const char *call, const dlb_attn *a) {
   const long long rows = static_cast<long long>(a->batch) * a->heads * std::max(a->q_len, 1);
   DLB_REQUIRE(tiles < (1ll << 31) && rows < (1ll << 31), DLB_ERR_UNSUPPORTED,
               "%s: batch=%d heads=%d lengths %d, %d make too many rows", call, a->batch, a->heads, a->q_len, a->kv_len);
+  for (const void *p : {static_cast<const void *>(a->kv_lens), static_cast<const void *>(a->q_start), static_cast<const void *>(a->prefix),
+                        static_cast<const void *>(a->q_docs), static_cast<const void *>(a->kv_docs), static_cast<const void *>(a->slopes),
+                        static_cast<const void *>(a->table), static_cast<const void *>(a->bucket_of), static_cast<const void *>(a->lse)})
+    DLB_REQUIRE(on_elements(p, 4), DLB_ERR_INVALID_ARG, "%s: address %p is not a multiple of 4", call, p);
   const long long nq = static_cast<long long>(a->batch) * a->q_len, nk = static_cast<long long>(a->batch) * a->kv_len;
-  if (int st = check_heads(call, "q", a->q, nq)) return st;
-  if (int st = check_heads(call, "k", a->k, nk)) return st;
-  if (int st = check_heads(call, "v", a->v, nk)) return st;
-  return check_heads(call, "o", a->o, nq);
+  if (int st = check_heads(call, "q", a->q, nq, a->dtype)) return st;
+  if (int st = check_heads(call, "k", a->k, nk, a->dtype)) return st;
+  if (int st = check_heads(call, "v", a->v, nk, a->dtype)) return st;
+  return check_heads(call, "o", a->o, nq, a->dtype);
 }
 
 Heads heads_of(const dlb_heads &h) { return {h.ptr, h.batch_stride, h.token_stride, h.head_stride}; }
@@ -312,15 +317,16 @@ extern "C" int dlb_attn_bwd(const dlb_attn *a, const dlb_attn_grad *g, void *wor
   if (int st = check("attn_bwd", a)) return st;
   DLB_REQUIRE(g != nullptr, DLB_ERR_INVALID_ARG, "attn_bwd: null gradient block");
   const long long nq = static_cast<long long>(a->batch) * a->q_len, nk = static_cast<long long>(a->batch) * a->kv_len;
-  if (int st = check_heads("attn_bwd", "dout", g->dout, nq)) return st;
-  if (int st = check_heads("attn_bwd", "dq", g->dq, nq)) return st;
-  if (int st = check_heads("attn_bwd", "dk", g->dk, nk)) return st;
-  if (int st = check_heads("attn_bwd", "dv", g->dv, nk)) return st;
+  if (int st = check_heads("attn_bwd", "dout", g->dout, nq, a->dtype)) return st;
+  if (int st = check_heads("attn_bwd", "dq", g->dq, nq, a->dtype)) return st;
+  if (int st = check_heads("attn_bwd", "dk", g->dk, nk, a->dtype)) return st;
+  if (int st = check_heads("attn_bwd", "dv", g->dv, nk, a->dtype)) return st;
   if (int st = check_output("attn_bwd", "dq", g->dq, a->batch, a->q_len, a->heads)) return st;
   if (int st = check_output("attn_bwd", "dk", g->dk, a->batch, a->kv_len, a->kv_heads)) return st;
   if (int st = check_output("attn_bwd", "dv", g->dv, a->batch, a->kv_len, a->kv_heads)) return st;
   DLB_REQUIRE(a->lse != nullptr || nq == 0, DLB_ERR_INVALID_ARG, "attn_bwd: lse is needed");
   DLB_REQUIRE(g->dtable == nullptr || a->table != nullptr, DLB_ERR_INVALID_ARG, "attn_bwd: dtable without table");
+  DLB_REQUIRE(on_elements(g->dtable, 4), DLB_ERR_INVALID_ARG, "attn_bwd: address of dtable is not a multiple of 4");
   const BwdPlan plan = plan_bwd(a, g);
   if (int st = check_workspace("attn_bwd", workspace, workspace_bytes, plan.bytes)) return st;
   AttnArgs p = args_of(a);

@@ -4,6 +4,7 @@
 
 #include <climits>
 #include <cmath>
+#include <cstdint>
 
 #include "common.cuh"
 
@@ -24,6 +25,9 @@ int allow_smem(K kern, size_t smem, const char *name) {
   DLB_REQUIRE(e == cudaSuccess, DLB_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
   return DLB_OK;
 }
+
+// An address between two elements would fault in the kernel.
+inline bool on_elements(const void *p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 struct Heads {
   void *ptr;

@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(kBiasThreads) rel_bias_fwd_kernel(const __grid
 // bucket on either side and is summed in two registers; nearer elements go to a column of their own
 // thread per bucket in shared memory.
 template <typename T>
-__global__ void __launch_bounds__(kBiasThreads) rel_bias_bwd_kernel(const __grid_constant__ BiasArgs a, int parts, bool vec) {
+__global__ void __launch_bounds__(kBiasThreads) rel_bias_bwd_kernel(const __grid_constant__ BiasArgs a, int parts) {
   pdl_prologue();
   extern __shared__ float sums[];  // [buckets][threads], then the bucket of every distance
   constexpr int V = Store<T>::kPerVec, kInFlight = 4, kWarps = kBiasThreads / 32;
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kBiasThreads) rel_bias_bwd_kernel(const __grid
     const T *src = static_cast<const T *>(a.in) + ((static_cast<size_t>(b) * a.heads + h) * a.q_len + i) * a.kv_len;
     const int shift = a.reach - (a.start + i);
     auto add = [&](int j, float x) { sums[bucket_lut[max(0, min(2 * a.reach, j + shift))] * kBiasThreads + tid] += x; };
-    const RowCut<T> cut(src, a.kv_len, vec);
+    const RowCut<T> cut(src, a.kv_len, true);
     for (int e = lane; e < cut.head + cut.tail; e += 32) {
       const int j = e < cut.head ? e : cut.vectors * V + e;
       add(j, Store<T>::to_float(ld_co(src + j)));
@@ -189,12 +189,12 @@ int bias_parts(int batch, int heads, int q_len) {
   return static_cast<int>(std::max(1ll, std::min<long long>(ceil_div(rows, 8ll), ceil_div(6 * sm_count(), std::max(heads, 1)))));
 }
 
-// Can 16-byte accesses be used between the ragged ends of rows?  Addresses on element boundaries, and the
-// same place within 16 bytes for what is read and written.
-bool rows_can_be_cut(const void *p, const void *q, int esize) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(q);
-  return x % esize == 0 && (y == 0 || x % 16 == y % 16);
+// Can 16-byte accesses be used between the ragged ends of rows?  What is read and written has to have the
+// same place within 16 bytes.
+bool rows_can_be_cut(const void *p, const void *q) {
+  return q == nullptr || reinterpret_cast<uintptr_t>(p) % 16 == reinterpret_cast<uintptr_t>(q) % 16;
 }
+int esize_of(int dtype) { return dtype == DLB_F32 ? 4 : 2; }
 
 }  // namespace
 }  // namespace dlb
@@ -228,8 +228,10 @@ extern "C" int dlb_rel_bias_fwd(const void *scores, const float *table, const in
   if (int st = check_shape("rel_bias_fwd", batch, heads, q_len, kv_len, q_start, buckets, max_distance, dtype)) return st;
   if (batch == 0 || heads == 0 || q_len == 0 || kv_len == 0) return DLB_OK;
   DLB_REQUIRE(table && bucket_of && out, DLB_ERR_INVALID_ARG, "rel_bias_fwd: null pointer");
+  DLB_REQUIRE(on_elements(scores, esize_of(dtype)) && on_elements(out, esize_of(dtype)) && on_elements(table, 4) && on_elements(bucket_of, 4),
+              DLB_ERR_INVALID_ARG, "rel_bias_fwd: an address is not on an element");
   BiasArgs a = {scores, table, bucket_of, out, nullptr, batch, heads, q_len, kv_len, q_start, buckets, max_distance};
-  const bool vec = rows_can_be_cut(out, scores, dtype == DLB_F32 ? 4 : 2);
+  const bool vec = rows_can_be_cut(out, scores);
   const dim3 grid(ceil_div(q_len, kBiasRows) * heads * batch);
   const size_t smem = sizeof(float) * (2 * max_distance + 1);
   auto kern = dtype == DLB_F32 ? rel_bias_fwd_kernel<float> : rel_bias_fwd_kernel<__nv_bfloat16>;
@@ -250,6 +252,8 @@ extern "C" int dlb_rel_bias_bwd(const void *dscores, const int32_t *bucket_of, f
   if (heads == 0) return DLB_OK;
   const bool empty = batch == 0 || q_len == 0 || kv_len == 0;
   DLB_REQUIRE((dscores || empty) && bucket_of && dtable, DLB_ERR_INVALID_ARG, "rel_bias_bwd: null pointer");
+  DLB_REQUIRE(on_elements(dscores, esize_of(dtype)) && on_elements(dtable, 4) && on_elements(bucket_of, 4), DLB_ERR_INVALID_ARG,
+              "rel_bias_bwd: an address is not on an element");
   const size_t need = dlb_rel_bias_bwd_workspace_bytes(batch, heads, q_len, kv_len, buckets);
   DLB_REQUIRE(workspace != nullptr && workspace_bytes >= need && aligned16(workspace), DLB_ERR_WORKSPACE,
               "rel_bias_bwd: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
@@ -257,10 +261,9 @@ extern "C" int dlb_rel_bias_bwd(const void *dscores, const int32_t *bucket_of, f
   BiasArgs a = {dscores, nullptr, bucket_of, nullptr, static_cast<float *>(workspace), batch, heads, q_len, kv_len,
                 q_start, buckets, max_distance};
   const size_t smem = sizeof(float) * buckets * kBiasThreads + 2 * max_distance + 1;
-  const bool vec = rows_can_be_cut(dscores, nullptr, dtype == DLB_F32 ? 4 : 2);
   auto kern = dtype == DLB_F32 ? rel_bias_bwd_kernel<float> : rel_bias_bwd_kernel<__nv_bfloat16>;
   if (int rc = allow_smem(kern, smem, "rel_bias_bwd")) return rc;
-  launch_pdl(kern, dim3(heads * parts), dim3(kBiasThreads), smem, as_stream(stream), a, parts, vec);
+  launch_pdl(kern, dim3(heads * parts), dim3(kBiasThreads), smem, as_stream(stream), a, parts);
   DLB_LAUNCH_CHECK("rel_bias_bwd");
   launch_pdl(rel_bias_sum_kernel, dim3(heads * buckets), dim3(128), 0, as_stream(stream),
              static_cast<const float *>(a.part), dtable, parts, buckets);

@@ -508,7 +508,8 @@ DLB_API int dlb_ce_from_ids_bwd(const int32_t *target_ids, const float *y_pred,
  * q, o [batch, q_len, heads, head_dim] and k, v [batch, kv_len, kv_heads, head_dim] are given by
  * an address and three strides in elements (columns are contiguous), so that the views of one
  * fused projection, a cache larger than kv_len and [batch, head, token] layouts go in as they
- * are; a stride of 0 repeats an input.  Outputs must not overlap anything else the call touches.
+ * are; a stride of 0 repeats an input.  Every address is a multiple of its element's size.  Outputs
+ * must not overlap anything else the call touches.
  * k and v at keys that no query of the batch may reach (j >= kv_lens[b], or behind the last
  * query's position and the prefix under a causal mask) may hold anything, NaN included; the
  * values in front of that bound have to be finite, masked or not.

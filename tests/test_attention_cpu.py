@@ -66,6 +66,40 @@ def test_null_blocks_and_overlapping_outputs():
     assert lib.dlb_attn_bwd(ctypes.byref(block()), ctypes.byref(g), FAKE, 1 << 30, None) == capi.ERR_INVALID_ARG  # no lse
 
 
+@pytest.mark.parametrize("dtype,off", [(capi.F32, 1), (capi.F32, 2), (capi.BF16, 1)])
+def test_addresses_between_elements(dtype, off):
+    """They would fault on the GPU; the host refuses them."""
+    lib = capi.lib()
+    size = 4 if dtype == capi.F32 else 2
+    need = 1 << 30
+    h, bad = capi.Heads(FAKE, 4096, 64, 16), capi.Heads(FAKE + off, 4096, 64, 16)
+    for name in ("q", "k", "v", "o"):
+        a = block(dtype=dtype, lse=FAKE, **{name: bad})
+        assert lib.dlb_attn_fwd(ctypes.byref(a), FAKE, need, None) == capi.ERR_INVALID_ARG, name
+        assert name.encode() in lib.dlb_last_error()
+    for name in ("dout", "dq", "dk", "dv"):
+        g = capi.AttnGrad(dout=h, dq=h, dk=h, dv=h)
+        setattr(g, name, bad)
+        assert lib.dlb_attn_bwd(ctypes.byref(block(dtype=dtype, lse=FAKE)), ctypes.byref(g), FAKE, need, None) == capi.ERR_INVALID_ARG, name
+    pair = dict(table=FAKE, bucket_of=FAKE)
+    for extra in (dict(kv_lens=FAKE + off), dict(q_start=FAKE + off), dict(prefix=FAKE + off), dict(q_docs=FAKE, kv_docs=FAKE + off),
+                  dict(q_docs=FAKE + off, kv_docs=FAKE), dict(slopes=FAKE + off), dict(pair, table=FAKE + off),
+                  dict(pair, bucket_of=FAKE + off), dict(lse=FAKE + off)):
+        assert lib.dlb_attn_fwd(ctypes.byref(block(dtype=dtype, **extra)), FAKE, need, None) == capi.ERR_INVALID_ARG, extra
+    g = capi.AttnGrad(dout=h, dq=h, dk=h, dv=h, dtable=FAKE + off)
+    assert lib.dlb_attn_bwd(ctypes.byref(block(dtype=dtype, lse=FAKE, **pair)), ctypes.byref(g), FAKE, need, None) == capi.ERR_INVALID_ARG
+
+    def bias(scores=FAKE, table=FAKE, of=FAKE, out=FAKE):
+        return lib.dlb_rel_bias_fwd(scores, table, of, out, 1, 2, 3, 4, 0, 8, 16, dtype, None)
+
+    def gradient(scores=FAKE, of=FAKE, out=FAKE):
+        return lib.dlb_rel_bias_bwd(scores, of, out, FAKE, need, 1, 2, 3, 4, 0, 8, 16, dtype, None)
+
+    for call in (bias, gradient):
+        assert call(scores=FAKE + off) == call(of=FAKE + off) == call(out=FAKE + off) == capi.ERR_INVALID_ARG
+    assert bias(table=FAKE + size // 2) == capi.ERR_INVALID_ARG
+
+
 def test_documents_of_an_empty_side():
     """The address of an array without elements says nothing: an empty tensor's is NULL."""
     lib = capi.lib()
