@@ -173,7 +173,11 @@ def dtype_of(t) -> int:
     raise TypeError(f"unsupported storage type {t.dtype}")
 
 
-def current_stream() -> int:
+def current_stream(device: int | None = None) -> int:
+    """Address of the current stream of `device` (default: the current one)."""
     import torch
-    # the address alone: building a Stream object costs several microseconds a call
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    if device is None:
+        device = torch.cuda.current_device()
+    # The address alone, where torch gives it: building a Stream object costs several microseconds a call.
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream

@@ -303,10 +303,6 @@ def _current_device(t):
     return device
 
 
-def _stream(device):
-    return torch._C._cuda_getCurrentRawStream(device)
-
-
 def _address(name, t, dtype, shape, device):
     """Address of a contiguous tensor of this type, shape and place; 0 for None."""
     if t is None:
@@ -395,7 +391,7 @@ def attn_fwd(q, k, v, scale=None, cap=0.0, causal=False, kv_lens=None, q_start=N
                         slopes, table, bucket_of)
     library = capi.lib()
     space, size, _keep = _space(workspace, library.dlb_attn_fwd_workspace_bytes(block) if workspace is None else 0, q)
-    check(library.dlb_attn_fwd(block, space, size, _stream(device)))
+    check(library.dlb_attn_fwd(block, space, size, current_stream(device)))
     return out, lse
 
 
@@ -425,7 +421,7 @@ def attn_bwd(dout, q, k, v, o, lse, scale=None, cap=0.0, causal=False, kv_lens=N
                            table_to)
     library = capi.lib()
     space, size, _keep = _space(workspace, library.dlb_attn_bwd_workspace_bytes(block, grad) if workspace is None else 0, q)
-    check(library.dlb_attn_bwd(block, grad, space, size, _stream(device)))
+    check(library.dlb_attn_bwd(block, grad, space, size, current_stream(device)))
     return dq, dk, dv, dtable
 
 
@@ -452,7 +448,7 @@ def rel_bias_fwd(table, bucket_of, scores=None, shape=None, q_start=0, dtype=tor
                                       _address("table", table, torch.float32, (heads, buckets), device),
                                       _address("bucket_of", bucket_of, torch.int32, (2 * reach + 1,), device),
                                       _address("out", out, dtype, shape, device), batch, heads, q_len, kv_len, q_start,
-                                      buckets, reach, dtype_of(out), _stream(device)))
+                                      buckets, reach, dtype_of(out), current_stream(device)))
     return out
 
 
@@ -472,7 +468,7 @@ def rel_bias_bwd(dscores, bucket_of, buckets, q_start=0, dtable=None, workspace=
                                    _address("bucket_of", bucket_of, torch.int32, (2 * reach + 1,), device),
                                    _address("dtable", dtable, torch.float32, (heads, buckets), device), space, size,
                                    batch, heads, q_len, kv_len, q_start, buckets, reach, dtype_of(dscores),
-                                   _stream(device)))
+                                   current_stream(device)))
     return dtable
 
 

@@ -194,3 +194,20 @@ def test_bucket_map_refusals():
     for buckets, top, both in ((0, 10, True), (7, 10, True), (32, 4, False), (66, 100, False), (32, 2000, True), (1, 5, False)):
         with pytest.raises(capi.DlbError):
             ops.rel_bucket_map(buckets, top, both)
+
+
+@pytest.mark.parametrize("private", [True, False])
+def test_stream_with_and_without_the_private_call(monkeypatch, private):
+    """The address of the current stream also comes from torch's public interface alone."""
+    class Stream:
+        def __init__(self, device):
+            self.cuda_stream = 100 + device
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    monkeypatch.setattr(torch.cuda, "current_stream", Stream)
+    if private:
+        monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 200 + device, raising=False)
+    else:
+        monkeypatch.delattr(torch._C, "_cuda_getCurrentRawStream", raising=False)
+    first = 200 if private else 100
+    assert capi.current_stream() == first + 3 and capi.current_stream(1) == first + 1
