@@ -506,6 +506,27 @@ def test_64_buckets_and_the_longest_map(D, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("kind", ["causal", "lens", "cap+table+causal", "prefix+causal+slopes", "returning_docs", "returning_docs+causal"])
+@pytest.mark.parametrize("shape", [(1, 1700, 1700, 8, 2, 128), (1, 2300, 2300, 4, 1, 64), (2, 1100, 1500, 4, 2, 40)])
+def test_long_sequences(shape, kind, dtype):
+    """Many tiles in the rings of both passes, times the heads of a group; documents that come back leave gaps in
+    the list of tiles."""
+    B, Sq, Sk, H, Hk, D = shape
+    q, k, v, dout = make(sum(shape), dtype, *shape, layout="plain", std=1.0)
+    how = options(kind.replace("returning_docs", "plain"), B, Sq, Sk, H)
+    if Sq != Sk:
+        how["q_start"] = ints([Sk - Sq] * B)
+    if "returning_docs" in kind:  # three numbers in runs of 170 tokens
+        runs = torch.randint(0, 3, (B, Sk // 170 + 1), generator=torch.Generator().manual_seed(Sk))
+        docs = runs.repeat_interleave(170, 1)[:, :Sk].int().cuda()
+        how["q_docs"], how["kv_docs"] = docs[:, Sk - Sq:].contiguous(), docs.contiguous()
+    values, bounds = reference(q, k, v, dout, exact_delta=dtype == "bf16", **how)
+    o, lse = ops.attn_fwd(q, k, v, **how)
+    dq, dk, dv, dtable = ops.attn_bwd(dout, q, k, v, o, lse, **how)
+    check(dict(o=o, lse=lse, dq=dq, dk=dk, dv=dv, dtable=dtable), values, bounds)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_bucket_map_edges(dtype):
     """A map of one entry; values outside 0..buckets-1 count as the nearest bucket."""
     q, k, v, dout = make(87, dtype, 1, 40, 40, 2, 2, 64, "plain")
