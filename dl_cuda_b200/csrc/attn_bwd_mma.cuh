@@ -9,8 +9,11 @@
 // next S.  TMEM holds S, G and the sums; for heads up to 64 wide it has room for more, and S does not wait
 // for P: the key pass keeps P beside S, the query pass two S where its ring has four stages to feed them.
 //
+// P and D are rounded to bf16, the operand type of the next product (in two parts these products would
+// double); sums, delta, row statistics and the gradient of the table are fp32.
+//
 // Tiles of 64 columns with two buffers each were slower (889 instead of 811 us for both passes over 4096
-// x 4096 tokens, 32 heads of 128): a product of 128 x 64 takes the tensor cores as long as one of 128 x
+// x 4096 tokens, 32 heads of 128; 908 us since R is made): a product of 128 x 64 takes the tensor cores as long as one of 128 x
 // 128, 65 cycles for 16 inner columns, so S and G cost twice as much.  What bounds the key pass now, by the
 // clock: 2800 cycles a tile, of which P takes 1430 (1024 of them are the special-function units' 16 a
 // clock) and dV with the next S, which cannot start before P is complete, 1260; the tensor cores are busy
@@ -54,7 +57,6 @@ struct BwdShape {
   static constexpr int kStage = 2 * NB * kBlockBytes;
   static constexpr int kStats = kRing + ST * kStage, kRest = kStats + ST * kStatsBytes;
 };
-
 
 // Where in the padded tables a warp's 16 pairs from distance d0 on (FOR_KEYS: back) lie when all its
 // rows' pairs are beyond the reach; -1 when some are not (then all are near enough for the padding).

@@ -9,13 +9,16 @@
 // no maximum stands between a score and its exponential, and O is hardly ever rescaled; keys are walked
 // from where the queries stand outwards, so that a distance bias shows its largest scores at once (from
 // the far end of a prefix, every tile moved the reference: 64 instead of 53 us for 3 x 1531 tokens).
-// The sum behind the quotient adds the ROUNDED probabilities, so that a row's weights add up to one
-// exactly as the product sees them (bf16 output 1.9e-3 instead of 2.3e-3 from the exact one, of which the
-// output's own rounding is 1.7e-3); lse comes from the unrounded ones.
+// Probabilities are rounded to bf16, the operand type of the second product: in two bf16 parts they would
+// need that product twice.  The sum behind the quotient adds the ROUNDED ones, so that a row's weights add
+// up to one exactly as the product sees them (one prompt's output 1.9e-3 instead of 2.3e-3 from the exact
+// one, 1.9e-3 to 2.4e-3 over 150 random cases, of which the output's own rounding is 1.7e-3); lse comes from
+// the unrounded ones.
 //
-// Measured (32 heads of 128, 4096 tokens): 270 us, 1.01 PFLOP/s, of the 1.66 that the library's plain
-// product reaches; causal 141 us, causal with a cap 177 us.  By the clock a pair of tiles takes 3500 cycles
-// where the tensor cores need 2470 of issue: a tile's own chain of scores, softmax (1700 cycles a tile,
+// Measured (4096 tokens, 32 heads of 128 on 8 key heads): 268 us, 1.03 PFLOP/s, of the 1.66 that the
+// library's plain product reaches; causal 147 us, causal with a cap 184 us (205 us from a cold L2).
+// By the clock a pair of tiles takes 3500 cycles where the tensor cores need 2470 of issue: a tile's own
+// chain of scores, softmax (1700 cycles a tile,
 // half of which are exponentials) and product is what remains, since TMEM has no room for a second S.
 // Taking a quarter of the exponentials as polynomials on the fp32 pipes changed nothing (275 us).
 #include <algorithm>
@@ -278,8 +281,10 @@ attn_fwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       }
       tc_fence_after();
       // One pass over the scores against the reference, which the keys so far fit.  Only if some row's
-      // sum says that it does not (too large, or nothing left of visible keys) the maximum is taken, the
-      // reference moved, what has been summed rescaled, and the pass repeated.
+      // sum says that it may not (too large, or nothing left of visible keys) the maximum is taken, the
+      // reference moved where that is out of its range, what has been summed rescaled, and the pass repeated.
+      // (A sum above 2^32 of many weights that are all below it repeats the pass and moves nothing: the
+      // result is the same, the softmax of such a tile takes three times as long.)
       uint32_t packed[32];
       float2 part, part_rounded;
       for (int pass = 0;; pass++) {

@@ -15,10 +15,13 @@ enum { kNoBias = 0, kSlope = 1, kTable = 2 };          // kTable: with or withou
 
 // Capped scores times log2(e), L tanh(k x) with L = cap * log2(e), k = scale / cap, as odd polynomials:
 // least-squares fits of tanh(x) / x in x^2, reweighted until the relative error was level.
-//   |k x| <= 0.25: degree 2, error 4e-7 of a score, powers of k and L folded into the coefficients (4
-//                  operations a score; scores up to a quarter of the cap are the usual case)
-//   |k x| <= 1:    degree 6, error 5e-8 (1.2e-7 in fp32), 10 operations
-// Anything larger takes two special-function operations per score.  A warp takes one road.
+//   |k x| <= 0.25: degree 2, error 4.2e-7 of a score (5.0e-7 in fp32), powers of k and L folded into the
+//                  coefficients (4 operations a score)
+//   |k x| <= 1:    degree 6, error 7.2e-8 (1.6e-7 in fp32), 10 operations
+// Anything larger takes two special-function operations per score.  A warp takes one road, for the largest of
+// the scores that it holds at a time, which are others in the forward and in either pass of the backward:
+// the same score may differ by 5.0e-7 of itself between them.  Roads of one accuracy would cost a degree
+// more; against what bf16 leaves of a probability (2^-8) the difference is nothing.
 struct CapCoef {
   float c0, c1, c2, k, out;
   bool folded;  // k^5 must not fall under fp32's range

@@ -522,8 +522,10 @@ DLB_API int dlb_ce_from_ids_bwd(const int32_t *target_ids, const float *y_pred,
  * product is split into two parts of 11 bits and three of their products are summed in fp32, which
  * leaves out 2^-21 of |x||y|; DLB_BF16 multiplies on the tensor cores with fp32 sums and softmax
  * statistics and rounds probabilities (in the backward also the gradients of the scores) to bf16 in
- * front of the next product.  head_dim 1..128; bf16 with head_dim, strides and addresses in
- * multiples of 16 bytes takes the tensor cores, anything else kernels with fp32 arithmetic.
+ * front of the next product.  head_dim 1..128; bf16 takes the tensor cores when head_dim, strides and
+ * addresses are multiples of 16 bytes, no stride is 0 (of a dimension with more than one entry), scale > 0
+ * and q_len and kv_len are at most 524288; anything else takes kernels with fp32 arithmetic, which are
+ * ten times slower and more at length.
  * The result does not depend on scheduling: same call, same bits.  As with the other pipelined
  * kernels, make the first call of a kind on a device before capturing.
  *
@@ -567,7 +569,11 @@ DLB_API int dlb_attn_fwd(const dlb_attn *a, void *workspace, size_t workspace_by
  * key/value heads get the sum over their query heads, table entries the sum over the batch; the
  * probabilities are rebuilt from lse.  Keys that no query reaches get zero.  Every sum has a fixed
  * order.  dout has to be finite, and lse within about +-1e4: the rebuilt probabilities carry a
- * relative error of |lse| * 2^-23.  slopes are constants: they get no gradient.
+ * relative error of |lse| * 2^-23, and with a cap and DLB_BF16 another of 5e-7 * |score| (the tanh is a
+ * polynomial chosen by the scores around).  A row's probabilities over the keys of the call have to add
+ * up to one: with DLB_BF16, o is a first guess of <dout, o>, which the row's sum of score gradients
+ * corrects, so that o and lse of a call over other or more keys do not do.  slopes are constants: they get
+ * no gradient.
  * Replaces the attention part of TransformerLayer::backward (src/transformer.cuh:604-658). */
 typedef struct dlb_attn_grad {
   dlb_heads dout, dq, dk, dv;
