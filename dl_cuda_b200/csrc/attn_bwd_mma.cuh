@@ -27,7 +27,8 @@
 // pass therefore takes it as a first guess only.  Its rows add up D in fp32; with the true delta a row's D
 // add up to zero, so the sum e is what the guess is off by, and
 //     dQ = scale (sum_j D_ij k_j - e_i R_i),  R_i = sum_j P_ij k_j (times the cap's derivative)
-// at the price of one product; delta + e goes to the key pass, which runs second.  dq and dk of 70 causal
+// at the price of one product; delta + e goes to the key pass, which runs second.  (A row whose P do not add
+// up to one has o and lse of more keys than the call's: its guess stays.)  dq and dk of 70 causal
 // tokens come from 2.7e-3 to 2.35e-3 of the exact ones (the output's and D's own rounding make 2.35e-3),
 // both passes over 4096 tokens, 32 heads of 128 on 8, causal with a cap, from 537 to 578 us.
 #pragma once
@@ -147,7 +148,8 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
   __shared__ uint64_t x_full, full[ST], empty[ST], s_full[2], g_full, p_full[2], d_full, v_full, acc_full, drain;
   __shared__ uint32_t tmem_slot;
   __shared__ int dead_flag, doc_range[2];
-  __shared__ float delta_part[FOR_KEYS ? 1 : PARTS][kTileRows], sum_part[FOR_KEYS ? 1 : PARTS][kTileRows];
+  __shared__ float delta_part[FOR_KEYS ? 1 : PARTS][kTileRows], d_part[FOR_KEYS ? 1 : PARTS][kTileRows];
+  __shared__ float p_part[FOR_KEYS ? 1 : PARTS][kTileRows];
   __shared__ __align__(16) int doc_tile[kTileRows];
   volatile int *dead = &dead_flag;
   // s_full and p_full come in pairs, used in turn: with two S the tensor cores may finish the next tile's
@@ -283,7 +285,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
       bucket_sum = 0.f;
       bucket_now = next;
     };
-    float2 ds_sum[2] = {both(0.f), both(0.f)};  // of this thread's D, for e
+    float2 d_sum[2] = {both(0.f), both(0.f)}, p_sum = both(0.f);  // of this thread's D and P, for e
     int it = -1;
     for (int g = 0; g < heads_here; g++) {
       const int h = FOR_KEYS ? hk * a.group + g : unit;
@@ -449,7 +451,11 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 #pragma unroll
           for (int e = 0; e < 8; e++) {
             const float2 d2 = make_float2(dp[2 * e], dp[2 * e + 1]), y = mul2(through_cap(e0 + 2 * e), d2);
-            if (!FOR_KEYS) ds_sum[e & 1] = fma2(make_float2(p[e0 + 2 * e], p[e0 + 2 * e + 1]), d2, ds_sum[e & 1]);
+            if (!FOR_KEYS) {
+              const float2 p2 = make_float2(p[e0 + 2 * e], p[e0 + 2 * e + 1]);
+              d_sum[e & 1] = fma2(p2, d2, d_sum[e & 1]);
+              p_sum = add2(p_sum, p2);
+            }
             packed[e] = pack_bf16(y.x, y.y);
           }
           tmem_store8(g_at + e0, packed);
@@ -498,11 +504,17 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
     }
     float off = 0.f;  // what delta was off by
     if constexpr (!FOR_KEYS) {
-      const float2 sum = add2(ds_sum[0], ds_sum[1]);
-      sum_part[part][row] = sum.x + sum.y;
+      const float2 sum = add2(d_sum[0], d_sum[1]);
+      d_part[part][row] = sum.x + sum.y;
+      p_part[part][row] = p_sum.x + p_sum.y;
       named_bar_sync(1, kRowThreads);
+      float total = 0.f;
 #pragma unroll
-      for (int k = 0; k < PARTS; k++) off += sum_part[k][row];
+      for (int k = 0; k < PARTS; k++) {
+        off += d_part[k][row];
+        total += p_part[k][row];
+      }
+      if (!row_is_whole(total)) off = 0.f;
       if (part == 0) stats_tile(a, b, unit, tile)[kStatRows + row] = row_stat.y - off;
     }
     mbar_wait(&acc_full, 0, dead, timeouts);

@@ -62,6 +62,11 @@ __host__ __device__ inline int stat_tiles(int q_len) { return (q_len + kStatRows
 __device__ __forceinline__ float *stats_tile(const AttnArgs &a, int b, int h, int tile) {
   return a.row_stats + ((static_cast<size_t>(b) * a.heads + h) * stat_tiles(a.q_len) + tile) * (2 * kStatRows);
 }
+// Backward: are these all the keys of a row (its probabilities, rebuilt from lse, add up to one), so that its
+// score gradients add up to zero?  Not for a call over some of the keys with o and lse of all.  What the
+// rounding of lse may move the sum by stays under the limit up to |lse| = 8000.
+__device__ __forceinline__ bool row_is_whole(float sum) { return fabsf(sum - 1.f) <= 0x1p-10f; }
+
 __device__ __forceinline__ float2 stat_at(const AttnArgs &a, int b, int h, int i) {
   const float *t = stats_tile(a, b, h, i / kStatRows) + i % kStatRows;
   return make_float2(t[0], t[kStatRows]);

@@ -2,8 +2,8 @@
 //
 // The products run on the warp-level tensor path (mma.sync m16n8k8, tf32) with every operand split in
 // two, x = hi + lo with 11 bits each: hi*hi + hi*lo + lo*hi leaves out 2^-21 of |x||y|.  fp32
-// results are up to 2.6 times as far from the exact ones as those of plain fp32 arithmetic (2-norm at most
-// 6.6e-7 over 150 random cases, 1.1e-6 for the gradient of a table); bf16 values need no lo, but take the
+// results are up to three times as far from the exact ones as those of plain fp32 arithmetic (2-norm at most
+// 9e-7 over 210 random cases, 1.1e-6 for the gradient of a table); bf16 values need no lo, but take the
 // same road.  Three such products run at 90 TFLOP/s where scalar multiply-adds reach 67 at best (both
 // measured on a B200), and they need a quarter of the shared-memory reads: the 64x64 scalar tiles this
 // replaces were bound by those.
@@ -547,7 +547,7 @@ __device__ __forceinline__ void attn_bwd_generic(const AttnArgs &a, bool vec, in
   __shared__ float2 col_stat_tiles[2][kGenCols];
   __shared__ int col_doc_tiles[2][kGenCols];
   constexpr bool kFixDelta = !FOR_KEYS && sizeof(T) == 2;
-  __shared__ float ds_sums[CG][kRows];
+  __shared__ float2 row_sums[CG][kRows];
   const bool want_table = !FOR_KEYS && a.dtable != nullptr;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int r0 = (warp % RG) * 16, cg = warp / RG, w0 = cg * 8 * NT;  // this warp's rows and columns
@@ -590,7 +590,7 @@ __device__ __forceinline__ void attn_bwd_generic(const AttnArgs &a, bool vec, in
     end[x] = (!FOR_KEYS && valid) ? row_end(a, view, row0 + r) : 0;
     row_stat[x] = (!FOR_KEYS && valid) ? stat_at(a, b, unit, row0 + r) : make_float2(-INFINITY, 0.f);
   }
-  float acc_x[DP / 32][4][4], acc_y[DP / 32][4][4], ds_sum[2] = {0.f, 0.f};
+  float acc_x[DP / 32][4][4], acc_y[DP / 32][4][4], ds_sum[2] = {0.f, 0.f}, p_sum[2] = {0.f, 0.f};
 #pragma unroll
   for (int q = 0; q < DP / 32; q++)
 #pragma unroll
@@ -685,7 +685,10 @@ __device__ __forceinline__ void attn_bwd_generic(const AttnArgs &a, bool vec, in
             ds_tile[r * kPitch + cc] = grad;
             p_tile[r * kPitch + cc] = prob;
           }
-          if (kFixDelta) ds_sum[x] += grad;
+          if (kFixDelta) {
+            ds_sum[x] += grad;
+            p_sum[x] += prob;
+          }
           p[k][e] = kFixDelta ? prob * dcap * a.scale : prob;
           d[k][e] = grad * dcap * a.scale;  // through the cap and the scale: the gradient of <q, k>
         }
@@ -727,15 +730,21 @@ __device__ __forceinline__ void attn_bwd_generic(const AttnArgs &a, bool vec, in
   if constexpr (kFixDelta) {
 #pragma unroll
     for (int x = 0; x < 2; x++) {
-      const float sum = quad_sum(ds_sum[x]);
-      if (c == 0) ds_sums[cg][r0 + g + 8 * x] = sum;
+      const float2 sum = make_float2(quad_sum(ds_sum[x]), quad_sum(p_sum[x]));
+      if (c == 0) row_sums[cg][r0 + g + 8 * x] = sum;
     }
     __syncthreads();
-    float off[2] = {0.f, 0.f};
+    float off[2];
 #pragma unroll
-    for (int k = 0; k < CG; k++)
+    for (int x = 0; x < 2; x++) {
+      float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int x = 0; x < 2; x++) off[x] += ds_sums[k][r0 + g + 8 * x];
+      for (int k = 0; k < CG; k++) {
+        sum.x += row_sums[k][r0 + g + 8 * x].x;
+        sum.y += row_sums[k][r0 + g + 8 * x].y;
+      }
+      off[x] = row_is_whole(sum.y) ? sum.x : 0.f;
+    }
 #pragma unroll
     for (int q = 0; q < DP / 32; q++)
 #pragma unroll
@@ -769,8 +778,8 @@ __device__ __forceinline__ void attn_bwd_generic(const AttnArgs &a, bool vec, in
   if (want_table) {
     __syncthreads();
     if (threadIdx.x < kRows) {
-      // A row's gradients of its scores add up to zero: what rounding left (in delta above all) is taken
-      // off again in proportion to P.
+      // The gradients of a whole row's scores add up to zero: what rounding left (in delta above all) is
+      // taken off again in proportion to P.
       const int r = threadIdx.x;
       float e = 0.f, total = 0.f;
       for (int n = 0; n < a.buckets; n++) {
@@ -782,7 +791,7 @@ __device__ __forceinline__ void attn_bwd_generic(const AttnArgs &a, bool vec, in
         e += v.x;
         total += v.y;
       }
-      e = total > 0.f ? e / total : 0.f;
+      e = row_is_whole(total) ? e / total : 0.f;
       for (int n = 0; n < a.buckets; n++) sums[n * kRows + r].x -= e * sums[n * kRows + r].y;
     }
     __syncthreads();

@@ -570,10 +570,10 @@ DLB_API int dlb_attn_fwd(const dlb_attn *a, void *workspace, size_t workspace_by
  * probabilities are rebuilt from lse.  Keys that no query reaches get zero.  Every sum has a fixed
  * order.  dout has to be finite, and lse within about +-1e4: the rebuilt probabilities carry a
  * relative error of |lse| * 2^-23, and with a cap and DLB_BF16 another of 5e-7 * |score| (the tanh is a
- * polynomial chosen by the scores around).  A row's probabilities over the keys of the call have to add
- * up to one: with DLB_BF16, o is a first guess of <dout, o>, which the row's sum of score gradients
- * corrects, so that o and lse of a call over other or more keys do not do.  slopes are constants: they get
- * no gradient.
+ * polynomial chosen by the scores around).  slopes are constants: they get no gradient.
+ * A call over some of the keys with o and lse of all of them gives that share's dk and dv and its part of dq
+ * and dtable.  Where a row's probabilities add up to one over the call's keys, its score gradients add up
+ * to zero, and the rounding of o is taken out of them by that; a row of a share keeps it.
  * Replaces the attention part of TransformerLayer::backward (src/transformer.cuh:604-658). */
 typedef struct dlb_attn_grad {
   dlb_heads dout, dq, dk, dv;

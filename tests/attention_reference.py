@@ -23,9 +23,9 @@ the tensor cores in it (else w = 0), entry by entry:
          on the tensor cores in proportion to sums of P that are kept in fp16 times 2^15: off by 2^-11 of the
          sum, or by 2^-40 (half a step of the smallest fp16, 2^-24, over 2^15), an addition, at most
          Sk / 128 + 2 of them by each of four threads; and the error taken off is at most e_delta + e_dp.
-         With exact_delta nothing is taken off: sums of 2 (d |dS| + P e_dp) + P e_delta without the term in w,
-         and of (Sq / 4 + 32) 2^-24 |dS| for a thread's own additions (a quarter of a key's queries), its
-         warp's and its row's
+         With exact_delta, or where the keys are shared out over several calls (shares), nothing is taken
+         off: sums of 2 (d |dS| + P e_dp) + P e_delta without its term in w, and of (Sq / 4 + 32) 2^-24 |dS|
+         for a thread's own additions (a quarter of a key's queries), its warp's and its row's
 """
 import math
 
@@ -35,7 +35,8 @@ F64 = torch.float64
 
 
 def reference(q, k, v, dout=None, scale=None, cap=0.0, causal=False, kv_lens=None, q_start=None, prefix=None,
-              q_docs=None, kv_docs=None, slopes=None, table=None, bucket_of=None, tensor_cores=None, exact_delta=False):
+              q_docs=None, kv_docs=None, slopes=None, table=None, bucket_of=None, tensor_cores=None, exact_delta=False,
+              shares=False):
     """(values, bounds): dicts of o, lse and, with dout, dq, dk, dv, dtable in float64 on the inputs' device."""
     B, Sq, H, D = q.shape
     Sk, Hk = k.shape[1], k.shape[2]
@@ -115,8 +116,8 @@ def reference(q, k, v, dout=None, scale=None, cap=0.0, causal=False, kv_lens=Non
         values["dtable"] = torch.einsum("bhij,bijn->hn", dS, one)
         b_t = 2 * (d * dS.abs() + d * P * (dP.abs() + delta.abs()) + P * e_dp)
         bounds["dtable"] = torch.einsum("bhij,bijn->hn", b_t, one) + tiny
-        if exact_delta:
-            b_t = 2 * (d * dS.abs() + P * e_dp) + P * (e_delta - w * from_output) + (Sq / 4 + 32) * 2.0 ** -24 * dS.abs()
+        if exact_delta or shares:
+            b_t = 2 * (d * dS.abs() + P * e_dp) + P * (e_delta - (w * from_output if exact_delta else 0.0)) + (Sq / 4 + 32) * 2.0 ** -24 * dS.abs()
             bounds["dtable"] = torch.einsum("bhij,bijn->hn", b_t, one) + tiny
         elif w:
             most = from_output + (e_dp.amax(-1, keepdim=True) if Sk else 0.0)

@@ -272,6 +272,33 @@ def test_bucket_map_that_alternates(D, buckets, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("D", [64, 128, 20])
+@pytest.mark.parametrize("kind", ["plain", "cap+causal", "slopes", "table", "table+causal+docs"])
+def test_backward_of_shares_of_the_keys(kind, D, dtype):
+    """The keys in three calls with o and lse of all of them: each its own dk and dv and a part of dq and dtable."""
+    B, Sq, Sk, H, Hk = 2, 150, 400, 4, 2
+    q, k, v, dout = make(D, dtype, B, Sq, Sk, H, Hk, D, "plain", std=1.0)
+    how = options(kind, B, Sq, Sk, H)
+    values, bounds = reference(q, k, v, dout, shares=True, q_start=ints([250, 100]), **how)
+    o, lse = ops.attn_fwd(q, k, v, q_start=ints([250, 100]), **how)
+    u = torch.finfo(q.dtype).eps / 2
+    dq, dk, dv, dtable = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), [], [], 0.0
+    for first, last in ((0, 130), (130, 257), (257, 400)):
+        share = dict(how, q_start=ints([250 - first, 100 - first]))
+        if "kv_docs" in how:
+            share["kv_docs"] = how["kv_docs"][:, first:last].contiguous()
+        got = ops.attn_bwd(dout, q, k[:, first:last], v[:, first:last], o, lse, **share)
+        dq += got[0].double()
+        bounds["dq"] += u / (1 - u) * got[0].double().abs()  # each share's dq is rounded by itself
+        dk.append(got[1])
+        dv.append(got[2])
+        if got[3] is not None:
+            dtable = dtable + got[3].double()
+    got = dict(o=o, lse=lse, dq=dq, dk=torch.cat(dk, 1), dv=torch.cat(dv, 1))
+    check(dict(got, dtable=dtable) if how.get("table") is not None else got, values, bounds)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_empty_sizes_with_documents(dtype):
     dt = DTYPES[dtype]
     full = lambda *s: torch.ones(*s, dtype=dt, device="cuda")  # noqa: E731
