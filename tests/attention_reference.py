@@ -19,10 +19,11 @@ the tensor cores in it (else w = 0), entry by entry:
     |dx' - dx| <= scale (c b + 4 d_s (|dS| + b)) =: bx for dx = scale c dS, c = 1 - tanh^2 off by at most
          4 d_s (twice the tanh's error and a rounding): (c + e1)(dS + e2) - c dS = c e2 + e1 dS + e1 e2
     |dq' - dq| <= bx |K| + u |dq|, |dk' - dk| <= bx^T |Q| + u |dk|
-    dtable: sums of d |dS| + d P (|dP| + |delta|) + P e_dp, doubled: the rows' common error is taken off;
-         on the tensor cores in proportion to sums of P that are kept in fp16 times 2^15: off by 2^-11 of the
-         sum, or by 2^-40 (half a step of the smallest fp16, 2^-24, over 2^15), an addition, at most
-         Sk / 128 + 2 of them by each of four threads; and the error taken off is at most e_delta + e_dp.
+    dtable: sums of d |dS| + d P (|dP| + |delta|) + P e_dp, doubled: the rows' common error is taken off.
+         With bf16, room for taking it off in proportion to sums of P in fp16 times 2^15 (no kernel needs it
+         any more): off by 2^-11 of the sum, or by 2^-40 (half a step of the smallest fp16, 2^-24, over
+         2^15), an addition, at most Sk / 128 + 2 of them by each of four threads; and the error taken off
+         is at most e_delta + e_dp.
          With exact_delta, or where the keys are shared out over several calls (shares), nothing is taken
          off: sums of 2 (d |dS| + P e_dp) + P e_delta without its term in w, and of (Sq / 4 + 32) 2^-24 |dS|
          for a thread's own additions (a quarter of a key's queries), its warp's and its row's
