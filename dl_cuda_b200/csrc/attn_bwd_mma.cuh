@@ -13,8 +13,8 @@
 // double); sums, delta, row statistics and the gradient of the table are fp32.
 //
 // Tiles of 64 columns with two buffers each were slower (889 instead of 811 us for both passes over 4096
-// x 4096 tokens, 32 heads of 128; 908 us since R is made): a product of 128 x 64 takes the tensor cores as long as one of 128 x
-// 128, 65 cycles for 16 inner columns, so S and G cost twice as much.  What bounds the key pass now, by the
+// x 4096 tokens, 32 heads of 128; 908 us since R is made): a product of 128 x 64 takes the tensor cores as
+// long as one of 128 x 128, 65 cycles for 16 inner columns, so S and G cost twice as much.  What bounds the key pass now, by the
 // clock: 2800 cycles a tile, of which P takes 1430 (1024 of them are the special-function units' 16 a
 // clock) and dV with the next S, which cannot start before P is complete, 1260; the tensor cores are busy
 // for 2048.
@@ -316,7 +316,6 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         // Probabilities, from S alone.  A chunk's P and D go over the first 8 columns of its own S and G.
         const uint32_t s_at = s_base + (kTwoS && (it & 1) ? 384 : 0);
         float p[kCols], capped[CAP ? kCols : 1];  // P, P times the cap's derivative
-        auto through_cap = [&](int e) { return make_float2(CAP ? capped[CAP ? e : 0] : p[e], CAP ? capped[CAP ? e + 1 : 0] : p[e + 1]); };
 #pragma unroll
         for (int q = 0; q < kChunks; q++) {
           const int e0 = q * 16, c1 = c0 + part * kCols + e0;
@@ -400,6 +399,9 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[it & 1]);  // (S has been read, also where P is of no use)
 
+        auto through_cap = [&](int e) {
+          return CAP ? make_float2(capped[CAP ? e : 0], capped[CAP ? e + 1 : 0]) : make_float2(p[e], p[e + 1]);
+        };
         mbar_wait(&g_full, it & 1, dead, timeouts);
         tc_fence_after();
 #pragma unroll
@@ -686,9 +688,10 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
 }
 
 // What the sums of the most buckets and the longest map leave room for.
-constexpr int kMostSums = 4 * DLB_ATTN_MAX_BUCKETS * kTileRows * 2, kMostLuts = 5 * (2 * (DLB_ATTN_MAX_DISTANCE + kLutPad) + 4) + 16;
-static_assert(1024 + BwdShape<1, 2>::kRest + kMostSums + kMostLuts + kMaxTiles <= kMaxDynamicSmem &&
-              1024 + BwdShape<2, 1>::kRest + kMostSums + kMostLuts + kMaxTiles <= kMaxDynamicSmem, "a table must fit in some shape");
+constexpr int kMostSums = 4 * DLB_ATTN_MAX_BUCKETS * kTileRows * 2;  // two parts
+constexpr int kMostLuts = 5 * (2 * (DLB_ATTN_MAX_DISTANCE + kLutPad) + 4) + 16;
+static_assert(1024 + BwdShape<1, 2>::kRest + kMostSums + kMostLuts + kMaxTiles <= kMaxDynamicSmem, "any table must fit");
+static_assert(1024 + BwdShape<2, 1>::kRest + kMostSums + kMostLuts + kMaxTiles <= kMaxDynamicSmem, "any table must fit");
 
 template <bool FOR_KEYS>
 int bwd_mma_launch(const AttnArgs &a, const BwdMaps &maps, cudaStream_t st) {

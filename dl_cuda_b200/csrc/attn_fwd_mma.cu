@@ -18,8 +18,8 @@
 // Measured (4096 tokens, 32 heads of 128 on 8 key heads): 268 us, 1.03 PFLOP/s, of the 1.66 that the
 // library's plain product reaches; causal 147 us, causal with a cap 184 us (205 us from a cold L2).
 // By the clock a pair of tiles takes 3500 cycles where the tensor cores need 2470 of issue: a tile's own
-// chain of scores, softmax (1700 cycles a tile,
-// half of which are exponentials) and product is what remains, since TMEM has no room for a second S.
+// chain of scores, softmax (1700 cycles a tile, half of which are exponentials) and product is what remains,
+// since TMEM has no room for a second S.
 // Taking a quarter of the exponentials as polynomials on the fp32 pipes changed nothing (275 us).
 #include <algorithm>
 

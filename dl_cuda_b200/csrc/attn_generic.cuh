@@ -1,9 +1,9 @@
 // Attention in fp32 arithmetic: every storage type, head width, stride and alignment.
 //
 // The products run on the warp-level tensor path (mma.sync m16n8k8, tf32) with every operand split in
-// two, x = hi + lo with 11 bits each: hi*hi + hi*lo + lo*hi leaves out 2^-21 of |x||y|.  fp32
-// results are up to three times as far from the exact ones as those of plain fp32 arithmetic (2-norm at most
-// 9e-7 over 210 random cases, 1.1e-6 for the gradient of a table); bf16 values need no lo, but take the
+// two, x = hi + lo with 11 bits each: hi*hi + hi*lo + lo*hi leaves out 2^-21 of |x||y|.
+// fp32 results are up to three times as far from the exact ones as those of plain fp32 arithmetic (2-norm at
+// most 9e-7 over 210 random cases, 1.1e-6 for the gradient of a table); bf16 values need no lo, but take the
 // same road.  Three such products run at 90 TFLOP/s where scalar multiply-adds reach 67 at best (both
 // measured on a B200), and they need a quarter of the shared-memory reads: the 64x64 scalar tiles this
 // replaces were bound by those.
@@ -475,7 +475,8 @@ static __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __
 }
 
 // Fills row_stats: -lse * log2(e) and -delta, delta = <dout_i, o_i> (= sum_j P_ij dP_ij; from a bf16 output
-// a first guess, see attn_bwd_generic).  A row is taken by LANES lanes with one 16-byte vector of each at a time, or by a warp element by element.
+// a first guess, see attn_bwd_generic).  A row is taken by LANES lanes with one 16-byte vector of each at a
+// time, or by a warp element by element.
 template <typename T, int LANES, bool VEC>
 static __global__ void __launch_bounds__(256) attn_row_stats_kernel(const __grid_constant__ AttnArgs a) {
   pdl_prologue();

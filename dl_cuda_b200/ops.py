@@ -399,7 +399,8 @@ def attn_bwd(dout, q, k, v, o, lse, scale=None, cap=0.0, causal=False, kv_lens=N
              q_docs=None, kv_docs=None, slopes=None, table=None, bucket_of=None, dq=None, dk=None, dv=None, dtable=None,
              want_dtable=True, workspace=None):
     """Returns (dq, dk, dv, dtable) from dout, with o and lse as attn_fwd returned them for the same arguments (or for
-    more keys: then dq and dtable are the parts of these keys); dtable (fp32 [heads, buckets]) is None without a table or when want_dtable is False."""
+    more keys: then dq and dtable are the parts of these keys); dtable (fp32 [heads, buckets]) is None without a
+    table or when want_dtable is False."""
     shape, dtype = q.shape, q.dtype
     if len(shape) != 4:
         raise ValueError("q is [batch, token, head, column]")
