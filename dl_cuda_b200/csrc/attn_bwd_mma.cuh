@@ -516,7 +516,7 @@ attn_bwd_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ 
         off += d_part[k][row];
         total += p_part[k][row];
       }
-      if (!row_is_whole(total)) off = 0.f;
+      if (!row_is_whole<__nv_bfloat16>(a, total, row_stat.x)) off = 0.f;
       if (part == 0) stats_tile(a, b, unit, tile)[kStatRows + row] = row_stat.y - off;
     }
     mbar_wait(&acc_full, 0, dead, timeouts);

@@ -63,9 +63,16 @@ __device__ __forceinline__ float *stats_tile(const AttnArgs &a, int b, int h, in
   return a.row_stats + ((static_cast<size_t>(b) * a.heads + h) * stat_tiles(a.q_len) + tile) * (2 * kStatRows);
 }
 // Backward: are these all the keys of a row (its probabilities, rebuilt from lse, add up to one), so that its
-// score gradients add up to zero?  Not for a call over some of the keys with o and lse of all.  What the
-// rounding of lse may move the sum by stays under the limit up to |lse| = 8000.
-__device__ __forceinline__ bool row_is_whole(float sum) { return fabsf(sum - 1.f) <= 0x1p-10f; }
+// score gradients add up to zero?  Not for a call over some of the keys with o and lse of all.  The sum may be
+// off by twice what the rounding of lse makes of a probability, by what two kernels make of a score, and with
+// bf16 by the roads of a cap (2^-21 of a score in each pass).  A share that lacks less of a row's weight than
+// that passes for the whole, and what it lacks is lost in the same roundings.
+template <typename T>
+__device__ __forceinline__ bool row_is_whole(const AttnArgs &a, float sum, float minus_lse_log2) {
+  const bool half = sizeof(T) == 2;
+  const float limit = fmaf(fabsf(minus_lse_log2), 0x1p-22f * kLn2, half ? fmaf(a.cap, 0x1p-20f, 0x1p-15f) : 0x1p-18f);
+  return fabsf(sum - 1.f) <= fminf(limit, 0x1p-10f);  // (lse = -infinity: the sum is 0)
+}
 
 __device__ __forceinline__ float2 stat_at(const AttnArgs &a, int b, int h, int i) {
   const float *t = stats_tile(a, b, h, i / kStatRows) + i % kStatRows;

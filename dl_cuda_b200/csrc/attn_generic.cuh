@@ -744,7 +744,7 @@ __device__ __forceinline__ void attn_bwd_generic(const AttnArgs &a, bool vec, in
         sum.x += row_sums[k][r0 + g + 8 * x].x;
         sum.y += row_sums[k][r0 + g + 8 * x].y;
       }
-      off[x] = row_is_whole(sum.y) ? sum.x : 0.f;
+      off[x] = row_is_whole<T>(a, sum.y, row_stat[x].x) ? sum.x : 0.f;
     }
 #pragma unroll
     for (int q = 0; q < DP / 32; q++)
@@ -792,7 +792,7 @@ __device__ __forceinline__ void attn_bwd_generic(const AttnArgs &a, bool vec, in
         e += v.x;
         total += v.y;
       }
-      e = row_is_whole(total) ? e / total : 0.f;
+      e = r < rows && row_is_whole<T>(a, total, stat_at(a, b, unit, row0 + r).x) ? e / total : 0.f;
       for (int n = 0; n < a.buckets; n++) sums[n * kRows + r].x -= e * sums[n * kRows + r].y;
     }
     __syncthreads();

@@ -299,6 +299,31 @@ def test_backward_of_shares_of_the_keys(kind, D, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("D", [64, 128, 20])
+def test_a_share_with_nearly_all_the_weight(D, dtype):
+    """A first share of the keys that holds all but some 1e-4 of every row's weight is not taken for the whole."""
+    B, Sq, Sk, H = 1, 100, 300, 2
+    q, k, v, dout = make(D + 3, dtype, B, Sq, Sk, H, H, D, "plain", std=0.3)
+    q[..., 0] = 4.5 * D ** 0.25
+    k[:, :150, :, 0], k[:, 150:, :, 0] = D ** 0.25, -D ** 0.25  # 9 between the shares' scores
+    v[:, 150:] += 30.0  # and one sign for what the little weight brings
+    dout = 1.0 + 0.1 * dout
+    u = torch.finfo(q.dtype).eps / 2
+    how = options("table", B, Sq, Sk, H)
+    values, bounds = reference(q, k, v, dout, shares=True, **how)
+    o, lse = ops.attn_fwd(q, k, v, **how)
+    dq, dtable, dk, dv = 0.0, 0.0, [], []
+    for first, last in ((0, 150), (150, 300)):
+        got = ops.attn_bwd(dout, q, k[:, first:last], v[:, first:last], o, lse, **dict(how, q_start=ints([-first])))
+        dq = dq + got[0].double()
+        bounds["dq"] += u / (1 - u) * got[0].double().abs()
+        dk.append(got[1])
+        dv.append(got[2])
+        dtable = dtable + got[3].double()
+    check(dict(dq=dq, dk=torch.cat(dk, 1), dv=torch.cat(dv, 1), dtable=dtable), values, bounds)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_empty_sizes_with_documents(dtype):
     dt = DTYPES[dtype]
     full = lambda *s: torch.ones(*s, dtype=dt, device="cuda")  # noqa: E731
